@@ -12,7 +12,10 @@ from .attention import (apply_fused_attention_patch, quantized_scaled_dot_produc
 from .block_pool import (AgentBlocks, BlockPool, KVBlock, ModelCacheSpec, PoolExhaustedError,
                          BLOCK_SIZE_TOKENS)
 from .cache import BatchQuantizedKVCache, QuantizedKVCache, validate_q4_pipeline
+from .experts import (ExpertRouting, combine_experts, expert_matmul, expert_swiglu,
+                      route_experts)
 from .kernels import dequantize, quantize
+from .linear import Q4Weight, quantized_matmul, quantized_swiglu
 from .masks import CausalMask, create_causal_mask
 from .paged import PagedLayerCache, PagedQ4Pool, lpt_partition, shuffled_allocator
 from .paged_cache import (DeviceBlockPool, PagedBatchQuantizedKVCache, PagedKV, PagedMask,
@@ -20,11 +23,12 @@ from .paged_cache import (DeviceBlockPool, PagedBatchQuantizedKVCache, PagedKV, 
 
 __all__ = [
     "AgentBlocks", "BLOCK_SIZE_TOKENS", "BatchQuantizedKVCache", "BlockPool", "CausalMask",
-    "DeviceBlockPool", "KVBlock", "ModelCacheSpec", "PagedBatchQuantizedKVCache", "PagedKV",
+    "DeviceBlockPool", "ExpertRouting", "KVBlock", "ModelCacheSpec", "PagedBatchQuantizedKVCache", "PagedKV",
     "PagedLayerCache", "PagedMask", "PagedQ4Pool", "PoolExhaustedError",
-    "Q4KernelError", "Q4KernelUnavailable", "QuantizedKVCache", "apply_fused_attention_patch",
-    "create_causal_mask", "dequantize", "extract_agent_blocks", "lpt_partition", "quantize",
-    "reconstruct_cache", "slice_cache_to_length",
-    "quantized_scaled_dot_product_attention", "scaled_dot_product_attention",
+    "Q4KernelError", "Q4KernelUnavailable", "Q4Weight", "QuantizedKVCache",
+    "apply_fused_attention_patch", "combine_experts", "create_causal_mask", "dequantize",
+    "expert_matmul", "expert_swiglu", "extract_agent_blocks", "lpt_partition", "quantize",
+    "quantized_matmul", "quantized_swiglu", "reconstruct_cache", "route_experts",
+    "slice_cache_to_length", "quantized_scaled_dot_product_attention", "scaled_dot_product_attention",
     "shuffled_allocator", "validate_q4_pipeline",
 ]

@@ -48,6 +48,14 @@ EXPORTED_SYMBOLS = (
     "am_q4_blocks_unpack",
     "am_block_reserve",
     "am_block_release",
+    "am_q4_weight_pack",
+    "am_q4_linear_workspace_bytes",
+    "am_q4_linear",
+    "am_q4_expert_linear_workspace_bytes",
+    "am_q4_expert_linear",
+    "am_route_experts_workspace_bytes",
+    "am_route_experts",
+    "am_combine_experts",
 )
 STATIC_DECODE_SCRATCH_BYTES = 16 << 20
 
@@ -111,6 +119,20 @@ class AttnArgs(ctypes.Structure):
         ("mask_stride_n", c_int64),
         ("status", c_void_p),
         ("sinks", c_void_p),
+    ]
+
+
+class Q4WeightDesc(ctypes.Structure):
+    """Mirror of ``am_q4_weight``."""
+
+    _fields_ = [
+        ("codes", c_void_p),
+        ("params", c_void_p),
+        ("row_scale", c_void_p),
+        ("n_out", c_int32),
+        ("n_in", c_int32),
+        ("experts", c_int32),
+        ("dtype", c_int32),
     ]
 
 
@@ -186,6 +208,29 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     lib.am_block_release.argtypes = [c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int32,
                                      c_void_p, c_void_p, c_void_p]
     lib.am_block_release.restype = c_int32
+    weight = ctypes.POINTER(Q4WeightDesc)
+    lib.am_q4_weight_pack.argtypes = [c_void_p, c_void_p, c_int32, c_int64, c_int32, c_void_p,
+                                      c_void_p, c_void_p]
+    lib.am_q4_linear_workspace_bytes.argtypes = [weight, weight, c_int32]
+    lib.am_q4_linear.argtypes = [weight, weight, c_void_p, c_int64, c_int32, c_void_p, c_int64,
+                                 c_void_p, c_size_t, c_void_p, c_void_p]
+    lib.am_q4_expert_linear_workspace_bytes.argtypes = [weight, weight, c_int32, c_int32]
+    lib.am_q4_expert_linear.argtypes = [weight, weight, c_void_p, c_int64, c_int32, c_void_p,
+                                        c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p,
+                                        c_size_t, c_void_p, c_void_p]
+    lib.am_route_experts_workspace_bytes.argtypes = [c_int32, c_int32, c_int32]
+    lib.am_route_experts.argtypes = [c_void_p, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_size_t, c_void_p]
+    lib.am_combine_experts.argtypes = [c_void_p, c_int32, c_int64, c_int32, c_void_p, c_void_p,
+                                       c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32,
+                                       c_int32, c_void_p, c_void_p]
+    for fn in ("am_q4_weight_pack", "am_q4_linear", "am_q4_expert_linear", "am_route_experts",
+               "am_combine_experts"):
+        getattr(lib, fn).restype = c_int32
+    for fn in ("am_q4_linear_workspace_bytes", "am_q4_expert_linear_workspace_bytes",
+               "am_route_experts_workspace_bytes"):
+        getattr(lib, fn).restype = c_size_t
     ver = lib.am_abi_version()
     if ver != ABI_VERSION:
         raise Q4KernelUnavailable(f"{p} has ABI version {ver}, expected {ABI_VERSION}")

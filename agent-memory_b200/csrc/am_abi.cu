@@ -16,6 +16,7 @@
 
 #include "am_common.cuh"
 #include "am_internal.h"
+#include "am_linear.cuh"
 
 namespace am {
 
@@ -681,6 +682,216 @@ int am_block_release(int32_t* free_ids, int32_t* free_top, int32_t num_blocks, i
   p.counts = keep_blocks;
   p.status = status;
   return cuda_status(launch_block_release(p, static_cast<cudaStream_t>(stream)), "am_block_release");
+}
+
+// ---------------------------------------------------------------- 4-bit weights and experts
+
+int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int64_t rows, int32_t n_in,
+                      uint32_t* params, float* row_scale, void* stream) {
+  clear_error();
+  if (!valid_half_dtype(dtype) || rows < 0 || rows > (int64_t)INT_MAX || n_in <= 0 || n_in % 64) {
+    set_error("am_q4_weight_pack: F16 or BF16, rows in [0, 2^31), n_in a positive multiple of 64 required");
+    return AM_ERR_INVALID;
+  }
+  if (rows == 0) return AM_OK;
+  if (!scales || !biases || !params || !row_scale || !aligned(params, 16) || !aligned(scales, 2) ||
+      !aligned(biases, 2) || !aligned(row_scale, 4)) {
+    set_error("am_q4_weight_pack: scales, biases, params (16-byte aligned) and row_scale required");
+    return AM_ERR_INVALID;
+  }
+  return cuda_status(launch_weight_pack(scales, biases, dtype == AM_DTYPE_BF16, rows, n_in / 64, params,
+                                        row_scale, static_cast<cudaStream_t>(stream)),
+                     "am_q4_weight_pack");
+}
+
+static int check_weight(const am_q4_weight* w, const char* fn) {
+  if (w == nullptr || !w->codes || !w->params || !w->row_scale) {
+    set_error("%s: a packed weight (codes, params, row_scale) is required", fn);
+    return AM_ERR_INVALID;
+  }
+  if (!valid_half_dtype(w->dtype) || w->n_out <= 0 || w->n_in <= 0 || w->n_in % 64 || w->experts <= 0 ||
+      (int64_t)w->experts * w->n_out > (int64_t)INT_MAX) {
+    set_error("%s: weight needs F16 or BF16, n_out > 0, n_in %% 64 == 0, experts > 0 (got %d, %d, %d, %d)", fn,
+              w->dtype, w->n_out, w->n_in, w->experts);
+    return AM_ERR_INVALID;
+  }
+  if (!aligned(w->codes, 16) || !aligned(w->params, 16) || !aligned(w->row_scale, 4)) {
+    set_error("%s: codes and params must be 16-byte and row_scale 4-byte aligned", fn);
+    return AM_ERR_INVALID;
+  }
+  return AM_OK;
+}
+
+// Fills p from a call's arguments; `offsets` null: one matrix over all rows.
+static int linear_params(LinearParams& p, const am_q4_weight* w, const am_q4_weight* up, const void* x,
+                         int64_t x_stride, int32_t x_rows, const int32_t* offsets, const int32_t* order,
+                         int32_t top_k, int32_t rows, void* out, int64_t out_stride, int32_t* status,
+                         const char* fn) {
+  clear_error();
+  int rc = check_weight(w, fn);
+  if (rc == AM_OK && up != nullptr) rc = check_weight(up, fn);
+  if (rc) return rc;
+  if (up != nullptr && (up->n_out != w->n_out || up->n_in != w->n_in || up->experts != w->experts ||
+                        up->dtype != w->dtype)) {
+    set_error("%s: the two weights of a gated call must have the same shape and dtype", fn);
+    return AM_ERR_INVALID;
+  }
+  if (rows < 0 || x_rows < 0 || (order != nullptr ? top_k <= 0 : x_rows < rows)) {
+    set_error("%s: rows and x_rows >= 0, top_k > 0 with an order, x_rows >= rows without one", fn);
+    return AM_ERR_INVALID;
+  }
+  if (rows > 0 && (x == nullptr || out == nullptr || !aligned(x, 16) || !aligned(out, 2) ||
+                   x_stride < w->n_in || x_stride % 8 || out_stride < w->n_out)) {
+    set_error("%s: x (16-byte aligned, row stride a multiple of 8 and at least n_in) and out (row stride at "
+              "least n_out) required", fn);
+    return AM_ERR_INVALID;
+  }
+  p.codes[0] = w->codes;
+  p.params[0] = w->params;
+  p.row_scale[0] = w->row_scale;
+  p.codes[1] = up ? up->codes : nullptr;
+  p.params[1] = up ? up->params : nullptr;
+  p.row_scale[1] = up ? up->row_scale : nullptr;
+  p.n_out = w->n_out;
+  p.n_in = w->n_in;
+  p.groups = w->n_in / 64;
+  p.pstride = (p.groups + 3) & ~3;
+  p.experts = w->experts;
+  p.bf16 = w->dtype == AM_DTYPE_BF16;
+  p.x = static_cast<const uint16_t*>(x);
+  p.x_stride = x_stride;
+  p.x_rows = x_rows;
+  p.offsets = offsets;
+  p.order = order;
+  p.top_k = top_k;
+  p.rows = rows;
+  p.out = static_cast<uint16_t*>(out);
+  p.out_stride = out_stride;
+  p.status = status;
+  return AM_OK;
+}
+
+size_t am_q4_linear_workspace_bytes(const am_q4_weight*, const am_q4_weight*, int32_t) { return 0; }
+
+size_t am_q4_expert_linear_workspace_bytes(const am_q4_weight*, const am_q4_weight*, int32_t, int32_t) {
+  return 0;
+}
+
+static int run_linear(const LinearParams& p, void* workspace, size_t workspace_bytes, void* stream,
+                      const char* fn) {
+  (void)workspace;
+  (void)workspace_bytes;
+  if (p.rows == 0) return AM_OK;
+  return cuda_status(launch_linear(p, static_cast<cudaStream_t>(stream)), fn);
+}
+
+int am_q4_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, int64_t x_stride, int32_t rows,
+                 void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, int32_t* status,
+                 void* stream) {
+  LinearParams p{};
+  int rc = linear_params(p, w, up, x, x_stride, rows, nullptr, nullptr, 1, rows, out, out_stride, status,
+                         "am_q4_linear");
+  if (rc) return rc;
+  if (w->experts != 1) {
+    set_error("am_q4_linear: one matrix expected, the weight holds %d", w->experts);
+    return AM_ERR_INVALID;
+  }
+  return run_linear(p, workspace, workspace_bytes, stream, "am_q4_linear");
+}
+
+int am_q4_expert_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, int64_t x_stride,
+                        int32_t x_rows, const int32_t* offsets, const int32_t* order, int32_t top_k,
+                        int32_t rows, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                        int32_t* status, void* stream) {
+  LinearParams p{};
+  if (offsets == nullptr) {
+    set_error("am_q4_expert_linear: offsets required");
+    return AM_ERR_INVALID;
+  }
+  int rc = linear_params(p, w, up, x, x_stride, x_rows, offsets, order, order ? top_k : 1, rows, out,
+                         out_stride, status, "am_q4_expert_linear");
+  if (rc) return rc;
+  return run_linear(p, workspace, workspace_bytes, stream, "am_q4_expert_linear");
+}
+
+static int check_route(int32_t tokens, int32_t n_experts, int32_t top_k) {
+  return tokens >= 0 && n_experts > 0 && n_experts <= 1024 && top_k > 0 && top_k <= 32 && top_k <= n_experts &&
+         (int64_t)tokens * top_k <= (int64_t)INT_MAX;
+}
+
+size_t am_route_experts_workspace_bytes(int32_t, int32_t, int32_t) { return 0; }
+
+int am_route_experts(const void* logits, int32_t dtype, int64_t stride, int32_t tokens, int32_t n_experts,
+                     int32_t top_k, int32_t normalize, int32_t* experts, float* weights, int32_t* offsets,
+                     int32_t* order, int32_t* positions, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  clear_error();
+  if (!check_route(tokens, n_experts, top_k)) {
+    set_error("am_route_experts: tokens >= 0, 1 <= top_k <= min(32, n_experts), n_experts <= 1024 and fewer "
+              "than 2^31 pairs required (got %d, %d, %d)", tokens, n_experts, top_k);
+    return AM_ERR_INVALID;
+  }
+  if (!(valid_half_dtype(dtype) || dtype == AM_DTYPE_F32) || stride < n_experts) {
+    set_error("am_route_experts: logits are F16, BF16 or F32 rows at least n_experts apart");
+    return AM_ERR_INVALID;
+  }
+  if (!offsets || (tokens > 0 && (!logits || !experts || !weights || !order || !positions))) {
+    set_error("am_route_experts: a buffer is NULL");
+    return AM_ERR_INVALID;
+  }
+  if (workspace_bytes < am_route_experts_workspace_bytes(tokens, n_experts, top_k)) {
+    set_error("am_route_experts: workspace of %zu bytes required",
+              am_route_experts_workspace_bytes(tokens, n_experts, top_k));
+    return AM_ERR_WORKSPACE;
+  }
+  RouteParams p{};
+  p.logits = logits;
+  p.dtype = dtype;
+  p.stride = stride;
+  p.tokens = tokens;
+  p.n_experts = n_experts;
+  p.top_k = top_k;
+  p.normalize = normalize != 0;
+  p.experts = experts;
+  p.weights = weights;
+  p.offsets = offsets;
+  p.order = order;
+  p.positions = positions;
+  p.ws = static_cast<int32_t*>(workspace);
+  return cuda_status(launch_route(p, static_cast<cudaStream_t>(stream)), "am_route_experts");
+}
+
+int am_combine_experts(const void* y, int32_t dtype, int64_t y_stride, int32_t y_rows, const float* weights,
+                       const int32_t* positions, const void* residual, int64_t residual_stride, void* out,
+                       int64_t out_stride, int32_t tokens, int32_t top_k, int32_t width, int32_t* status,
+                       void* stream) {
+  clear_error();
+  if (!valid_half_dtype(dtype) || tokens < 0 || top_k <= 0 || width < 0 || y_rows < 0) {
+    set_error("am_combine_experts: F16 or BF16, tokens, width, y_rows >= 0 and top_k > 0 required");
+    return AM_ERR_INVALID;
+  }
+  if (tokens == 0 || width == 0) return AM_OK;
+  if (!y || !weights || !positions || !out || y_stride < width || out_stride < width ||
+      (residual && residual_stride < width)) {
+    set_error("am_combine_experts: y, weights, positions and out, with row strides of at least width, required");
+    return AM_ERR_INVALID;
+  }
+  CombineParams p{};
+  p.y = static_cast<const uint16_t*>(y);
+  p.residual = static_cast<const uint16_t*>(residual);
+  p.out = static_cast<uint16_t*>(out);
+  p.y_stride = y_stride;
+  p.residual_stride = residual_stride;
+  p.out_stride = out_stride;
+  p.weights = weights;
+  p.positions = positions;
+  p.y_rows = y_rows;
+  p.tokens = tokens;
+  p.top_k = top_k;
+  p.width = width;
+  p.bf16 = dtype == AM_DTYPE_BF16;
+  p.status = status;
+  return cuda_status(launch_combine(p, static_cast<cudaStream_t>(stream)), "am_combine_experts");
 }
 
 }  // extern "C"

@@ -13,6 +13,9 @@ struct AppendParams;
 struct DecodeParams;
 struct BlockCopyParams;
 struct BlockListParams;
+struct LinearParams;
+struct RouteParams;
+struct CombineParams;
 
 cudaError_t launch_quantize(const void* x, bool bf16, int64_t rows, int dim, uint32_t* codes,
                             void* scales, void* biases, cudaStream_t stream);
@@ -53,6 +56,13 @@ int decode_max_cluster(int k_dim, int v_dim);
 int decode_active_clusters(int k_dim, int v_dim, int size);
 // Resident decode CTAs per SM on the current device for a (k_dim, v_dim) pair.
 int decode_ctas_per_sm(int k_dim, int v_dim);
+
+// 4-bit linear layers (am_linear.cu) and expert routing (am_experts.cu).
+cudaError_t launch_weight_pack(const void* scales, const void* biases, bool bf16, int64_t rows,
+                               int groups, uint32_t* params, float* row_scale, cudaStream_t stream);
+cudaError_t launch_linear(const LinearParams& p, cudaStream_t stream);
+cudaError_t launch_route(const RouteParams& p, cudaStream_t stream);
+cudaError_t launch_combine(const CombineParams& p, cudaStream_t stream);
 
 cudaError_t launch_blocks_copy(const BlockCopyParams& p, int n_blocks, cudaStream_t stream);
 cudaError_t launch_block_reserve(const BlockListParams& p, cudaStream_t stream);

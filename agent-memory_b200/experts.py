@@ -1,0 +1,211 @@
+"""Mixture-of-experts layers over 4-bit weights: routing, grouped products, combination.
+
+A layer of experts runs as::
+
+    r = route_experts(logits, top_k)              # which experts, their weights, sorted rows
+    h = expert_swiglu(x, gate, up, r)             # [tokens * top_k, inner], rows by expert
+    y = expert_matmul(h, down, r)                 # [tokens * top_k, width], rows by expert
+    out = combine_experts(y, r.weights, r.positions, residual=x)
+
+Nothing of it comes back to the host: the experts' row counts stay on the device, and the
+products read each expert that has rows once.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from ._lib import check
+from .kernels import _half_code, dtype_code
+from .linear import (Q4Weight, _check_pair, _out, _raw_stream, _row_stride, _rows_of, _workspace)
+
+MAX_EXPERTS, MAX_TOP_K = 1024, 32
+
+
+class ExpertRouting(NamedTuple):
+    """Which experts each token goes to (int32 tensors but for the weights).
+
+    experts, weights, positions: [tokens, top_k]; offsets: [n_experts + 1]; order: [tokens *
+    top_k], the (token, slot) pairs ``t * top_k + j`` sorted by expert (stable).  Rows
+    ``[offsets[e], offsets[e + 1])`` of a sorted tensor are expert e's, and pair (t, j) is row
+    ``positions[t, j]``."""
+
+    experts: torch.Tensor
+    weights: torch.Tensor
+    offsets: torch.Tensor
+    order: torch.Tensor
+    positions: torch.Tensor
+
+
+def _int32(t: torch.Tensor, shape, device, what: str) -> torch.Tensor:
+    if t.dtype is not torch.int32 or tuple(t.shape) != tuple(shape) or t.device != device:
+        raise ValueError(f"{what} must be int32 {tuple(shape)} on {device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _status_ptr(status, device):
+    if status is None:
+        return None
+    if status.dtype is not torch.int32 or status.device != device or status.numel() < 1:
+        raise ValueError(f"status must be an int32 tensor on {device}")
+    return status.data_ptr()
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, normalize: bool = True) -> ExpertRouting:
+    """Top-k routing of logits [tokens, n_experts] (float32, float16 or bfloat16).
+
+    Per token the ``top_k`` largest logits in falling order, the lower index first among equal
+    ones (NaN counts as -inf), with softmax weights over the chosen logits (``normalize``) or
+    over all of them.  A token whose logits are all -inf has weights 0; infinite logits share
+    the weight equally."""
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [tokens, n_experts], got {tuple(logits.shape)}")
+    tokens, n_experts = logits.shape
+    if not 1 <= top_k <= min(MAX_TOP_K, n_experts) or n_experts > MAX_EXPERTS:
+        raise ValueError(f"top_k in 1..min({MAX_TOP_K}, n_experts) and n_experts <= {MAX_EXPERTS} "
+                         f"required, got {top_k} of {n_experts}")
+    dev = logits.device
+    if not logits.is_cuda:
+        raise ValueError("Q4 kernels run on CUDA tensors only (no CPU path)")
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("route_experts has no backward pass: detach the logits or use no_grad")
+    if logits.stride(1) != 1 or (tokens > 1 and logits.stride(0) < n_experts):
+        logits = logits.contiguous()
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _route_call(logits, tokens, n_experts, top_k, normalize, dev)
+    return _route_call(logits, tokens, n_experts, top_k, normalize, dev)
+
+
+def _route_call(logits, tokens, n_experts, top_k, normalize, dev):
+    pairs = tokens * top_k
+    # one buffer: experts, positions, order, offsets
+    buf = torch.empty(3 * pairs + n_experts + 1, dtype=torch.int32, device=dev)
+    weights = torch.empty(tokens, top_k, dtype=torch.float32, device=dev)
+    experts = buf[:pairs].view(tokens, top_k)
+    positions = buf[pairs:2 * pairs].view(tokens, top_k)
+    order, offsets = buf[2 * pairs:3 * pairs], buf[3 * pairs:]
+    base = buf.data_ptr()
+    lib = _lib.load()
+    need = int(lib.am_route_experts_workspace_bytes(tokens, n_experts, top_k))
+    ws = _workspace(need, dev)
+    rc = lib.am_route_experts(logits.data_ptr(), dtype_code(logits.dtype), _row_stride(logits), tokens,
+                              n_experts, top_k, 1 if normalize else 0, base, weights.data_ptr(),
+                              base + 12 * pairs, base + 8 * pairs, base + 4 * pairs,
+                              ws.data_ptr() if ws is not None else None, need,
+                              _raw_stream(dev.index))
+    if rc:
+        check("am_route_experts", rc)
+    return ExpertRouting(experts, weights, offsets, order, positions)
+
+
+def _expert_linear(x, w: Q4Weight, up, routing: ExpertRouting, gather: bool, out, status):
+    if w.codes.dim() != 3:
+        raise ValueError(f"{w} is one matrix: use quantized_matmul / quantized_swiglu")
+    if x.dim() != 2:
+        raise ValueError(f"x must be [rows, {w.n_in}], got {tuple(x.shape)}")
+    x = _rows_of(x, w)
+    rows = routing.order.shape[0]
+    offsets = _int32(routing.offsets, (w.experts + 1,), w.device, "routing.offsets")
+    order, top_k = None, 1
+    if gather:
+        order = _int32(routing.order, (rows,), w.device, "routing.order")
+        top_k = routing.experts.shape[1]
+        if x.shape[0] * top_k != rows:
+            raise ValueError(f"x has {x.shape[0]} tokens, the routing {rows} rows of {top_k} each")
+    elif x.shape[0] != rows:
+        raise ValueError(f"x has {x.shape[0]} rows, the routing {rows}")
+    if w.index != torch.cuda.current_device():
+        with torch.cuda.device(w.device):
+            return _expert_call(x, w, up, offsets, order, top_k, rows, out, status)
+    return _expert_call(x, w, up, offsets, order, top_k, rows, out, status)
+
+
+def _expert_call(x, w, up, offsets, order, top_k, rows, out, status):
+    out = _out(out, rows, w, (rows, w.n_out))
+    lib = _lib.load()
+    key = (up is not None, x.shape[0], rows)
+    need = w.bytes_cache.get(key)
+    up_ref = up.ref if up is not None else None
+    if need is None:
+        need = w.bytes_cache[key] = int(
+            lib.am_q4_expert_linear_workspace_bytes(w.ref, up_ref, x.shape[0], rows))
+    ws = _workspace(need, w.device)
+    rc = lib.am_q4_expert_linear(w.ref, up_ref, x.data_ptr(), _row_stride(x), x.shape[0],
+                                 offsets.data_ptr(), order.data_ptr() if order is not None else None,
+                                 top_k, rows, out.data_ptr(), w.n_out,
+                                 ws.data_ptr() if ws is not None else None, need,
+                                 _status_ptr(status, w.device), _raw_stream(w.index))
+    if rc:
+        check("am_q4_expert_linear", rc)
+    return out
+
+
+def expert_matmul(x: torch.Tensor, weight: Q4Weight, routing: ExpertRouting, *, gather: bool = False,
+                  out: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """Row r of x [tokens * top_k, n_in], sorted by expert, times its expert's matrix (with
+    ``gather`` x is [tokens, n_in] and each pair's row is fetched through ``routing.order``)
+    -> [tokens * top_k, n_out] sorted by expert.  ``status``: optional int32 device word that
+    gets AM_STATUS_* bits for order entries outside x."""
+    return _expert_linear(x, weight, None, routing, gather, out, status)
+
+
+def expert_swiglu(x: torch.Tensor, gate: Q4Weight, up: Q4Weight, routing: ExpertRouting, *,
+                  gather: bool = True, out: torch.Tensor | None = None,
+                  status: torch.Tensor | None = None):
+    """silu(x gate_e^T) * (x up_e^T) for each (token, slot) pair's expert e, from x [tokens, n_in]
+    -> [tokens * top_k, n_out] sorted by expert (``gather=False``: x holds the sorted rows)."""
+    _check_pair(gate, up)
+    return _expert_linear(x, gate, up, routing, gather, out, status)
+
+
+def combine_experts(y: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor, *,
+                    residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    status: torch.Tensor | None = None):
+    """out[t] = residual[t] + sum_j weights[t, j] * y[positions[t, j]]: y [rows, width] float16
+    or bfloat16, weights float32 and positions int32 [tokens, top_k].  fp32 sums, rounded once."""
+    if not y.is_cuda:
+        raise ValueError("Q4 kernels run on CUDA tensors only (no CPU path)")
+    if y.dim() != 2 or positions.dim() != 2:
+        raise ValueError("y must be [rows, width] and positions [tokens, top_k]")
+    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
+        raise RuntimeError("combine_experts has no backward pass: detach its inputs or use no_grad")
+    dev, (tokens, top_k), width = y.device, positions.shape, y.shape[1]
+    if top_k == 0:
+        raise ValueError("positions must hold at least one slot a token")
+    positions = _int32(positions, (tokens, top_k), dev, "positions")
+    if weights.dtype is not torch.float32 or weights.shape != positions.shape or weights.device != dev:
+        raise ValueError(f"weights must be float32 {(tokens, top_k)} on {dev}")
+    weights = weights if weights.is_contiguous() else weights.contiguous()
+    code = _half_code(y.dtype)
+
+    def rows(t):
+        return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
+
+    y = rows(y)
+    if residual is not None:
+        if residual.shape != (tokens, width) or residual.dtype is not y.dtype or residual.device != dev:
+            raise ValueError(f"residual must be {y.dtype} {(tokens, width)} on {dev}")
+        residual = rows(residual)
+    if out is None:
+        out = torch.empty(tokens, width, dtype=y.dtype, device=dev)
+    elif (out.shape != (tokens, width) or out.dtype is not y.dtype or out.device != dev
+          or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous {y.dtype} tensor {(tokens, width)} on {dev}")
+    args = (y.data_ptr(), code, _row_stride(y), y.shape[0], weights.data_ptr(), positions.data_ptr(),
+            residual.data_ptr() if residual is not None else None,
+            _row_stride(residual) if residual is not None else 0, out.data_ptr(), width, tokens, top_k,
+            width, _status_ptr(status, dev), _raw_stream(dev.index))
+    lib = _lib.load()
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            rc = lib.am_combine_experts(*args)
+    else:
+        rc = lib.am_combine_experts(*args)
+    if rc:
+        check("am_combine_experts", rc)
+    return out

@@ -274,6 +274,94 @@ int am_block_release(int32_t* free_ids, int32_t* free_top, int32_t num_blocks, i
                      int32_t table_stride, int32_t rows, const int32_t* keep_blocks,
                      int32_t* status, void* stream);
 
+/* ---------------------------------------------------------------- 4-bit weights and experts
+ *
+ * The products around the attention of a model whose weights are held in the cache's 4-bit
+ * format (what mlx's quantized matrices are to the models the reference loads): linear
+ * layers, gated pairs of them, the same per expert, and the routing of tokens to experts.
+ * The weights are frozen codes; there is no backward pass. */
+
+/*
+ * One 4-bit matrix [n_out, n_in], or one per expert.  codes as mx.quantize writes them
+ * (element i of a row in word i/8 at bits 4*(i%8)); params / row_scale are the scales and
+ * biases as am_q4_weight_pack lays them out, once, when the weights are loaded.
+ */
+typedef struct am_q4_weight {
+  const uint32_t* codes;      /* device [experts, n_out, n_in/8], 16-byte aligned */
+  const uint32_t* params;     /* device [experts, n_out, ceil4(n_in/64)] */
+  const float* row_scale;     /* device [experts, n_out] */
+  int32_t n_out;
+  int32_t n_in;               /* multiple of 64 */
+  int32_t experts;            /* 1 for a plain matrix */
+  int32_t dtype;              /* AM_DTYPE_F16 or AM_DTYPE_BF16: activations and outputs */
+} am_q4_weight;
+
+/*
+ * Lays out the scales and biases (device [rows, n_in/64] of dtype F16 or BF16) of `rows`
+ * weight rows for the kernels: row_scale[r] = 2^e with e chosen so that every
+ * scale * 2^(24-e) and bias * 2^-e of row r fits fp16, and params[r, g] = the two as fp16
+ * (low half: the scale).  Both keep their value unless a group's is below about 2^-28 of
+ * its row's largest; entries past n_in/64 of a params row are zero.
+ */
+int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int64_t rows,
+                      int32_t n_in, uint32_t* params, float* row_scale, void* stream);
+
+/*
+ * y = x W^T (replaces mx.quantized_matmul(x, w, scales, biases, transpose=True)), or with a
+ * second matrix `up` of the same shape y = silu(x W^T) * (x up^T).  x: device [rows, n_in],
+ * out: device [rows, n_out], both of w->dtype, row strides in elements (x_stride % 8 == 0, x
+ * 16-byte aligned).  Sums are fp32; y is rounded once.  Weights enter the products rounded
+ * to fp16 (11 bits), activations exactly.
+ */
+size_t am_q4_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up, int32_t rows);
+int am_q4_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, int64_t x_stride,
+                 int32_t rows, void* out, int64_t out_stride, void* workspace,
+                 size_t workspace_bytes, int32_t* status, void* stream);
+
+/*
+ * The same with one matrix per expert (replaces mx.gather_qmm over sorted rows): output row
+ * r in [offsets[e], offsets[e+1]) is made with expert e's matrix from row order[r] / top_k of
+ * x (order given), or from row r of x (order NULL).  offsets: device int32 [experts + 1],
+ * non-decreasing, used clamped to [0, rows]; rows no expert holds are not written.  An order
+ * entry that points outside [0, x_rows) reads as a row of zeros and sets
+ * AM_STATUS_BAD_POSITION.
+ */
+size_t am_q4_expert_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up,
+                                           int32_t x_rows, int32_t rows);
+int am_q4_expert_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x,
+                        int64_t x_stride, int32_t x_rows, const int32_t* offsets,
+                        const int32_t* order, int32_t top_k, int32_t rows, void* out,
+                        int64_t out_stride, void* workspace, size_t workspace_bytes,
+                        int32_t* status, void* stream);
+
+/*
+ * Routing of tokens to experts.  logits: device [tokens, n_experts] of dtype F16, BF16 or F32,
+ * row stride in elements.  Per token the top_k largest logits in falling order (equal ones:
+ * the lower index first; NaN counts as -inf), and their softmax weights over all experts
+ * (normalize 0) or over the chosen ones (1); a token whose logits are all -inf has weights 0,
+ * and infinite logits share the weight equally.  experts / weights / positions: device
+ * [tokens, top_k]; offsets: device [n_experts + 1]; order: device [tokens * top_k]: the
+ * (token, slot) pairs t * top_k + j sorted by expert, equal ones in rising order, and
+ * positions[t, j] the place of pair (t, j) in it.  n_experts <= 1024, top_k <= 32.
+ */
+size_t am_route_experts_workspace_bytes(int32_t tokens, int32_t n_experts, int32_t top_k);
+int am_route_experts(const void* logits, int32_t dtype, int64_t stride, int32_t tokens,
+                     int32_t n_experts, int32_t top_k, int32_t normalize, int32_t* experts,
+                     float* weights, int32_t* offsets, int32_t* order, int32_t* positions,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * out[t] = residual[t] + sum over j of weights[t, j] * y[positions[t, j]] (fp32 sum in slot
+ * order, rounded once).  y: device [y_rows, width], residual (or NULL) and out: device
+ * [tokens, width], of dtype F16 or BF16, row strides in elements; weights / positions: device
+ * [tokens, top_k].  A position outside [0, y_rows) adds nothing and sets
+ * AM_STATUS_BAD_POSITION.
+ */
+int am_combine_experts(const void* y, int32_t dtype, int64_t y_stride, int32_t y_rows,
+                       const float* weights, const int32_t* positions, const void* residual,
+                       int64_t residual_stride, void* out, int64_t out_stride, int32_t tokens,
+                       int32_t top_k, int32_t width, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
