@@ -60,7 +60,13 @@ int decode_ctas_per_sm(int k_dim, int v_dim);
 // 4-bit linear layers (am_linear.cu) and expert routing (am_experts.cu).
 cudaError_t launch_weight_pack(const void* scales, const void* biases, bool bf16, int64_t rows,
                                int groups, uint32_t* params, float* row_scale, cudaStream_t stream);
-cudaError_t launch_linear(const LinearParams& p, cudaStream_t stream);
+// Linear layers: the tensor-tile kernel (tcgen05, am_linear_tc.cu; it needs the workspace and the
+// tensor maps of LinearParams) or the few-token kernel (am_linear.cu).
+bool linear_uses_tensor_tiles(int rows, int experts, bool grouped);
+// Rows of a token tile of the tensor-tile kernel for a call (the x map's box rows).
+int linear_token_tile(int rows, int experts, bool grouped);
+cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream);
+cudaError_t launch_linear_tiles(const LinearParams& p, cudaStream_t stream);
 cudaError_t launch_route(const RouteParams& p, cudaStream_t stream);
 cudaError_t launch_combine(const CombineParams& p, cudaStream_t stream);
 

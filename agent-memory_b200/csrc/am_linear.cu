@@ -93,61 +93,10 @@ struct FewParams {
   int32_t x_groups;   // groups staged at a time (a multiple of 4)
 };
 
-__device__ __forceinline__ uint32_t hfma2_bits(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-
-// The four weight pairs of one word: inputs (0, 4), (1, 5), (2, 6), (3, 7) of its eight.
-__device__ __forceinline__ void dequant_word(uint32_t w, uint32_t s24, uint32_t s20, uint32_t b, uint32_t (&o)[4]) {
-  const uint32_t h = w >> 8;
-  o[0] = hfma2_bits(w & 0x000f000fu, s24, b);
-  o[1] = hfma2_bits(w & 0x00f000f0u, s20, b);
-  o[2] = hfma2_bits(h & 0x000f000fu, s24, b);
-  o[3] = hfma2_bits(h & 0x00f000f0u, s20, b);
-}
-
 __device__ __forceinline__ uint2 ld_codes(const uint32_t* p) {
   uint2 v;
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
-}
-
-// The work item of blockIdx.y: rows [lo, hi) of one expert, at most 8 * NT of them.  Returns
-// the expert, or -1 past the last item.  Every thread of the CTA calls it.
-template <int TOK>
-__device__ __forceinline__ int find_item(const LinearParams& p, int item, int& lo, int& hi) {
-  if (p.offsets == nullptr) {
-    lo = item * TOK;
-    hi = min(lo + TOK, p.rows);
-    return lo < hi ? 0 : -1;
-  }
-  // each warp scans the experts, 32 at a time
-  const int lane = threadIdx.x & 31;
-  int base = 0;
-  for (int e0 = 0; e0 < p.experts; e0 += 32) {
-    int a = 0, b = 0;
-    if (e0 + lane < p.experts) expert_range(p, e0 + lane, a, b);
-    const int n = (b - a + TOK - 1) / TOK;
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    const int total = __shfl_sync(0xffffffffu, incl, 31);
-    if (item < base + total) {
-      const bool mine = item >= base + incl - n && item < base + incl;
-      const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
-      const int first = a + (item - (base + incl - n)) * TOK;
-      lo = __shfl_sync(0xffffffffu, first, src);
-      hi = min(__shfl_sync(0xffffffffu, b, src), lo + TOK);
-      return e0 + src;
-    }
-    base += total;
-  }
-  return -1;
 }
 
 template <int NT, int MT, bool GATED, int GQ>
@@ -216,10 +165,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) linear_few_kernel(const __g
       const int row = tok_row[tok];
       if (v < vecs && row >= 0) {
         const uint4 u = *reinterpret_cast<const uint4*>(p.x + (int64_t)row * p.x_stride + xg0 * 64 + v * 8);
-        const uint32_t a = __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);
-        const uint32_t b = __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu);
-        const uint32_t c = __vmaxu2(a, b);
-        mx = max(c & 0xffffu, c >> 16);
+        mx = max_abs_bits(u);
       }
       mx = __reduce_max_sync(0xffffffffu, mx);
       if (lane == 0) atomicMax(&tok_max[tok], static_cast<int>(mx));
@@ -227,10 +173,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) linear_few_kernel(const __g
     __syncthreads();
   }
   if (tid < TOK) {
-    // bf16 bits: the exponent field is bits 7..14; zero and subnormal rows count as 2^-126
-    int ex = 0;
-    if (p.bf16) ex = min(max(tok_max[tid] >> 7, 1), 254) - 127 - 14;
-    ex = max(ex, -126);
+    const int ex = p.bf16 ? row_exponent(tok_max[tid]) : 0;
     tok_scale[tid] = exp2f(static_cast<float>(ex));
     tok_max[tid] = __float_as_int(exp2f(static_cast<float>(-ex)));
   }
@@ -321,21 +264,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) linear_few_kernel(const __g
       uint4 o = make_uint4(0, 0, 0, 0);
       if (row >= 0) {
         const uint4 u = *reinterpret_cast<const uint4*>(p.x + (int64_t)row * p.x_stride + (int64_t)s0 * 64 + v * 8);
-        if (p.bf16) {
-          const float sc = tok_inv[tok];
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-          float x8[8];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x8[2 * j] = __uint_as_float(w[j] << 16) * sc;
-            x8[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * sc;
-          }
-          o = make_uint4(pack_half2(x8[0], x8[4]), pack_half2(x8[1], x8[5]), pack_half2(x8[2], x8[6]),
-                         pack_half2(x8[3], x8[7]));
-        } else {
-          o = make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632),
-                         __byte_perm(u.y, u.w, 0x5410), __byte_perm(u.y, u.w, 0x7632));
-        }
+        o = p.bf16 ? permute_bf16(u, tok_inv[tok]) : permute_f16(u);
       }
       // word c of the group: lane c / 2 of the quad, half c & 1
       reinterpret_cast<uint4*>(sx)[((int64_t)grp * 2 + (c & 1)) * m * 4 + tok * 4 + (c >> 1)] = o;
@@ -496,7 +425,14 @@ static cudaError_t launch_few(const LinearParams& p, cudaStream_t stream) {
   return launch_few_t<NT, 2, false, GQ>(p, static_cast<int>(items), stream);
 }
 
-cudaError_t launch_linear(const LinearParams& p, cudaStream_t stream) {
+// Which kernel: the mean number of rows of a matrix decides (a grouped call's counts are on the
+// device).
+bool linear_uses_tensor_tiles(int rows, int experts, bool grouped) {
+  const int mean = grouped ? (rows + experts - 1) / experts : rows;
+  return mean > 32;
+}
+
+cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream) {
   if (p.rows == 0) return cudaSuccess;
   const int mean = p.offsets != nullptr ? (p.rows + p.experts - 1) / p.experts : p.rows;
   if (mean <= 8) return launch_few<1>(p, stream);

@@ -23,6 +23,13 @@ struct LinearParams {
   uint16_t* out;
   int64_t out_stride;
   int32_t* status;
+  uint64_t wait_ns;           // limit of the bounded waits
+  // tensor-tile kernel: the activations as fp16 rows [x_rows][n_in] in its input order and their
+  // powers of two, in the caller's workspace; tensor maps of them and of the codes
+  uint16_t* xh;
+  float* xscale;
+  alignas(64) CUtensorMap tmap_w[2];
+  alignas(64) CUtensorMap tmap_x;
 };
 
 struct RouteParams {
@@ -70,6 +77,80 @@ __device__ __forceinline__ int source_row(const LinearParams& p, int r) {
     return -1;
   }
   return t;
+}
+
+__device__ __forceinline__ uint32_t hfma2_bits(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
+// The four weight pairs of one word: inputs (0, 4), (1, 5), (2, 6), (3, 7) of its eight.
+__device__ __forceinline__ void dequant_word(uint32_t w, uint32_t s24, uint32_t s20, uint32_t b, uint32_t (&o)[4]) {
+  const uint32_t h = w >> 8;
+  o[0] = hfma2_bits(w & 0x000f000fu, s24, b);
+  o[1] = hfma2_bits(w & 0x00f000f0u, s20, b);
+  o[2] = hfma2_bits(h & 0x000f000fu, s24, b);
+  o[3] = hfma2_bits(h & 0x00f000f0u, s20, b);
+}
+
+// Activations under a power of two: the largest |bf16| of eight as its 15 bits, the exponent that
+// takes a row's largest to [2^14, 2^15) (zero rows and the smallest numbers: 2^-126), and eight
+// inputs as fp16 pairs (0, 4), (1, 5), (2, 6), (3, 7), the order of dequant_word.
+__device__ __forceinline__ uint32_t max_abs_bits(uint4 u) {
+  const uint32_t a = __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);
+  const uint32_t b = __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu);
+  const uint32_t c = __vmaxu2(a, b);
+  return max(c & 0xffffu, c >> 16);
+}
+__device__ __forceinline__ int row_exponent(uint32_t max_bits) {
+  return max(min(max(static_cast<int>(max_bits >> 7), 1), 254) - 127 - 14, -126);
+}
+__device__ __forceinline__ uint4 permute_f16(uint4 u) {
+  return make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
+                    __byte_perm(u.y, u.w, 0x7632));
+}
+__device__ __forceinline__ uint4 permute_bf16(uint4 u, float f) {
+  auto lo = [f](uint32_t w) { return __uint_as_float(w << 16) * f; };
+  auto hi = [f](uint32_t w) { return __uint_as_float(w & 0xffff0000u) * f; };
+  return make_uint4(pack_half2(lo(u.x), lo(u.z)), pack_half2(hi(u.x), hi(u.z)), pack_half2(lo(u.y), lo(u.w)),
+                    pack_half2(hi(u.y), hi(u.w)));
+}
+
+// The work item of blockIdx.y: rows [lo, hi) of one expert, at most TOK of them.  Returns
+// the expert, or -1 past the last item.  Every thread of the CTA calls it.
+template <int TOK>
+__device__ __forceinline__ int find_item(const LinearParams& p, int item, int& lo, int& hi) {
+  if (p.offsets == nullptr) {
+    lo = item * TOK;
+    hi = min(lo + TOK, p.rows);
+    return lo < hi ? 0 : -1;
+  }
+  // each warp scans the experts, 32 at a time
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int e0 = 0; e0 < p.experts; e0 += 32) {
+    int a = 0, b = 0;
+    if (e0 + lane < p.experts) expert_range(p, e0 + lane, a, b);
+    const int n = (b - a + TOK - 1) / TOK;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    if (item < base + total) {
+      const bool mine = item >= base + incl - n && item < base + incl;
+      const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+      const int first = a + (item - (base + incl - n)) * TOK;
+      lo = __shfl_sync(0xffffffffu, first, src);
+      hi = min(__shfl_sync(0xffffffffu, b, src), lo + TOK);
+      return e0 + src;
+    }
+    base += total;
+  }
+  return -1;
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
