@@ -246,6 +246,12 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ float2 ld_dsmem_f32x2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 // Final softmax normalisation of one query row from its running max m and sum l (log2
 // units), with an optional attention sink s2 (log2 units): returns the factor that turns
 // the unnormalised output O into O * w / den, i.e. w / den, so that

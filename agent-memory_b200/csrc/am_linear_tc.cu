@@ -69,6 +69,9 @@ struct TilesLayout {
   static constexpr int CS = NT == 128 ? 3 : 2;              // code stages (256 rows x 256 inputs)
   static constexpr int XS = NT == 128 ? 6 : (NT == 64 ? 5 : 8);  // activation slabs (NT x 64 inputs)
   static constexpr int AB = (TMEM_COLS - 2 * NT) / 64;      // TMEM operand buffers (2 tiles x 32 columns)
+  static constexpr int DG = NT == 128 ? 2 : 1;              // groups of 8 dequantization warps, slabs in turn
+  static constexpr int DW = 8 * DG;
+  static constexpr int THREADS = 32 * (DW + 3);             // + codes, activations, MMA
   static constexpr int CSTAGE = 2 * 128 * 128;
   static constexpr int XSLAB = NT * 128;
   static constexpr int OFF_C = 0;
@@ -78,14 +81,13 @@ struct TilesLayout {
   static constexpr int OFF_BAR = OFF_END > RED ? OFF_END : RED;
   static constexpr int B_CFULL = 0, B_CEMPTY = CS, B_XFULL = 2 * CS, B_XEMPTY = B_XFULL + XS;
   static constexpr int B_AFULL = B_XEMPTY + XS, B_AEMPTY = B_AFULL + AB, B_DFULL = B_AEMPTY + AB;
-  static constexpr int B_DRAIN = B_DFULL + 1, B_COUNT = B_DRAIN + 1;
-  static constexpr int SMEM = OFF_BAR + B_COUNT * 8 + 16;
+  static constexpr int B_DRAIN = B_DFULL + 1, B_SCALE = B_DRAIN + 1, B_COUNT = B_SCALE + 1;
+  static constexpr int OFF_SCALE = OFF_BAR + B_COUNT * 8 + 16;
+  static constexpr int SMEM = OFF_SCALE + NT * 4;
   static constexpr int A_COL = 2 * NT;  // D[tile] at tile * NT, A[buffer][tile] at A_COL + 64 b + 32 tile
-  static_assert(AB >= 2, "the operand needs two buffers");
+  static_assert(AB >= 2 && (DG == 1 || AB % DG == 0), "the operand needs two buffers");
   static_assert(SMEM * CTAS <= 232448 - 1024 * (CTAS - 1), "shared memory of a SM");
 };
-
-constexpr int kTilesThreads = 352;  // 8 dequantization warps, codes, activations, MMA
 
 // gather4 load of four rows of a map with one-row boxes of 128 bytes.
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, int r0, int r1, int r2,
@@ -103,17 +105,19 @@ struct TilesParams {
 };
 
 template <int NT, bool GATED>
-__global__ void __launch_bounds__(kTilesThreads, TilesLayout<NT>::CTAS)
+__global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTAS)
     linear_tiles_kernel(const __grid_constant__ TilesParams f) {
   using LY = TilesLayout<NT>;
   constexpr int CS = LY::CS, XS = LY::XS, AB = LY::AB;
-  constexpr int CODES_WARP = 8, X_WARP = 9, MMA_WARP = 10;
+  constexpr int DW = LY::DW, DG = LY::DG;
+  constexpr int CODES_WARP = DW, X_WARP = DW + 1, MMA_WARP = DW + 2;
   const LinearParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t s_base = smem_u32(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + LY::OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + LY::OFF_BAR + LY::B_COUNT * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + LY::OFF_BAR + LY::B_COUNT * 8 + 4);
+  float* tok_scale = reinterpret_cast<float*>(smem + LY::OFF_SCALE);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -135,8 +139,9 @@ __global__ void __launch_bounds__(kTilesThreads, TilesLayout<NT>::CTAS)
 
   if (tid == 0) {
     for (int i = 0; i < LY::B_COUNT; ++i) {
-      const bool by_warps = (i >= LY::B_CEMPTY && i < LY::B_CEMPTY + CS) || (i >= LY::B_AFULL && i < LY::B_AFULL + AB);
-      mbar_init(bar(i), by_warps ? 8 : 1);
+      const bool c_empty = i >= LY::B_CEMPTY && i < LY::B_CEMPTY + CS;
+      const bool a_full = i >= LY::B_AFULL && i < LY::B_AFULL + AB;
+      mbar_init(bar(i), c_empty ? DW : (a_full ? 8 : 1));
     }
     fence_mbar_init();
     *abort_flag = 0;
@@ -182,7 +187,21 @@ __global__ void __launch_bounds__(kTilesThreads, TilesLayout<NT>::CTAS)
     }
     griddep_wait();  // the activations are written
     bool ok = true;
+    auto scales = [&]() {  // the tokens' powers of two, for the epilogue
+      for (int j = lane; j < NT; j += 32) {
+        const int r = lo + j;
+        float v = 0.0f;
+        if (r < hi) {
+          const int src = p.order != nullptr ? p.order[r] / p.top_k : r;
+          if (src >= 0 && src < p.x_rows) v = p.xscale[src];
+        }
+        tok_scale[j] = v;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(LY::B_SCALE));
+    };
     for (int i = 0; i < slabs; ++i) {
+      if (i == min(XS, slabs) - 1) scales();  // behind the first loads
       const int s = i % XS;
       if (i >= XS) ok = wait_or_abort(bar(LY::B_XEMPTY + s), ((i - XS) / XS) & 1, p.wait_ns, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
@@ -227,14 +246,26 @@ __global__ void __launch_bounds__(kTilesThreads, TilesLayout<NT>::CTAS)
       if (!ok) *abort_flag = 1;
     }
   } else {
-    // ---- dequantization: weight row `wrow` of tile t, one 64-input slab at a time
-    const int t = warp >> 2, quarter = warp & 3;
+    // ---- dequantization: one weight row of tile t a thread, 64 inputs (a slab) at a time; with two
+    // groups of warps each takes every other slab.  A slab's store into TMEM completes while
+    // the next one is dequantized, and only then is it handed to the MMA thread.
+    const int group = warp >> 3, t = (warp >> 2) & 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const int n = min(n0 + (GATED ? 0 : t * 128) + r, p.n_out - 1);
     const uint32_t* prow = p.params[GATED ? t : 0] + ((int64_t)e * p.n_out + n) * p.pstride;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t a_base = tmem + LY::A_COL + t * 32 + lane_base;
     uint4 pv = __ldg(reinterpret_cast<const uint4*>(prow) + q0);
     bool ok = true;
+    int stored = -1;  // buffer of the store in flight
+    auto publish = [&]() {
+      if (stored >= 0) {
+        tc::tmem_wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(LY::B_AFULL + stored));
+      }
+    };
     for (int c = 0; c < q1 - q0 && ok; ++c) {
       const int cs = c % CS;
       const uint4 pnext = c + 1 < q1 - q0 ? __ldg(reinterpret_cast<const uint4*>(prow) + q0 + c + 1) : pv;
@@ -244,12 +275,14 @@ __global__ void __launch_bounds__(kTilesThreads, TilesLayout<NT>::CTAS)
       const uint32_t pw[4] = {pv.x, pv.y, pv.z, pv.w};
       const int in_stage = min(4, slabs - 4 * c);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
+      for (int s4 = 0; s4 < 4; s4 += DG) {
+        const int s = s4 + group;
         if (s >= in_stage) break;
         const int i = 4 * c + s, b = i % AB;
         const uint4 w0 = *reinterpret_cast<const uint4*>(crow + (((2 * s) ^ (r & 7)) << 4));
         const uint4 w1 = *reinterpret_cast<const uint4*>(crow + (((2 * s + 1) ^ (r & 7)) << 4));
-        const uint32_t s24 = __byte_perm(pw[s], pw[s], 0x1010), bb = __byte_perm(pw[s], pw[s], 0x3232);
+        const uint32_t ps = DG == 1 ? pw[s4] : (group == 0 ? pw[s4] : pw[(s4 + 1) & 3]);
+        const uint32_t s24 = __byte_perm(ps, ps, 0x1010), bb = __byte_perm(ps, ps, 0x3232);
         const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);
         const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
         uint32_t o[32];
@@ -260,92 +293,133 @@ __global__ void __launch_bounds__(kTilesThreads, TilesLayout<NT>::CTAS)
 #pragma unroll
           for (int k = 0; k < 4; ++k) o[4 * j + k] = d[k];
         }
-        if (s + 1 == in_stage) {  // the stage's codes are in registers
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(LY::B_CEMPTY + cs));
-        }
+        publish();
         if (i >= AB) {
           ok = __all_sync(0xffffffffu,
                           wait_or_abort(bar(LY::B_AEMPTY + b), ((i - AB) / AB) & 1, p.wait_ns, abort_flag));
           if (!ok) break;
           tc::fence_after();
         }
-        tc::tmem_st32(tmem + LY::A_COL + b * 64 + t * 32 + lane_base, o);
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(LY::B_AFULL + b));
+        tc::tmem_st32_nowait(a_base + b * 64, o);
+        stored = b;
       }
+      __syncwarp();  // the stage's codes are in registers
+      if (lane == 0) mbar_arrive(bar(LY::B_CEMPTY + cs));
       pv = pnext;
     }
-    if (ok) ok = __all_sync(0xffffffffu, wait_or_abort(bar(LY::B_DFULL), 0, p.wait_ns, abort_flag));
-    if (!ok) {
-      *abort_flag = 1;
-    } else {
-      tc::fence_after();
-      griddep_wait();  // the tokens' powers of two are read below
-      if (f.ck == 1) {
-        // ---- output: lane = weight row, columns = tokens
-        const int half = warp >> 2;
-        const int row = n0 + (GATED ? 0 : half * 128) + r;
-        const int64_t wr = (int64_t)e * p.n_out + min(row, p.n_out - 1);
-        const float rs0 = p.row_scale[0][wr], rs1 = GATED ? p.row_scale[1][wr] : 0.0f;
-        constexpr int COLS = GATED ? NT / 2 : NT;  // gated: the two warps of a lane quarter share the tokens
-        const int col0 = GATED ? half * COLS : 0;
+    if (ok) {
+      publish();
+      ok = __all_sync(0xffffffffu, wait_or_abort(bar(LY::B_DFULL), 0, p.wait_ns, abort_flag) &&
+                                       wait_or_abort(bar(LY::B_SCALE), 0, p.wait_ns, abort_flag));
+    }
+    if (!ok) *abort_flag = 1;
+    // the output warps meet here also after an abort (each may have seen it at another step)
+    tc::fence_after();
+    if (f.ck == 1) {
+      // ---- output: lane = weight row, columns = tokens; rounded values to shared memory as
+      // [token][row], then whole rows of them to global memory
+      constexpr int PARTS = GATED ? DW / 4 : DW / 8;  // warps that share a lane quarter (and tile)
+      constexpr int COLS = NT / PARTS;
+      const int part = GATED ? warp >> 2 : group;
+      const int row = n0 + (GATED ? 0 : t * 128) + r;
+      const int64_t wr = (int64_t)e * p.n_out + min(row, p.n_out - 1);
+      const float rs0 = p.row_scale[0][wr], rs1 = GATED ? p.row_scale[1][wr] : 0.0f;
+      uint16_t* so = reinterpret_cast<uint16_t*>(smem);
+      if (ok) {
 #pragma unroll 1
-        for (int cb = 0; cb < COLS; cb += 16) {
-          if (lo + col0 + cb >= hi) break;
+        for (int cb = part * COLS; cb < (part + 1) * COLS; cb += 16) {
+          if (lo + cb >= hi) break;
           float g[16], u[16];
-          tc::tmem_ld16(tmem + (GATED ? 0 : half * NT) + col0 + cb + lane_base, g);
-          if constexpr (GATED) tc::tmem_ld16(tmem + NT + col0 + cb + lane_base, u);
+          tc::tmem_ld16(tmem + (GATED ? 0 : t * NT) + cb + lane_base, g);
+          if constexpr (GATED) tc::tmem_ld16(tmem + NT + cb + lane_base, u);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const int out_row = lo + col0 + cb + j;
-            if (out_row < hi && row < p.n_out) {
-              const int src = p.order != nullptr ? min(max(p.order[out_row] / p.top_k, 0), p.x_rows - 1) : out_row;
-              const float ts = p.xscale[src];
-              const float y = GATED ? silu_mul(g[j] * (rs0 * ts), u[j] * (rs1 * ts)) : g[j] * (rs0 * ts);
-              p.out[(int64_t)out_row * p.out_stride + row] = p.bf16 ? f2h<true>(y) : f2h<false>(y);
-            }
+            const float ts = tok_scale[cb + j];
+            const float y = GATED ? silu_mul(g[j] * (rs0 * ts), u[j] * (rs1 * ts)) : g[j] * (rs0 * ts);
+            so[(cb + j) * CTA_ROWS + (GATED ? 0 : t * 128) + r] = p.bf16 ? f2h<true>(y) : f2h<false>(y);
           }
         }
-      } else {
-        // ---- fp32 sums to shared memory, [tile][token][128 rows]
-        float* red = reinterpret_cast<float*>(smem) + t * NT * 128 + r;
-#pragma unroll 1
-        for (int cb = 0; cb < NT; cb += 16) {
-          float v[16];
-          tc::tmem_ld16(tmem + t * NT + cb + lane_base, v);
+      }
+      asm volatile("bar.sync 1, %0;\n" ::"n"(DW * 32) : "memory");
+      if (!*abort_flag) {
+        const int m = hi - lo;
+        const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+        constexpr int VPR = CTA_ROWS / 8;  // 16-byte vectors of a token
+        for (int v = tid; v < m * VPR; v += DW * 32) {
+          const int tok = v / VPR, col = (v % VPR) * 8;
+          const int left = p.n_out - (n0 + col);
+          if (left <= 0) continue;
+          const uint4 d = *reinterpret_cast<const uint4*>(so + tok * CTA_ROWS + col);
+          uint16_t* dst = p.out + (int64_t)(lo + tok) * p.out_stride + n0 + col;
+          if (wide && left >= 8) {
+            *reinterpret_cast<uint4*>(dst) = d;
+          } else {
+            const uint32_t w[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-          for (int j = 0; j < 16; ++j) red[(cb + j) * 128] = v[j];
+            for (int j = 0; j < 8; ++j)
+              if (j < left) dst[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+          }
         }
+      }
+    } else if (ok) {
+      // ---- fp32 sums to shared memory, [tile][token][128 rows]
+      constexpr int COLS = NT / DG;
+      float* red = reinterpret_cast<float*>(smem) + t * NT * 128 + r;
+#pragma unroll 1
+      for (int cb = group * COLS; cb < (group + 1) * COLS; cb += 16) {
+        float v[16];
+        tc::tmem_ld16(tmem + t * NT + cb + lane_base, v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) red[(cb + j) * 128] = v[j];
       }
     }
   }
   __syncwarp();
   if (f.ck > 1) {
-    griddep_wait();
+    // the ranks' sums of a token and row, added in rank order; a rank finishes its share of the
+    // tokens, two rows a thread
     cluster_sync_all();
     if (!*abort_flag) {
       const int m = hi - lo;
-      const uint32_t base = s_base;
-      for (int o = tid; o < CTA_ROWS * m; o += kTilesThreads) {
-        const int tok = o / CTA_ROWS, rr = o % CTA_ROWS;
-        if (tok % f.ck != rank) continue;
+      const int t0 = m * rank / f.ck, t1 = m * (rank + 1) / f.ck;
+      constexpr int PAIRS = CTA_ROWS / 2;
+      const bool wide = (p.out_stride & 1) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0;
+      for (int o = tid; o < PAIRS * (t1 - t0); o += LY::THREADS) {
+        const int tok = t0 + o / PAIRS, rr = (o % PAIRS) * 2;
         const int row = n0 + rr;
         if (row >= p.n_out) continue;
-        const uint32_t at = base + (((GATED ? 0 : rr >> 7) * NT + tok) * 128 + (rr & 127)) * 4;
-        float s0 = 0.0f, s1 = 0.0f;
-        for (int c = 0; c < f.ck; ++c) {
-          s0 += ld_dsmem_f32(dsmem_addr(at, c));
-          if constexpr (GATED) s1 += ld_dsmem_f32(dsmem_addr(at + NT * 128 * 4, c));
+        const uint32_t at = s_base + (((GATED ? 0 : rr >> 7) * NT + tok) * 128 + (rr & 127)) * 4;
+        float2 a[8], b[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          a[c] = c < f.ck ? ld_dsmem_f32x2(dsmem_addr(at, c)) : make_float2(0.0f, 0.0f);
+          if constexpr (GATED) b[c] = c < f.ck ? ld_dsmem_f32x2(dsmem_addr(at + NT * 128 * 4, c)) : make_float2(0.0f, 0.0f);
         }
-        const int out_row = lo + tok;
-        const int src = p.order != nullptr ? min(max(p.order[out_row] / p.top_k, 0), p.x_rows - 1) : out_row;
-        const float ts = p.xscale[src];
+#pragma unroll
+        for (int c = 1; c < 8; ++c) {
+          a[0].x += a[c].x;
+          a[0].y += a[c].y;
+          if constexpr (GATED) {
+            b[0].x += b[c].x;
+            b[0].y += b[c].y;
+          }
+        }
+        const float ts = tok_scale[tok];
         const int64_t wr = (int64_t)e * p.n_out + row;
-        const float y = GATED ? silu_mul(s0 * (p.row_scale[0][wr] * ts), s1 * (p.row_scale[1][wr] * ts))
-                              : s0 * (p.row_scale[0][wr] * ts);
-        p.out[(int64_t)out_row * p.out_stride + row] = p.bf16 ? f2h<true>(y) : f2h<false>(y);
+        const bool two = row + 1 < p.n_out;
+        float y0 = a[0].x * (p.row_scale[0][wr] * ts), y1 = two ? a[0].y * (p.row_scale[0][wr + 1] * ts) : 0.0f;
+        if constexpr (GATED) {
+          y0 = silu_mul(y0, b[0].x * (p.row_scale[1][wr] * ts));
+          if (two) y1 = silu_mul(y1, b[0].y * (p.row_scale[1][wr + 1] * ts));
+        }
+        const uint32_t h0 = p.bf16 ? f2h<true>(y0) : f2h<false>(y0), h1 = p.bf16 ? f2h<true>(y1) : f2h<false>(y1);
+        uint16_t* dst = p.out + (int64_t)(lo + tok) * p.out_stride + row;
+        if (wide && two) {
+          *reinterpret_cast<uint32_t*>(dst) = h0 | (h1 << 16);
+        } else {
+          dst[0] = static_cast<uint16_t>(h0);
+          if (two) dst[1] = static_cast<uint16_t>(h1);
+        }
       }
     }
     cluster_sync_all();
@@ -405,7 +479,7 @@ static cudaError_t launch_tiles_t(const LinearParams& p, int64_t items, cudaStre
   while (f.ck < 8 && (int64_t)row_tiles * items * f.ck * 2 <= (int64_t)sms * LY::CTAS && f.ck * 4 <= quads) f.ck *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(row_tiles * f.ck, static_cast<unsigned>(items));
-  cfg.blockDim = dim3(kTilesThreads);
+  cfg.blockDim = dim3(LY::THREADS);
   cfg.dynamicSmemBytes = LY::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
