@@ -117,8 +117,22 @@ __device__ __forceinline__ uint4 permute_bf16(uint4 u, float f) {
                     pack_half2(hi(u.y), hi(u.w)));
 }
 
-// The work item of blockIdx.y: rows [lo, hi) of one expert, at most TOK of them.  Returns
-// the expert, or -1 past the last item.  Every thread of the CTA calls it.
+// Work items of a call: pieces of at most TOK rows of one expert.  The warp's lanes agree.
+template <int TOK>
+__device__ __forceinline__ int count_items(const LinearParams& p) {
+  if (p.offsets == nullptr) return (p.rows + TOK - 1) / TOK;
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+  for (int e = lane; e < p.experts; e += 32) {
+    int a, b;
+    expert_range(p, e, a, b);
+    n += (b - a + TOK - 1) / TOK;
+  }
+  return __reduce_add_sync(0xffffffffu, n);
+}
+
+// Item `item`: rows [lo, hi) of one expert.  Returns the expert, or -1 past the last item.  All
+// lanes of a warp call it.
 template <int TOK>
 __device__ __forceinline__ int find_item(const LinearParams& p, int item, int& lo, int& hi) {
   if (p.offsets == nullptr) {

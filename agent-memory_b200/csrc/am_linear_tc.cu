@@ -15,9 +15,10 @@
 //    * warps 0-7 dequantize: a thread owns a weight row; 64 codes a step become 32 registers of
 //      fp16 pairs (9 operations for 8 weights, see am_linear.cu) and go to TMEM with one
 //      tcgen05.st -- no shared-memory round trip, and the MMA reads its A operand there;
-//    * one thread issues tcgen05.mma (kind::f16, M = 128, N = NT, K = 16) over both tiles.
+//    * two threads, one a weight tile, issue tcgen05.mma (kind::f16, M = 128, N = NT, K = 16).
 //    The accumulators are read back by the dequantization warps, scaled by the row's and the
-//    token's powers of two, gated, rounded once and stored.
+//    token's powers of two, gated, rounded once and stored.  A CTA walks the tiles with stride
+//    gridDim.x; the loads of its next tile run during the output of the last one.
 //    With few tiles the inputs are split over the CTAs of a cluster, whose fp32 sums meet in
 //    distributed shared memory, in rank order.
 // Every wait is bounded (LinearParams::wait_ns); on timeout the kernel flags AM_STATUS_TIMEOUT,
@@ -26,6 +27,9 @@
 // The codes and parameters are read before griddepcontrol.wait: linear_rows_kernel starts only
 // when everything before it in the stream is complete (it is launched without programmatic
 // serialization), and it writes nothing but the activations.
+#include <algorithm>
+#include <climits>
+
 #include "am_internal.h"
 #include "am_linear.cuh"
 #include "am_tcgen05.cuh"
@@ -66,27 +70,40 @@ struct TilesLayout {
   // 128 tokens: one CTA a SM, 512 TMEM columns; fewer: two CTAs a SM of 256 columns each
   static constexpr int CTAS = NT == 128 ? 1 : 2;
   static constexpr uint32_t TMEM_COLS = 512 / CTAS;
-  static constexpr int CS = NT == 128 ? 3 : 2;              // code stages (256 rows x 256 inputs)
-  static constexpr int XS = NT == 128 ? 6 : (NT == 64 ? 5 : 8);  // activation slabs (NT x 64 inputs)
-  static constexpr int AB = (TMEM_COLS - 2 * NT) / 64;      // TMEM operand buffers (2 tiles x 32 columns)
-  static constexpr int DG = NT == 128 ? 2 : 1;              // groups of 8 dequantization warps, slabs in turn
-  static constexpr int DW = 8 * DG;
-  static constexpr int THREADS = 32 * (DW + 3);             // + codes, activations, MMA
+  static constexpr int SP = NT == 128 ? 2 : 1;             // slabs (64 inputs) of a pipeline step
+  static constexpr int CS = NT == 128 ? 3 : 2;             // code stages (256 rows x 256 inputs)
+  static constexpr int XS = NT == 128 ? 3 : (NT == 64 ? 5 : 8);  // activation steps (NT x 64 SP inputs)
+  static constexpr int AB = (TMEM_COLS - 2 * NT) / (64 * SP);    // TMEM operand buffers (2 tiles x 32 SP columns)
+  static constexpr int DW = 8 * SP;                        // dequantization warps: 8 a slab of the step
+  static constexpr int THREADS = 32 * (DW + 4);            // + codes, activations, two MMA warps
   static constexpr int CSTAGE = 2 * 128 * 128;
   static constexpr int XSLAB = NT * 128;
   static constexpr int OFF_C = 0;
   static constexpr int OFF_X = OFF_C + CS * CSTAGE;
-  static constexpr int OFF_END = OFF_X + XS * XSLAB;
-  static constexpr int RED = 2 * NT * 128 * 4;              // fp32 sums of a split (over the rings)
-  static constexpr int OFF_BAR = OFF_END > RED ? OFF_END : RED;
+  static constexpr int OFF_END = OFF_X + XS * SP * XSLAB;
+  static constexpr int RED = 2 * NT * 128 * 4;             // fp32 sums of a split (over the rings)
+  static constexpr int OFF_OUT = OFF_END > RED ? OFF_END : RED;  // 1 KB a dequantization warp
+  static constexpr int OFF_SCALE = OFF_OUT + DW * 1024;    // two tiles' token scales
+  static constexpr int OFF_BAR = OFF_SCALE + 2 * NT * 4;
   static constexpr int B_CFULL = 0, B_CEMPTY = CS, B_XFULL = 2 * CS, B_XEMPTY = B_XFULL + XS;
   static constexpr int B_AFULL = B_XEMPTY + XS, B_AEMPTY = B_AFULL + AB, B_DFULL = B_AEMPTY + AB;
-  static constexpr int B_DRAIN = B_DFULL + 1, B_SCALE = B_DRAIN + 1, B_COUNT = B_SCALE + 1;
-  static constexpr int OFF_SCALE = OFF_BAR + B_COUNT * 8 + 16;
-  static constexpr int SMEM = OFF_SCALE + NT * 4;
-  static constexpr int A_COL = 2 * NT;  // D[tile] at tile * NT, A[buffer][tile] at A_COL + 64 b + 32 tile
-  static_assert(AB >= 2 && (DG == 1 || AB % DG == 0), "the operand needs two buffers");
-  static_assert(SMEM * CTAS <= 232448 - 1024 * (CTAS - 1), "shared memory of a SM");
+  static constexpr int B_DEMPTY = B_DFULL + 1, B_SFULL = B_DEMPTY + 1, B_SEMPTY = B_SFULL + 2;
+  static constexpr int B_DRAIN = B_SEMPTY + 2, B_COUNT = B_DRAIN + 2;
+  static constexpr int SMEM = OFF_BAR + B_COUNT * 8 + 16;
+  static constexpr int A_COL = 2 * NT;  // D[tile] at tile * NT, A[buffer][tile] at A_COL + 32 SP (2 b + tile)
+  static_assert(AB >= 2, "the operand needs two buffers");
+  static_assert((SMEM + 1024) * CTAS <= 233472 && SMEM <= 232448, "shared memory of a SM");
+  // Arrivals that complete a phase of barrier i.
+  static __device__ int arrivals(int i) {
+    if (i >= B_CEMPTY && i < B_CEMPTY + CS) return DW;
+    if (i >= B_XEMPTY && i < B_XEMPTY + XS) return 2;
+    if (i >= B_AFULL && i < B_AFULL + AB) return DW;
+    if (i >= B_AEMPTY && i < B_AEMPTY + AB) return 2;
+    if (i == B_DFULL) return 2;
+    if (i == B_DEMPTY) return DW;
+    if (i >= B_SEMPTY && i < B_SEMPTY + 2) return DW;
+    return 1;
+  }
 };
 
 // gather4 load of four rows of a map with one-row boxes of 128 bytes.
@@ -99,18 +116,32 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// Position in a ring of N buffers and the parity of its current round.
+template <int N>
+struct Ring {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      ph ^= 1u;
+    }
+  }
+};
+
 struct TilesParams {
   LinearParams p;
-  int32_t ck;  // CTAs of a cluster that split the inputs
+  int32_t ck;         // CTAs of a cluster that split the inputs (then a CTA has one tile)
+  int32_t row_tiles;  // tiles of CTA_ROWS weight rows
 };
 
 template <int NT, bool GATED>
 __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTAS)
     linear_tiles_kernel(const __grid_constant__ TilesParams f) {
   using LY = TilesLayout<NT>;
-  constexpr int CS = LY::CS, XS = LY::XS, AB = LY::AB;
-  constexpr int DW = LY::DW, DG = LY::DG;
+  constexpr int CS = LY::CS, XS = LY::XS, AB = LY::AB, SP = LY::SP, DW = LY::DW;
   constexpr int CODES_WARP = DW, X_WARP = DW + 1, MMA_WARP = DW + 2;
+  constexpr int STEPS = 4 / SP;  // steps of a code stage
   const LinearParams& p = f.p;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t s_base = smem_u32(smem);
@@ -119,144 +150,156 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + LY::OFF_BAR + LY::B_COUNT * 8 + 4);
   float* tok_scale = reinterpret_cast<float*>(smem + LY::OFF_SCALE);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  auto wait = [&](int i, uint32_t parity) { return wait_or_abort(bar(i), parity, p.wait_ns, abort_flag); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  griddep_launch_dependents();
   if (s_base & 1023u) {  // swizzled tiles need a 1024-byte aligned window (the whole grid returns)
     if (tid == 0) flag_status(p.status, AM_STATUS_BAD_POSITION);
     return;
   }
-  int lo, hi;
-  const int e = find_item<NT>(p, blockIdx.y, lo, hi);
-  if (e < 0) return;  // the whole cluster: it shares blockIdx.y
   const int rank = f.ck > 1 ? static_cast<int>(blockIdx.x) % f.ck : 0;
-  const int tile = static_cast<int>(blockIdx.x) / f.ck;
+  const int first = static_cast<int>(blockIdx.x) / f.ck, step = static_cast<int>(gridDim.x) / f.ck;
+  const int tiles = count_items<NT>(p) * f.row_tiles;
+  if (first >= tiles) return;  // the whole cluster
   constexpr int CTA_ROWS = GATED ? 128 : 256;
-  const int n0 = tile * CTA_ROWS;
-  // this CTA's inputs: quads of groups [q0, q1), slabs of 64 inputs
+  // this CTA's inputs: quads of groups [q0, q1), slabs of 64 inputs, steps of SP slabs
   const int quads = p.pstride >> 2;
   const int q0 = quads * rank / f.ck, q1 = quads * (rank + 1) / f.ck;
   const int slabs = min(q1 * 4, p.groups) - q0 * 4;
+  const int steps = (slabs + SP - 1) / SP;
 
-  if (tid == 0) {
-    for (int i = 0; i < LY::B_COUNT; ++i) {
-      const bool c_empty = i >= LY::B_CEMPTY && i < LY::B_CEMPTY + CS;
-      const bool a_full = i >= LY::B_AFULL && i < LY::B_AFULL + AB;
-      mbar_init(bar(i), c_empty ? DW : (a_full ? 8 : 1));
-    }
-    fence_mbar_init();
-    *abort_flag = 0;
-  }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)),
                  "r"(LY::TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
+  } else if (warp == CODES_WARP) {
+    for (int i = lane; i < LY::B_COUNT; i += 32) mbar_init(bar(i), LY::arrivals(i));
+    if (lane == 0) *abort_flag = 0;
+    fence_mbar_init();
   }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  int issued_c = 0, issued_x = 0;  // loads in flight (their own threads' counts)
+  int issued_c = 0, issued_x = 0;  // loads issued (their own threads' counts)
   bool mma_issued = false;
+  bool ok = true;
   if (warp == CODES_WARP) {
-    if (lane == 0) {
-      const int y = e * p.n_out + n0;
-      bool ok = true;
-      for (int c = 0; c < q1 - q0; ++c) {
-        const int s = c % CS;
-        if (c >= CS) ok = wait_or_abort(bar(LY::B_CEMPTY + s), ((c - CS) / CS) & 1, p.wait_ns, abort_flag);
-        if (!ok) break;
-        mbar_arrive_expect_tx(bar(LY::B_CFULL + s), LY::CSTAGE);
-        const uint32_t dst = s_base + LY::OFF_C + s * LY::CSTAGE;
-        tma_load_2d(dst, &p.tmap_w[0], (q0 + c) * 128, y, bar(LY::B_CFULL + s));
-        tma_load_2d(dst + LY::CSTAGE / 2, &p.tmap_w[GATED ? 1 : 0], (q0 + c) * 128, GATED ? y : y + 128,
-                    bar(LY::B_CFULL + s));
-        issued_c = c + 1;
+    Ring<CS> ring;
+    for (int tile = first; tile < tiles; tile += step) {
+      int lo, hi;
+      const int e = find_item<NT>(p, tile / f.row_tiles, lo, hi);
+      const int y = e * p.n_out + tile % f.row_tiles * CTA_ROWS;
+      if (lane == 0) {
+        for (int c = q0; c < q1; ++c) {
+          ok = wait(LY::B_CEMPTY + ring.s, ring.ph ^ 1u);
+          if (!ok) break;
+          const uint32_t full = bar(LY::B_CFULL + ring.s), dst = s_base + LY::OFF_C + ring.s * LY::CSTAGE;
+          mbar_arrive_expect_tx(full, LY::CSTAGE);
+          tma_load_2d(dst, &p.tmap_w[0], c * 128, y, full);
+          tma_load_2d(dst + LY::CSTAGE / 2, &p.tmap_w[GATED ? 1 : 0], c * 128, GATED ? y : y + 128, full);
+          ++issued_c;
+          ring.next();
+        }
       }
-      if (!ok) *abort_flag = 1;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
     }
   } else if (warp == X_WARP) {
-    int rows4[4] = {};
-    if (p.order != nullptr) {
+    griddep_wait();  // the activations are written
+    Ring<XS> ring;
+    int k = 0;
+    for (int tile = first; tile < tiles && ok; tile += step, ++k) {
+      int lo, hi;
+      find_item<NT>(p, tile / f.row_tiles, lo, hi);
+      // lane i: rows 4 i .. 4 i + 3 of the item
+      int rows4[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = lo + 4 * lane + j;
         const int src = 4 * lane < NT && r < hi ? source_row(p, r) : -1;
         rows4[j] = src >= 0 ? src : p.x_rows;  // past the map: zeros
       }
-    }
-    griddep_wait();  // the activations are written
-    bool ok = true;
-    auto scales = [&]() {  // the tokens' powers of two, for the epilogue
-      for (int j = lane; j < NT; j += 32) {
-        const int r = lo + j;
-        float v = 0.0f;
-        if (r < hi) {
-          const int src = p.order != nullptr ? p.order[r] / p.top_k : r;
-          if (src >= 0 && src < p.x_rows) v = p.xscale[src];
+      for (int i = 0; i < steps; ++i) {
+        ok = __all_sync(0xffffffffu, wait(LY::B_XEMPTY + ring.s, ring.ph ^ 1u));
+        if (!ok) break;
+        const uint32_t full = bar(LY::B_XFULL + ring.s), dst = s_base + LY::OFF_X + ring.s * SP * LY::XSLAB;
+        const int n = min(SP, slabs - i * SP);
+        if (lane == 0) mbar_arrive_expect_tx(full, n * LY::XSLAB);
+        __syncwarp();
+        for (int s = 0; s < n; ++s) {
+          const int x = (q0 * 4 + i * SP + s) * 128;
+          if (p.order != nullptr) {
+            if (4 * lane < NT)
+              tma_gather4(dst + s * LY::XSLAB + lane * 512, &p.tmap_x, x, rows4[0], rows4[1], rows4[2], rows4[3], full);
+          } else if (lane == 0) {
+            tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, x, lo, full);
+          }
         }
-        tok_scale[j] = v;
+        ++issued_x;
+        ring.next();
+        if (i == min(XS, steps) - 1) {  // behind the first loads: the tokens' powers of two
+          const int b = k & 1;
+          ok = __all_sync(0xffffffffu, wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1));
+          if (!ok) break;
+          if (4 * lane < NT) {
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = rows4[j] < p.x_rows ? p.xscale[rows4[j]] : 0.0f;
+            *reinterpret_cast<float4*>(tok_scale + b * NT + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(LY::B_SFULL + b));
+        }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(LY::B_SCALE));
-    };
-    for (int i = 0; i < slabs; ++i) {
-      if (i == min(XS, slabs) - 1) scales();  // behind the first loads
-      const int s = i % XS;
-      if (i >= XS) ok = wait_or_abort(bar(LY::B_XEMPTY + s), ((i - XS) / XS) & 1, p.wait_ns, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
-      const uint32_t dst = s_base + LY::OFF_X + s * LY::XSLAB;
-      if (lane == 0) mbar_arrive_expect_tx(bar(LY::B_XFULL + s), LY::XSLAB);
-      __syncwarp();
-      if (p.order != nullptr) {
-        if (4 * lane < NT)
-          tma_gather4(dst + lane * 512, &p.tmap_x, (q0 * 4 + i) * 128, rows4[0], rows4[1], rows4[2], rows4[3],
-                      bar(LY::B_XFULL + s));
-      } else if (lane == 0) {
-        tma_load_2d(dst, &p.tmap_x, (q0 * 4 + i) * 128, lo, bar(LY::B_XFULL + s));
-      }
-      issued_x = i + 1;
     }
-    if (!ok) *abort_flag = 1;
-  } else if (warp == MMA_WARP) {
+  } else if (warp >= MMA_WARP) {
+    // Two issuing threads, one a weight tile: the waits and commits of one hide behind the MMAs
+    // of the other (one thread for both left the tensor pipe idle half of the time).
     if (lane == 0) {
       constexpr uint32_t ID = tc::idesc(128, NT, false);
-      bool ok = true;
-      for (int i = 0; i < slabs && ok; ++i) {
-        const int b = i % AB, s = i % XS;
-        ok = wait_or_abort(bar(LY::B_XFULL + s), (i / XS) & 1, p.wait_ns, abort_flag) &&
-             wait_or_abort(bar(LY::B_AFULL + b), (i / AB) & 1, p.wait_ns, abort_flag);
-        if (!ok) break;
-        tc::fence_after();
-        const uint32_t xs = s_base + LY::OFF_X + s * LY::XSLAB;
+      const int t = warp - MMA_WARP;
+      const uint32_t d = tmem + t * NT;
+      Ring<XS> xr;
+      Ring<AB> ar;
+      uint32_t dph = 1;
+      for (int tile = first; tile < tiles && ok; tile += step, dph ^= 1u) {
+        ok = wait(LY::B_DEMPTY, dph);
+        for (int i = 0; i < steps && ok; ++i) {
+          ok = wait(LY::B_XFULL + xr.s, xr.ph) && wait(LY::B_AFULL + ar.s, ar.ph);
+          if (!ok) break;
+          tc::fence_after();
+          const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + xr.s * SP * LY::XSLAB, 16, 1024);
+          const uint32_t a = tmem + LY::A_COL + ar.s * 64 * SP + t * 32;
+          // (descriptor addresses count 16-byte units: 32 bytes of a swizzled row are 16 inputs)
+          tc::mma_ts(d, a, xd, ID, i > 0 ? 1u : 0u);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int ks = 1; ks < 4; ++ks) tc::mma_ts(d, a + ks * 8, xd + ks * 2, ID, 1u);
+          if (SP == 2 && 2 * i + 1 < slabs) {
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            tc::mma_ts(tmem + t * NT, tmem + LY::A_COL + b * 64 + t * 32 + ks * 8, tc::sdesc(xs + ks * 32, 16, 1024),
-                       ID, (i > 0 || ks > 0) ? 1u : 0u);
-        mma_issued = true;
-        tc::commit(bar(LY::B_XEMPTY + s));
-        tc::commit(bar(LY::B_AEMPTY + b));
+            for (int ks = 0; ks < 4; ++ks) tc::mma_ts(d, a + 64 + ks * 8, xd + LY::XSLAB / 16 + ks * 2, ID, 1u);
+          }
+          mma_issued = true;
+          tc::commit(bar(LY::B_XEMPTY + xr.s));
+          tc::commit(bar(LY::B_AEMPTY + ar.s));
+          xr.next();
+          ar.next();
+        }
+        if (ok) tc::commit(bar(LY::B_DFULL));
       }
-      if (ok) tc::commit(bar(LY::B_DFULL));
-      if (!ok) *abort_flag = 1;
     }
   } else {
-    // ---- dequantization: one weight row of tile t a thread, 64 inputs (a slab) at a time; with two
-    // groups of warps each takes every other slab.  A slab's store into TMEM completes while
-    // the next one is dequantized, and only then is it handed to the MMA thread.
+    // ---- dequantization: one weight row of tile t a thread, slab `group` of every step.  A slab's
+    // store into TMEM completes while the next one is dequantized, and only then is it handed
+    // to the MMA threads.
     const int group = warp >> 3, t = (warp >> 2) & 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    const int n = min(n0 + (GATED ? 0 : t * 128) + r, p.n_out - 1);
-    const uint32_t* prow = p.params[GATED ? t : 0] + ((int64_t)e * p.n_out + n) * p.pstride;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t a_base = tmem + LY::A_COL + t * 32 + lane_base;
-    uint4 pv = __ldg(reinterpret_cast<const uint4*>(prow) + q0);
-    bool ok = true;
+    const uint32_t a_base = tmem + LY::A_COL + group * 64 + t * 32 + lane_base;
+    Ring<CS> cr;
+    Ring<AB> ar;
     int stored = -1;  // buffer of the store in flight
     auto publish = [&]() {
       if (stored >= 0) {
@@ -266,120 +309,151 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
         if (lane == 0) mbar_arrive(bar(LY::B_AFULL + stored));
       }
     };
-    for (int c = 0; c < q1 - q0 && ok; ++c) {
-      const int cs = c % CS;
-      const uint4 pnext = c + 1 < q1 - q0 ? __ldg(reinterpret_cast<const uint4*>(prow) + q0 + c + 1) : pv;
-      ok = __all_sync(0xffffffffu, wait_or_abort(bar(LY::B_CFULL + cs), (c / CS) & 1, p.wait_ns, abort_flag));
-      if (!ok) break;
-      const uint8_t* crow = smem + LY::OFF_C + cs * LY::CSTAGE + t * (LY::CSTAGE / 2) + r * 128;
-      const uint32_t pw[4] = {pv.x, pv.y, pv.z, pv.w};
-      const int in_stage = min(4, slabs - 4 * c);
+    int k = 0;
+    for (int tile = first; tile < tiles && ok; tile += step, ++k) {
+      int lo, hi;
+      const int e = find_item<NT>(p, tile / f.row_tiles, lo, hi);
+      const int n0 = tile % f.row_tiles * CTA_ROWS;
+      const int64_t wrow = (int64_t)e * p.n_out + min(n0 + (GATED ? 0 : t * 128) + r, p.n_out - 1);
+      const uint4* prow = reinterpret_cast<const uint4*>(p.params[GATED ? t : 0] + wrow * p.pstride);
+      uint4 pv = __ldg(prow + q0);
+      for (int c = q0; c < q1; ++c) {
+        const uint4 pnext = __ldg(prow + min(c + 1, q1 - 1));
+        ok = __all_sync(0xffffffffu, wait(LY::B_CFULL + cr.s, cr.ph));
+        if (!ok) break;
+        const uint8_t* crow = smem + LY::OFF_C + cr.s * LY::CSTAGE + t * (LY::CSTAGE / 2) + r * 128;
+        const uint32_t pw[4] = {pv.x, pv.y, pv.z, pv.w};
+        const int in_stage = min(4, slabs - 4 * (c - q0));
 #pragma unroll
-      for (int s4 = 0; s4 < 4; s4 += DG) {
-        const int s = s4 + group;
-        if (s >= in_stage) break;
-        const int i = 4 * c + s, b = i % AB;
-        const uint4 w0 = *reinterpret_cast<const uint4*>(crow + (((2 * s) ^ (r & 7)) << 4));
-        const uint4 w1 = *reinterpret_cast<const uint4*>(crow + (((2 * s + 1) ^ (r & 7)) << 4));
-        const uint32_t ps = DG == 1 ? pw[s4] : (group == 0 ? pw[s4] : pw[(s4 + 1) & 3]);
-        const uint32_t s24 = __byte_perm(ps, ps, 0x1010), bb = __byte_perm(ps, ps, 0x3232);
-        const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);
-        const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-        uint32_t o[32];
+        for (int st = 0; st < STEPS; ++st) {
+          if (st * SP >= in_stage) break;
+          const int s = st * SP + group;
+          uint32_t o[32];
+          if (s < in_stage) {
+            const uint4 w0 = *reinterpret_cast<const uint4*>(crow + (((2 * s) ^ (r & 7)) << 4));
+            const uint4 w1 = *reinterpret_cast<const uint4*>(crow + (((2 * s + 1) ^ (r & 7)) << 4));
+            const uint32_t ps = SP == 1 || group == 0 ? pw[st * SP] : pw[(st * SP + 1) & 3];
+            const uint32_t s24 = __byte_perm(ps, ps, 0x1010), bb = __byte_perm(ps, ps, 0x3232);
+            const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);
+            const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t d[4];
-          dequant_word(words[j], s24, s20, bb, d);
+            for (int j = 0; j < 8; ++j) {
+              uint32_t d[4];
+              dequant_word(words[j], s24, s20, bb, d);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[4 * j + k] = d[k];
-        }
-        publish();
-        if (i >= AB) {
-          ok = __all_sync(0xffffffffu,
-                          wait_or_abort(bar(LY::B_AEMPTY + b), ((i - AB) / AB) & 1, p.wait_ns, abort_flag));
+              for (int q = 0; q < 4; ++q) o[4 * j + q] = d[q];
+            }
+          }
+          publish();
+          ok = __all_sync(0xffffffffu, wait(LY::B_AEMPTY + ar.s, ar.ph ^ 1u));
           if (!ok) break;
           tc::fence_after();
+          if (s < in_stage) tc::tmem_st32_nowait(a_base + ar.s * 64 * SP, o);
+          stored = ar.s;
+          ar.next();
         }
-        tc::tmem_st32_nowait(a_base + b * 64, o);
-        stored = b;
+        if (!ok) break;
+        __syncwarp();  // the stage's codes are in registers
+        if (lane == 0) mbar_arrive(bar(LY::B_CEMPTY + cr.s));
+        cr.next();
+        pv = pnext;
       }
-      __syncwarp();  // the stage's codes are in registers
-      if (lane == 0) mbar_arrive(bar(LY::B_CEMPTY + cs));
-      pv = pnext;
-    }
-    if (ok) {
+      if (!ok) break;
       publish();
-      ok = __all_sync(0xffffffffu, wait_or_abort(bar(LY::B_DFULL), 0, p.wait_ns, abort_flag) &&
-                                       wait_or_abort(bar(LY::B_SCALE), 0, p.wait_ns, abort_flag));
-    }
-    if (!ok) *abort_flag = 1;
-    // the output warps meet here also after an abort (each may have seen it at another step)
-    tc::fence_after();
-    if (f.ck == 1) {
-      // ---- output: lane = weight row, columns = tokens; rounded values to shared memory as
-      // [token][row], then whole rows of them to global memory
+      stored = -1;
+      const int b = k & 1;
+      ok = __all_sync(0xffffffffu, wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1));
+      if (!ok) break;
+      tc::fence_after();
+      if (f.ck > 1) {
+        // ---- fp32 sums to shared memory, [tile][token][128 rows]
+        constexpr int COLS = NT / SP;
+        float* red = reinterpret_cast<float*>(smem) + t * NT * 128 + r;
+#pragma unroll 1
+        for (int cb = group * COLS; cb < (group + 1) * COLS; cb += 16) {
+          float v[16];
+          tc::tmem_ld16(tmem + t * NT + cb + lane_base, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) red[(cb + j) * 128] = v[j];
+        }
+        break;
+      }
+      // ---- output: lane = weight row, columns = tokens; 16 tokens at a time through the warp's
+      // own shared memory, so that a token's 32 rows leave as 64 bytes
       constexpr int PARTS = GATED ? DW / 4 : DW / 8;  // warps that share a lane quarter (and tile)
       constexpr int COLS = NT / PARTS;
       const int part = GATED ? warp >> 2 : group;
-      const int row = n0 + (GATED ? 0 : t * 128) + r;
-      const int64_t wr = (int64_t)e * p.n_out + min(row, p.n_out - 1);
+      const int row0 = n0 + (GATED ? 0 : t * 128) + quarter * 32;
+      const int64_t wr = (int64_t)e * p.n_out + min(row0 + lane, p.n_out - 1);
       const float rs0 = p.row_scale[0][wr], rs1 = GATED ? p.row_scale[1][wr] : 0.0f;
-      uint16_t* so = reinterpret_cast<uint16_t*>(smem);
-      if (ok) {
+      uint16_t* so = reinterpret_cast<uint16_t*>(smem + LY::OFF_OUT + warp * 1024);
+      const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 #pragma unroll 1
-        for (int cb = part * COLS; cb < (part + 1) * COLS; cb += 16) {
-          if (lo + cb >= hi) break;
-          float g[16], u[16];
-          tc::tmem_ld16(tmem + (GATED ? 0 : t * NT) + cb + lane_base, g);
-          if constexpr (GATED) tc::tmem_ld16(tmem + NT + cb + lane_base, u);
+      for (int cb = part * COLS; cb < (part + 1) * COLS; cb += 16) {
+        if (lo + cb >= hi) break;
+        float g[16], u[16];
+        tc::tmem_ld16(tmem + (GATED ? 0 : t * NT) + cb + lane_base, g);
+        if constexpr (GATED) tc::tmem_ld16(tmem + NT + cb + lane_base, u);
+        const float4* ts4 = reinterpret_cast<const float4*>(tok_scale + b * NT + cb);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float ts = tok_scale[cb + j];
-            const float y = GATED ? silu_mul(g[j] * (rs0 * ts), u[j] * (rs1 * ts)) : g[j] * (rs0 * ts);
-            so[(cb + j) * CTA_ROWS + (GATED ? 0 : t * 128) + r] = p.bf16 ? f2h<true>(y) : f2h<false>(y);
-          }
+        for (int j = 0; j < 16; ++j) {
+          const float4 tv = ts4[j >> 2];
+          const float ts = (j & 3) == 0 ? tv.x : (j & 3) == 1 ? tv.y : (j & 3) == 2 ? tv.z : tv.w;
+          g[j] *= rs0 * ts;
+          if constexpr (GATED) g[j] = silu_mul(g[j], u[j] * (rs1 * ts));
         }
-      }
-      asm volatile("bar.sync 1, %0;\n" ::"n"(DW * 32) : "memory");
-      if (!*abort_flag) {
-        const int m = hi - lo;
-        const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-        constexpr int VPR = CTA_ROWS / 8;  // 16-byte vectors of a token
-        for (int v = tid; v < m * VPR; v += DW * 32) {
-          const int tok = v / VPR, col = (v % VPR) * 8;
-          const int left = p.n_out - (n0 + col);
-          if (left <= 0) continue;
-          const uint4 d = *reinterpret_cast<const uint4*>(so + tok * CTA_ROWS + col);
-          uint16_t* dst = p.out + (int64_t)(lo + tok) * p.out_stride + n0 + col;
-          if (wide && left >= 8) {
-            *reinterpret_cast<uint4*>(dst) = d;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          uint32_t h;
+          if (p.bf16) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(g[j], g[j + 1]);
+            h = *reinterpret_cast<const uint32_t*>(&v);
           } else {
-            const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+            h = pack_half2(g[j], g[j + 1]);
+          }
+          so[j * 32 + lane] = static_cast<uint16_t>(h);
+          so[(j + 1) * 32 + lane] = static_cast<uint16_t>(h >> 16);
+        }
+        __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (j < left) dst[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+        for (int h = 0; h < 2; ++h) {
+          const int tok = h * 8 + (lane >> 2), col = (lane & 3) * 8;
+          const int left = p.n_out - (row0 + col);
+          const uint4 d = *reinterpret_cast<const uint4*>(so + tok * 32 + col);
+          if (lo + cb + tok < hi && left > 0) {
+            uint16_t* dst = p.out + (int64_t)(lo + cb + tok) * p.out_stride + row0 + col;
+            if (wide && left >= 8) {
+              *reinterpret_cast<uint4*>(dst) = d;
+            } else {
+              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (j < left) dst[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+            }
           }
         }
+        __syncwarp();
       }
-    } else if (ok) {
-      // ---- fp32 sums to shared memory, [tile][token][128 rows]
-      constexpr int COLS = NT / DG;
-      float* red = reinterpret_cast<float*>(smem) + t * NT * 128 + r;
-#pragma unroll 1
-      for (int cb = group * COLS; cb < (group + 1) * COLS; cb += 16) {
-        float v[16];
-        tc::tmem_ld16(tmem + t * NT + cb + lane_base, v);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) red[(cb + j) * 128] = v[j];
+      // the accumulators and the tokens' scales are read
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(LY::B_DEMPTY));
+        mbar_arrive(bar(LY::B_SEMPTY + b));
       }
     }
   }
+  if (!ok) *abort_flag = 1;
   __syncwarp();
   if (f.ck > 1) {
     // the ranks' sums of a token and row, added in rank order; a rank finishes its share of the
     // tokens, two rows a thread
+    griddep_wait();
     cluster_sync_all();
     if (!*abort_flag) {
+      int lo, hi;
+      const int e = find_item<NT>(p, first / f.row_tiles, lo, hi);
+      const int n0 = first % f.row_tiles * CTA_ROWS;
       const int m = hi - lo;
       const int t0 = m * rank / f.ck, t1 = m * (rank + 1) / f.ck;
       constexpr int PAIRS = CTA_ROWS / 2;
@@ -435,9 +509,9 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     if (warp == X_WARP && lane == 0)
       for (int j = max(0, issued_x - XS); j < issued_x; ++j)
         mbar_wait_bounded(bar(LY::B_XFULL + j % XS), (j / XS) & 1, kDrainNs);
-    if (warp == MMA_WARP && lane == 0 && mma_issued) {
-      tc::commit(bar(LY::B_DRAIN));
-      mbar_wait_bounded(bar(LY::B_DRAIN), 0, kDrainNs);
+    if (warp >= MMA_WARP && lane == 0 && mma_issued) {
+      tc::commit(bar(LY::B_DRAIN + warp - MMA_WARP));
+      mbar_wait_bounded(bar(LY::B_DRAIN + warp - MMA_WARP), 0, kDrainNs);
     }
     if (tid == 0) flag_status(p.status, AM_STATUS_TIMEOUT);
   }
@@ -472,13 +546,15 @@ static cudaError_t launch_tiles_t(const LinearParams& p, int64_t items, cudaStre
   }
   const int rows_per_cta = GATED ? 128 : 256;
   const int row_tiles = (p.n_out + rows_per_cta - 1) / rows_per_cta;
+  if (row_tiles * items > INT_MAX) return cudaErrorNotSupported;
   const int quads = p.pstride / 4;
   TilesParams f{};
   f.p = p;
   f.ck = 1;
   while (f.ck < 8 && (int64_t)row_tiles * items * f.ck * 2 <= (int64_t)sms * LY::CTAS && f.ck * 4 <= quads) f.ck *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(row_tiles * f.ck, static_cast<unsigned>(items));
+  f.row_tiles = row_tiles;
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(row_tiles * items * f.ck, (int64_t)sms * LY::CTAS)));
   cfg.blockDim = dim3(LY::THREADS);
   cfg.dynamicSmemBytes = LY::SMEM;
   cfg.stream = stream;
@@ -498,7 +574,6 @@ template <int NT>
 static cudaError_t launch_tiles(const LinearParams& p, cudaStream_t stream) {
   const int64_t items = p.offsets != nullptr ? (int64_t)min(p.experts, p.rows) + p.rows / NT
                                              : ((int64_t)p.rows + NT - 1) / NT;
-  if (items > 65535) return cudaErrorInvalidConfiguration;
   return p.codes[1] != nullptr ? launch_tiles_t<NT, true>(p, items, stream) : launch_tiles_t<NT, false>(p, items, stream);
 }
 
