@@ -214,7 +214,7 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     lib.am_q4_linear_workspace_bytes.argtypes = [weight, weight, c_int32]
     lib.am_q4_linear.argtypes = [weight, weight, c_void_p, c_int64, c_int32, c_void_p, c_int64,
                                  c_void_p, c_size_t, c_void_p, c_void_p]
-    lib.am_q4_expert_linear_workspace_bytes.argtypes = [weight, weight, c_int32, c_int32]
+    lib.am_q4_expert_linear_workspace_bytes.argtypes = [weight, weight, c_int32]
     lib.am_q4_expert_linear.argtypes = [weight, weight, c_void_p, c_int64, c_int32, c_void_p,
                                         c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p,
                                         c_size_t, c_void_p, c_void_p]

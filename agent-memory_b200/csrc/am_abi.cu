@@ -772,20 +772,19 @@ static int linear_params(LinearParams& p, const am_q4_weight* w, const am_q4_wei
 }
 
 // Workspace of the tensor-tile kernel: the activations as fp16 rows and one float a row.
-static size_t linear_workspace(const am_q4_weight* w, int32_t x_rows, int32_t rows, bool grouped) {
-  if (w == nullptr || w->n_in <= 0 || w->experts <= 0 || rows <= 0 || x_rows <= 0 ||
+static size_t linear_workspace(const am_q4_weight* w, int32_t rows, bool grouped) {
+  if (w == nullptr || w->n_in <= 0 || w->experts <= 0 || rows <= 0 ||
       !linear_uses_tensor_tiles(rows, w->experts, grouped))
     return 0;
-  return (size_t)x_rows * ((size_t)w->n_in * 2 + 4);
+  return (size_t)rows * ((size_t)w->n_in * 2 + 4);
 }
 
 size_t am_q4_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight*, int32_t rows) {
-  return linear_workspace(w, rows, rows, false);
+  return linear_workspace(w, rows, false);
 }
 
-size_t am_q4_expert_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight*, int32_t x_rows,
-                                           int32_t rows) {
-  return linear_workspace(w, x_rows, rows, true);
+size_t am_q4_expert_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight*, int32_t rows) {
+  return linear_workspace(w, rows, true);
 }
 
 // A 2-D map over rows of `row_bytes` bytes, read in boxes of 128 bytes x box_rows with the
@@ -807,20 +806,16 @@ static int run_linear(LinearParams& p, void* workspace, size_t workspace_bytes, 
   const bool grouped = p.offsets != nullptr;
   if (!linear_uses_tensor_tiles(p.rows, p.experts, grouped))
     return cuda_status(launch_linear_few(p, static_cast<cudaStream_t>(stream)), fn);
-  if (p.x_rows == 0) {
-    set_error("%s: rows without any x rows", fn);
-    return AM_ERR_INVALID;
-  }
-  const size_t need = (size_t)p.x_rows * ((size_t)p.n_in * 2 + 4);
+  const size_t need = (size_t)p.rows * ((size_t)p.n_in * 2 + 4);
   if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)) {
     set_error("%s: a 256-byte aligned workspace of %zu bytes required (got %zu)", fn, need, workspace_bytes);
     return AM_ERR_WORKSPACE;
   }
   p.xh = static_cast<uint16_t*>(workspace);
-  p.xscale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)p.x_rows * p.n_in * 2);
+  p.xscale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)p.rows * p.n_in * 2);
   p.wait_ns = wait_limit_ns();
   const int tile = linear_token_tile(p.rows, p.experts, grouped);
-  bool ok = encode_rows_map(&p.tmap_x, p.xh, p.x_rows, (int64_t)p.n_in * 2, p.order != nullptr ? 1 : tile);
+  bool ok = encode_rows_map(&p.tmap_x, p.xh, p.rows, (int64_t)p.n_in * 2, tile);
   for (int i = 0; i < 2 && ok; ++i)
     if (p.codes[i] != nullptr)
       ok = encode_rows_map(&p.tmap_w[i], p.codes[i], (int64_t)p.experts * p.n_out, p.n_in / 2, 128);

@@ -429,7 +429,7 @@ static cudaError_t launch_few(const LinearParams& p, cudaStream_t stream) {
 // device).
 bool linear_uses_tensor_tiles(int rows, int experts, bool grouped) {
   const int mean = grouped ? (rows + experts - 1) / experts : rows;
-  return mean > 32;
+  return mean > 8;
 }
 
 cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream) {

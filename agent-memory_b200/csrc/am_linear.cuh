@@ -24,7 +24,7 @@ struct LinearParams {
   int64_t out_stride;
   int32_t* status;
   uint64_t wait_ns;           // limit of the bounded waits
-  // tensor-tile kernel: the activations as fp16 rows [x_rows][n_in] in its input order and their
+  // tensor-tile kernel: the activations as fp16 rows [rows][n_in] in its input order and their
   // powers of two, in the caller's workspace; tensor maps of them and of the codes
   uint16_t* xh;
   float* xscale;

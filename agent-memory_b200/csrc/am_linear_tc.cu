@@ -3,15 +3,15 @@
 // y^T = W x^T: weight rows are the M side (128 lanes of TMEM), tokens the N side, so a weight is
 // dequantized once for up to 128 tokens, straight into the TMEM operand.
 //
-// 1. linear_rows_kernel writes the activations as fp16 rows of the workspace, each under a power
-//    of two (exact for fp16 and bf16 values) and with its inputs in the order in which the
-//    dequantization below produces the weights.
+// 1. linear_rows_kernel writes the activations as fp16 rows of the workspace, in output order (a
+//    grouped call's tokens are gathered here: tile::gather4 loads in the tile kernel measured
+//    2.5x slower than plain boxes, ~75 clocks per four rows), each under a power of two (exact
+//    for fp16 and bf16 values) and with its inputs in the order in which the dequantization
+//    below produces the weights.
 // 2. linear_tiles_kernel: a CTA owns two 128-row weight tiles (plain: 256 rows of the matrix;
 //    gated: 128 rows of each matrix) and NT tokens of one matrix or expert.
 //    * one thread streams the codes (TMA, 128 rows x 256 inputs a box, 128-byte swizzle), one
-//      warp the activations (TMA boxes of NT rows x 64 inputs; through `order` by
-//      tile::gather4, four rows an instruction; rows past the item or behind a bad index lie
-//      outside the map and read as zeros);
+//      the activations (TMA boxes of NT rows x 64 inputs);
 //    * warps 0-7 dequantize: a thread owns a weight row; 64 codes a step become 32 registers of
 //      fp16 pairs (9 operations for 8 weights, see am_linear.cu) and go to TMEM with one
 //      tcgen05.st -- no shared-memory round trip, and the MMA reads its A operand there;
@@ -41,9 +41,15 @@ __global__ void __launch_bounds__(128) linear_rows_kernel(const __grid_constant_
   __shared__ uint32_t wmax[4];
   griddep_launch_dependents();
   const int row = blockIdx.x, tid = threadIdx.x;
-  const uint4* src = reinterpret_cast<const uint4*>(p.x + (int64_t)row * p.x_stride);
+  const int from = source_row(p, row);
+  const uint4* src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(from, 0) * p.x_stride);
   uint4* dst = reinterpret_cast<uint4*>(p.xh + (int64_t)row * p.n_in);
   const int vecs = p.n_in / 8;
+  if (from < 0) {
+    for (int i = tid; i < vecs; i += 128) dst[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) p.xscale[row] = 1.0f;
+    return;
+  }
   if (!p.bf16) {
     for (int i = tid; i < vecs; i += 128) {
       const uint4 u = src[i];
@@ -105,16 +111,6 @@ struct TilesLayout {
     return 1;
   }
 };
-
-// gather4 load of four rows of a map with one-row boxes of 128 bytes.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, int r0, int r1, int r2,
-                                            int r3, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, "
-      "{%2, %3, %4, %5, %6}], [%7];\n" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
-      : "memory");
-}
 
 // Position in a ring of N buffers and the parity of its current round.
 template <int N>
@@ -214,29 +210,15 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     for (int tile = first; tile < tiles && ok; tile += step, ++k) {
       int lo, hi;
       find_item<NT>(p, tile / f.row_tiles, lo, hi);
-      // lane i: rows 4 i .. 4 i + 3 of the item
-      int rows4[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = lo + 4 * lane + j;
-        const int src = 4 * lane < NT && r < hi ? source_row(p, r) : -1;
-        rows4[j] = src >= 0 ? src : p.x_rows;  // past the map: zeros
-      }
       for (int i = 0; i < steps; ++i) {
         ok = __all_sync(0xffffffffu, wait(LY::B_XEMPTY + ring.s, ring.ph ^ 1u));
         if (!ok) break;
         const uint32_t full = bar(LY::B_XFULL + ring.s), dst = s_base + LY::OFF_X + ring.s * SP * LY::XSLAB;
         const int n = min(SP, slabs - i * SP);
-        if (lane == 0) mbar_arrive_expect_tx(full, n * LY::XSLAB);
-        __syncwarp();
-        for (int s = 0; s < n; ++s) {
-          const int x = (q0 * 4 + i * SP + s) * 128;
-          if (p.order != nullptr) {
-            if (4 * lane < NT)
-              tma_gather4(dst + s * LY::XSLAB + lane * 512, &p.tmap_x, x, rows4[0], rows4[1], rows4[2], rows4[3], full);
-          } else if (lane == 0) {
-            tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, x, lo, full);
-          }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(full, n * LY::XSLAB);
+          for (int s = 0; s < n; ++s)
+            tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, (q0 * 4 + i * SP + s) * 128, lo, full);
         }
         ++issued_x;
         ring.next();
@@ -244,12 +226,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
           const int b = k & 1;
           ok = __all_sync(0xffffffffu, wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1));
           if (!ok) break;
-          if (4 * lane < NT) {
-            float v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = rows4[j] < p.x_rows ? p.xscale[rows4[j]] : 0.0f;
-            *reinterpret_cast<float4*>(tok_scale + b * NT + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
-          }
+          for (int j = lane; j < NT; j += 32) tok_scale[b * NT + j] = lo + j < hi ? p.xscale[lo + j] : 0.0f;
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(LY::B_SFULL + b));
         }
@@ -578,7 +555,7 @@ static cudaError_t launch_tiles(const LinearParams& p, cudaStream_t stream) {
 }
 
 cudaError_t launch_linear_tiles(const LinearParams& p, cudaStream_t stream) {
-  linear_rows_kernel<<<p.x_rows, 128, 0, stream>>>(p);
+  linear_rows_kernel<<<p.rows, 128, 0, stream>>>(p);
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   switch (linear_token_tile(p.rows, p.experts, p.offsets != nullptr)) {

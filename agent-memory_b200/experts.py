@@ -128,12 +128,12 @@ def _expert_linear(x, w: Q4Weight, up, routing: ExpertRouting, gather: bool, out
 def _expert_call(x, w, up, offsets, order, top_k, rows, out, status):
     out = _out(out, rows, w, (rows, w.n_out))
     lib = _lib.load()
-    key = (up is not None, x.shape[0], rows)
+    key = (up is not None, rows)
     need = w.bytes_cache.get(key)
     up_ref = up.ref if up is not None else None
     if need is None:
         need = w.bytes_cache[key] = int(
-            lib.am_q4_expert_linear_workspace_bytes(w.ref, up_ref, x.shape[0], rows))
+            lib.am_q4_expert_linear_workspace_bytes(w.ref, up_ref, rows))
     ws = _workspace(need, w.device)
     rc = lib.am_q4_expert_linear(w.ref, up_ref, x.data_ptr(), _row_stride(x), x.shape[0],
                                  offsets.data_ptr(), order.data_ptr() if order is not None else None,

@@ -327,7 +327,7 @@ int am_q4_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, i
  * AM_STATUS_BAD_POSITION.
  */
 size_t am_q4_expert_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up,
-                                           int32_t x_rows, int32_t rows);
+                                           int32_t rows);
 int am_q4_expert_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x,
                         int64_t x_stride, int32_t x_rows, const int32_t* offsets,
                         const int32_t* order, int32_t top_k, int32_t rows, void* out,
