@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   constexpr bool GATED = MT == 2;
   constexpr int STAGE = MT * kFewStage;
   const LinearParams& p = f.p;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g8 = lane >> 2, t4 = lane & 3;
   const int rank = f.ck > 1 ? static_cast<int>(blockIdx.x) % f.ck : 0;
@@ -139,46 +139,62 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   const int64_t total = (int64_t)items * f.tiles;
   const int64_t p0 = total * cluster / clusters, p1 = total * (cluster + 1) / clusters;
 
-  // ---- load side: position, stage and expert of the next stage to fetch
-  int64_t l_pos = p0;
-  int l_stage = 0, l_item = -1, l_e = 0, l_buf = 0;
+  // ---- load side: walks the positions [p0, p1) a few stages ahead of the sums.  A lane fetches 16
+  // bytes of rows lane / 8 + 4 j of the tile and a parameter of rows lane / 4 + 8 j.
+  int l_left = static_cast<int>(p1 - p0);
+  int l_item = static_cast<int>(p0 / f.tiles);
+  int l_pos = static_cast<int>(p0 - (int64_t)l_item * f.tiles);  // position in the item
+  int l_stage = 0, l_buf = 0, l_e = 0;
+  const int row_bytes = p.n_in / 2;
+  const int64_t tile_bytes = (int64_t)wr_n * 16 * row_bytes, tile_params = (int64_t)wr_n * 16 * p.pstride;
+  const uint8_t* l_codes = nullptr;   // this lane's first chunk of the tile, matrix 0
+  const uint32_t* l_params = nullptr;
+  const int64_t codes_diff = GATED ? reinterpret_cast<const uint8_t*>(p.codes[1]) - reinterpret_cast<const uint8_t*>(p.codes[0]) : 0;
+  const int64_t params_diff = GATED ? p.params[1] - p.params[0] : 0;
+  const uint32_t l_dst = smem_u32(ring) + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);  // row + 4: chunk ^ 4
+  const uint32_t l_pdst = smem_u32(ring) + 2048 + (lane >> 2) * 16 + (lane & 3) * 4;
+  auto l_open = [&]() {  // pointers of position l_pos of item l_item
+    int lo, hi;
+    l_e = find_item<kFewTokens>(p, l_item, lo, hi);
+    const int64_t row = (int64_t)max(l_e, 0) * p.n_out + (int64_t)(l_pos * wr_n + wr) * 16;
+    l_codes = reinterpret_cast<const uint8_t*>(p.codes[0]) + (row + (lane >> 3)) * row_bytes + ga * 32 + (lane & 7) * 16;
+    l_params = p.params[0] + (row + (lane >> 2)) * p.pstride + ga + (lane & 3);
+  };
+  if (l_left > 0) l_open();
   auto fetch = [&]() {
-    if (l_pos < p1 && stages > 0) {
-      const int item = static_cast<int>(l_pos / f.tiles);
-      if (item != l_item) {
-        int lo, hi;
-        l_e = find_item<kFewTokens>(p, item, lo, hi);
-        l_item = item;
+    if (l_left > 0) {
+      const int first_row = (l_pos * wr_n + wr) * 16;
+      const int ng = min(4, gb - ga - 4 * l_stage);
+      const uint32_t dst = l_dst + l_buf * STAGE, pdst = l_pdst + l_buf * STAGE;
+      const uint8_t* src = l_codes + l_stage * 128;
+      const uint32_t* psrc = l_params + l_stage * 4;
+      const int rows = p.n_out - first_row;  // rows past the matrix are neither loaded nor stored
+      if ((lane & 7) < 2 * ng) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((lane >> 3) + 4 * j < rows)
+              cp_async16_s((dst ^ ((j & 1) << 6)) + i * kFewStage + j * 512, src + i * codes_diff + j * 4 * row_bytes);
       }
-      const int tile = static_cast<int>(l_pos - (int64_t)item * f.tiles) * wr_n + wr;
-      const int g0 = ga + l_stage * 4, ng = min(4, gb - g0);
-      if (tile < row_tiles) {
-        uint8_t* dst = ring + l_buf * STAGE;
-        const int c = lane & 7;
+      if ((lane & 3) < ng) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const int64_t wbase = (int64_t)l_e * p.n_out;
-          if (c < 2 * ng) {
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int r = (lane >> 3) + 4 * j;
-              const int64_t row = wbase + min(tile * 16 + r, p.n_out - 1);  // (rows past the matrix are not stored)
-              cp_async16(dst + i * kFewStage + r * 128 + ((c ^ (r & 7)) << 4),
-                         reinterpret_cast<const uint8_t*>(p.codes[i]) + row * (p.n_in / 2) + g0 * 32 + c * 16);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = (lane >> 2) + 8 * j, q = lane & 3;
-            const int64_t row = wbase + min(tile * 16 + r, p.n_out - 1);
-            if (q < ng)
-              cp_async4(dst + i * kFewStage + 2048 + r * 16 + q * 4, p.params[i] + row * p.pstride + g0 + q);
-          }
-        }
+          for (int j = 0; j < 2; ++j)
+            if ((lane >> 2) + 8 * j < rows)
+              cp_async4_s(pdst + i * kFewStage + j * 128, psrc + i * params_diff + j * 8 * p.pstride);
       }
       if (++l_stage == stages) {
         l_stage = 0;
-        ++l_pos;
+        --l_left;
+        l_codes += tile_bytes;
+        l_params += tile_params;
+        if (++l_pos == f.tiles) {
+          l_pos = 0;
+          ++l_item;
+          if (l_left > 0) l_open();
+        }
       }
       if (++l_buf == D) l_buf = 0;
     }
@@ -219,18 +235,21 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
     __syncwarp();
   };
 
-  int64_t pos = p0;
-  while (pos < p1) {
+  // byte offsets of this lane's two words of group q in a row pair's stage
+  uint32_t woff[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) woff[q] = g8 * 128 + (((2 * q + (t4 >> 1)) ^ g8) << 4) + (t4 & 1) * 8;
+  int left = static_cast<int>(p1 - p0), it = static_cast<int>(p0 / f.tiles);
+  int tile0 = static_cast<int>(p0 - (int64_t)it * f.tiles);
+  while (left > 0) {
     // a batch: positions of one item
-    const int it = static_cast<int>(pos / f.tiles);
     if (it != item) {
       e = find_item<kFewTokens>(p, it, lo, hi);
       item = it;
       m = hi - lo;
       stage_x();
     }
-    const int tile0 = static_cast<int>(pos - (int64_t)it * f.tiles);
-    const int nb = static_cast<int>(min((int64_t)min(f.batch, f.tiles - tile0), p1 - pos));
+    const int nb = min(min(f.batch, f.tiles - tile0), left);
     for (int b = 0; b < nb; ++b) {
       float acc[MT][4] = {};
       const int tile = (tile0 + b) * wr_n + wr;
@@ -261,9 +280,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
               uint32_t a[2][2][4];  // [row half][word][pair]
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const int r = g8 + 8 * h;
-                const uint2 w = *reinterpret_cast<const uint2*>(
-                    src + i * kFewStage + r * 128 + (((2 * q + (t4 >> 1)) ^ (r & 7)) << 4) + (t4 & 1) * 8);
+                const uint2 w = *reinterpret_cast<const uint2*>(src + i * kFewStage + woff[q] + h * 1024);
                 const uint32_t v = q == 0 ? pq[i][h].x : q == 1 ? pq[i][h].y : q == 2 ? pq[i][h].z : pq[i][h].w;
                 const uint32_t s24 = __byte_perm(v, v, 0x1010), bb = __byte_perm(v, v, 0x3232);
                 const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);  // * 2^-4
@@ -328,7 +345,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
       cluster_sync_all();
     else
       __syncthreads();
-    pos += nb;
+    left -= nb;
+    if ((tile0 += nb) == f.tiles) {
+      tile0 = 0;
+      ++it;
+    }
   }
 }
 
@@ -386,7 +407,7 @@ cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream) {
   const int row_tiles = (p.n_out + 15) / 16;
   const int wr_n = kFewWarps / f.wk;
   f.tiles = (row_tiles + wr_n - 1) / wr_n;
-  f.batch = 4 / mt;
+  f.batch = std::max(1, std::min(16, 32 / (mt * tok)));  // 32 KB of sums
   const int red = f.batch * mt * kFewWarps * tok * 64;
   // A cluster splits the inputs when the activations of a CTA would leave no room for two stages.
   f.ck = 1;
