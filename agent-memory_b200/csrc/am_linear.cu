@@ -65,23 +65,23 @@ cudaError_t launch_weight_pack(const void* scales, const void* biases, bool bf16
 }
 
 // ---------------------------------------------------------------- few tokens (HBM-bound)
-// Up to 8 tokens of one matrix or expert: y^T = W x^T on mma.sync m16n8k16 with the weights as the A
-// operand straight from their packed words.  tcgen05 would take the dequantized weights through
+// Up to 8 tokens of one matrix or expert: y^T = W x^T on mma.sync m16n8k16 with the codes as the A
+// operand straight from their packed words.  tcgen05 would take dequantized weights through
 // TMEM; here a weight is used for at most 8 tokens and the kernel is bound by the bytes of the
 // codes, so the operand that needs no staging wins.
 //
-// * Dequantization: one AND turns two nibbles of a word into fp16 subnormals code * 2^-24 (or
-//   * 2^-20), one packed FMA with (scale * 2^24 or 2^20, bias) makes the two weights, rounded
-//   once: 9 operations for 8 weights.  The row's exponent (am_q4_weight_pack) keeps scale * 2^24
-//   inside fp16 and is undone on the fp32 result.
-// * The inputs of a group of 64 are permuted over the MMA's k slots so that lane t of a quad owns
-//   words 2t and 2t + 1 of its row.  The activations are staged in the same order, as fp16 under
-//   a power of two per token (exact), in fragment order: one 16-byte load per two MMAs.
-// * A CTA of 16 warps a SM.  wk of them split the inputs (each stages only its own slice of the
-//   activations, so nothing waits for the whole CTA before the sums), the others take further
-//   row tiles; with long inputs CK CTAs of a cluster split them again.  Every warp streams its
-//   slices of the row tiles (16 rows x up to 4 groups a stage) through a private cp.async ring:
-//   the warps of a SM keep 70 to 110 KB in flight, across tile and expert ends.
+// * Per group of 64 inputs y += scale * (codes . x) + bias * sum(x), the first dot product on
+//   the tensor cores (exact products, fp32 sums), the rest in fp32: no weight is rounded.  One
+//   AND turns two nibbles of a word into fp16 subnormals code * 2^-24, or 16 code * 2^-24 for
+//   the odd nibbles, whose activations are staged divided by 16: 5 integer operations for 8
+//   weights; the parameters hold scale * 2^24 (am_q4_weight_pack).
+// * The inputs of a group are permuted over the MMA's k slots so that lane t of a quad owns words
+//   2t and 2t + 1 of its row.  The activations are staged in the same order, as fp16 under a
+//   power of two per token and slice (exact), in fragment order, with their group sums.
+// * A CTA of 16 warps a SM.  wk of them split the inputs, the others take further row tiles; when
+//   the activations do not fit, CK CTAs of a cluster split the inputs again.  Every warp
+//   streams its slices of the row tiles (16 rows x up to 4 groups a stage) through a private
+//   cp.async ring: the warps of a SM keep 74 to 110 KB in flight, across tile and expert ends.
 // * Partial sums meet in shared memory every few tiles, in a fixed order.
 // * The work of all experts is one sequence of row tiles, cut evenly over the CTAs.
 // * Before griddepcontrol.wait the CTA only asks L2 for its first codes (a prefetch reads
@@ -92,18 +92,52 @@ constexpr int kFewStage = 16 * 128 + 16 * 16;  // codes and parameters of 16 row
 
 struct FewParams {
   LinearParams p;
-  int32_t wk;       // warps along the inputs (1, 2, 4, 8 or 16)
-  int32_t ck;       // CTAs of a cluster along the inputs
-  int32_t tiles;    // positions of one item: row tiles / (16 / wk), rounded up
-  int32_t batch;    // positions between two sums
-  int32_t slice;    // groups of a warp's slice, at most
-  int32_t x_stride; // staged bytes of a warp's activations
+  int32_t wk;     // warps along the inputs (1, 2, 4, 8 or 16)
+  int32_t ck;     // CTAs of a cluster along the inputs
+  int32_t tiles;  // positions of one item: row tiles / (16 / wk), rounded up
+  int32_t batch;  // positions between two sums
 };
 
-template <int MT, int D>
+// Ring depth of a warp: what leaves room for the activations of a few thousand inputs.
+template <int MT, int TK>
+constexpr int kFewDepth = MT == 2 ? 2 : (TK == 8 ? 3 : 4);
+
+// D = A x B with a zero accumulator.
+__device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                   uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// Eight activations of a token times `f` (a power of two) in the order of the A operand, the odd
+// inputs of a word divided by 16; `sum` gets their fp32 sum (of the scaled values).
+template <bool BF16>
+__device__ __forceinline__ uint4 stage_inputs(uint4 u, float f, float& sum) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  float v[8];
+  sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = h2f<BF16>(static_cast<uint16_t>(w[j])) * f;
+    v[2 * j + 1] = h2f<BF16>(static_cast<uint16_t>(w[j] >> 16)) * f;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum += v[j];
+  constexpr float k = 0.0625f;
+  return make_uint4(pack_half2(v[0], v[4]), pack_half2(v[1] * k, v[5] * k), pack_half2(v[2], v[6]),
+                    pack_half2(v[3] * k, v[7] * k));
+}
+
+// TK: tokens of an item, padded to 1, 2, 4 or 8.
+template <int MT, int TK>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __grid_constant__ FewParams f) {
   constexpr bool GATED = MT == 2;
+  constexpr int D = kFewDepth<MT, TK>;
   constexpr int STAGE = MT * kFewStage;
+  constexpr int XG = 128 * TK;  // staged bytes of a group
   const LinearParams& p = f.p;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -112,14 +146,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   const int cluster = static_cast<int>(blockIdx.x) / f.ck, clusters = static_cast<int>(gridDim.x) / f.ck;
   const int wk = f.wk, wr_n = kFewWarps / wk;
   const int kslice = warp % wk, wr = warp / wk;
-  uint8_t* ring = smem + warp * (D * STAGE);
-  uint8_t* sx = smem + kFewWarps * D * STAGE + warp * f.x_stride;
-  float* red = reinterpret_cast<float*>(smem + kFewWarps * (D * STAGE + f.x_stride));
-  const int row_tiles = (p.n_out + 15) >> 4;
-  // this warp's groups
-  const int slices = wk * f.ck, slot = rank * wk + kslice;
-  const int ga = p.groups * slot / slices, gb = p.groups * (slot + 1) / slices;
+  // this CTA's and this warp's groups
+  const int slices = wk * f.ck;
+  const int ca = p.groups * (rank * wk) / slices;
+  const int ga = p.groups * (rank * wk + kslice) / slices, gb = p.groups * (rank * wk + kslice + 1) / slices;
   const int stages = (gb - ga + 3) >> 2;  // of one row tile
+  const int cta_groups = (p.groups + f.ck - 1) / f.ck;  // at most
+  uint8_t* ring = smem + warp * (D * STAGE);
+  uint8_t* sx = smem + kFewWarps * D * STAGE;                         // [group][half][TK][4] x 16 bytes
+  float* sxsum = reinterpret_cast<float*>(sx + (cta_groups + 1) * XG);  // [group][TK]
+  float* sxscale = sxsum + (cta_groups + 1) * TK;                       // [slice][TK]
+  float* red = sxscale + kFewWarps * TK;
+  const int row_tiles = (p.n_out + 15) >> 4;
 
   griddep_launch_dependents();
   if (p.offsets == nullptr) {  // L2 prefetch of the CTA's first tiles: a lane pair a row
@@ -129,7 +167,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const char* c = reinterpret_cast<const char*>(p.codes[i] + n * (p.n_in / 8));
-        for (int g = ga + (lane & 1) * 4; g < gb; g += 8)
+        for (int g = ga + (lane & 1) * 4; g < min(gb, ga + 16); g += 8)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(c + g * 32));
       }
     }
@@ -144,7 +182,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   int l_left = static_cast<int>(p1 - p0);
   int l_item = static_cast<int>(p0 / f.tiles);
   int l_pos = static_cast<int>(p0 - (int64_t)l_item * f.tiles);  // position in the item
-  int l_stage = 0, l_buf = 0, l_e = 0;
+  int l_stage = 0, l_buf = 0;
   const int row_bytes = p.n_in / 2;
   const int64_t tile_bytes = (int64_t)wr_n * 16 * row_bytes, tile_params = (int64_t)wr_n * 16 * p.pstride;
   const uint8_t* l_codes = nullptr;   // this lane's first chunk of the tile, matrix 0
@@ -155,20 +193,19 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   const uint32_t l_pdst = smem_u32(ring) + 2048 + (lane >> 2) * 16 + (lane & 3) * 4;
   auto l_open = [&]() {  // pointers of position l_pos of item l_item
     int lo, hi;
-    l_e = find_item<kFewTokens>(p, l_item, lo, hi);
-    const int64_t row = (int64_t)max(l_e, 0) * p.n_out + (int64_t)(l_pos * wr_n + wr) * 16;
+    const int e = find_item<kFewTokens>(p, l_item, lo, hi);
+    const int64_t row = (int64_t)max(e, 0) * p.n_out + (int64_t)(l_pos * wr_n + wr) * 16;
     l_codes = reinterpret_cast<const uint8_t*>(p.codes[0]) + (row + (lane >> 3)) * row_bytes + ga * 32 + (lane & 7) * 16;
     l_params = p.params[0] + (row + (lane >> 2)) * p.pstride + ga + (lane & 3);
   };
   if (l_left > 0) l_open();
   auto fetch = [&]() {
     if (l_left > 0) {
-      const int first_row = (l_pos * wr_n + wr) * 16;
       const int ng = min(4, gb - ga - 4 * l_stage);
       const uint32_t dst = l_dst + l_buf * STAGE, pdst = l_pdst + l_buf * STAGE;
       const uint8_t* src = l_codes + l_stage * 128;
       const uint32_t* psrc = l_params + l_stage * 4;
-      const int rows = p.n_out - first_row;  // rows past the matrix are neither loaded nor stored
+      const int rows = p.n_out - (l_pos * wr_n + wr) * 16;  // rows past the matrix are neither loaded nor stored
       if ((lane & 7) < 2 * ng) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -205,40 +242,44 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
 
   // ---- compute side
   int item = -1, e = 0, lo = 0, hi = 0, m = 0, buf = 0;
-  float scale2[2] = {};  // powers of two of tokens 2 t4 and 2 t4 + 1
-  // this warp's slice of the item's activations: largest |x| of a token to [2^14, 2^15), fragment order
+  // The item's activations of slice kslice, tokens wr, wr + wr_n, ..: largest |x| to [2^14, 2^15).
   auto stage_x = [&]() {
     const int vecs = (gb - ga) * 8;  // 16-byte vectors of a token's slice
-    __syncwarp();
-    for (int tok = 0; tok < m; ++tok) {
+    for (int tok = wr; tok < m; tok += wr_n) {
       const int row = source_row(p, lo + tok);
       const uint4* src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(row, 0) * p.x_stride + ga * 64);
-      float inv = 1.0f, sc = 1.0f;
-      if (p.bf16) {
-        uint32_t mx = 0;
-        if (row >= 0)
-          for (int v = lane; v < vecs; v += 32) mx = max(mx, max_abs_bits(src[v]));
-        const int ex = row_exponent(__reduce_max_sync(0xffffffffu, mx));
-        inv = exp2f(static_cast<float>(-ex));
-        sc = exp2f(static_cast<float>(ex));
-      }
-      if (tok == 2 * t4) scale2[0] = sc;
-      if (tok == 2 * t4 + 1) scale2[1] = sc;
-      for (int v = lane; v < vecs; v += 32) {
-        uint4 o = make_uint4(0, 0, 0, 0);
-        if (row >= 0) o = p.bf16 ? permute_bf16(src[v], inv) : permute_f16(src[v]);
+      uint32_t mx = 0;
+      if (row >= 0)
+        for (int v = lane; v < vecs; v += 32) mx = max(mx, max_abs_bits(src[v]));
+      mx = __reduce_max_sync(0xffffffffu, mx);
+      const int ex = p.bf16 ? row_exponent(mx) : row_exponent_f16(mx);
+      const float inv = exp2f(static_cast<float>(-ex));
+      if (lane == 0) sxscale[kslice * TK + tok] = exp2f(static_cast<float>(ex));
+      for (int v0 = 0; v0 < vecs; v0 += 32) {
+        const int v = v0 + lane;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (row >= 0 && v < vecs) u = src[v];
+        float sum;
+        const uint4 o = p.bf16 ? stage_inputs<true>(u, inv, sum) : stage_inputs<false>(u, inv, sum);
+#pragma unroll
+        for (int s = 1; s < 8; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
         // word c of the group: lane c / 2 of the quad, half c & 1
-        const int grp = v >> 3, c = v & 7;
-        reinterpret_cast<uint4*>(sx)[((grp * 2 + (c & 1)) * m + tok) * 4 + (c >> 1)] = o;
+        const int grp = ga - ca + (v >> 3), c = v & 7;
+        if (v < vecs) {
+          *reinterpret_cast<uint4*>(sx + grp * XG + ((c & 1) * TK + tok) * 64 + (c >> 1) * 16) = o;
+          if (c == 0) sxsum[grp * TK + tok] = sum;
+        }
       }
     }
-    __syncwarp();
   };
 
-  // byte offsets of this lane's two words of group q in a row pair's stage
+  // byte offsets of this lane's two words of group q in a row pair's stage, and of its token's
+  // activations and its two columns' sums in a group
   uint32_t woff[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) woff[q] = g8 * 128 + (((2 * q + (t4 >> 1)) ^ g8) << 4) + (t4 & 1) * 8;
+  const uint8_t* xlane = sx + (ga - ca) * XG + (g8 & (TK - 1)) * 64 + t4 * 16;
+  const float* slane = sxsum + (ga - ca) * TK + ((2 * t4) & (TK - 1));
   int left = static_cast<int>(p1 - p0), it = static_cast<int>(p0 / f.tiles);
   int tile0 = static_cast<int>(p0 - (int64_t)it * f.tiles);
   while (left > 0) {
@@ -248,18 +289,21 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
       item = it;
       m = hi - lo;
       stage_x();
+      __syncthreads();  // (the last batch ended with a barrier after its last read of the activations)
     }
     const int nb = min(min(f.batch, f.tiles - tile0), left);
     for (int b = 0; b < nb; ++b) {
       float acc[MT][4] = {};
       const int tile = (tile0 + b) * wr_n + wr;
+      const uint8_t* xs = xlane;
+      const float* ss = slane;
       for (int st = 0; st < stages; ++st) {
         fetch();
         cp_async_wait<D - 1>();
         __syncwarp();
         if (tile < row_tiles) {
           const uint8_t* src = ring + buf * STAGE;
-          const int ng = min(4, gb - ga - 4 * st);
+          const int ng = gb - ga - 4 * st;
           uint4 pq[MT][2];
 #pragma unroll
           for (int i = 0; i < MT; ++i)
@@ -269,44 +313,63 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             if (q >= ng) break;
-            const uint4* bx = reinterpret_cast<const uint4*>(sx) + (4 * st + q) * 8 * m;
-            uint4 b0 = make_uint4(0, 0, 0, 0), b1 = b0;
-            if (g8 < m) {
-              b0 = bx[g8 * 4 + t4];
-              b1 = bx[(m + g8) * 4 + t4];
-            }
+            const uint4 b0 = *reinterpret_cast<const uint4*>(xs + q * XG);
+            const uint4 b1 = *reinterpret_cast<const uint4*>(xs + q * XG + TK * 64);
+            float2 sm;
+            if constexpr (TK == 1)
+              sm = make_float2(ss[q], 0.0f);
+            else
+              sm = *reinterpret_cast<const float2*>(ss + q * TK);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-              uint32_t a[2][2][4];  // [row half][word][pair]
+              uint32_t a[2][8];  // [row half][pair]
+              float sc[2], bi[2];
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const uint2 w = *reinterpret_cast<const uint2*>(src + i * kFewStage + woff[q] + h * 1024);
                 const uint32_t v = q == 0 ? pq[i][h].x : q == 1 ? pq[i][h].y : q == 2 ? pq[i][h].z : pq[i][h].w;
-                const uint32_t s24 = __byte_perm(v, v, 0x1010), bb = __byte_perm(v, v, 0x3232);
-                const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);  // * 2^-4
-                dequant_word(w.x, s24, s20, bb, a[h][0]);
-                dequant_word(w.y, s24, s20, bb, a[h][1]);
+                const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                sc[h] = sb.x;
+                bi[h] = sb.y;
+                const uint32_t wh = w.x >> 8, xh = w.y >> 8;
+                a[h][0] = w.x & 0x000f000fu;
+                a[h][1] = w.x & 0x00f000f0u;
+                a[h][2] = wh & 0x000f000fu;
+                a[h][3] = wh & 0x00f000f0u;
+                a[h][4] = w.y & 0x000f000fu;
+                a[h][5] = w.y & 0x00f000f0u;
+                a[h][6] = xh & 0x000f000fu;
+                a[h][7] = xh & 0x00f000f0u;
               }
-              mma_f16_16816(acc[i], a[0][0][0], a[1][0][0], a[0][0][1], a[1][0][1], b0.x, b0.y);
-              mma_f16_16816(acc[i], a[0][0][2], a[1][0][2], a[0][0][3], a[1][0][3], b0.z, b0.w);
-              mma_f16_16816(acc[i], a[0][1][0], a[1][1][0], a[0][1][1], a[1][1][1], b1.x, b1.y);
-              mma_f16_16816(acc[i], a[0][1][2], a[1][1][2], a[0][1][3], a[1][1][3], b1.z, b1.w);
+              float d[4];
+              mma_f16_16816_zero(d, a[0][0], a[1][0], a[0][1], a[1][1], b0.x, b0.y);
+              mma_f16_16816(d, a[0][2], a[1][2], a[0][3], a[1][3], b0.z, b0.w);
+              mma_f16_16816(d, a[0][4], a[1][4], a[0][5], a[1][5], b1.x, b1.y);
+              mma_f16_16816(d, a[0][6], a[1][6], a[0][7], a[1][7], b1.z, b1.w);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                acc[i][2 * h] = fmaf(bi[h], sm.x, fmaf(sc[h], d[2 * h], acc[i][2 * h]));
+                if constexpr (TK > 1) acc[i][2 * h + 1] = fmaf(bi[h], sm.y, fmaf(sc[h], d[2 * h + 1], acc[i][2 * h + 1]));
+              }
             }
           }
+          xs += 4 * XG;
+          ss += 4 * TK;
         }
         __syncwarp();  // the stage is read before it is loaded again
         if (++buf == D) buf = 0;
       }
       // partial sums [batch][matrix][wr][slice][token][16 rows]
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int c = 0; c < 4; ++c) {
+        const int tok = 2 * t4 + (c & 1);
+        if (tok < m) {
+          const float ts = sxscale[kslice * TK + tok];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int tok = 2 * t4 + (c & 1);
-          if (tok < m)
-            red[((((b * MT + i) * wr_n + wr) * wk + kslice) * m + tok) * 16 + g8 + 8 * (c >> 1)] =
-                acc[i][c] * scale2[c & 1];
+          for (int i = 0; i < MT; ++i)
+            red[((((b * MT + i) * wr_n + wr) * wk + kslice) * m + tok) * 16 + g8 + 8 * (c >> 1)] = acc[i][c] * ts;
         }
+      }
     }
     // ---- sums over the slices, the row's power of two, the gate, the output
     if (f.ck > 1)
@@ -353,20 +416,54 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   }
 }
 
-constexpr int kFewSmem = 220 * 1024;
+constexpr int kFewSmem = 226 * 1024;
 
-template <int MT, int D>
-static cudaError_t launch_few_t(const FewParams& f, int smem, int ctas, int dev, cudaStream_t stream) {
+template <int MT, int TK>
+static cudaError_t launch_few_t(FewParams& f, int64_t items, cudaStream_t stream) {
+  const LinearParams& p = f.p;
+  int dev = 0, sms = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (err != cudaSuccess) return err;
   static unsigned long long done = 0;
-  auto kfn = linear_few_kernel<MT, D>;
+  auto kfn = linear_few_kernel<MT, TK>;
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
   if (!bit || !(__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) {
-    cudaError_t err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+    err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
     if (err != cudaSuccess) return err;
     if (bit) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
   }
+  constexpr int ring = kFewWarps * kFewDepth<MT, TK> * MT * kFewStage;
+  f.batch = std::max(1, 16 / (MT * TK));  // 16 KB of sums
+  const int red = f.batch * MT * kFewWarps * TK * 64;
+  auto smem_for = [&](int ck) {
+    const int groups = (p.groups + ck - 1) / ck + 1;
+    return ring + groups * (128 + 4) * TK + kFewWarps * TK * 4 + red;
+  };
+  f.ck = 1;
+  while (f.ck < 8 && smem_for(f.ck) > kFewSmem) f.ck *= 2;
+  const int smem = smem_for(f.ck);
+  if (smem > kFewSmem) return cudaErrorNotSupported;
+  // Warps along the inputs: the split whose CTAs finish first, a position costing its groups and
+  // about one and a half groups' time for the sums; a warp gets at least a whole stage.
+  const int row_tiles = (p.n_out + 15) / 16;
+  const int ctas = sms / f.ck;
+  double best = 0.0;
+  for (int wk = 1; wk <= kFewWarps; wk *= 2) {
+    if (wk > 1 && p.groups < 4 * wk * f.ck) break;
+    const int wr = kFewWarps / wk;
+    const int64_t positions = (int64_t)((row_tiles + wr - 1) / wr) * items;
+    const double rounds = static_cast<double>((positions + ctas - 1) / ctas);
+    const double cost = rounds * ((p.groups + wk * f.ck - 1) / (wk * f.ck) + 1.5);
+    if (wk == 1 || cost < best) {
+      best = cost;
+      f.wk = wk;
+    }
+  }
+  const int wr = kFewWarps / f.wk;
+  f.tiles = (row_tiles + wr - 1) / wr;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
+  cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(items * f.tiles, ctas)) * f.ck));
   cfg.blockDim = dim3(kFewWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -382,6 +479,14 @@ static cudaError_t launch_few_t(const FewParams& f, int smem, int ctas, int dev,
   return cudaLaunchKernelEx(&cfg, kfn, f);
 }
 
+template <int MT>
+static cudaError_t launch_few(FewParams& f, int tok, int64_t items, cudaStream_t stream) {
+  if (tok <= 1) return launch_few_t<MT, 1>(f, items, stream);
+  if (tok <= 2) return launch_few_t<MT, 2>(f, items, stream);
+  if (tok <= 4) return launch_few_t<MT, 4>(f, items, stream);
+  return launch_few_t<MT, 8>(f, items, stream);
+}
+
 // Which kernel: the mean number of rows of a matrix decides (a grouped call's counts are on the
 // device).
 bool linear_uses_tensor_tiles(int rows, int experts, bool grouped) {
@@ -391,43 +496,12 @@ bool linear_uses_tensor_tiles(int rows, int experts, bool grouped) {
 
 cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream) {
   if (p.rows == 0) return cudaSuccess;
-  int dev = 0, sms = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (err != cudaSuccess) return err;
-  const int mt = p.codes[1] != nullptr ? 2 : 1;
-  const int tok = min(p.rows, kFewTokens);
-  const int64_t items = p.offsets != nullptr ? (int64_t)min(p.experts, p.rows) + p.rows / kFewTokens
+  const int64_t items = p.offsets != nullptr ? (int64_t)std::min(p.experts, p.rows) + p.rows / kFewTokens
                                              : (p.rows + kFewTokens - 1) / kFewTokens;
   FewParams f{};
   f.p = p;
-  // Slices along the inputs: up to 16 warps with at least 4 groups (a whole stage) each.
-  f.wk = 1;
-  while (f.wk < kFewWarps && p.groups >= f.wk * 8) f.wk *= 2;
-  const int row_tiles = (p.n_out + 15) / 16;
-  const int wr_n = kFewWarps / f.wk;
-  f.tiles = (row_tiles + wr_n - 1) / wr_n;
-  f.batch = std::max(1, std::min(16, 32 / (mt * tok)));  // 32 KB of sums
-  const int red = f.batch * mt * kFewWarps * tok * 64;
-  // A cluster splits the inputs when the activations of a CTA would leave no room for two stages.
-  f.ck = 1;
-  for (;; f.ck *= 2) {
-    f.slice = (p.groups + f.wk * f.ck - 1) / (f.wk * f.ck);
-    f.x_stride = f.slice * 128 * tok;
-    if (f.ck == 8 || kFewWarps * (2 * mt * kFewStage + f.x_stride) + red <= kFewSmem) break;
-  }
-  const int room = kFewSmem - red - kFewWarps * f.x_stride;
-  const int d = min(mt == 2 ? 3 : 5, room / (kFewWarps * mt * kFewStage));
-  if (d < 2) return cudaErrorNotSupported;  // (more than 8 x 16 x 19 groups of 64 inputs)
-  const int smem = kFewWarps * (d * mt * kFewStage + f.x_stride) + red;
-  const int ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items * f.tiles, sms / f.ck))) * f.ck;
-  if (mt == 2) return d == 2 ? launch_few_t<2, 2>(f, smem, ctas, dev, stream) : launch_few_t<2, 3>(f, smem, ctas, dev, stream);
-  switch (d) {
-    case 2: return launch_few_t<1, 2>(f, smem, ctas, dev, stream);
-    case 3: return launch_few_t<1, 3>(f, smem, ctas, dev, stream);
-    case 4: return launch_few_t<1, 4>(f, smem, ctas, dev, stream);
-    default: return launch_few_t<1, 5>(f, smem, ctas, dev, stream);
-  }
+  const int tok = std::min(p.rows, kFewTokens);
+  return p.codes[1] != nullptr ? launch_few<2>(f, tok, items, stream) : launch_few<1>(f, tok, items, stream);
 }
 
 }  // namespace am

@@ -106,6 +106,11 @@ __device__ __forceinline__ uint32_t max_abs_bits(uint4 u) {
 __device__ __forceinline__ int row_exponent(uint32_t max_bits) {
   return max(min(max(static_cast<int>(max_bits >> 7), 1), 254) - 127 - 14, -126);
 }
+// The same for fp16 bits.
+__device__ __forceinline__ int row_exponent_f16(uint32_t max_bits) {
+  const float v = fminf(__half2float(__ushort_as_half(static_cast<uint16_t>(max_bits))), 65504.0f);
+  return v > 0.0f ? ilogbf(v) - 14 : 0;
+}
 __device__ __forceinline__ uint4 permute_f16(uint4 u) {
   return make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
                     __byte_perm(u.y, u.w, 0x7632));
