@@ -2,6 +2,7 @@
 // per group of 64 inputs; gated: silu(x G^T) * (x U^T); and both per expert over rows sorted
 // by expert.
 #include <algorithm>
+#include <climits>
 
 #include "am_internal.h"
 #include "am_linear.cuh"
@@ -86,30 +87,39 @@ cudaError_t launch_weight_pack(const void* scales, const void* biases, bool bf16
 // * The work of all experts is one sequence of row tiles, cut evenly over the CTAs.
 // * Before griddepcontrol.wait the CTA only asks L2 for its first codes (a prefetch reads
 //   nothing, so it may run before the previous kernel is done).
-constexpr int kFewWarps = 16;
+constexpr int kFewWarps = 16, kFewLogWarps = 4;
 constexpr int kFewTokens = 8;
-constexpr int kFewStage = 16 * 128 + 16 * 16;  // codes and parameters of 16 rows x 4 groups
+constexpr int kFewCodes = 16 * 128, kFewPar = 16 * 16;  // bytes of 16 rows x 4 groups
 
 struct FewParams {
   LinearParams p;
-  int32_t wk;     // warps along the inputs (1, 2, 4, 8 or 16)
-  int32_t ck;     // CTAs of a cluster along the inputs
+  int32_t lwk;    // log2 of the warps along the inputs (1 to 16)
+  int32_t lck;    // log2 of the CTAs of a cluster along the inputs (1 to 8)
   int32_t tiles;  // positions of one item: row tiles / (16 / wk), rounded up
   int32_t batch;  // positions between two sums
 };
 
 // Ring depth of a warp: what leaves room for the activations of a few thousand inputs.
 template <int MT, int TK>
-constexpr int kFewDepth = MT == 2 ? 2 : (TK == 8 ? 3 : 4);
+constexpr int kFewDepth = MT == 2 ? 2 : (TK == 8 ? 3 : 5);
 
 // D = A x B with a zero accumulator.
 __device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                    uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};\n"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// D += A x B (as mma_f16_16816, free to be scheduled among other tiles' operations).
+__device__ __forceinline__ void mma_f16_16816_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                  uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // Eight activations of a token times `f` (a power of two) in the order of the A operand, the odd
@@ -132,131 +142,168 @@ __device__ __forceinline__ uint4 stage_inputs(uint4 u, float f, float& sum) {
 }
 
 // TK: tokens of an item, padded to 1, 2, 4 or 8.
-template <int MT, int TK>
+template <bool GATED, int MT, int TK>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __grid_constant__ FewParams f) {
-  constexpr bool GATED = MT == 2;
+  constexpr int TROWS = GATED ? 16 : 16 * MT;  // output rows of a tile
   constexpr int D = kFewDepth<MT, TK>;
-  constexpr int STAGE = MT * kFewStage;
   constexpr int XG = 128 * TK;  // staged bytes of a group
+  static_assert(!GATED || MT == 2, "a gated tile holds 16 rows of each matrix");
   const LinearParams& p = f.p;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g8 = lane >> 2, t4 = lane & 3;
-  const int rank = f.ck > 1 ? static_cast<int>(blockIdx.x) % f.ck : 0;
-  const int cluster = static_cast<int>(blockIdx.x) / f.ck, clusters = static_cast<int>(gridDim.x) / f.ck;
-  const int wk = f.wk, wr_n = kFewWarps / wk;
-  const int kslice = warp % wk, wr = warp / wk;
-  // this CTA's and this warp's groups
-  const int slices = wk * f.ck;
-  const int ca = p.groups * (rank * wk) / slices;
-  const int ga = p.groups * (rank * wk + kslice) / slices, gb = p.groups * (rank * wk + kslice + 1) / slices;
-  const int stages = (gb - ga + 3) >> 2;  // of one row tile
-  const int cta_groups = (p.groups + f.ck - 1) / f.ck;  // at most
+  const int rank = static_cast<int>(blockIdx.x) & ((1 << f.lck) - 1);
+  const int cluster = static_cast<int>(blockIdx.x) >> f.lck, clusters = static_cast<int>(gridDim.x) >> f.lck;
+  const int lwr = kFewLogWarps - f.lwk, wr_n = 1 << lwr, wk = 1 << f.lwk;
+  const int kslice = warp & (wk - 1), wr = warp >> f.lwk;
+  // this CTA's groups [ca, cb) and this warp's [ga, gb): whole quads (16 bytes of parameters)
+  const int quads = p.pstride >> 2, lsl = f.lwk + f.lck;
+  const int ca = (quads * rank >> f.lck) * 4, cb = min((quads * (rank + 1) >> f.lck) * 4, p.groups);
+  const int qa = quads * ((rank << f.lwk) + kslice) >> lsl, qb = quads * ((rank << f.lwk) + kslice + 1) >> lsl;
+  const int ga = qa * 4, gb = min(qb * 4, p.groups);
+  const int stages = qb - qa;  // of one row tile
+  const int cta_groups = ((quads + (1 << f.lck) - 1) >> f.lck) * 4;  // at most
+  constexpr int STAGE = MT * (kFewCodes + kFewPar);
   uint8_t* ring = smem + warp * (D * STAGE);
-  uint8_t* sx = smem + kFewWarps * D * STAGE;                         // [group][half][TK][4] x 16 bytes
-  float* sxsum = reinterpret_cast<float*>(sx + (cta_groups + 1) * XG);  // [group][TK]
-  float* sxscale = sxsum + (cta_groups + 1) * TK;                       // [slice][TK]
-  float* red = sxscale + kFewWarps * TK;
-  const int row_tiles = (p.n_out + 15) >> 4;
+  uint8_t* sx = smem + kFewWarps * D * STAGE;  // [group][half][TK][4] x 16 bytes
+  float* sxsum = reinterpret_cast<float*>(sx + cta_groups * XG);     // [group][TK]
+  float* sxmax = sxsum + cta_groups * TK;  // [warp]: largest |x| of its part of a token, as bits
+  float* red = sxmax + kFewWarps;
+  const int row_tiles = (p.n_out + TROWS - 1) / TROWS;
 
   griddep_launch_dependents();
-  if (p.offsets == nullptr) {  // L2 prefetch of the CTA's first tiles: a lane pair a row
-    const int64_t pos0 = (int64_t)f.tiles * cluster / clusters;
-    const int64_t n = (pos0 * wr_n + wr) * 16 + (lane >> 1);
-    if (n < p.n_out) {
-#pragma unroll
+  // positions [p0, p0 + n_pos) of the sequence of all items' positions
+  int items = (p.rows + kFewTokens - 1) / kFewTokens, p0, n_pos;
+  auto share = [&]() {
+    const int total = items * f.tiles, each = total / clusters, more = total - each * clusters;
+    p0 = each * cluster + min(cluster, more);
+    n_pos = each + (cluster < more);
+  };
+  if (p.offsets == nullptr) {
+    share();
+    // L2 prefetch of the first tiles' codes: a lane pair a row
+    if (p0 < f.tiles) {
+#pragma unroll 1
       for (int i = 0; i < MT; ++i) {
-        const char* c = reinterpret_cast<const char*>(p.codes[i] + n * (p.n_in / 8));
-        for (int g = ga + (lane & 1) * 4; g < min(gb, ga + 16); g += 8)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(c + g * 32));
+        const int64_t n = (int64_t)((p0 << lwr) + wr) * TROWS + (lane >> 1) + (GATED ? 0 : 16 * i);
+        if (n < p.n_out) {
+          const char* c = reinterpret_cast<const char*>(p.codes[GATED ? i : 0] + n * (p.n_in / 8));
+          for (int g = ga + (lane & 1) * 4; g < min(gb, ga + 16); g += 8)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(c + g * 32));
+        }
       }
     }
   }
   griddep_wait();
-  const int items = count_items<kFewTokens>(p);
-  const int64_t total = (int64_t)items * f.tiles;
-  const int64_t p0 = total * cluster / clusters, p1 = total * (cluster + 1) / clusters;
+  if (p.offsets != nullptr) {
+    items = count_items<kFewTokens>(p);
+    share();
+  }
 
-  // ---- load side: walks the positions [p0, p1) a few stages ahead of the sums.  A lane fetches 16
-  // bytes of rows lane / 8 + 4 j of the tile and a parameter of rows lane / 4 + 8 j.
-  int l_left = static_cast<int>(p1 - p0);
-  int l_item = static_cast<int>(p0 / f.tiles);
-  int l_pos = static_cast<int>(p0 - (int64_t)l_item * f.tiles);  // position in the item
-  int l_stage = 0, l_buf = 0;
+  // ---- load side: walks the positions [p0, p1) D - 1 stages ahead of the sums.  A lane fetches 16
+  // bytes of rows lane / 8 + 4 j of the tile and a parameter of rows lane / 4 + 8 j.  (cp.async:
+  // tensor-map boxes of 16 rows reached 3.5 TB/s here, these copies 6.1.)
   const int row_bytes = p.n_in / 2;
-  const int64_t tile_bytes = (int64_t)wr_n * 16 * row_bytes, tile_params = (int64_t)wr_n * 16 * p.pstride;
-  const uint8_t* l_codes = nullptr;   // this lane's first chunk of the tile, matrix 0
-  const uint32_t* l_params = nullptr;
-  const int64_t codes_diff = GATED ? reinterpret_cast<const uint8_t*>(p.codes[1]) - reinterpret_cast<const uint8_t*>(p.codes[0]) : 0;
-  const int64_t params_diff = GATED ? p.params[1] - p.params[0] : 0;
-  const uint32_t l_dst = smem_u32(ring) + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);  // row + 4: chunk ^ 4
-  const uint32_t l_pdst = smem_u32(ring) + 2048 + (lane >> 2) * 16 + (lane & 3) * 4;
-  auto l_open = [&]() {  // pointers of position l_pos of item l_item
+  const int64_t codes4 = (int64_t)4 * row_bytes, par8 = (int64_t)8 * p.pstride * 4;  // bytes to the next j
+  const int64_t tile_bytes = (int64_t)wr_n * TROWS * row_bytes - stages * 128;  // from a tile's end to the next
+  const int64_t tile_par = (int64_t)wr_n * TROWS * p.pstride * 4 - stages * 16;
+  const uint8_t *l_codes = nullptr, *l_par = nullptr;  // this lane's bytes of the next stage, matrix 0
+  const int64_t codes_diff = GATED ? reinterpret_cast<const uint8_t*>(p.codes[1]) - reinterpret_cast<const uint8_t*>(p.codes[0])
+                                   : (int64_t)16 * row_bytes;
+  const int64_t par_diff = GATED ? reinterpret_cast<const uint8_t*>(p.params[1]) - reinterpret_cast<const uint8_t*>(p.params[0])
+                                 : (int64_t)16 * p.pstride * 4;
+  const uint32_t l_dst0 = smem_u32(ring) + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);  // row + 4: chunk ^ 4
+  const uint32_t l_flip = ((l_dst0 ^ 64) - l_dst0);
+  const uint32_t l_pdst0 = smem_u32(ring) + 2048 + (lane >> 2) * 16 + (lane & 3) * 4;
+  const int item0 = p0 / f.tiles;
+  int l_left = n_pos, l_item = item0, l_pos = p0 - item0 * f.tiles;  // (position in the item)
+  int l_stage = 0;
+  uint32_t l_off = 0;  // of the next stage's buffer
+  int l_rows = 0;      // weight rows from the tile's first one to the matrix's end
+  auto l_open = [&]() {  // position l_pos of item l_item
     int lo, hi;
     const int e = find_item<kFewTokens>(p, l_item, lo, hi);
-    const int64_t row = (int64_t)max(e, 0) * p.n_out + (int64_t)(l_pos * wr_n + wr) * 16;
-    l_codes = reinterpret_cast<const uint8_t*>(p.codes[0]) + (row + (lane >> 3)) * row_bytes + ga * 32 + (lane & 7) * 16;
-    l_params = p.params[0] + (row + (lane >> 2)) * p.pstride + ga + (lane & 3);
+    const int first = (l_pos * wr_n + wr) * TROWS;
+    const int64_t row = (int64_t)max(e, 0) * p.n_out + first;
+    l_rows = p.n_out - first;
+    l_codes = reinterpret_cast<const uint8_t*>(p.codes[0]) + (row + (lane >> 3)) * row_bytes + qa * 128 + (lane & 7) * 16;
+    l_par = reinterpret_cast<const uint8_t*>(p.params[0]) + ((row + (lane >> 2)) * p.pstride + qa * 4 + (lane & 3)) * 4;
   };
   if (l_left > 0) l_open();
   auto fetch = [&]() {
     if (l_left > 0) {
-      const int ng = min(4, gb - ga - 4 * l_stage);
-      const uint32_t dst = l_dst + l_buf * STAGE, pdst = l_pdst + l_buf * STAGE;
-      const uint8_t* src = l_codes + l_stage * 128;
-      const uint32_t* psrc = l_params + l_stage * 4;
-      const int rows = p.n_out - (l_pos * wr_n + wr) * 16;  // rows past the matrix are neither loaded nor stored
-      if ((lane & 7) < 2 * ng) {
+      const uint32_t dst = l_dst0 + l_off, pdst = l_pdst0 + l_off;
+      // rows past the matrix are neither loaded nor stored, groups past the last neither loaded nor used
+      const int chunks = min(8, (p.groups - (qa + l_stage) * 4) * 2);
+      if (l_rows >= TROWS && chunks == 8) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const uint8_t* src = l_codes + i * codes_diff;
+          cp_async16_s(dst + i * (kFewCodes + kFewPar), src);
+          cp_async16_s(dst + l_flip + i * (kFewCodes + kFewPar) + 512, src + codes4);
+          cp_async16_s(dst + i * (kFewCodes + kFewPar) + 1024, src + 2 * codes4);
+          cp_async16_s(dst + l_flip + i * (kFewCodes + kFewPar) + 1536, src + 3 * codes4);
+          cp_async4_s(pdst + i * (kFewCodes + kFewPar), l_par + i * par_diff);
+          cp_async4_s(pdst + i * (kFewCodes + kFewPar) + 128, l_par + i * par_diff + par8);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < MT; ++i) {
+          const int rows = l_rows - (GATED ? 0 : 16 * i);
           for (int j = 0; j < 4; ++j)
-            if ((lane >> 3) + 4 * j < rows)
-              cp_async16_s((dst ^ ((j & 1) << 6)) + i * kFewStage + j * 512, src + i * codes_diff + j * 4 * row_bytes);
-      }
-      if ((lane & 3) < ng) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
+            if ((lane >> 3) + 4 * j < rows && (lane & 7) < chunks)
+              cp_async16_s(dst + (j & 1) * l_flip + i * (kFewCodes + kFewPar) + j * 512, l_codes + i * codes_diff + j * codes4);
           for (int j = 0; j < 2; ++j)
             if ((lane >> 2) + 8 * j < rows)
-              cp_async4_s(pdst + i * kFewStage + j * 128, psrc + i * params_diff + j * 8 * p.pstride);
+              cp_async4_s(pdst + i * (kFewCodes + kFewPar) + j * 128, l_par + i * par_diff + j * par8);
+        }
       }
+      l_codes += 128;
+      l_par += 16;
+      if ((l_off += STAGE) == D * STAGE) l_off = 0;
       if (++l_stage == stages) {
         l_stage = 0;
         --l_left;
         l_codes += tile_bytes;
-        l_params += tile_params;
+        l_par += tile_par;
+        l_rows -= wr_n * TROWS;
         if (++l_pos == f.tiles) {
           l_pos = 0;
           ++l_item;
           if (l_left > 0) l_open();
         }
       }
-      if (++l_buf == D) l_buf = 0;
     }
     cp_async_commit();
   };
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < D - 1; ++i) fetch();
 
   // ---- compute side
   int item = -1, e = 0, lo = 0, hi = 0, m = 0, buf = 0;
-  // The item's activations of slice kslice, tokens wr, wr + wr_n, ..: largest |x| to [2^14, 2^15).
+  // The item's activations of this CTA's inputs, the largest |x| of a token to [2^14, 2^15): 16 / TK
+  // warps a token, a lane's vectors read for the maximum and again (from L1) for the conversion.
+  constexpr int WPT = kFewWarps / TK;
   auto stage_x = [&]() {
-    const int vecs = (gb - ga) * 8;  // 16-byte vectors of a token's slice
-    for (int tok = wr; tok < m; tok += wr_n) {
-      const int row = source_row(p, lo + tok);
-      const uint4* src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(row, 0) * p.x_stride + ga * 64);
-      uint32_t mx = 0;
-      if (row >= 0)
-        for (int v = lane; v < vecs; v += 32) mx = max(mx, max_abs_bits(src[v]));
-      mx = __reduce_max_sync(0xffffffffu, mx);
-      const int ex = p.bf16 ? row_exponent(mx) : row_exponent_f16(mx);
-      const float inv = exp2f(static_cast<float>(-ex));
-      if (lane == 0) sxscale[kslice * TK + tok] = exp2f(static_cast<float>(ex));
-      for (int v0 = 0; v0 < vecs; v0 += 32) {
-        const int v = v0 + lane;
+    const int tok = warp / WPT, part = warp % WPT;
+    const int vecs = (cb - ca) * 8;  // 16-byte vectors of the token
+    const int row = tok < m ? source_row(p, lo + tok) : -1;
+    const uint4* src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(row, 0) * p.x_stride + (int64_t)ca * 64);
+    const int v0 = part * 32 + lane;
+    uint32_t mx = 0;
+    if (row >= 0) {
+#pragma unroll 8
+      for (int v = v0; v < vecs; v += 32 * WPT) mx = max(mx, max_abs_bits(src[v]));
+    }
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if (lane == 0) sxmax[warp] = __uint_as_float(mx);
+    __syncthreads();
+    if (tok < m) {
+      const uint32_t all = lane < WPT ? __float_as_uint(sxmax[tok * WPT + lane]) : 0u;
+      mx = __reduce_max_sync(0xffffffffu, all);
+      const float inv = exp2_int(-(p.bf16 ? row_exponent(mx) : row_exponent_f16(mx)));
+#pragma unroll 2
+      for (int v = v0; v - lane < vecs; v += 32 * WPT) {
         uint4 u = make_uint4(0, 0, 0, 0);
         if (row >= 0 && v < vecs) u = src[v];
         float sum;
@@ -264,13 +311,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
 #pragma unroll
         for (int s = 1; s < 8; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
         // word c of the group: lane c / 2 of the quad, half c & 1
-        const int grp = ga - ca + (v >> 3), c = v & 7;
+        const int grp = v >> 3, c = v & 7;
         if (v < vecs) {
           *reinterpret_cast<uint4*>(sx + grp * XG + ((c & 1) * TK + tok) * 64 + (c >> 1) * 16) = o;
           if (c == 0) sxsum[grp * TK + tok] = sum;
         }
       }
     }
+    __syncthreads();
   };
 
   // byte offsets of this lane's two words of group q in a row pair's stage, and of its token's
@@ -280,21 +328,36 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   for (int q = 0; q < 4; ++q) woff[q] = g8 * 128 + (((2 * q + (t4 >> 1)) ^ g8) << 4) + (t4 & 1) * 8;
   const uint8_t* xlane = sx + (ga - ca) * XG + (g8 & (TK - 1)) * 64 + t4 * 16;
   const float* slane = sxsum + (ga - ca) * TK + ((2 * t4) & (TK - 1));
-  int left = static_cast<int>(p1 - p0), it = static_cast<int>(p0 / f.tiles);
-  int tile0 = static_cast<int>(p0 - (int64_t)it * f.tiles);
+  int left = n_pos, it = item0, tile0 = p0 - item0 * f.tiles;
+  float tscale[2] = {};  // powers of two of this lane's columns
   while (left > 0) {
     // a batch: positions of one item
     if (it != item) {
       e = find_item<kFewTokens>(p, it, lo, hi);
       item = it;
       m = hi - lo;
-      stage_x();
-      __syncthreads();  // (the last batch ended with a barrier after its last read of the activations)
+      stage_x();  // (the last batch ended with a barrier after its last read of the activations)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t mx = 0;
+#pragma unroll
+        for (int k = 0; k < WPT; ++k) mx = max(mx, __float_as_uint(sxmax[((2 * t4 + c) & (TK - 1)) * WPT + k]));
+        tscale[c] = exp2_int(p.bf16 ? row_exponent(mx) : row_exponent_f16(mx));
+      }
     }
     const int nb = min(min(f.batch, f.tiles - tile0), left);
     for (int b = 0; b < nb; ++b) {
       float acc[MT][4] = {};
-      const int tile = (tile0 + b) * wr_n + wr;
+      const int tile = ((tile0 + b) << lwr) + wr;
+      // the rows' powers of two, needed after the sums
+      float rs[MT][2];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int n = tile * TROWS + (GATED ? 0 : 16 * i) + g8 + 8 * h;
+          rs[i][h] = n < p.n_out ? __ldg(p.row_scale[GATED ? i : 0] + (int64_t)e * p.n_out + n) : 0.0f;
+        }
       const uint8_t* xs = xlane;
       const float* ss = slane;
       for (int st = 0; st < stages; ++st) {
@@ -302,17 +365,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
         cp_async_wait<D - 1>();
         __syncwarp();
         if (tile < row_tiles) {
-          const uint8_t* src = ring + buf * STAGE;
-          const int ng = gb - ga - 4 * st;
+          const uint8_t* src = ring + buf;
           uint4 pq[MT][2];
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              pq[i][h] = *reinterpret_cast<const uint4*>(src + i * kFewStage + 2048 + (g8 + 8 * h) * 16);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (q >= ng) break;
+              pq[i][h] = *reinterpret_cast<const uint4*>(src + i * (kFewCodes + kFewPar) + 2048 + (g8 + 8 * h) * 16);
+          auto group = [&](int q) {
             const uint4 b0 = *reinterpret_cast<const uint4*>(xs + q * XG);
             const uint4 b1 = *reinterpret_cast<const uint4*>(xs + q * XG + TK * 64);
             float2 sm;
@@ -326,7 +386,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
               float sc[2], bi[2];
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const uint2 w = *reinterpret_cast<const uint2*>(src + i * kFewStage + woff[q] + h * 1024);
+                const uint2 w = *reinterpret_cast<const uint2*>(src + i * (kFewCodes + kFewPar) + woff[q] + h * 1024);
                 const uint32_t v = q == 0 ? pq[i][h].x : q == 1 ? pq[i][h].y : q == 2 ? pq[i][h].z : pq[i][h].w;
                 const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(&v));
                 sc[h] = sb.x;
@@ -343,68 +403,78 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
               }
               float d[4];
               mma_f16_16816_zero(d, a[0][0], a[1][0], a[0][1], a[1][1], b0.x, b0.y);
-              mma_f16_16816(d, a[0][2], a[1][2], a[0][3], a[1][3], b0.z, b0.w);
-              mma_f16_16816(d, a[0][4], a[1][4], a[0][5], a[1][5], b1.x, b1.y);
-              mma_f16_16816(d, a[0][6], a[1][6], a[0][7], a[1][7], b1.z, b1.w);
+              mma_f16_16816_add(d, a[0][2], a[1][2], a[0][3], a[1][3], b0.z, b0.w);
+              mma_f16_16816_add(d, a[0][4], a[1][4], a[0][5], a[1][5], b1.x, b1.y);
+              mma_f16_16816_add(d, a[0][6], a[1][6], a[0][7], a[1][7], b1.z, b1.w);
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 acc[i][2 * h] = fmaf(bi[h], sm.x, fmaf(sc[h], d[2 * h], acc[i][2 * h]));
                 if constexpr (TK > 1) acc[i][2 * h + 1] = fmaf(bi[h], sm.y, fmaf(sc[h], d[2 * h + 1], acc[i][2 * h + 1]));
               }
             }
+          };
+          const int ng = gb - ga - 4 * st;
+          if (ng >= 4) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) group(q);
+          } else {
+            group(0);
+            if (ng > 1) group(1);
+            if (ng > 2) group(2);
           }
           xs += 4 * XG;
           ss += 4 * TK;
         }
         __syncwarp();  // the stage is read before it is loaded again
-        if (++buf == D) buf = 0;
+        if ((buf += STAGE) == D * STAGE) buf = 0;
       }
-      // partial sums [batch][matrix][wr][slice][token][16 rows]
+      // partial sums [batch][matrix or half][wr][slice][token][16 rows]
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int tok = 2 * t4 + (c & 1);
-        if (tok < m) {
-          const float ts = sxscale[kslice * TK + tok];
+        if (tok < TK) {
 #pragma unroll
           for (int i = 0; i < MT; ++i)
-            red[((((b * MT + i) * wr_n + wr) * wk + kslice) * m + tok) * 16 + g8 + 8 * (c >> 1)] = acc[i][c] * ts;
+            red[(((((((b * MT + i) << lwr) + wr) << f.lwk) + kslice) * TK + tok) << 4) + g8 + 8 * (c >> 1)] =
+                acc[i][c] * (tscale[c & 1] * rs[i][c >> 1]);
         }
       }
     }
-    // ---- sums over the slices, the row's power of two, the gate, the output
-    if (f.ck > 1)
+    // ---- sums over the slices, the gate, the output: rows fastest, then tiles of a position, tokens
+    if (f.lck > 0)
       cluster_sync_all();
     else
       __syncthreads();
-    const int outs = nb * wr_n * 16 * m;
+    constexpr int LROWS = TROWS == 16 ? 4 : 5, LTK = TK == 1 ? 0 : TK == 2 ? 1 : TK == 4 ? 2 : 3;
+    const int outs = nb << (lwr + LROWS + LTK);
     const uint32_t red_addr = smem_u32(red);
-    for (int o = tid + rank * kFewWarps * 32; o < outs; o += kFewWarps * 32 * f.ck) {
-      const int r = o & 15, rest = o >> 4;
-      const int w = rest % wr_n, bt = rest / wr_n;  // rows fastest over the tiles of a position
-      const int b = bt % nb, tok = bt / nb;
-      const int n = ((tile0 + b) * wr_n + w) * 16 + r;
-      if (n >= p.n_out) continue;
+    for (int o = tid + rank * kFewWarps * 32; o < outs; o += kFewWarps * 32 << f.lck) {
+      const int r = o & (TROWS - 1), w = (o >> LROWS) & (wr_n - 1), rest = o >> (LROWS + lwr);
+      const int tok = rest & (TK - 1), b = rest >> LTK;
+      const int n = (((tile0 + b) << lwr) + w) * TROWS + r;
+      if (n >= p.n_out || tok >= m) continue;
       float sum[2];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int at = (((b * MT + i) * wr_n + w) * wk * m + tok) * 16 + r;
+      for (int i = 0; i < (GATED ? 2 : 1); ++i) {
+        const int half = GATED ? i : r >> 4;
+        const int at = ((((((b * MT + half) << lwr) + w) << f.lwk) * TK + tok) << 4) + (r & 15);
         float s = 0.0f;
-        if (f.ck > 1) {
-          for (int c = 0; c < f.ck; ++c) {
+        if (f.lck > 0) {
+          for (int c = 0; c < 1 << f.lck; ++c) {
             const uint32_t base = dsmem_addr(red_addr, c) + at * 4;
 #pragma unroll 4
-            for (int k = 0; k < wk; ++k) s += ld_dsmem_f32(base + k * m * 64);
+            for (int k = 0; k < wk; ++k) s += ld_dsmem_f32(base + k * TK * 64);
           }
         } else {
 #pragma unroll 4
-          for (int k = 0; k < wk; ++k) s += red[at + k * m * 16];
+          for (int k = 0; k < wk; ++k) s += red[at + k * TK * 16];
         }
-        sum[i] = s * p.row_scale[i][(int64_t)e * p.n_out + n];
+        sum[i] = s;
       }
       const float y = GATED ? silu_mul(sum[0], sum[1]) : sum[0];
       p.out[(int64_t)(lo + tok) * p.out_stride + n] = p.bf16 ? f2h<true>(y) : f2h<false>(y);
     }
-    if (f.ck > 1)
+    if (f.lck > 0)
       cluster_sync_all();
     else
       __syncthreads();
@@ -416,9 +486,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   }
 }
 
-constexpr int kFewSmem = 226 * 1024;
+constexpr int kFewSmem = 227 * 1024;
 
-template <int MT, int TK>
+template <bool GATED, int MT, int TK>
 static cudaError_t launch_few_t(FewParams& f, int64_t items, cudaStream_t stream) {
   const LinearParams& p = f.p;
   int dev = 0, sms = 0;
@@ -426,44 +496,51 @@ static cudaError_t launch_few_t(FewParams& f, int64_t items, cudaStream_t stream
   if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (err != cudaSuccess) return err;
   static unsigned long long done = 0;
-  auto kfn = linear_few_kernel<MT, TK>;
+  auto kfn = linear_few_kernel<GATED, MT, TK>;
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
   if (!bit || !(__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) {
     err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
     if (err != cudaSuccess) return err;
     if (bit) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
   }
-  constexpr int ring = kFewWarps * kFewDepth<MT, TK> * MT * kFewStage;
+  constexpr int ring = kFewWarps * kFewDepth<MT, TK> * MT * (kFewCodes + kFewPar);
   f.batch = std::max(1, 16 / (MT * TK));  // 16 KB of sums
   const int red = f.batch * MT * kFewWarps * TK * 64;
+  const int quads = p.pstride / 4;
   auto smem_for = [&](int ck) {
-    const int groups = (p.groups + ck - 1) / ck + 1;
-    return ring + groups * (128 + 4) * TK + kFewWarps * TK * 4 + red;
+    const int groups = (quads + ck - 1) / ck * 4;
+    return ring + groups * (128 + 4) * TK + kFewWarps * 4 + red;
   };
-  f.ck = 1;
-  while (f.ck < 8 && smem_for(f.ck) > kFewSmem) f.ck *= 2;
-  const int smem = smem_for(f.ck);
+  int ck = 1;
+  while (ck < 8 && smem_for(ck) > kFewSmem) ck *= 2;
+  const int smem = smem_for(ck);
   if (smem > kFewSmem) return cudaErrorNotSupported;
   // Warps along the inputs: the split whose CTAs finish first, a position costing its groups and
   // about one and a half groups' time for the sums; a warp gets at least a whole stage.
-  const int row_tiles = (p.n_out + 15) / 16;
-  const int ctas = sms / f.ck;
+  constexpr int TROWS = GATED ? 16 : 16 * MT;
+  const int row_tiles = (p.n_out + TROWS - 1) / TROWS;
+  const int ctas = sms / ck;
   double best = 0.0;
-  for (int wk = 1; wk <= kFewWarps; wk *= 2) {
-    if (wk > 1 && p.groups < 4 * wk * f.ck) break;
-    const int wr = kFewWarps / wk;
+  int wk = 1;
+  for (int k = 1; k <= kFewWarps; k *= 2) {
+    if (k > 1 && quads < k * ck) break;
+    const int wr = kFewWarps / k;
     const int64_t positions = (int64_t)((row_tiles + wr - 1) / wr) * items;
     const double rounds = static_cast<double>((positions + ctas - 1) / ctas);
-    const double cost = rounds * ((p.groups + wk * f.ck - 1) / (wk * f.ck) + 1.5);
-    if (wk == 1 || cost < best) {
+    const double cost = rounds * ((quads + k * ck - 1) / (k * ck) * 4 + 1.5);
+    if (k == 1 || cost < best) {
       best = cost;
-      f.wk = wk;
+      wk = k;
     }
   }
-  const int wr = kFewWarps / f.wk;
+  auto log2_of = [](int v) { return 31 - __builtin_clz(v); };
+  f.lwk = log2_of(wk);
+  f.lck = log2_of(ck);
+  const int wr = kFewWarps / wk;
   f.tiles = (row_tiles + wr - 1) / wr;
+  if (items * f.tiles > INT_MAX) return cudaErrorNotSupported;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(items * f.tiles, ctas)) * f.ck));
+  cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(items * f.tiles, ctas)) * ck));
   cfg.blockDim = dim3(kFewWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -471,20 +548,20 @@ static cudaError_t launch_few_t(FewParams& f, int64_t items, cudaStream_t stream
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = f.ck;
+  attr[1].val.clusterDim.x = ck;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = f.ck > 1 ? 2 : 1;
+  cfg.numAttrs = ck > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kfn, f);
 }
 
-template <int MT>
+template <bool GATED, int MT, int MT8>
 static cudaError_t launch_few(FewParams& f, int tok, int64_t items, cudaStream_t stream) {
-  if (tok <= 1) return launch_few_t<MT, 1>(f, items, stream);
-  if (tok <= 2) return launch_few_t<MT, 2>(f, items, stream);
-  if (tok <= 4) return launch_few_t<MT, 4>(f, items, stream);
-  return launch_few_t<MT, 8>(f, items, stream);
+  if (tok <= 1) return launch_few_t<GATED, MT, 1>(f, items, stream);
+  if (tok <= 2) return launch_few_t<GATED, MT, 2>(f, items, stream);
+  if (tok <= 4) return launch_few_t<GATED, MT, 4>(f, items, stream);
+  return launch_few_t<GATED, MT8, 8>(f, items, stream);
 }
 
 // Which kernel: the mean number of rows of a matrix decides (a grouped call's counts are on the
@@ -501,7 +578,8 @@ cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream) {
   FewParams f{};
   f.p = p;
   const int tok = std::min(p.rows, kFewTokens);
-  return p.codes[1] != nullptr ? launch_few<2>(f, tok, items, stream) : launch_few<1>(f, tok, items, stream);
+  return p.codes[1] != nullptr ? launch_few<true, 2, 2>(f, tok, items, stream)
+                               : launch_few<false, 1, 1>(f, tok, items, stream);
 }
 
 }  // namespace am

@@ -106,6 +106,8 @@ __device__ __forceinline__ uint32_t max_abs_bits(uint4 u) {
 __device__ __forceinline__ int row_exponent(uint32_t max_bits) {
   return max(min(max(static_cast<int>(max_bits >> 7), 1), 254) - 127 - 14, -126);
 }
+// 2^e for e in [-126, 127].
+__device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }
 // The same for fp16 bits.
 __device__ __forceinline__ int row_exponent_f16(uint32_t max_bits) {
   const float v = fminf(__half2float(__ushort_as_half(static_cast<uint16_t>(max_bits))), 65504.0f);
