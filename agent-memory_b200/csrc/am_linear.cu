@@ -101,7 +101,7 @@ struct FewParams {
 
 // Ring depth of a warp: what leaves room for the activations of a few thousand inputs.
 template <int MT, int TK>
-constexpr int kFewDepth = MT == 2 ? 2 : (TK == 8 ? 3 : 5);
+constexpr int kFewDepth = MT == 2 ? 2 : (TK == 8 ? 3 : 4);
 
 // D = A x B with a zero accumulator.
 __device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
