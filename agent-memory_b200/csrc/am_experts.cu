@@ -30,17 +30,15 @@ static cudaError_t launch_chained(K kfn, const P& p, dim3 grid, int threads, int
 }
 
 // ---------------------------------------------------------------- routing
-// One cluster of up to 8 CTAs, each with a contiguous part of the tokens, in one launch: a token's
-// work is a few hundred cycles of shuffles, so the launch and the barriers cost more than the data
-// (4096 tokens of 32 experts are 0.5 MB), and a second launch more than the SMs left idle.
-//
-// 1. Top-k by a team of TEAM lanes a token (TEAM * PER >= n_experts): each round takes the maximum
-//    of 64-bit keys (the logit as an ordered integer, then the complemented index: ties go to
-//    the lower one) over the team.  NaN counts as -inf.
-// 2. A stable counting sort by expert of the (token, slot) pairs: a warp walks its contiguous part
-//    32 pairs at a time (match_any ranks equal experts among the lanes) with counters per
-//    (warp, expert); the counters' prefix over warps, CTAs (distributed shared memory) and
-//    experts gives the places.
+// 1. Top-k by a warp a token: each round takes the largest logit (as an ordered integer) and the
+//    lowest index that has it, two warp reductions.  NaN counts as -inf.
+// 2. A stable counting sort by expert of the (token, slot) pairs in one cluster of up to 8 CTAs: a
+//    warp walks its contiguous part 32 pairs at a time (match_any ranks equal experts among the
+//    lanes) with counters per (warp, expert); the counters' prefix over warps, CTAs (distributed
+//    shared memory) and experts gives the places.
+// Up to 64 tokens one CTA does both.  More go through a top-k launch over all SMs first (4096
+// tokens of 32 experts: 22 us with the top-k inside the sorting cluster).  Both are bound by the
+// launch and the barriers: the data of 4096 tokens are 0.8 MB.
 __device__ __forceinline__ float load_logit(const RouteParams& p, int64_t i) {
   const float v = p.dtype == AM_DTYPE_F32 ? static_cast<const float*>(p.logits)[i]
                                           : h2f_rt(static_cast<const uint16_t*>(p.logits)[i],
@@ -62,111 +60,121 @@ __device__ __forceinline__ float weight_of(float v, float top) {
   return top == -INFINITY ? 0.0f : (v == top ? 1.0f : expf(v - top));
 }
 
-// Routes token t (t < 0: only takes part in the shuffles).  Slot j is written by lane j % TEAM.
-template <int TEAM, int PER>
+// A warp routes token t (PER * 32 >= n_experts); lane j writes slot j.
+template <int PER>
 __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lane) {
-  constexpr int SLOTS = 32 / TEAM;  // top_k <= 32
-  const int l = lane & (TEAM - 1);
   float v[PER];
-  uint64_t key[PER];  // 0: taken, or no expert
+  uint32_t key[PER];  // 0: taken, or no expert
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = i * TEAM + l;
-    v[i] = t >= 0 && e < p.n_experts ? load_logit(p, (int64_t)t * p.stride + e) : -INFINITY;
-    key[i] = e < p.n_experts ? (static_cast<uint64_t>(ordered(v[i])) << 32) | static_cast<uint32_t>(~e) : 0;
+    const int e = i * 32 + lane;
+    v[i] = e < p.n_experts ? load_logit(p, (int64_t)t * p.stride + e) : -INFINITY;
+    key[i] = e < p.n_experts ? ordered(v[i]) : 0u;
   }
-  float top = 0.0f, sum = 0.0f, mine[SLOTS];
-  int mine_e[SLOTS];
-#pragma unroll
-  for (int s = 0; s < SLOTS; ++s) {
-    mine[s] = -INFINITY;
-    mine_e[s] = 0;
-  }
+  float top = 0.0f, sum = 0.0f, my_v = -INFINITY;
+  int my_e = 0;
   for (int j = 0; j < p.top_k; ++j) {
-    uint64_t best = key[0];
+    uint32_t best = key[0];
 #pragma unroll
-    for (int i = 1; i < PER; ++i) best = key[i] > best ? key[i] : best;
+    for (int i = 1; i < PER; ++i) best = max(best, key[i]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    uint32_t at = 0xffffffffu;
 #pragma unroll
-    for (int o = TEAM / 2; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
-    }
+    for (int i = PER - 1; i >= 0; --i)
+      if (key[i] == best) at = i * 32 + lane;
+    at = __reduce_min_sync(0xffffffffu, at);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (key[i] == best) key[i] = 0;
-    const float bv = unordered(static_cast<uint32_t>(best >> 32));
+      if (i * 32 + lane == static_cast<int>(at)) key[i] = 0;
+    const float bv = unordered(best);
     if (j == 0) top = bv;
-#pragma unroll
-    for (int s = 0; s < SLOTS; ++s)
-      if (j == s * TEAM + l) {
-        mine[s] = bv;
-        mine_e[s] = static_cast<int>(~static_cast<uint32_t>(best));
-      }
+    if (j == lane) {
+      my_v = bv;
+      my_e = static_cast<int>(at);
+    }
     if (p.normalize) sum += weight_of(bv, top);
   }
   if (!p.normalize) {
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (i * TEAM + l < p.n_experts) sum += weight_of(v[i], top);
+      if (i * 32 + lane < p.n_experts) sum += weight_of(v[i], top);
 #pragma unroll
-    for (int o = TEAM / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-#pragma unroll
-  for (int s = 0; s < SLOTS; ++s) {
-    const int j = s * TEAM + l;
-    if (t >= 0 && j < p.top_k) {
-      p.experts[(int64_t)t * p.top_k + j] = mine_e[s];
-      p.weights[(int64_t)t * p.top_k + j] = sum > 0.0f ? weight_of(mine[s], top) / sum : 0.0f;
-    }
+  if (lane < p.top_k) {
+    p.experts[(int64_t)t * p.top_k + lane] = my_e;
+    p.weights[(int64_t)t * p.top_k + lane] = sum > 0.0f ? weight_of(my_v, top) / sum : 0.0f;
   }
 }
 
-// Shared memory: counters [warps][n_experts], this CTA's totals [n_experts], one word a warp.
-template <int TEAM, int PER>
-__global__ void __launch_bounds__(1024) route_kernel(const __grid_constant__ RouteParams p) {
+template <int PER>
+__global__ void __launch_bounds__(256) route_topk_kernel(const __grid_constant__ RouteParams p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (t < p.tokens) route_token<PER>(p, t, threadIdx.x & 31);
+}
+
+constexpr int kRouteHeld = 4096;  // pairs of a CTA whose expert and rank stay in shared memory
+
+// Shared memory: counters [warps][n_experts], totals and first places [n_experts], a word a warp,
+// then the held pairs' expert and rank.  PER > 0: the top-k too.
+template <int PER>
+__global__ void __launch_bounds__(1024) route_sort_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ int32_t counts[];
   const int E = p.n_experts, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int threads = blockDim.x, warps = threads >> 5;
   int32_t* totals = counts + warps * E;
-  int32_t* carry = totals + E;
+  int32_t* first = totals + E;
+  int32_t* carry = first + E;
+  int32_t* held_e = carry + 32;
   const int rank = blockIdx.x, ctas = gridDim.x;  // one cluster
   const int t0 = static_cast<int>((int64_t)p.tokens * rank / ctas);
   const int t1 = static_cast<int>((int64_t)p.tokens * (rank + 1) / ctas);
+  const int i0 = t0 * p.top_k, n = (t1 - t0) * p.top_k;
+  const bool held = n <= kRouteHeld;
+  int32_t* held_r = held_e + (held ? n : 0);
   for (int i = tid; i < warps * E; i += threads) counts[i] = 0;
   griddep_launch_dependents();
   griddep_wait();
-
-  constexpr int TEAMS = 32 / TEAM;  // of a warp
-  for (int t = t0 + warp * TEAMS; t < t1; t += warps * TEAMS) {
-    const int mine = t + lane / TEAM;
-    route_token<TEAM, PER>(p, mine < t1 ? mine : -1, lane);
+  if constexpr (PER > 0) {
+    for (int t = t0 + warp; t < t1; t += warps) route_token<PER>(p, t, lane);
   }
   __syncthreads();
 
   // places among the warp's pairs of the same expert, and the warp's counts
-  const int i0 = t0 * p.top_k, n = (t1 - t0) * p.top_k;
-  const int a = i0 + static_cast<int>((int64_t)n * warp / warps), b = i0 + static_cast<int>((int64_t)n * (warp + 1) / warps);
+  const int a = static_cast<int>((int64_t)n * warp / warps), b = static_cast<int>((int64_t)n * (warp + 1) / warps);
   int32_t* mine = counts + warp * E;
   for (int i = a; i < b; i += 32) {
     const bool live = i + lane < b;
-    const int e = live ? p.experts[i + lane] : -1;
+    const int e = live ? p.experts[i0 + i + lane] : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, e);
     const int before = __popc(same & ((1u << lane) - 1u));
-    if (live) p.positions[i + lane] = mine[e] + before;
+    if (live) {
+      const int r = mine[e] + before;
+      if (held) {
+        held_e[i + lane] = e;
+        held_r[i + lane] = r;
+      } else {
+        p.positions[i0 + i + lane] = r;
+      }
+    }
     __syncwarp();
     if (live && before == 0) mine[e] += __popc(same);
     __syncwarp();
   }
   __syncthreads();
-  // exclusive prefix over the warps; the CTA's totals
-  for (int e = tid; e < E; e += threads) {
-    int run = 0;
-    for (int w = 0; w < warps; ++w) {
-      const int c = counts[w * E + e];
-      counts[w * E + e] = run;
-      run += c;
+  // exclusive prefix over the warps (a lane a warp); the CTA's totals
+  for (int e = warp; e < E; e += warps) {
+    const int c = lane < warps ? counts[lane * E + e] : 0;
+    int incl = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
     }
-    totals[e] = run;
+    if (lane < warps) counts[lane * E + e] = incl - c;
+    if (lane == 31) totals[e] = incl;
   }
   if (ctas > 1)
     cluster_sync_all();
@@ -179,11 +187,16 @@ __global__ void __launch_bounds__(1024) route_kernel(const __grid_constant__ Rou
     const int e = e0 + tid;
     int all = 0, before = 0;
     if (e < E) {
-      const uint32_t addr = smem_u32(&totals[e]);
-      for (int c = 0; c < ctas; ++c) {
-        const int v = ctas > 1 ? __float_as_int(ld_dsmem_f32(dsmem_addr(addr, c))) : totals[e];
-        before += c < rank ? v : 0;
-        all += v;
+      if (ctas > 1) {
+        const uint32_t addr = smem_u32(&totals[e]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int v = c < ctas ? __float_as_int(ld_dsmem_f32(dsmem_addr(addr, c))) : 0;
+          before += c < rank ? v : 0;
+          all += v;
+        }
+      } else {
+        all = totals[e];
       }
     }
     int incl = all;
@@ -194,36 +207,30 @@ __global__ void __launch_bounds__(1024) route_kernel(const __grid_constant__ Rou
     }
     if (lane == 31) carry[warp] = incl;
     __syncthreads();
-    int pre = 0, sum = 0;
-    for (int w = 0; w < warps; ++w) {
-      pre += w < warp ? carry[w] : 0;
-      sum += carry[w];
-    }
-    const int start = base + pre + incl - all;
-    base += sum;
+    const int cw = lane < warps ? carry[lane] : 0;
+    const int start = base + __reduce_add_sync(0xffffffffu, lane < warp ? cw : 0) + incl - all;
+    base += __reduce_add_sync(0xffffffffu, cw);
     if (e < E) {
       if (rank == 0) p.offsets[e] = start;
-      for (int w = 0; w < warps; ++w) counts[w * E + e] += start + before;
+      first[e] = start + before;
     }
     __syncthreads();
   }
   if (rank == 0 && tid == 0) p.offsets[E] = base;
   for (int i = a + lane; i < b; i += 32) {
-    const int pos = p.positions[i] + mine[p.experts[i]];
-    p.positions[i] = pos;
-    p.order[pos] = i;
+    const int e = held ? held_e[i] : p.experts[i0 + i];
+    const int pos = (held ? held_r[i] : p.positions[i0 + i]) + mine[e] + first[e];
+    p.positions[i0 + i] = pos;
+    p.order[pos] = i0 + i;
   }
   if (ctas > 1) cluster_sync_all();  // peers have read this CTA's totals
 }
 
-template <int TEAM, int PER>
-static cudaError_t launch_route_t(const RouteParams& p, cudaStream_t stream) {
-  // a CTA for every 64 tokens; few tokens in a small CTA, whose barriers are cheaper
-  int ctas = 1;
-  while (ctas < 8 && p.tokens > ctas * 64) ctas *= 2;
-  const int threads = p.tokens * TEAM <= 256 ? 256 : 1024;
-  const int smem = (threads / 32 * p.n_experts + p.n_experts + 32) * 4;
-  auto kfn = route_kernel<TEAM, PER>;
+template <int PER>
+static cudaError_t launch_sort(const RouteParams& p, int ctas, int threads, cudaStream_t stream) {
+  const int held = std::min((p.tokens + ctas - 1) / ctas * p.top_k, kRouteHeld);
+  const int smem = (threads / 32 * p.n_experts + 2 * p.n_experts + 32 + 2 * held) * 4;
+  auto kfn = route_sort_kernel<PER>;
   if (smem > 48 * 1024) {
     const cudaError_t err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
@@ -231,12 +238,24 @@ static cudaError_t launch_route_t(const RouteParams& p, cudaStream_t stream) {
   return launch_chained(kfn, p, dim3(ctas), threads, smem, ctas, stream);
 }
 
+template <int PER>
+static cudaError_t launch_route_t(const RouteParams& p, cudaStream_t stream) {
+  // few tokens in a small CTA, whose barriers are cheaper
+  if (p.tokens <= 64) return launch_sort<PER>(p, 1, p.tokens <= 8 ? 256 : 1024, stream);
+  const cudaError_t err =
+      launch_chained(route_topk_kernel<PER>, p, dim3((p.tokens + 7) / 8), 256, 0, 1, stream);
+  if (err != cudaSuccess) return err;
+  int ctas = 1;  // a CTA for every 1024 pairs: one pair a thread
+  while (ctas < 8 && (int64_t)p.tokens * p.top_k > ctas * 1024) ctas *= 2;
+  return launch_sort<0>(p, ctas, 1024, stream);
+}
+
 cudaError_t launch_route(const RouteParams& p, cudaStream_t stream) {
-  if (p.n_experts <= 32) return launch_route_t<8, 4>(p, stream);
-  if (p.n_experts <= 64) return launch_route_t<16, 4>(p, stream);
-  if (p.n_experts <= 128) return launch_route_t<32, 4>(p, stream);
-  if (p.n_experts <= 256) return launch_route_t<32, 8>(p, stream);
-  return launch_route_t<32, 32>(p, stream);
+  if (p.n_experts <= 32) return launch_route_t<1>(p, stream);
+  if (p.n_experts <= 64) return launch_route_t<2>(p, stream);
+  if (p.n_experts <= 128) return launch_route_t<4>(p, stream);
+  if (p.n_experts <= 256) return launch_route_t<8>(p, stream);
+  return launch_route_t<32>(p, stream);
 }
 
 // ---------------------------------------------------------------- combine
