@@ -53,7 +53,6 @@ EXPORTED_SYMBOLS = (
     "am_q4_linear",
     "am_q4_expert_linear_workspace_bytes",
     "am_q4_expert_linear",
-    "am_route_experts_workspace_bytes",
     "am_route_experts",
     "am_combine_experts",
 )
@@ -218,18 +217,15 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     lib.am_q4_expert_linear.argtypes = [weight, weight, c_void_p, c_int64, c_int32, c_void_p,
                                         c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p,
                                         c_size_t, c_void_p, c_void_p]
-    lib.am_route_experts_workspace_bytes.argtypes = [c_int32, c_int32, c_int32]
     lib.am_route_experts.argtypes = [c_void_p, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
-                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                     c_size_t, c_void_p]
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     lib.am_combine_experts.argtypes = [c_void_p, c_int32, c_int64, c_int32, c_void_p, c_void_p,
                                        c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32,
                                        c_int32, c_void_p, c_void_p]
     for fn in ("am_q4_weight_pack", "am_q4_linear", "am_q4_expert_linear", "am_route_experts",
                "am_combine_experts"):
         getattr(lib, fn).restype = c_int32
-    for fn in ("am_q4_linear_workspace_bytes", "am_q4_expert_linear_workspace_bytes",
-               "am_route_experts_workspace_bytes"):
+    for fn in ("am_q4_linear_workspace_bytes", "am_q4_expert_linear_workspace_bytes"):
         getattr(lib, fn).restype = c_size_t
     ver = lib.am_abi_version()
     if ver != ABI_VERSION:

@@ -860,12 +860,9 @@ static int check_route(int32_t tokens, int32_t n_experts, int32_t top_k) {
          (int64_t)tokens * top_k <= (int64_t)INT_MAX;
 }
 
-size_t am_route_experts_workspace_bytes(int32_t, int32_t, int32_t) { return 0; }
-
 int am_route_experts(const void* logits, int32_t dtype, int64_t stride, int32_t tokens, int32_t n_experts,
                      int32_t top_k, int32_t normalize, int32_t* experts, float* weights, int32_t* offsets,
-                     int32_t* order, int32_t* positions, void* workspace, size_t workspace_bytes,
-                     void* stream) {
+                     int32_t* order, int32_t* positions, void* stream) {
   clear_error();
   if (!check_route(tokens, n_experts, top_k)) {
     set_error("am_route_experts: tokens >= 0, 1 <= top_k <= min(32, n_experts), n_experts <= 1024 and fewer "
@@ -880,11 +877,6 @@ int am_route_experts(const void* logits, int32_t dtype, int64_t stride, int32_t 
     set_error("am_route_experts: a buffer is NULL");
     return AM_ERR_INVALID;
   }
-  if (workspace_bytes < am_route_experts_workspace_bytes(tokens, n_experts, top_k)) {
-    set_error("am_route_experts: workspace of %zu bytes required",
-              am_route_experts_workspace_bytes(tokens, n_experts, top_k));
-    return AM_ERR_WORKSPACE;
-  }
   RouteParams p{};
   p.logits = logits;
   p.dtype = dtype;
@@ -898,7 +890,6 @@ int am_route_experts(const void* logits, int32_t dtype, int64_t stride, int32_t 
   p.offsets = offsets;
   p.order = order;
   p.positions = positions;
-  p.ws = static_cast<int32_t*>(workspace);
   return cuda_status(launch_route(p, static_cast<cudaStream_t>(stream)), "am_route_experts");
 }
 

@@ -57,6 +57,9 @@ int decode_active_clusters(int k_dim, int v_dim, int size);
 // Resident decode CTAs per SM on the current device for a (k_dim, v_dim) pair.
 int decode_ctas_per_sm(int k_dim, int v_dim);
 
+// SMs of the current device (looked up once per device); 0 on error.
+int sm_count(int* device);
+
 // 4-bit linear layers (am_linear.cu) and expert routing (am_experts.cu).
 cudaError_t launch_weight_pack(const void* scales, const void* biases, bool bf16, int64_t rows,
                                int groups, uint32_t* params, float* row_scale, cudaStream_t stream);

@@ -9,6 +9,17 @@
 
 namespace am {
 
+int sm_count(int* device) {
+  static int counts[64] = {};
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  *device = dev;
+  if (dev < 64) n = __atomic_load_n(&counts[dev], __ATOMIC_RELAXED);
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) __atomic_store_n(&counts[dev], n, __ATOMIC_RELAXED);
+  return n;
+}
+
 // ---------------------------------------------------------------- weight parameters
 // One warp per weight row: the row's exponent e is the smallest with every |scale| * 2^(24-e)
 // and |bias| * 2^-e at most 2^15 (fp16 holds up to 65504), then the groups' pairs are scaled by
@@ -491,10 +502,10 @@ constexpr int kFewSmem = 227 * 1024;
 template <bool GATED, int MT, int TK>
 static cudaError_t launch_few_t(FewParams& f, int64_t items, cudaStream_t stream) {
   const LinearParams& p = f.p;
-  int dev = 0, sms = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (err != cudaSuccess) return err;
+  int dev = 0;
+  const int sms = sm_count(&dev);
+  if (sms == 0) return cudaErrorInvalidDevice;
+  cudaError_t err = cudaSuccess;
   static unsigned long long done = 0;
   auto kfn = linear_few_kernel<GATED, MT, TK>;
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0;

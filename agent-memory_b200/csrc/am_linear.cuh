@@ -42,7 +42,6 @@ struct RouteParams {
   int32_t* offsets;
   int32_t* order;
   int32_t* positions;
-  int32_t* ws;
 };
 
 struct CombineParams {

@@ -509,10 +509,10 @@ int linear_token_tile(int rows, int experts, bool grouped) {
 template <int NT, bool GATED>
 static cudaError_t launch_tiles_t(const LinearParams& p, int64_t items, cudaStream_t stream) {
   using LY = TilesLayout<NT>;
-  int dev = 0, sms = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (err != cudaSuccess) return err;
+  int dev = 0;
+  const int sms = sm_count(&dev);
+  if (sms == 0) return cudaErrorInvalidDevice;
+  cudaError_t err = cudaSuccess;
   auto kfn = linear_tiles_kernel<NT, GATED>;
   static unsigned long long done = 0;
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0;

@@ -20,7 +20,8 @@ import torch
 from . import _lib
 from ._lib import check
 from .kernels import _half_code, dtype_code
-from .linear import (Q4Weight, _check_pair, _out, _raw_stream, _row_stride, _rows_of, _workspace)
+from .linear import (Q4Weight, _check_out, _check_pair, _current_device, _raw_stream, _row_stride,
+                     _rows_of)
 
 MAX_EXPERTS, MAX_TOP_K = 1024, 32
 
@@ -41,7 +42,7 @@ class ExpertRouting(NamedTuple):
 
 
 def _int32(t: torch.Tensor, shape, device, what: str) -> torch.Tensor:
-    if t.dtype is not torch.int32 or tuple(t.shape) != tuple(shape) or t.device != device:
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device:
         raise ValueError(f"{what} must be int32 {tuple(shape)} on {device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return t if t.is_contiguous() else t.contiguous()
@@ -75,7 +76,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, normalize: bool = True) -
         raise RuntimeError("route_experts has no backward pass: detach the logits or use no_grad")
     if logits.stride(1) != 1 or (tokens > 1 and logits.stride(0) < n_experts):
         logits = logits.contiguous()
-    if dev.index != torch.cuda.current_device():
+    if dev.index != _current_device():
         with torch.cuda.device(dev):
             return _route_call(logits, tokens, n_experts, top_k, normalize, dev)
     return _route_call(logits, tokens, n_experts, top_k, normalize, dev)
@@ -86,25 +87,22 @@ def _route_call(logits, tokens, n_experts, top_k, normalize, dev):
     # one buffer: experts, positions, order, offsets
     buf = torch.empty(3 * pairs + n_experts + 1, dtype=torch.int32, device=dev)
     weights = torch.empty(tokens, top_k, dtype=torch.float32, device=dev)
-    experts = buf[:pairs].view(tokens, top_k)
-    positions = buf[pairs:2 * pairs].view(tokens, top_k)
-    order, offsets = buf[2 * pairs:3 * pairs], buf[3 * pairs:]
     base = buf.data_ptr()
-    lib = _lib.load()
-    need = int(lib.am_route_experts_workspace_bytes(tokens, n_experts, top_k))
-    ws = _workspace(need, dev)
-    rc = lib.am_route_experts(logits.data_ptr(), dtype_code(logits.dtype), _row_stride(logits), tokens,
-                              n_experts, top_k, 1 if normalize else 0, base, weights.data_ptr(),
-                              base + 12 * pairs, base + 8 * pairs, base + 4 * pairs,
-                              ws.data_ptr() if ws is not None else None, need,
-                              _raw_stream(dev.index))
+    rc = _lib.load().am_route_experts(
+        logits.data_ptr(), dtype_code(logits.dtype), _row_stride(logits), tokens, n_experts, top_k,
+        1 if normalize else 0, base, weights.data_ptr(), base + 12 * pairs, base + 8 * pairs,
+        base + 4 * pairs, _raw_stream(dev.index))
     if rc:
         check("am_route_experts", rc)
-    return ExpertRouting(experts, weights, offsets, order, positions)
+    shape, strides = (tokens, top_k), (top_k, 1)
+    return ExpertRouting(buf.as_strided(shape, strides, 0), weights,
+                         buf.as_strided((n_experts + 1,), (1,), 3 * pairs),
+                         buf.as_strided((pairs,), (1,), 2 * pairs),
+                         buf.as_strided(shape, strides, pairs))
 
 
 def _expert_linear(x, w: Q4Weight, up, routing: ExpertRouting, gather: bool, out, status):
-    if w.codes.dim() != 3:
+    if not w.grouped:
         raise ValueError(f"{w} is one matrix: use quantized_matmul / quantized_swiglu")
     if x.dim() != 2:
         raise ValueError(f"x must be [rows, {w.n_in}], got {tuple(x.shape)}")
@@ -119,27 +117,25 @@ def _expert_linear(x, w: Q4Weight, up, routing: ExpertRouting, gather: bool, out
             raise ValueError(f"x has {x.shape[0]} tokens, the routing {rows} rows of {top_k} each")
     elif x.shape[0] != rows:
         raise ValueError(f"x has {x.shape[0]} rows, the routing {rows}")
-    if w.index != torch.cuda.current_device():
+    if w.index != _current_device():
         with torch.cuda.device(w.device):
             return _expert_call(x, w, up, offsets, order, top_k, rows, out, status)
     return _expert_call(x, w, up, offsets, order, top_k, rows, out, status)
 
 
 def _expert_call(x, w, up, offsets, order, top_k, rows, out, status):
-    out = _out(out, rows, w, (rows, w.n_out))
+    if out is not None:
+        _check_out(out, w, (rows, w.n_out))
+    else:
+        out = torch.empty(rows, w.n_out, dtype=w.dtype, device=w.device)
     lib = _lib.load()
-    key = (up is not None, rows)
-    need = w.bytes_cache.get(key)
     up_ref = up.ref if up is not None else None
-    if need is None:
-        need = w.bytes_cache[key] = int(
-            lib.am_q4_expert_linear_workspace_bytes(w.ref, up_ref, rows))
-    ws = _workspace(need, w.device)
+    need = int(lib.am_q4_expert_linear_workspace_bytes(w.ref, up_ref, rows))
+    ws = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
     rc = lib.am_q4_expert_linear(w.ref, up_ref, x.data_ptr(), _row_stride(x), x.shape[0],
                                  offsets.data_ptr(), order.data_ptr() if order is not None else None,
-                                 top_k, rows, out.data_ptr(), w.n_out,
-                                 ws.data_ptr() if ws is not None else None, need,
-                                 _status_ptr(status, w.device), _raw_stream(w.index))
+                                 top_k, rows, out.data_ptr(), w.n_out, ws.data_ptr() if need else None,
+                                 need, _status_ptr(status, w.device), _raw_stream(w.index))
     if rc:
         check("am_q4_expert_linear", rc)
     return out
@@ -174,38 +170,41 @@ def combine_experts(y: torch.Tensor, weights: torch.Tensor, positions: torch.Ten
         raise ValueError("y must be [rows, width] and positions [tokens, top_k]")
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
         raise RuntimeError("combine_experts has no backward pass: detach its inputs or use no_grad")
-    dev, (tokens, top_k), width = y.device, positions.shape, y.shape[1]
+    dev, shape, width = y.device, positions.shape, y.shape[1]
+    tokens, top_k = shape
     if top_k == 0:
         raise ValueError("positions must hold at least one slot a token")
-    positions = _int32(positions, (tokens, top_k), dev, "positions")
-    if weights.dtype is not torch.float32 or weights.shape != positions.shape or weights.device != dev:
-        raise ValueError(f"weights must be float32 {(tokens, top_k)} on {dev}")
-    weights = weights if weights.is_contiguous() else weights.contiguous()
+    positions = _int32(positions, shape, dev, "positions")
+    if weights.dtype is not torch.float32 or weights.shape != shape or weights.device != dev:
+        raise ValueError(f"weights must be float32 {tuple(shape)} on {dev}")
+    if not weights.is_contiguous():
+        weights = weights.contiguous()
     code = _half_code(y.dtype)
-
-    def rows(t):
-        return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
-
-    y = rows(y)
+    y = _dense_rows(y, width)
+    res, res_stride = None, 0
     if residual is not None:
         if residual.shape != (tokens, width) or residual.dtype is not y.dtype or residual.device != dev:
             raise ValueError(f"residual must be {y.dtype} {(tokens, width)} on {dev}")
-        residual = rows(residual)
+        residual = _dense_rows(residual, width)
+        res, res_stride = residual.data_ptr(), _row_stride(residual)
     if out is None:
         out = torch.empty(tokens, width, dtype=y.dtype, device=dev)
     elif (out.shape != (tokens, width) or out.dtype is not y.dtype or out.device != dev
           or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous {y.dtype} tensor {(tokens, width)} on {dev}")
     args = (y.data_ptr(), code, _row_stride(y), y.shape[0], weights.data_ptr(), positions.data_ptr(),
-            residual.data_ptr() if residual is not None else None,
-            _row_stride(residual) if residual is not None else 0, out.data_ptr(), width, tokens, top_k,
-            width, _status_ptr(status, dev), _raw_stream(dev.index))
-    lib = _lib.load()
-    if dev.index != torch.cuda.current_device():
+            res, res_stride, out.data_ptr(), width, tokens, top_k, width, _status_ptr(status, dev),
+            _raw_stream(dev.index))
+    if dev.index != _current_device():
         with torch.cuda.device(dev):
-            rc = lib.am_combine_experts(*args)
+            rc = _lib.load().am_combine_experts(*args)
     else:
-        rc = lib.am_combine_experts(*args)
+        rc = _lib.load().am_combine_experts(*args)
     if rc:
         check("am_combine_experts", rc)
     return out
+
+
+def _dense_rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    stride = t.stride()
+    return t if stride[1] == 1 and (stride[0] >= width or t.shape[0] <= 1) else t.contiguous()

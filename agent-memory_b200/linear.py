@@ -24,6 +24,8 @@ from ._lib import Q4WeightDesc, check
 from .kernels import GROUP_SIZE, _check_params, _half_code, as_codes, _require_cuda
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+FEW_TOKENS = 8  # a single matrix with at most so many tokens needs no workspace
 
 
 class Q4Weight:
@@ -35,7 +37,7 @@ class Q4Weight:
     biases are packed into a buffer of the same size on the current stream."""
 
     __slots__ = ("codes", "params", "row_scale", "dtype", "device", "index", "n_out", "n_in",
-                 "experts", "desc", "ref", "bytes_cache")
+                 "experts", "grouped", "desc", "ref")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
                  group_size: int = 64, bits: int = 4):
@@ -50,7 +52,8 @@ class Q4Weight:
             raise TypeError("scales and biases must share one dtype")
         self.dtype = scales.dtype
         self.n_out, self.n_in = codes.shape[-2], codes.shape[-1] * 8
-        self.experts = codes.shape[0] if codes.dim() == 3 else 1
+        self.grouped = codes.dim() == 3
+        self.experts = codes.shape[0] if self.grouped else 1
         if self.n_in == 0 or self.n_in % GROUP_SIZE or self.n_out == 0 or self.experts == 0:
             raise ValueError(f"a weight of {self.experts} x {self.n_out} x {self.n_in} needs n_in a "
                              f"positive multiple of {GROUP_SIZE} and no empty dimension")
@@ -74,27 +77,27 @@ class Q4Weight:
         d.n_out, d.n_in, d.experts, d.dtype = self.n_out, self.n_in, self.experts, _half_code(self.dtype)
         self.desc = d
         self.ref = ctypes.byref(d)
-        self.bytes_cache: dict = {}
 
     def __repr__(self) -> str:
-        e = f"{self.experts} x " if self.codes.dim() == 3 else ""
+        e = f"{self.experts} x " if self.grouped else ""
         return f"Q4Weight({e}{self.n_out} x {self.n_in}, {self.dtype}, {self.device})"
 
 
 def _rows_of(x: torch.Tensor, w: Q4Weight) -> torch.Tensor:
     """x as rows [M, n_in] the kernels can read (a copy only where the strides need one)."""
-    if x.shape[-1] != w.n_in:
-        raise ValueError(f"x has {x.shape[-1]} inputs, the weight {w.n_in}")
+    shape = x.shape
+    if shape[-1] != w.n_in:
+        raise ValueError(f"x has {shape[-1]} inputs, the weight {w.n_in}")
     if x.dtype is not w.dtype:
         raise TypeError(f"x must be {w.dtype} like the weight's scales, got {x.dtype}")
     if x.device != w.device:
         raise ValueError(f"x is on {x.device}, the weight on {w.device} (no CPU path)")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("4-bit linear layers have no backward pass: detach x or use no_grad")
-    if x.dim() != 2:
+    if len(shape) != 2:
         x = x.reshape(-1, w.n_in)
-    st = x.stride()
-    if st[1] != 1 or (st[0] % 8 and x.shape[0] > 1) or x.data_ptr() % 16:
+    stride = x.stride()
+    if stride[1] != 1 or x.data_ptr() % 16 or (stride[0] % 8 and x.shape[0] > 1):
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
@@ -106,49 +109,43 @@ def _row_stride(x: torch.Tensor) -> int:
 
 
 def _check_pair(w: Q4Weight, up: Q4Weight) -> None:
-    if (up.n_out, up.n_in, up.experts, up.dtype, up.device) != (w.n_out, w.n_in, w.experts, w.dtype,
-                                                                w.device):
+    if (up.n_out != w.n_out or up.n_in != w.n_in or up.experts != w.experts or up.dtype is not w.dtype
+            or up.device != w.device):
         raise ValueError(f"the matrices of a gated layer must be alike, got {w} and {up}")
 
 
-def _out(out, rows: int, w: Q4Weight, shape) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=w.dtype, device=w.device)
+def _check_out(out: torch.Tensor, w: Q4Weight, shape) -> None:
     if (tuple(out.shape) != tuple(shape) or out.dtype is not w.dtype or out.device != w.device
             or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous {w.dtype} tensor {tuple(shape)} on {w.device}")
-    return out
-
-
-def _workspace(nbytes: int, device):
-    """Scratch of one call from the caching allocator, on the call's stream."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _linear(x: torch.Tensor, w: Q4Weight, up: Q4Weight | None, out):
-    if w.codes.dim() != 2:
+    if w.grouped:
         raise ValueError(f"{w} holds one matrix per expert: use expert_matmul / expert_swiglu")
-    lead = x.shape[:-1]
-    x = _rows_of(x, w)
-    rows = x.shape[0]
-    if w.index != torch.cuda.current_device():
+    rows2 = _rows_of(x, w)
+    if w.index != _current_device():
         with torch.cuda.device(w.device):
-            return _linear_call(x, w, up, out, rows, lead)
-    return _linear_call(x, w, up, out, rows, lead)
+            return _linear_call(x, rows2, w, up, out)
+    return _linear_call(x, rows2, w, up, out)
 
 
-def _linear_call(x, w, up, out, rows, lead):
-    out = _out(out, rows, w, (*lead, w.n_out))
+def _linear_call(x, rows2, w, up, out):
+    rows = rows2.shape[0]
+    if out is not None:
+        _check_out(out, w, (*x.shape[:-1], w.n_out))
+    elif x.dim() == 2:
+        out = torch.empty(rows, w.n_out, dtype=w.dtype, device=w.device)
+    else:
+        out = torch.empty(*x.shape[:-1], w.n_out, dtype=w.dtype, device=w.device)
     lib = _lib.load()
-    key = (up is not None, rows)
-    need = w.bytes_cache.get(key)
     up_ref = up.ref if up is not None else None
-    if need is None:
-        need = w.bytes_cache[key] = int(lib.am_q4_linear_workspace_bytes(w.ref, up_ref, rows))
-    ws = _workspace(need, w.device)
-    rc = lib.am_q4_linear(w.ref, up_ref, x.data_ptr(), _row_stride(x), rows, out.data_ptr(), w.n_out,
-                          ws.data_ptr() if ws is not None else None, need, None,
-                          _raw_stream(w.index))
+    need, ws = 0, None
+    if rows > FEW_TOKENS:  # (scratch of the call from the caching allocator, on the call's stream)
+        need = int(lib.am_q4_linear_workspace_bytes(w.ref, up_ref, rows))
+        ws = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
+    rc = lib.am_q4_linear(w.ref, up_ref, rows2.data_ptr(), _row_stride(rows2), rows, out.data_ptr(),
+                          w.n_out, ws.data_ptr() if need else None, need, None, _raw_stream(w.index))
     if rc:
         check("am_q4_linear", rc)
     return out

@@ -344,11 +344,10 @@ int am_q4_expert_linear(const am_q4_weight* w, const am_q4_weight* up, const voi
  * (token, slot) pairs t * top_k + j sorted by expert, equal ones in rising order, and
  * positions[t, j] the place of pair (t, j) in it.  n_experts <= 1024, top_k <= 32.
  */
-size_t am_route_experts_workspace_bytes(int32_t tokens, int32_t n_experts, int32_t top_k);
 int am_route_experts(const void* logits, int32_t dtype, int64_t stride, int32_t tokens,
                      int32_t n_experts, int32_t top_k, int32_t normalize, int32_t* experts,
                      float* weights, int32_t* offsets, int32_t* order, int32_t* positions,
-                     void* workspace, size_t workspace_bytes, void* stream);
+                     void* stream);
 
 /*
  * out[t] = residual[t] + sum over j of weights[t, j] * y[positions[t, j]] (fp32 sum in slot
