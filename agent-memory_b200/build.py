@@ -19,7 +19,7 @@ INCLUDE = REPO / "include"
 OUT = PKG_DIR / "libamq4.so"
 
 SOURCES = ["am_abi.cu", "am_quantize.cu", "am_decode.cu", "am_prefill.cu", "am_noalloc.cu",
-           "am_blocks.cu", "am_linear.cu", "am_linear_tc.cu",
+           "am_blocks.cu", "am_linear.cu", "am_linear_tc.cu", "am_linear_pair.cu",
            "am_experts.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -814,16 +814,18 @@ static int run_linear(LinearParams& p, void* workspace, size_t workspace_bytes, 
   p.xh = static_cast<uint16_t*>(workspace);
   p.xscale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)p.rows * p.n_in * 2);
   p.wait_ns = wait_limit_ns();
-  const int tile = linear_token_tile(p.rows, p.experts, grouped);
+  const bool gated = p.codes[1] != nullptr;
+  const bool pairs = linear_uses_pairs(p.rows, p.experts, p.n_out, grouped, gated);
+  const int tile = pairs ? 128 : linear_token_tile(p.rows, p.experts, grouped);
   bool ok = encode_rows_map(&p.tmap_x, p.xh, p.rows, (int64_t)p.n_in * 2, tile);
   for (int i = 0; i < 2 && ok; ++i)
     if (p.codes[i] != nullptr)
-      ok = encode_rows_map(&p.tmap_w[i], p.codes[i], (int64_t)p.experts * p.n_out, p.n_in / 2, 128);
+      ok = encode_rows_map(&p.tmap_w[i], p.codes[i], (int64_t)p.experts * p.n_out, p.n_in / 2, pairs ? 64 : 128);
   if (!ok) {
     set_error("%s: cannot describe the operands to the TMA unit (cuTensorMapEncodeTiled is required)", fn);
     return AM_ERR_CUDA;
   }
-  return cuda_status(launch_linear_tiles(p, static_cast<cudaStream_t>(stream)), fn);
+  return cuda_status(launch_linear_tiles(p, pairs, static_cast<cudaStream_t>(stream)), fn);
 }
 
 int am_q4_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, int64_t x_stride, int32_t rows,

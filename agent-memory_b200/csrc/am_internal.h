@@ -69,7 +69,10 @@ bool linear_uses_tensor_tiles(int rows, int experts, bool grouped);
 // Rows of a token tile of the tensor-tile kernel for a call (the x map's box rows).
 int linear_token_tile(int rows, int experts, bool grouped);
 cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream);
-cudaError_t launch_linear_tiles(const LinearParams& p, cudaStream_t stream);
+bool linear_uses_pairs(int rows, int experts, int n_out, bool grouped, bool gated);
+cudaError_t launch_linear_tiles(const LinearParams& p, bool pairs, cudaStream_t stream);
+// Tiles of pairs of SMs (am_linear_pair.cu), after the activations' rows are written.
+cudaError_t launch_linear_pair(const LinearParams& p, cudaStream_t stream);
 cudaError_t launch_route(const RouteParams& p, cudaStream_t stream);
 cudaError_t launch_combine(const CombineParams& p, cudaStream_t stream);
 

@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   }
   griddep_wait();
   if (p.offsets != nullptr) {
-    items = count_items<kFewTokens>(p);
+    items = count_items(p, kFewTokens);
     share();
   }
 
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   int l_rows = 0;      // weight rows from the tile's first one to the matrix's end
   auto l_open = [&]() {  // position l_pos of item l_item
     int lo, hi;
-    const int e = find_item<kFewTokens>(p, l_item, lo, hi);
+    const int e = find_item(p, l_item, kFewTokens, lo, hi);
     const int first = (l_pos * wr_n + wr) * TROWS;
     const int64_t row = (int64_t)max(e, 0) * p.n_out + first;
     l_rows = p.n_out - first;
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   while (left > 0) {
     // a batch: positions of one item
     if (it != item) {
-      e = find_item<kFewTokens>(p, it, lo, hi);
+      e = find_item(p, it, kFewTokens, lo, hi);
       item = it;
       m = hi - lo;
       stage_x();  // (the last batch ended with a barrier after its last read of the activations)

@@ -123,27 +123,25 @@ __device__ __forceinline__ uint4 permute_bf16(uint4 u, float f) {
                     pack_half2(hi(u.y), hi(u.w)));
 }
 
-// Work items of a call: pieces of at most TOK rows of one expert.  The warp's lanes agree.
-template <int TOK>
-__device__ __forceinline__ int count_items(const LinearParams& p) {
-  if (p.offsets == nullptr) return (p.rows + TOK - 1) / TOK;
+// Work items of a call: pieces of at most `tok` rows of one expert.  The warp's lanes agree.
+__device__ __forceinline__ int count_items(const LinearParams& p, int tok) {
+  if (p.offsets == nullptr) return (p.rows + tok - 1) / tok;
   const int lane = threadIdx.x & 31;
   int n = 0;
   for (int e = lane; e < p.experts; e += 32) {
     int a, b;
     expert_range(p, e, a, b);
-    n += (b - a + TOK - 1) / TOK;
+    n += (b - a + tok - 1) / tok;
   }
   return __reduce_add_sync(0xffffffffu, n);
 }
 
 // Item `item`: rows [lo, hi) of one expert.  Returns the expert, or -1 past the last item.  All
 // lanes of a warp call it.
-template <int TOK>
-__device__ __forceinline__ int find_item(const LinearParams& p, int item, int& lo, int& hi) {
+__device__ __forceinline__ int find_item(const LinearParams& p, int item, int tok, int& lo, int& hi) {
   if (p.offsets == nullptr) {
-    lo = item * TOK;
-    hi = min(lo + TOK, p.rows);
+    lo = item * tok;
+    hi = min(lo + tok, p.rows);
     return lo < hi ? 0 : -1;
   }
   // each warp scans the experts, 32 at a time
@@ -152,7 +150,7 @@ __device__ __forceinline__ int find_item(const LinearParams& p, int item, int& l
   for (int e0 = 0; e0 < p.experts; e0 += 32) {
     int a = 0, b = 0;
     if (e0 + lane < p.experts) expert_range(p, e0 + lane, a, b);
-    const int n = (b - a + TOK - 1) / TOK;
+    const int n = (b - a + tok - 1) / tok;
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -163,9 +161,9 @@ __device__ __forceinline__ int find_item(const LinearParams& p, int item, int& l
     if (item < base + total) {
       const bool mine = item >= base + incl - n && item < base + incl;
       const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
-      const int first = a + (item - (base + incl - n)) * TOK;
+      const int first = a + (item - (base + incl - n)) * tok;
       lo = __shfl_sync(0xffffffffu, first, src);
-      hi = min(__shfl_sync(0xffffffffu, b, src), lo + TOK);
+      hi = min(__shfl_sync(0xffffffffu, b, src), lo + tok);
       return e0 + src;
     }
     base += total;

@@ -1,0 +1,510 @@
+// Linear layers over 4-bit weights for many tokens: tcgen05 on pairs of SMs (cta_group::2).
+//
+// The tiles of am_linear_tc.cu with twice the tokens: two CTAs of a cluster share one product of 256
+// weight rows x up to 256 tokens.  Each dequantizes 128 of the rows into its own TMEM and loads
+// half of the tokens' activations; the leader's MMAs (M = 256) read the operands of both.  A
+// weight is dequantized once for 256 tokens instead of 128, and an activation is brought into
+// shared memory and read from it for 256 weight rows by each SM: at the power cap that these sizes
+// run at, the work saved beside the MMAs is clock rate gained for them.
+//
+// Per CTA: one thread streams the codes (plain: 128 rows of the matrix; gated: 64 rows of each, so
+// that a row's gate and its partner lie 64 TMEM lanes apart in the same CTA), one the
+// activations; their full barrier and that of the dequantized operand are the leader's.  8
+// warps dequantize (two groups of 4, a 64-input slab each) and write the output: TMEM holds the
+// 256-column accumulator and eight operand slabs.  The MMA shape follows the item: N is its tokens
+// rounded up to 32.  Waits are bounded as in am_linear_tc.cu; the CTAs of a pair leave together.
+#include <algorithm>
+#include <climits>
+
+#include "am_internal.h"
+#include "am_linear.cuh"
+#include "am_tcgen05.cuh"
+
+namespace am {
+
+namespace tc2 {
+
+// D (TMEM of both CTAs) [+]= A (TMEM of both, 128 rows each) x B (shared memory of both, N / 2 rows
+// each, at the same offset).  Issued by the leader.
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t id, uint32_t accum) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b), "r"(id), "r"(accum));
+}
+
+// Arrive on both CTAs' copy of `bar` once every MMA this thread issued before has completed.
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+// Tile load into this CTA's shared memory that completes on the leader's copy of `bar`.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar & 0xFEFFFFFFu)
+      : "memory");
+}
+
+// Arrive on an mbarrier of the cluster (address from mapa), releasing to the cluster.
+__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
+}
+
+// wait_or_abort on a barrier that the peer CTA arrives on too.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, uint64_t limit_ns, const volatile int* abort_flag) {
+  if (limit_ns == 0) return false;
+  constexpr uint32_t kSuspendNs = 100000;
+  uint64_t t0 = 0;
+  for (uint32_t it = 0;; ++it) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n"
+        "selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "r"(kSuspendNs)
+        : "memory");
+    if (done) return true;
+    if (*abort_flag) return false;
+    if (it == 0) {
+      t0 = globaltimer_ns();
+    } else if (globaltimer_ns() - t0 > limit_ns) {
+      return false;
+    }
+  }
+}
+
+// Whether any of the `count` threads that meet at named barrier `id` passes true.
+__device__ __forceinline__ bool any_of_group(int id, bool v, int count) {
+  uint32_t r;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, %2, %3, p;\n"
+      "selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(v)), "r"(id), "r"(count)
+      : "memory");
+  return r != 0;
+}
+
+}  // namespace tc2
+
+struct PairLayout {
+  static constexpr int CS = 4, XS = 4, AB = 4, SP = 2, DW = 8;  // AB: steps of SP slabs
+  static constexpr int THREADS = 32 * (DW + 3);                  // + codes, activations, MMA
+  static constexpr int CSTAGE = 128 * 128;                       // 128 rows x 256 inputs
+  static constexpr int XSLAB = 128 * 128;                        // 128 tokens x 64 inputs
+  static constexpr int OFF_C = 0;
+  static constexpr int OFF_X = OFF_C + CS * CSTAGE;
+  static constexpr int OFF_OUT = OFF_X + XS * SP * XSLAB;        // 1 KB a warp
+  static constexpr int OFF_SWAP = OFF_OUT + DW * 1024;           // two buffers of 2 KB a pair of warps
+  static constexpr int OFF_SCALE = OFF_SWAP + 4 * 2 * 2048;      // two tiles' token scales
+  static constexpr int OFF_BAR = OFF_SCALE + 2 * 256 * 4;
+  static constexpr int B_CFULL = 0, B_CEMPTY = CS, B_XFULL = 2 * CS, B_XEMPTY = B_XFULL + XS;
+  static constexpr int B_AFULL = B_XEMPTY + XS, B_AEMPTY = B_AFULL + AB, B_DFULL = B_AEMPTY + AB;
+  static constexpr int B_DEMPTY = B_DFULL + 1, B_SFULL = B_DEMPTY + 1, B_SEMPTY = B_SFULL + 2;
+  static constexpr int B_DRAIN = B_SEMPTY + 2, B_COUNT = B_DRAIN + 1;
+  static constexpr int SMEM = OFF_BAR + B_COUNT * 8 + 16;
+  static constexpr int A_COL = 256;  // D at 0, A[step][slab] at A_COL + 32 (2 step + slab)
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
+  static __device__ int arrivals(int i) {
+    if (i >= B_CEMPTY && i < B_CEMPTY + CS) return DW;
+    if (i >= B_AFULL && i < B_AFULL + AB) return 2 * DW;  // (the leader's: both CTAs' warps)
+    if (i == B_DEMPTY) return 2 * DW;
+    if (i >= B_SEMPTY && i < B_SEMPTY + 2) return DW;
+    return 1;
+  }
+};
+
+struct PairParams {
+  LinearParams p;
+  int32_t row_tiles;    // tiles of 256 weight rows (gated: 128 of each matrix)
+  int32_t tile_tokens;  // tokens of an item, at most: a multiple of 32 up to 256
+};
+
+template <int N>
+struct PairRing {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      ph ^= 1u;
+    }
+  }
+};
+
+template <bool GATED>
+__global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams f) {
+  using LY = PairLayout;
+  constexpr int CS = LY::CS, XS = LY::XS, AB = LY::AB, SP = LY::SP, DW = LY::DW;
+  constexpr int CODES_WARP = DW, X_WARP = DW + 1, MMA_WARP = DW + 2;
+  constexpr int CTA_ROWS = GATED ? 64 : 128;  // output rows of a CTA
+  const LinearParams& p = f.p;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t s_base = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + LY::OFF_BAR);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + LY::OFF_BAR + LY::B_COUNT * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + LY::OFF_BAR + LY::B_COUNT * 8 + 4);
+  float* tok_scale = reinterpret_cast<float*>(smem + LY::OFF_SCALE);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  auto wait = [&](int i, uint32_t parity) { return wait_or_abort(bar(i), parity, p.wait_ns, abort_flag); };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  griddep_launch_dependents();
+  if (s_base & 1023u) {  // swizzled tiles need a 1024-byte aligned window (the whole grid returns)
+    if (tid == 0) flag_status(p.status, AM_STATUS_BAD_POSITION);
+    return;
+  }
+  const int rank = static_cast<int>(blockIdx.x) & 1;
+  const int first = static_cast<int>(blockIdx.x) >> 1, step = static_cast<int>(gridDim.x) >> 1;
+  const int tiles = count_items(p, f.tile_tokens) * f.row_tiles;
+  if (first >= tiles) return;  // both CTAs of the pair
+  const int stages = p.pstride >> 2;  // quads of groups
+  const int slabs = p.groups, steps = (slabs + SP - 1) / SP;
+
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::);
+  } else if (warp == CODES_WARP) {
+    for (int i = lane; i < LY::B_COUNT; i += 32) mbar_init(bar(i), LY::arrivals(i));
+    if (lane == 0) *abort_flag = 0;
+    fence_mbar_init();
+  }
+  tc::fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before either arrives on the other's
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  int issued_c = 0, issued_x = 0;  // loads issued (their own threads' counts)
+  bool mma_issued = false;
+  bool ok = true;
+  if (warp == CODES_WARP) {
+    PairRing<CS> ring;
+    for (int tile = first; tile < tiles && ok; tile += step) {
+      int lo, hi;
+      const int e = find_item(p, tile / f.row_tiles, f.tile_tokens, lo, hi);
+      const int y = e * p.n_out + tile % f.row_tiles * 2 * CTA_ROWS + rank * CTA_ROWS;
+      if (lane == 0) {
+        for (int c = 0; c < stages; ++c) {
+          ok = wait(LY::B_CEMPTY + ring.s, ring.ph ^ 1u);
+          if (!ok) break;
+          const uint32_t full = bar(LY::B_CFULL + ring.s), dst = s_base + LY::OFF_C + ring.s * LY::CSTAGE;
+          mbar_arrive_expect_tx(full, LY::CSTAGE);
+          am::tma_load_2d(dst, &p.tmap_w[0], c * 128, y, full);
+          am::tma_load_2d(dst + LY::CSTAGE / 2, &p.tmap_w[GATED ? 1 : 0], c * 128, GATED ? y : y + 64, full);
+          ++issued_c;
+          ring.next();
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+  } else if (warp == X_WARP) {
+    griddep_wait();  // the activations are written
+    PairRing<XS> ring;
+    int k = 0;
+    for (int tile = first; tile < tiles && ok; tile += step, ++k) {
+      int lo, hi;
+      find_item(p, tile / f.row_tiles, f.tile_tokens, lo, hi);
+      const int half = ((hi - lo + 31) & ~31) >> 1;  // tokens of a CTA
+      const int y = lo + rank * half;
+      for (int i = 0; i < steps; ++i) {
+        ok = __all_sync(0xffffffffu, wait(LY::B_XEMPTY + ring.s, ring.ph ^ 1u));
+        if (!ok) break;
+        const uint32_t dst = s_base + LY::OFF_X + ring.s * SP * LY::XSLAB;
+        const int n = min(SP, slabs - i * SP);
+        if (lane == 0) {
+          const uint32_t full = bar(LY::B_XFULL + ring.s);
+          if (rank == 0) mbar_arrive_expect_tx(full, 2 * n * LY::XSLAB);  // both CTAs' bytes
+          for (int s = 0; s < n; ++s) tc2::tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, (i * SP + s) * 128, y, full);
+        }
+        ++issued_x;
+        ring.next();
+        if (i == min(XS, steps) - 1) {  // behind the first loads: the tokens' powers of two
+          const int b = k & 1;
+          ok = __all_sync(0xffffffffu, wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1));
+          if (!ok) break;
+          for (int j = lane; j < 256; j += 32) tok_scale[b * 256 + j] = lo + j < hi ? p.xscale[lo + j] : 0.0f;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(LY::B_SFULL + b));
+        }
+      }
+    }
+  } else if (warp == MMA_WARP) {
+    PairRing<XS> xr;
+    PairRing<AB> ar;
+    uint32_t dph = 1;
+    for (int tile = first; tile < tiles && ok && rank == 0; tile += step, dph ^= 1u) {
+      int lo, hi;
+      find_item(p, tile / f.row_tiles, f.tile_tokens, lo, hi);
+      const uint32_t id = tc::idesc(256, (hi - lo + 31) & ~31, false);
+      if (lane == 0) {
+        ok = tc2::wait_cluster(bar(LY::B_DEMPTY), dph, p.wait_ns, abort_flag);
+        for (int i = 0; i < steps && ok; ++i) {
+          ok = wait(LY::B_XFULL + xr.s, xr.ph) &&
+               tc2::wait_cluster(bar(LY::B_AFULL + ar.s), ar.ph, p.wait_ns, abort_flag);
+          if (!ok) break;
+          tc::fence_after();
+          const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + xr.s * SP * LY::XSLAB, 16, 1024);
+          const uint32_t a = tmem + LY::A_COL + ar.s * 64;
+          // (descriptor addresses count 16-byte units: 32 bytes of a swizzled row are 16 inputs)
+          tc2::mma_ts(tmem, a, xd, id, i > 0 ? 1u : 0u);
+#pragma unroll
+          for (int ks = 1; ks < 4; ++ks) tc2::mma_ts(tmem, a + ks * 8, xd + ks * 2, id, 1u);
+          if (2 * i + 1 < slabs) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) tc2::mma_ts(tmem, a + 32 + ks * 8, xd + LY::XSLAB / 16 + ks * 2, id, 1u);
+          }
+          mma_issued = true;
+          tc2::commit(bar(LY::B_XEMPTY + xr.s));
+          tc2::commit(bar(LY::B_AEMPTY + ar.s));
+          xr.next();
+          ar.next();
+        }
+        if (ok) tc2::commit(bar(LY::B_DFULL));
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+  } else {
+    // ---- dequantization (as in linear_tiles_kernel): a weight row a thread, slab `group` of every step
+    const int group = warp >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const int which = GATED ? quarter >> 1 : 0;      // the matrix of this lane's rows
+    const int rr = GATED ? r & 63 : r;               // output row within the CTA
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t a_base = tmem + LY::A_COL + group * 32 + lane_base;
+    const uint32_t lead_afull = dsmem_addr(bar(LY::B_AFULL), 0), lead_dempty = dsmem_addr(bar(LY::B_DEMPTY), 0);
+    PairRing<CS> cr;
+    PairRing<AB> ar;
+    int stored = -1;  // step of the store in flight
+    auto publish = [&]() {
+      if (stored >= 0) {
+        tc::tmem_wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc2::arrive_cluster(lead_afull + stored * 8);
+      }
+    };
+    int k = 0;
+    for (int tile = first; tile < tiles && ok; tile += step, ++k) {
+      int lo, hi;
+      const int e = find_item(p, tile / f.row_tiles, f.tile_tokens, lo, hi);
+      const int n0 = tile % f.row_tiles * 2 * CTA_ROWS + rank * CTA_ROWS;
+      const int64_t wrow = (int64_t)e * p.n_out + min(n0 + rr, p.n_out - 1);
+      const uint4* prow = reinterpret_cast<const uint4*>(p.params[which] + wrow * p.pstride);
+      uint4 pv = __ldg(prow);
+      for (int c = 0; c < stages; ++c) {
+        const uint4 pnext = __ldg(prow + min(c + 1, stages - 1));
+        ok = __all_sync(0xffffffffu, wait(LY::B_CFULL + cr.s, cr.ph));
+        if (!ok) break;
+        const uint8_t* crow = smem + LY::OFF_C + cr.s * LY::CSTAGE + r * 128;
+        const uint32_t pw[4] = {pv.x, pv.y, pv.z, pv.w};
+        const int in_stage = min(4, slabs - 4 * c);
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          if (st * SP >= in_stage) break;
+          const int s = st * SP + group;
+          uint32_t o[32];
+          if (s < in_stage) {
+            const uint4 w0 = *reinterpret_cast<const uint4*>(crow + (((2 * s) ^ (r & 7)) << 4));
+            const uint4 w1 = *reinterpret_cast<const uint4*>(crow + (((2 * s + 1) ^ (r & 7)) << 4));
+            const uint32_t ps = group == 0 ? pw[st * SP] : pw[st * SP + 1];
+            const uint32_t s24 = __byte_perm(ps, ps, 0x1010), bb = __byte_perm(ps, ps, 0x3232);
+            const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);
+            const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint32_t d[4];
+              dequant_word(words[j], s24, s20, bb, d);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) o[4 * j + q] = d[q];
+            }
+          }
+          publish();
+          ok = __all_sync(0xffffffffu, wait(LY::B_AEMPTY + ar.s, ar.ph ^ 1u));
+          if (!ok) break;
+          tc::fence_after();
+          if (s < in_stage) tc::tmem_st32_nowait(a_base + ar.s * 64, o);
+          stored = ar.s;
+          ar.next();
+        }
+        if (!ok) break;
+        __syncwarp();  // the stage's codes are in registers
+        if (lane == 0) mbar_arrive(bar(LY::B_CEMPTY + cr.s));
+        cr.next();
+        pv = pnext;
+      }
+      if (ok) publish();
+      stored = -1;
+      const int b = k & 1;
+      ok = ok && __all_sync(0xffffffffu, wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1));
+      // the warps go on together or not at all: the output below has barriers among them
+      ok = !tc2::any_of_group(5, !ok, DW * 32);
+      if (!ok) break;
+      tc::fence_after();
+      // ---- output: lane = weight row, columns = tokens; group g takes every other 16 of them.  A token's
+      // 32 rows leave as 64 bytes through the warp's own shared memory.  Gated: the warps that hold a
+      // row's gate and its partner swap halves of the 16 columns and finish 8 each.
+      constexpr int COLS = GATED ? 8 : 16;  // tokens a warp finishes of 16
+      const int row0 = n0 + (GATED ? (quarter & 1) * 32 : quarter * 32);
+      const float rs = p.row_scale[which][wrow];
+      const int pair = group * 2 + (quarter & 1);
+      float* swap = reinterpret_cast<float*>(smem + LY::OFF_SWAP) + pair * 1024;
+      uint16_t* so = reinterpret_cast<uint16_t*>(smem + LY::OFF_OUT + warp * 1024);
+      const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+      int flip = 0;
+#pragma unroll 1
+      for (int cb = group * 16; lo + cb < hi; cb += 32, flip ^= 512) {
+        float v[16];
+        tc::tmem_ld16(tmem + cb + lane_base, v);
+        const float4* ts4 = reinterpret_cast<const float4*>(tok_scale + b * 256 + cb);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float4 tv = ts4[j >> 2];
+          v[j] *= rs * ((j & 3) == 0 ? tv.x : (j & 3) == 1 ? tv.y : (j & 3) == 2 ? tv.z : tv.w);
+        }
+        if constexpr (GATED) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) swap[flip + (which * 8 + j) * 32 + lane] = which == 0 ? v[8 + j] : v[j];
+          asm volatile("bar.sync %0, 64;\n" ::"r"(1 + pair) : "memory");
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float other = swap[flip + ((which ^ 1) * 8 + j) * 32 + lane];
+            v[j] = which == 0 ? silu_mul(v[j], other) : silu_mul(other, v[8 + j]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < COLS; j += 2) {
+          uint32_t h;
+          if (p.bf16) {
+            const __nv_bfloat162 q = __floats2bfloat162_rn(v[j], v[j + 1]);
+            h = *reinterpret_cast<const uint32_t*>(&q);
+          } else {
+            h = pack_half2(v[j], v[j + 1]);
+          }
+          so[j * 32 + lane] = static_cast<uint16_t>(h);
+          so[(j + 1) * 32 + lane] = static_cast<uint16_t>(h >> 16);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < COLS / 8; ++h) {
+          const int tok = h * 8 + (lane >> 2), col = (lane & 3) * 8;
+          const int out_row = lo + cb + (GATED ? which * 8 : 0) + tok;
+          const int left = p.n_out - (row0 + col);
+          const uint4 d = *reinterpret_cast<const uint4*>(so + tok * 32 + col);
+          if (out_row < hi && left > 0) {
+            uint16_t* dst = p.out + (int64_t)out_row * p.out_stride + row0 + col;
+            if (wide && left >= 8) {
+              *reinterpret_cast<uint4*>(dst) = d;
+            } else {
+              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (j < left) dst[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+            }
+          }
+        }
+        __syncwarp();
+      }
+      // the accumulator and the tokens' scales are read
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        tc2::arrive_cluster(lead_dempty);
+        mbar_arrive(bar(LY::B_SEMPTY + b));
+      }
+    }
+  }
+  if (!ok) *abort_flag = 1;
+  __syncthreads();
+
+  // ---- teardown: after an abort, this CTA's loads (and the leader's MMAs) in flight finish (bounded);
+  // then both CTAs are done with each other's memory
+  if (*abort_flag) {
+    constexpr uint64_t kDrainNs = 100000000ull;
+    if (warp == CODES_WARP && lane == 0)
+      for (int j = max(0, issued_c - CS); j < issued_c; ++j)
+        mbar_wait_bounded(bar(LY::B_CFULL + j % CS), (j / CS) & 1, kDrainNs);
+    if (warp == X_WARP && lane == 0 && rank == 0)  // (both CTAs' loads complete on the leader's barriers)
+      for (int j = max(0, issued_x - XS); j < issued_x; ++j)
+        mbar_wait_bounded(bar(LY::B_XFULL + j % XS), (j / XS) & 1, kDrainNs);
+    if (warp == MMA_WARP && lane == 0 && mma_issued) {
+      tc2::commit(bar(LY::B_DRAIN));
+      mbar_wait_bounded(bar(LY::B_DRAIN), 0, kDrainNs);
+    }
+    if (tid == 0) flag_status(p.status, AM_STATUS_TIMEOUT);
+  }
+  tc::fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 0) {
+    tc::fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
+  }
+}
+
+// ---------------------------------------------------------------- host
+template <bool GATED>
+static cudaError_t launch_pair_t(const PairParams& f, int clusters, int dev, cudaStream_t stream) {
+  auto kfn = linear_pair_kernel<GATED>;
+  static unsigned long long done = 0;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (!bit || !(__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) {
+    const cudaError_t err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, PairLayout::SMEM);
+    if (err != cudaSuccess) return err;
+    if (bit) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * clusters);
+  cfg.blockDim = dim3(PairLayout::THREADS);
+  cfg.dynamicSmemBytes = PairLayout::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kfn, f);
+}
+
+cudaError_t launch_linear_pair(const LinearParams& p, cudaStream_t stream) {
+  int dev = 0;
+  const int sms = sm_count(&dev);
+  if (sms == 0) return cudaErrorInvalidDevice;
+  const bool gated = p.codes[1] != nullptr;
+  const int rows = gated ? 128 : 256;
+  PairParams f{};
+  f.p = p;
+  f.row_tiles = (p.n_out + rows - 1) / rows;
+  const int pairs = sms / 2;
+  f.tile_tokens = 256;
+  int64_t items = p.offsets != nullptr ? (int64_t)std::min(p.experts, p.rows) + p.rows / 256 : 0;
+  if (p.offsets == nullptr) {
+    // One matrix: the cut of the tokens whose last round of tiles is fullest (a tile costs its tokens
+    // and about 24 more for its output and restart).
+    double best = 0.0;
+    for (int n = (p.rows + 255) / 256, tries = 0; tries < 4; ++n, ++tries) {
+      const int tokens = ((p.rows + n - 1) / n + 31) & ~31;
+      const int64_t tiles = (int64_t)f.row_tiles * ((p.rows + tokens - 1) / tokens);
+      const double cost = (double)((tiles + pairs - 1) / pairs) * (tokens + 24);
+      if (tries == 0 || cost < best) {
+        best = cost;
+        f.tile_tokens = tokens;
+      }
+    }
+    items = (p.rows + f.tile_tokens - 1) / f.tile_tokens;
+  }
+  if (f.row_tiles * items > INT_MAX) return cudaErrorNotSupported;
+  const int clusters = static_cast<int>(std::min<int64_t>(f.row_tiles * items, pairs));
+  return gated ? launch_pair_t<true>(f, clusters, dev, stream) : launch_pair_t<false>(f, clusters, dev, stream);
+}
+
+}  // namespace am

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
   }
   const int rank = f.ck > 1 ? static_cast<int>(blockIdx.x) % f.ck : 0;
   const int first = static_cast<int>(blockIdx.x) / f.ck, step = static_cast<int>(gridDim.x) / f.ck;
-  const int tiles = count_items<NT>(p) * f.row_tiles;
+  const int tiles = count_items(p, NT) * f.row_tiles;
   if (first >= tiles) return;  // the whole cluster
   constexpr int CTA_ROWS = GATED ? 128 : 256;
   // this CTA's inputs: quads of groups [q0, q1), slabs of 64 inputs, steps of SP slabs
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     Ring<CS> ring;
     for (int tile = first; tile < tiles; tile += step) {
       int lo, hi;
-      const int e = find_item<NT>(p, tile / f.row_tiles, lo, hi);
+      const int e = find_item(p, tile / f.row_tiles, NT, lo, hi);
       const int y = e * p.n_out + tile % f.row_tiles * CTA_ROWS;
       if (lane == 0) {
         for (int c = q0; c < q1; ++c) {
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     int k = 0;
     for (int tile = first; tile < tiles && ok; tile += step, ++k) {
       int lo, hi;
-      find_item<NT>(p, tile / f.row_tiles, lo, hi);
+      find_item(p, tile / f.row_tiles, NT, lo, hi);
       for (int i = 0; i < steps; ++i) {
         ok = __all_sync(0xffffffffu, wait(LY::B_XEMPTY + ring.s, ring.ph ^ 1u));
         if (!ok) break;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     int k = 0;
     for (int tile = first; tile < tiles && ok; tile += step, ++k) {
       int lo, hi;
-      const int e = find_item<NT>(p, tile / f.row_tiles, lo, hi);
+      const int e = find_item(p, tile / f.row_tiles, NT, lo, hi);
       const int n0 = tile % f.row_tiles * CTA_ROWS;
       const int64_t wrow = (int64_t)e * p.n_out + min(n0 + (GATED ? 0 : t * 128) + r, p.n_out - 1);
       const uint4* prow = reinterpret_cast<const uint4*>(p.params[GATED ? t : 0] + wrow * p.pstride);
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     cluster_sync_all();
     if (!*abort_flag) {
       int lo, hi;
-      const int e = find_item<NT>(p, first / f.row_tiles, lo, hi);
+      const int e = find_item(p, first / f.row_tiles, NT, lo, hi);
       const int n0 = first % f.row_tiles * CTA_ROWS;
       const int m = hi - lo;
       const int t0 = m * rank / f.ck, t1 = m * (rank + 1) / f.ck;
@@ -501,6 +501,15 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
 }
 
 // ---------------------------------------------------------------- host
+// Pairs of SMs where a matrix's mean number of rows fills most of a pair's 256 tokens and the tiles
+// fill the pairs.
+bool linear_uses_pairs(int rows, int experts, int n_out, bool grouped, bool gated) {
+  const int mean = grouped ? (rows + experts - 1) / experts : rows;
+  const int64_t tiles = (int64_t)((n_out + (gated ? 127 : 255)) / (gated ? 128 : 256)) *
+                        (grouped ? rows / 256 : (rows + 255) / 256);
+  return mean > 192 && tiles >= 64;
+}
+
 int linear_token_tile(int rows, int experts, bool grouped) {
   const int mean = grouped ? (rows + experts - 1) / experts : rows;
   return mean <= 32 ? 32 : (mean <= 64 ? 64 : 128);
@@ -554,10 +563,11 @@ static cudaError_t launch_tiles(const LinearParams& p, cudaStream_t stream) {
   return p.codes[1] != nullptr ? launch_tiles_t<NT, true>(p, items, stream) : launch_tiles_t<NT, false>(p, items, stream);
 }
 
-cudaError_t launch_linear_tiles(const LinearParams& p, cudaStream_t stream) {
+cudaError_t launch_linear_tiles(const LinearParams& p, bool pairs, cudaStream_t stream) {
   linear_rows_kernel<<<p.rows, 128, 0, stream>>>(p);
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
+  if (pairs) return launch_linear_pair(p, stream);
   switch (linear_token_tile(p.rows, p.experts, p.offsets != nullptr)) {
     case 32: return launch_tiles<32>(p, stream);
     case 64: return launch_tiles<64>(p, stream);

@@ -92,7 +92,10 @@ def test_linear_every_token_count(cuda, n, k, gated, dtype):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("m,n,k,gated", [(1, 4096, 4096, False), (3, 5000, 14336, False), (8, 9001, 1024, True),
                                          (20, 2049, 4096, True), (96, 4096, 4096, False),
-                                         (700, 1537, 2880, True), (1500, 2304, 1024, False)])
+                                         (700, 1537, 2880, True), (1500, 2304, 1024, False),
+                                         (2048, 2049, 320, False), (2300, 1030, 192, True),
+                                         (1000, 4097, 1024, False), (4096, 2048, 64, True),
+                                         (2100, 2304, 2880, True), (3333, 1100, 448, True)])
 def test_linear_larger(cuda, m, n, k, gated, dtype):
     ws = [make_weight((n, k), dtype, cuda, seed=i) for i in range(1 + gated)]
     x = make_x(m, k, dtype, cuda)
@@ -272,6 +275,19 @@ def test_experts_wide(cuda):
         q = [pkg.Q4Weight(*w) for w in ws]
         r = routing_of(choose("skewed", tokens, e, k, cuda), e)
         x = make_x(tokens, d, torch.bfloat16, cuda)
+        assert_within(pkg.expert_swiglu(x, *q, r), *expected_experts(x, ws, r, True))
+        assert_within(pkg.expert_matmul(x, q[1], r, gather=True), *expected_experts(x, ws[1:], r, True))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["even", "skewed", "one"])
+def test_experts_many_rows(cuda, kind, dtype):
+    """Hundreds of rows an expert: tiles of pairs of SMs with items of every size."""
+    for tokens, e, k, n, d in ((3000, 3, 2, 800, 320), (4000, 8, 1, 1200, 704)):
+        ws = [make_weight((e, n, d), dtype, cuda, seed=i) for i in range(2)]
+        q = [pkg.Q4Weight(*w) for w in ws]
+        r = routing_of(choose(kind, tokens, e, k, cuda), e)
+        x = make_x(tokens, d, dtype, cuda)
         assert_within(pkg.expert_swiglu(x, *q, r), *expected_experts(x, ws, r, True))
         assert_within(pkg.expert_matmul(x, q[1], r, gather=True), *expected_experts(x, ws[1:], r, True))
 
