@@ -50,32 +50,11 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// Arrive on an mbarrier of the cluster (address from mapa), releasing to the cluster.
+// Arrive on an mbarrier of the cluster (address from mapa).  What it hands over is TMEM, ordered by the
+// tcgen05 fences around the arrival and the wait; a cluster-scope release of all memory before it
+// would cost 320 cycles an arrival instead of 8 (measured).
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
-}
-
-// wait_or_abort on a barrier that the peer CTA arrives on too.
-__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, uint64_t limit_ns, const volatile int* abort_flag) {
-  if (limit_ns == 0) return false;
-  constexpr uint32_t kSuspendNs = 100000;
-  uint64_t t0 = 0;
-  for (uint32_t it = 0;; ++it) {
-    uint32_t done;
-    asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n"
-        "selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done)
-        : "r"(bar), "r"(parity), "r"(kSuspendNs)
-        : "memory");
-    if (done) return true;
-    if (*abort_flag) return false;
-    if (it == 0) {
-      t0 = globaltimer_ns();
-    } else if (globaltimer_ns() - t0 > limit_ns) {
-      return false;
-    }
-  }
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
 }
 
 // Whether any of the `count` threads that meet at named barrier `id` passes true.
@@ -99,8 +78,7 @@ struct PairLayout {
   static constexpr int XSLAB = 128 * 128;                        // 128 tokens x 64 inputs
   static constexpr int OFF_C = 0;
   static constexpr int OFF_X = OFF_C + CS * CSTAGE;
-  static constexpr int OFF_OUT = OFF_X + XS * SP * XSLAB;        // 1 KB a warp
-  static constexpr int OFF_SWAP = OFF_OUT + DW * 1024;           // two buffers of 2 KB a pair of warps
+  static constexpr int OFF_SWAP = OFF_X + XS * SP * XSLAB;       // two buffers of 2 KB a pair of warps
   static constexpr int OFF_SCALE = OFF_SWAP + 4 * 2 * 2048;      // two tiles' token scales
   static constexpr int OFF_BAR = OFF_SCALE + 2 * 256 * 4;
   static constexpr int B_CFULL = 0, B_CEMPTY = CS, B_XFULL = 2 * CS, B_XEMPTY = B_XFULL + XS;
@@ -151,7 +129,7 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + LY::OFF_BAR + LY::B_COUNT * 8 + 4);
   float* tok_scale = reinterpret_cast<float*>(smem + LY::OFF_SCALE);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  auto wait = [&](int i, uint32_t parity) { return wait_or_abort(bar(i), parity, p.wait_ns, abort_flag); };
+  auto wait = [&](int i, uint32_t parity) { return wait_quick(bar(i), parity, p.wait_ns, abort_flag); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   griddep_launch_dependents();
@@ -243,27 +221,33 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
       find_item(p, tile / f.row_tiles, f.tile_tokens, lo, hi);
       const uint32_t id = tc::idesc(256, (hi - lo + 31) & ~31, false);
       if (lane == 0) {
-        ok = tc2::wait_cluster(bar(LY::B_DEMPTY), dph, p.wait_ns, abort_flag);
+        // The barriers of step i + 1 are waited for between the MMAs of step i, whose queue is only a
+        // few deep.
+        ok = wait(LY::B_DEMPTY, dph) &&
+             wait(LY::B_XFULL + xr.s, xr.ph) && wait(LY::B_AFULL + ar.s, ar.ph);
         for (int i = 0; i < steps && ok; ++i) {
-          ok = wait(LY::B_XFULL + xr.s, xr.ph) &&
-               tc2::wait_cluster(bar(LY::B_AFULL + ar.s), ar.ph, p.wait_ns, abort_flag);
-          if (!ok) break;
           tc::fence_after();
           const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + xr.s * SP * LY::XSLAB, 16, 1024);
           const uint32_t a = tmem + LY::A_COL + ar.s * 64;
+          const uint32_t x_done = bar(LY::B_XEMPTY + xr.s), a_done = bar(LY::B_AEMPTY + ar.s);
+          const bool both = 2 * i + 1 < slabs, more = i + 1 < steps;
+          xr.next();
+          ar.next();
           // (descriptor addresses count 16-byte units: 32 bytes of a swizzled row are 16 inputs)
           tc2::mma_ts(tmem, a, xd, id, i > 0 ? 1u : 0u);
 #pragma unroll
           for (int ks = 1; ks < 4; ++ks) tc2::mma_ts(tmem, a + ks * 8, xd + ks * 2, id, 1u);
-          if (2 * i + 1 < slabs) {
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) tc2::mma_ts(tmem, a + 32 + ks * 8, xd + LY::XSLAB / 16 + ks * 2, id, 1u);
-          }
           mma_issued = true;
-          tc2::commit(bar(LY::B_XEMPTY + xr.s));
-          tc2::commit(bar(LY::B_AEMPTY + ar.s));
-          xr.next();
-          ar.next();
+          if (both) {
+            tc2::mma_ts(tmem, a + 32, xd + LY::XSLAB / 16, id, 1u);
+            tc2::mma_ts(tmem, a + 40, xd + LY::XSLAB / 16 + 2, id, 1u);
+          }
+          if (more) ok = wait(LY::B_XFULL + xr.s, xr.ph);
+          if (both) tc2::mma_ts(tmem, a + 48, xd + LY::XSLAB / 16 + 4, id, 1u);
+          if (more && ok) ok = wait(LY::B_AFULL + ar.s, ar.ph);
+          if (both) tc2::mma_ts(tmem, a + 56, xd + LY::XSLAB / 16 + 6, id, 1u);
+          tc2::commit(x_done);
+          tc2::commit(a_done);
         }
         if (ok) tc2::commit(bar(LY::B_DFULL));
       }
@@ -289,15 +273,11 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
         if (lane == 0) tc2::arrive_cluster(lead_afull + stored * 8);
       }
     };
-    int k = 0;
-    for (int tile = first; tile < tiles && ok; tile += step, ++k) {
-      int lo, hi;
-      const int e = find_item(p, tile / f.row_tiles, f.tile_tokens, lo, hi);
-      const int n0 = tile % f.row_tiles * 2 * CTA_ROWS + rank * CTA_ROWS;
-      const int64_t wrow = (int64_t)e * p.n_out + min(n0 + rr, p.n_out - 1);
-      const uint4* prow = reinterpret_cast<const uint4*>(p.params[which] + wrow * p.pstride);
-      uint4 pv = __ldg(prow);
-      for (int c = 0; c < stages; ++c) {
+    // stages [c0, c1) of the tile with parameter row prow
+    const uint4* prow = nullptr;
+    uint4 pv = make_uint4(0, 0, 0, 0);
+    auto dequant = [&](int c0, int c1) {
+      for (int c = c0; c < c1 && ok; ++c) {
         const uint4 pnext = __ldg(prow + min(c + 1, stages - 1));
         ok = __all_sync(0xffffffffu, wait(LY::B_CFULL + cr.s, cr.ph));
         if (!ok) break;
@@ -340,22 +320,25 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
       }
       if (ok) publish();
       stored = -1;
+    };
+    // ---- output of the k-th tile: lane = weight row, columns = tokens; group g takes every other 16 of
+    // them, a token's 32 rows leave as 64 bytes.  Gated: the warps that hold a row's gate and its
+    // partner swap halves of the 16 columns and finish 8 each.
+    bool left = false;  // a failure was seen by all warps: none meets the others again
+    auto output = [&](int k, int lo, int hi, int n0, int64_t wrow) {
       const int b = k & 1;
       ok = ok && __all_sync(0xffffffffu, wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1));
-      // the warps go on together or not at all: the output below has barriers among them
+      // the warps go on together or not at all: there are barriers among them below
       ok = !tc2::any_of_group(5, !ok, DW * 32);
-      if (!ok) break;
+      left = !ok;
+      if (!ok) return;
       tc::fence_after();
-      // ---- output: lane = weight row, columns = tokens; group g takes every other 16 of them.  A token's
-      // 32 rows leave as 64 bytes through the warp's own shared memory.  Gated: the warps that hold a
-      // row's gate and its partner swap halves of the 16 columns and finish 8 each.
       constexpr int COLS = GATED ? 8 : 16;  // tokens a warp finishes of 16
-      const int row0 = n0 + (GATED ? (quarter & 1) * 32 : quarter * 32);
+      const int row = n0 + rr;
       const float rs = p.row_scale[which][wrow];
       const int pair = group * 2 + (quarter & 1);
       float* swap = reinterpret_cast<float*>(smem + LY::OFF_SWAP) + pair * 1024;
-      uint16_t* so = reinterpret_cast<uint16_t*>(smem + LY::OFF_OUT + warp * 1024);
-      const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+      uint16_t* dst = p.out + (int64_t)(lo + (GATED ? which * 8 : 0)) * p.out_stride + row;
       int flip = 0;
 #pragma unroll 1
       for (int cb = group * 16; lo + cb < hi; cb += 32, flip ^= 512) {
@@ -377,38 +360,13 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
             v[j] = which == 0 ? silu_mul(v[j], other) : silu_mul(other, v[8 + j]);
           }
         }
+        if (row < p.n_out) {
+          uint16_t* d = dst + (int64_t)cb * p.out_stride;
+          const int live = hi - lo - cb - (GATED ? which * 8 : 0);
 #pragma unroll
-        for (int j = 0; j < COLS; j += 2) {
-          uint32_t h;
-          if (p.bf16) {
-            const __nv_bfloat162 q = __floats2bfloat162_rn(v[j], v[j + 1]);
-            h = *reinterpret_cast<const uint32_t*>(&q);
-          } else {
-            h = pack_half2(v[j], v[j + 1]);
-          }
-          so[j * 32 + lane] = static_cast<uint16_t>(h);
-          so[(j + 1) * 32 + lane] = static_cast<uint16_t>(h >> 16);
+          for (int j = 0; j < COLS; ++j)
+            if (j < live) d[j * p.out_stride] = p.bf16 ? f2h<true>(v[j]) : f2h<false>(v[j]);
         }
-        __syncwarp();
-#pragma unroll
-        for (int h = 0; h < COLS / 8; ++h) {
-          const int tok = h * 8 + (lane >> 2), col = (lane & 3) * 8;
-          const int out_row = lo + cb + (GATED ? which * 8 : 0) + tok;
-          const int left = p.n_out - (row0 + col);
-          const uint4 d = *reinterpret_cast<const uint4*>(so + tok * 32 + col);
-          if (out_row < hi && left > 0) {
-            uint16_t* dst = p.out + (int64_t)out_row * p.out_stride + row0 + col;
-            if (wide && left >= 8) {
-              *reinterpret_cast<uint4*>(dst) = d;
-            } else {
-              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (j < left) dst[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
-            }
-          }
-        }
-        __syncwarp();
       }
       // the accumulator and the tokens' scales are read
       tc::fence_before();
@@ -417,7 +375,28 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
         tc2::arrive_cluster(lead_dempty);
         mbar_arrive(bar(LY::B_SEMPTY + b));
       }
+    };
+    // The first AB steps of a tile are dequantized before the output of the one before it: they fill
+    // the operand buffers while its last MMAs run, and the next MMAs start with the output done.
+    constexpr int AHEAD = AB * SP / 4;  // stages
+    int k = 0, lo = 0, hi = 0, n0 = 0;
+    int64_t wrow = 0;
+    for (int tile = first; tile < tiles && ok; tile += step, ++k) {
+      int lo_n, hi_n;
+      const int e = find_item(p, tile / f.row_tiles, f.tile_tokens, lo_n, hi_n);
+      const int n0_n = tile % f.row_tiles * 2 * CTA_ROWS + rank * CTA_ROWS;
+      const int64_t wrow_n = (int64_t)e * p.n_out + min(n0_n + rr, p.n_out - 1);
+      prow = reinterpret_cast<const uint4*>(p.params[which] + wrow_n * p.pstride);
+      pv = __ldg(prow);
+      dequant(0, min(AHEAD, stages));
+      if (k > 0) output(k - 1, lo, hi, n0, wrow);
+      if (ok) dequant(min(AHEAD, stages), stages);
+      lo = lo_n;
+      hi = hi_n;
+      n0 = n0_n;
+      wrow = wrow_n;
     }
+    if (k > 0 && !left) output(k - 1, lo, hi, n0, wrow);
   }
   if (!ok) *abort_flag = 1;
   __syncthreads();

@@ -210,4 +210,24 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, uin
   }
 }
 
+// wait_or_abort for barriers that are mostly complete already: one try without a suspend-time hint
+// (14 cycles when complete; with the hint 100, measured), then the wait out of line.
+static __device__ __noinline__ bool wait_or_abort_slow(uint32_t bar, uint32_t parity, uint64_t limit_ns,
+                                                const volatile int* abort_flag) {
+  return wait_or_abort(bar, parity, limit_ns, abort_flag);
+}
+
+__device__ __forceinline__ bool wait_quick(uint32_t bar, uint32_t parity, uint64_t limit_ns,
+                                           const volatile int* abort_flag) {
+  if (limit_ns == 0) return false;
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done || wait_or_abort_slow(bar, parity, limit_ns, abort_flag);
+}
+
 }  // namespace am
