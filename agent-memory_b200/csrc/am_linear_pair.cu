@@ -71,6 +71,8 @@ __device__ __forceinline__ bool any_of_group(int id, bool v, int count) {
 
 }  // namespace tc2
 
+constexpr int kOutPitch = 80;  // bytes between tokens of a warp's 32 output rows: 64, and 16 against bank conflicts
+
 struct PairLayout {
   static constexpr int CS = 4, XS = 4, AB = 4, SP = 2, DW = 8;  // AB: steps of SP slabs
   static constexpr int THREADS = 32 * (DW + 3);                  // + codes, activations, MMA
@@ -78,7 +80,8 @@ struct PairLayout {
   static constexpr int XSLAB = 128 * 128;                        // 128 tokens x 64 inputs
   static constexpr int OFF_C = 0;
   static constexpr int OFF_X = OFF_C + CS * CSTAGE;
-  static constexpr int OFF_SWAP = OFF_X + XS * SP * XSLAB;       // two buffers of 2 KB a pair of warps
+  static constexpr int OFF_OUT = OFF_X + XS * SP * XSLAB;        // 16 tokens x kOutPitch bytes a warp
+  static constexpr int OFF_SWAP = OFF_OUT + DW * 16 * kOutPitch;  // two buffers of 2 KB a pair of warps
   static constexpr int OFF_SCALE = OFF_SWAP + 4 * 2 * 2048;      // two tiles' token scales
   static constexpr int OFF_BAR = OFF_SCALE + 2 * 256 * 4;
   static constexpr int B_CFULL = 0, B_CEMPTY = CS, B_XFULL = 2 * CS, B_XEMPTY = B_XFULL + XS;
@@ -321,11 +324,12 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
       if (ok) publish();
       stored = -1;
     };
-    // ---- output of the k-th tile: lane = weight row, columns = tokens; group g takes every other 16 of
-    // them, a token's 32 rows leave as 64 bytes.  Gated: the warps that hold a row's gate and its
-    // partner swap halves of the 16 columns and finish 8 each.
+    // ---- output of the k-th tile: group g takes every other 16 tokens.  The accumulators come in mma
+    // fragments (thread (g8, t4): rows g8 + 8 i, tokens 2 t4, + 1 of eight), leave transposed through
+    // the warp's own shared memory, a token's 32 rows as 64 bytes.  Gated: the warps that hold a
+    // row's gate and its partner swap eight of the 16 tokens and finish the other eight each.
     bool left = false;  // a failure was seen by all warps: none meets the others again
-    auto output = [&](int k, int lo, int hi, int n0, int64_t wrow) {
+    auto output = [&](int k, int lo, int hi, int n0, int64_t wbase) {
       const int b = k & 1;
       ok = ok && __all_sync(0xffffffffu, wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1));
       // the warps go on together or not at all: there are barriers among them below
@@ -333,40 +337,91 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
       left = !ok;
       if (!ok) return;
       tc::fence_after();
-      constexpr int COLS = GATED ? 8 : 16;  // tokens a warp finishes of 16
-      const int row = n0 + rr;
-      const float rs = p.row_scale[which][wrow];
+      const int g8 = lane >> 2, t4 = lane & 3;
+      const int row0 = n0 + (GATED ? (quarter & 1) * 32 : quarter * 32);  // of the warp's 32
+      float rs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        rs[i] = __ldg(p.row_scale[which] + wbase + min(row0 + g8 + 8 * i, p.n_out - 1));
       const int pair = group * 2 + (quarter & 1);
-      float* swap = reinterpret_cast<float*>(smem + LY::OFF_SWAP) + pair * 1024;
-      uint16_t* dst = p.out + (int64_t)(lo + (GATED ? which * 8 : 0)) * p.out_stride + row;
+      float4* swap = reinterpret_cast<float4*>(smem + LY::OFF_SWAP) + pair * 256;
+      uint8_t* so = smem + LY::OFF_OUT + warp * (16 * kOutPitch);
+      // rows of the transposed 8 x 8 matrices: tokens lane % 8 (+ 8), weight rows 8 (lane / 8)
+      const uint32_t st_addr = smem_u32(so) + (lane & 7) * kOutPitch + (lane >> 3) * 16;
+      const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+      const int left_rows = p.n_out - (row0 + (lane & 3) * 8);  // from this lane's 8 output rows on
       int flip = 0;
 #pragma unroll 1
-      for (int cb = group * 16; lo + cb < hi; cb += 32, flip ^= 512) {
-        float v[16];
-        tc::tmem_ld16(tmem + cb + lane_base, v);
-        const float4* ts4 = reinterpret_cast<const float4*>(tok_scale + b * 256 + cb);
+      for (int cb = group * 16; lo + cb < hi; cb += 32, flip ^= 128) {
+        float v[2][8];  // [16 rows][token block, row g8 or g8 + 8, token]
+        tc::tmem_ld_16x16_nowait(tmem + cb + lane_base, v[0]);
+        tc::tmem_ld_16x16_nowait(tmem + cb + lane_base + (16u << 16), v[1]);
+        float2 ts[2];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float4 tv = ts4[j >> 2];
-          v[j] *= rs * ((j & 3) == 0 ? tv.x : (j & 3) == 1 ? tv.y : (j & 3) == 2 ? tv.z : tv.w);
-        }
+        for (int j = 0; j < 2; ++j) ts[j] = *reinterpret_cast<const float2*>(tok_scale + b * 256 + cb + 8 * j + 2 * t4);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[h][i] *= rs[2 * h + ((i >> 1) & 1)] * ((i & 1) ? ts[i >> 2].y : ts[i >> 2].x);
+        uint32_t q[2][4];  // [token block][8 rows]: pairs of tokens
+        auto pack = [&](float x, float y) -> uint32_t {
+          if (p.bf16) {
+            const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
+            return *reinterpret_cast<const uint32_t*>(&z);
+          }
+          return pack_half2(x, y);
+        };
         if constexpr (GATED) {
+          const int give = which == 0 ? 1 : 0;  // the token block the other warp finishes
+          float keep[2][4];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) swap[flip + (which * 8 + j) * 32 + lane] = which == 0 ? v[8 + j] : v[j];
+          for (int h = 0; h < 2; ++h) {
+            swap[flip + (which * 2 + h) * 32 + lane] = give ? make_float4(v[h][4], v[h][5], v[h][6], v[h][7])
+                                                            : make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) keep[h][i] = give ? v[h][i] : v[h][4 + i];
+          }
           asm volatile("bar.sync %0, 64;\n" ::"r"(1 + pair) : "memory");
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float other = swap[flip + ((which ^ 1) * 8 + j) * 32 + lane];
-            v[j] = which == 0 ? silu_mul(v[j], other) : silu_mul(other, v[8 + j]);
+          for (int h = 0; h < 2; ++h) {
+            const float4 o4 = swap[flip + ((which ^ 1) * 2 + h) * 32 + lane];
+            const float o[4] = {o4.x, o4.y, o4.z, o4.w};
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = which == 0 ? silu_mul(keep[h][i], o[i]) : silu_mul(o[i], keep[h][i]);
+            q[0][2 * h] = pack(y[0], y[1]);
+            q[0][2 * h + 1] = pack(y[2], y[3]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              q[j][2 * h] = pack(v[h][4 * j], v[h][4 * j + 1]);
+              q[j][2 * h + 1] = pack(v[h][4 * j + 2], v[h][4 * j + 3]);
+            }
+        }
+        stsm_x4_trans(st_addr, q[0][0], q[0][1], q[0][2], q[0][3]);
+        if constexpr (!GATED) stsm_x4_trans(st_addr + 8 * kOutPitch, q[1][0], q[1][1], q[1][2], q[1][3]);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < (GATED ? 1 : 2); ++j) {
+          const int tok = lo + cb + (GATED ? which * 8 : j * 8) + (lane >> 2);
+          const uint4 d = *reinterpret_cast<const uint4*>(so + (j * 8 + (lane >> 2)) * kOutPitch + (lane & 3) * 16);
+          if (tok < hi && left_rows > 0) {
+            uint16_t* dst = p.out + (int64_t)tok * p.out_stride + row0 + (lane & 3) * 8;
+            if (wide && left_rows >= 8) {
+              *reinterpret_cast<uint4*>(dst) = d;
+            } else {
+              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (i < left_rows) dst[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+            }
           }
         }
-        if (row < p.n_out) {
-          uint16_t* d = dst + (int64_t)cb * p.out_stride;
-          const int live = hi - lo - cb - (GATED ? which * 8 : 0);
-#pragma unroll
-          for (int j = 0; j < COLS; ++j)
-            if (j < live) d[j * p.out_stride] = p.bf16 ? f2h<true>(v[j]) : f2h<false>(v[j]);
-        }
+        __syncwarp();
       }
       // the accumulator and the tokens' scales are read
       tc::fence_before();
@@ -380,23 +435,23 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
     // the operand buffers while its last MMAs run, and the next MMAs start with the output done.
     constexpr int AHEAD = AB * SP / 4;  // stages
     int k = 0, lo = 0, hi = 0, n0 = 0;
-    int64_t wrow = 0;
+    int64_t wbase = 0;
     for (int tile = first; tile < tiles && ok; tile += step, ++k) {
       int lo_n, hi_n;
       const int e = find_item(p, tile / f.row_tiles, f.tile_tokens, lo_n, hi_n);
       const int n0_n = tile % f.row_tiles * 2 * CTA_ROWS + rank * CTA_ROWS;
-      const int64_t wrow_n = (int64_t)e * p.n_out + min(n0_n + rr, p.n_out - 1);
-      prow = reinterpret_cast<const uint4*>(p.params[which] + wrow_n * p.pstride);
+      const int64_t wbase_n = (int64_t)e * p.n_out;
+      prow = reinterpret_cast<const uint4*>(p.params[which] + (wbase_n + min(n0_n + rr, p.n_out - 1)) * p.pstride);
       pv = __ldg(prow);
       dequant(0, min(AHEAD, stages));
-      if (k > 0) output(k - 1, lo, hi, n0, wrow);
+      if (k > 0) output(k - 1, lo, hi, n0, wbase);
       if (ok) dequant(min(AHEAD, stages), stages);
       lo = lo_n;
       hi = hi_n;
       n0 = n0_n;
-      wrow = wrow_n;
+      wbase = wbase_n;
     }
-    if (k > 0 && !left) output(k - 1, lo, hi, n0, wrow);
+    if (k > 0 && !left) output(k - 1, lo, hi, n0, wbase);
   }
   if (!ok) *abort_flag = 1;
   __syncthreads();

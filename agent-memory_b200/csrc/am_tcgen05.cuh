@@ -122,6 +122,14 @@ __device__ __forceinline__ void tmem_ld64_nowait(uint32_t taddr, float (&v)[64])
       : "r"(taddr));
 #undef AM_R8
 }
+// Warp loads 16 lanes x 16 columns from taddr on, without the wait: thread (g, t) = (lane / 4, lane % 4)
+// gets of columns 8 j + 2 t, + 1 (j = 0, 1) rows g (v[4 j], v[4 j + 1]) and g + 8 (v[4 j + 2], v[4 j + 3]).
+__device__ __forceinline__ void tmem_ld_16x16_nowait(uint32_t taddr, float (&v)[8]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 
 template <int N>
