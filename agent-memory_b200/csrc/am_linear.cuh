@@ -136,13 +136,14 @@ __device__ __forceinline__ int count_items(const LinearParams& p, int tok) {
   return __reduce_add_sync(0xffffffffu, n);
 }
 
-// Item `item`: rows [lo, hi) of one expert.  Returns the expert, or -1 past the last item.  All
-// lanes of a warp call it.
+// Item `item`: rows [lo, hi) of one expert, whose rows are cut evenly into as few items as hold them.
+// Returns the expert, or -1 past the last item.  All lanes of a warp call it.
 __device__ __forceinline__ int find_item(const LinearParams& p, int item, int tok, int& lo, int& hi) {
   if (p.offsets == nullptr) {
-    lo = item * tok;
-    hi = min(lo + tok, p.rows);
-    return lo < hi ? 0 : -1;
+    const int n = (p.rows + tok - 1) / tok, per = n > 0 ? (p.rows + n - 1) / n : 0;
+    lo = item * per;
+    hi = min(lo + per, p.rows);
+    return item < n ? 0 : -1;
   }
   // each warp scans the experts, 32 at a time
   const int lane = threadIdx.x & 31;
@@ -161,9 +162,10 @@ __device__ __forceinline__ int find_item(const LinearParams& p, int item, int to
     if (item < base + total) {
       const bool mine = item >= base + incl - n && item < base + incl;
       const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
-      const int first = a + (item - (base + incl - n)) * tok;
+      const int per = n > 0 ? (b - a + n - 1) / n : 0;
+      const int first = a + (item - (base + incl - n)) * per;
       lo = __shfl_sync(0xffffffffu, first, src);
-      hi = min(__shfl_sync(0xffffffffu, b, src), lo + tok);
+      hi = __shfl_sync(0xffffffffu, min(first + per, b), src);
       return e0 + src;
     }
     base += total;

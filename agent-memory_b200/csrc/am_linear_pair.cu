@@ -9,9 +9,9 @@
 //
 // Per CTA: one thread streams the codes (plain: 128 rows of the matrix; gated: 64 rows of each, so
 // that a row's gate and its partner lie 64 TMEM lanes apart in the same CTA), one the
-// activations; their full barrier and that of the dequantized operand are the leader's.  8
-// warps dequantize (two groups of 4, a 64-input slab each) and write the output: TMEM holds the
-// 256-column accumulator and eight operand slabs.  The MMA shape follows the item: N is its tokens
+// activations; their full barrier, shared with the dequantized operand's, is the leader's.  8
+// warps dequantize (two groups of 4, a 64-input slab of a step each) and write the output: TMEM holds
+// the 256-column accumulator and eight operand slabs.  The MMA shape follows the item: N is its tokens
 // rounded up to 32.  Waits are bounded as in am_linear_tc.cu; the CTAs of a pair leave together.
 #include <algorithm>
 #include <climits>
@@ -73,27 +73,32 @@ __device__ __forceinline__ bool any_of_group(int id, bool v, int count) {
 
 constexpr int kOutPitch = 80;  // bytes between tokens of a warp's 32 output rows: 64, and 16 against bank conflicts
 
+template <bool GATED>
 struct PairLayout {
-  static constexpr int CS = 4, XS = 4, AB = 4, SP = 2, DW = 8;  // AB: steps of SP slabs
-  static constexpr int THREADS = 32 * (DW + 3);                  // + codes, activations, MMA
-  static constexpr int CSTAGE = 128 * 128;                       // 128 rows x 256 inputs
-  static constexpr int XSLAB = 128 * 128;                        // 128 tokens x 64 inputs
+  static constexpr int CS = 4;               // code stages (128 rows x 256 inputs)
+  static constexpr int ST = 4;               // steps in flight: two slabs (64 inputs) of operand and activations
+  static constexpr int DW = 8;               // dequantization warps: 4 a slab of a step
+  static constexpr int THREADS = 32 * (DW + 3);  // + codes, activations, MMA
+  static constexpr int CSTAGE = 128 * 128;
+  static constexpr int XSLAB = 128 * 128;    // 128 tokens x 64 inputs
   static constexpr int OFF_C = 0;
   static constexpr int OFF_X = OFF_C + CS * CSTAGE;
-  static constexpr int OFF_OUT = OFF_X + XS * SP * XSLAB;        // 16 tokens x kOutPitch bytes a warp
-  static constexpr int OFF_SWAP = OFF_OUT + DW * 16 * kOutPitch;  // two buffers of 2 KB a pair of warps
-  static constexpr int OFF_SCALE = OFF_SWAP + 4 * 2 * 2048;      // two tiles' token scales
+  static constexpr int OFF_OUT = OFF_X + ST * 2 * XSLAB;           // kOutPitch bytes a token of a warp
+  static constexpr int OUT = (GATED ? 8 : 16) * kOutPitch;
+  static constexpr int OFF_SWAP = OFF_OUT + DW * OUT;              // two buffers of 2 KB a pair of warps
+  static constexpr int OFF_SCALE = OFF_SWAP + (GATED ? DW / 2 * 4096 : 0);  // two tiles' token scales
   static constexpr int OFF_BAR = OFF_SCALE + 2 * 256 * 4;
-  static constexpr int B_CFULL = 0, B_CEMPTY = CS, B_XFULL = 2 * CS, B_XEMPTY = B_XFULL + XS;
-  static constexpr int B_AFULL = B_XEMPTY + XS, B_AEMPTY = B_AFULL + AB, B_DFULL = B_AEMPTY + AB;
-  static constexpr int B_DEMPTY = B_DFULL + 1, B_SFULL = B_DEMPTY + 1, B_SEMPTY = B_SFULL + 2;
+  // FULL: a step's operand is in the TMEM of both CTAs and its activations in their shared memory (the
+  // leader's copy); EMPTY: the step's MMAs are done (both copies).
+  static constexpr int B_CFULL = 0, B_CEMPTY = CS, B_FULL = 2 * CS, B_EMPTY = B_FULL + ST;
+  static constexpr int B_DFULL = B_EMPTY + ST, B_DEMPTY = B_DFULL + 1, B_SFULL = B_DEMPTY + 1, B_SEMPTY = B_SFULL + 2;
   static constexpr int B_DRAIN = B_SEMPTY + 2, B_COUNT = B_DRAIN + 1;
   static constexpr int SMEM = OFF_BAR + B_COUNT * 8 + 16;
   static constexpr int A_COL = 256;  // D at 0, A[step][slab] at A_COL + 32 (2 step + slab)
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static __device__ int arrivals(int i) {
     if (i >= B_CEMPTY && i < B_CEMPTY + CS) return DW;
-    if (i >= B_AFULL && i < B_AFULL + AB) return 2 * DW;  // (the leader's: both CTAs' warps)
+    if (i >= B_FULL && i < B_FULL + ST) return 2 * DW + 1;  // both CTAs' warps, the activations' thread
     if (i == B_DEMPTY) return 2 * DW;
     if (i >= B_SEMPTY && i < B_SEMPTY + 2) return DW;
     return 1;
@@ -119,9 +124,9 @@ struct PairRing {
 };
 
 template <bool GATED>
-__global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams f) {
-  using LY = PairLayout;
-  constexpr int CS = LY::CS, XS = LY::XS, AB = LY::AB, SP = LY::SP, DW = LY::DW;
+__global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams f) {
+  using LY = PairLayout<GATED>;
+  constexpr int CS = LY::CS, ST = LY::ST, DW = LY::DW;
   constexpr int CODES_WARP = DW, X_WARP = DW + 1, MMA_WARP = DW + 2;
   constexpr int CTA_ROWS = GATED ? 64 : 128;  // output rows of a CTA
   const LinearParams& p = f.p;
@@ -145,7 +150,7 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
   const int tiles = count_items(p, f.tile_tokens) * f.row_tiles;
   if (first >= tiles) return;  // both CTAs of the pair
   const int stages = p.pstride >> 2;  // quads of groups
-  const int slabs = p.groups, steps = (slabs + SP - 1) / SP;
+  const int slabs = p.groups, steps = (slabs + 1) / 2;
 
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(tmem_slot)));
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
     }
   } else if (warp == X_WARP) {
     griddep_wait();  // the activations are written
-    PairRing<XS> ring;
+    PairRing<ST> ring;
     int k = 0;
     for (int tile = first; tile < tiles && ok; tile += step, ++k) {
       int lo, hi;
@@ -194,18 +199,18 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
       const int half = ((hi - lo + 31) & ~31) >> 1;  // tokens of a CTA
       const int y = lo + rank * half;
       for (int i = 0; i < steps; ++i) {
-        ok = __all_sync(0xffffffffu, wait(LY::B_XEMPTY + ring.s, ring.ph ^ 1u));
+        ok = __all_sync(0xffffffffu, wait(LY::B_EMPTY + ring.s, ring.ph ^ 1u));
         if (!ok) break;
-        const uint32_t dst = s_base + LY::OFF_X + ring.s * SP * LY::XSLAB;
-        const int n = min(SP, slabs - i * SP);
+        const uint32_t dst = s_base + LY::OFF_X + ring.s * 2 * LY::XSLAB;
+        const int n = min(2, slabs - 2 * i);
         if (lane == 0) {
-          const uint32_t full = bar(LY::B_XFULL + ring.s);
+          const uint32_t full = bar(LY::B_FULL + ring.s);
           if (rank == 0) mbar_arrive_expect_tx(full, 2 * n * LY::XSLAB);  // both CTAs' bytes
-          for (int s = 0; s < n; ++s) tc2::tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, (i * SP + s) * 128, y, full);
+          for (int s = 0; s < n; ++s) tc2::tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, (2 * i + s) * 128, y, full);
         }
         ++issued_x;
         ring.next();
-        if (i == min(XS, steps) - 1) {  // behind the first loads: the tokens' powers of two
+        if (i == min(ST, steps) - 1) {  // behind the first loads: the tokens' powers of two
           const int b = k & 1;
           ok = __all_sync(0xffffffffu, wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1));
           if (!ok) break;
@@ -216,26 +221,23 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
       }
     }
   } else if (warp == MMA_WARP) {
-    PairRing<XS> xr;
-    PairRing<AB> ar;
+    PairRing<ST> ring;
     uint32_t dph = 1;
     for (int tile = first; tile < tiles && ok && rank == 0; tile += step, dph ^= 1u) {
       int lo, hi;
       find_item(p, tile / f.row_tiles, f.tile_tokens, lo, hi);
       const uint32_t id = tc::idesc(256, (hi - lo + 31) & ~31, false);
       if (lane == 0) {
-        // The barriers of step i + 1 are waited for between the MMAs of step i, whose queue is only a
-        // few deep.
-        ok = wait(LY::B_DEMPTY, dph) &&
-             wait(LY::B_XFULL + xr.s, xr.ph) && wait(LY::B_AFULL + ar.s, ar.ph);
+        // One wait and one commit a step (8 MMAs of 128 cycles); the wait for step i + 1 stands before
+        // the last MMAs of step i.  With separate barriers for operand and activations the issuing
+        // thread itself took 1450 cycles a step.
+        ok = wait(LY::B_DEMPTY, dph) && wait(LY::B_FULL + ring.s, ring.ph);
         for (int i = 0; i < steps && ok; ++i) {
           tc::fence_after();
-          const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + xr.s * SP * LY::XSLAB, 16, 1024);
-          const uint32_t a = tmem + LY::A_COL + ar.s * 64;
-          const uint32_t x_done = bar(LY::B_XEMPTY + xr.s), a_done = bar(LY::B_AEMPTY + ar.s);
-          const bool both = 2 * i + 1 < slabs, more = i + 1 < steps;
-          xr.next();
-          ar.next();
+          const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + ring.s * 2 * LY::XSLAB, 16, 1024);
+          const uint32_t a = tmem + LY::A_COL + ring.s * 64, done = bar(LY::B_EMPTY + ring.s);
+          const bool both = 2 * i + 1 < slabs;
+          ring.next();
           // (descriptor addresses count 16-byte units: 32 bytes of a swizzled row are 16 inputs)
           tc2::mma_ts(tmem, a, xd, id, i > 0 ? 1u : 0u);
 #pragma unroll
@@ -245,12 +247,12 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
             tc2::mma_ts(tmem, a + 32, xd + LY::XSLAB / 16, id, 1u);
             tc2::mma_ts(tmem, a + 40, xd + LY::XSLAB / 16 + 2, id, 1u);
           }
-          if (more) ok = wait(LY::B_XFULL + xr.s, xr.ph);
-          if (both) tc2::mma_ts(tmem, a + 48, xd + LY::XSLAB / 16 + 4, id, 1u);
-          if (more && ok) ok = wait(LY::B_AFULL + ar.s, ar.ph);
-          if (both) tc2::mma_ts(tmem, a + 56, xd + LY::XSLAB / 16 + 6, id, 1u);
-          tc2::commit(x_done);
-          tc2::commit(a_done);
+          if (i + 1 < steps) ok = wait(LY::B_FULL + ring.s, ring.ph);
+          if (both) {
+            tc2::mma_ts(tmem, a + 48, xd + LY::XSLAB / 16 + 4, id, 1u);
+            tc2::mma_ts(tmem, a + 56, xd + LY::XSLAB / 16 + 6, id, 1u);
+          }
+          tc2::commit(done);
         }
         if (ok) tc2::commit(bar(LY::B_DFULL));
       }
@@ -264,39 +266,28 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
     const int rr = GATED ? r & 63 : r;               // output row within the CTA
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t a_base = tmem + LY::A_COL + group * 32 + lane_base;
-    const uint32_t lead_afull = dsmem_addr(bar(LY::B_AFULL), 0), lead_dempty = dsmem_addr(bar(LY::B_DEMPTY), 0);
+    const uint32_t lead_full = dsmem_addr(bar(LY::B_FULL), 0), lead_dempty = dsmem_addr(bar(LY::B_DEMPTY), 0);
     PairRing<CS> cr;
-    PairRing<AB> ar;
-    int stored = -1;  // step of the store in flight
-    auto publish = [&]() {
-      if (stored >= 0) {
-        tc::tmem_wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) tc2::arrive_cluster(lead_afull + stored * 8);
-      }
-    };
-    // stages [c0, c1) of the tile with parameter row prow
-    const uint4* prow = nullptr;
+    PairRing<ST> ring;
+    const uint4* prow = nullptr;  // parameters of this thread's weight row, a code stage each
     uint4 pv = make_uint4(0, 0, 0, 0);
-    auto dequant = [&](int c0, int c1) {
+    auto dequant = [&](int c0, int c1) {  // code stages [c0, c1)
       for (int c = c0; c < c1 && ok; ++c) {
-        const uint4 pnext = __ldg(prow + min(c + 1, stages - 1));
+        const uint32_t ps[2] = {group == 0 ? pv.x : pv.y, group == 0 ? pv.z : pv.w};
+        pv = __ldg(prow + min(c + 1, stages - 1));
         ok = __all_sync(0xffffffffu, wait(LY::B_CFULL + cr.s, cr.ph));
         if (!ok) break;
         const uint8_t* crow = smem + LY::OFF_C + cr.s * LY::CSTAGE + r * 128;
-        const uint32_t pw[4] = {pv.x, pv.y, pv.z, pv.w};
         const int in_stage = min(4, slabs - 4 * c);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          if (st * SP >= in_stage) break;
-          const int s = st * SP + group;
+          if (st * 2 >= in_stage) break;
+          const int s = st * 2 + group;
           uint32_t o[32];
           if (s < in_stage) {
             const uint4 w0 = *reinterpret_cast<const uint4*>(crow + (((2 * s) ^ (r & 7)) << 4));
             const uint4 w1 = *reinterpret_cast<const uint4*>(crow + (((2 * s + 1) ^ (r & 7)) << 4));
-            const uint32_t ps = group == 0 ? pw[st * SP] : pw[st * SP + 1];
-            const uint32_t s24 = __byte_perm(ps, ps, 0x1010), bb = __byte_perm(ps, ps, 0x3232);
+            const uint32_t s24 = __byte_perm(ps[st], ps[st], 0x1010), bb = __byte_perm(ps[st], ps[st], 0x3232);
             const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);
             const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
@@ -307,22 +298,20 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
               for (int q = 0; q < 4; ++q) o[4 * j + q] = d[q];
             }
           }
-          publish();
-          ok = __all_sync(0xffffffffu, wait(LY::B_AEMPTY + ar.s, ar.ph ^ 1u));
+          ok = __all_sync(0xffffffffu, wait(LY::B_EMPTY + ring.s, ring.ph ^ 1u));
           if (!ok) break;
           tc::fence_after();
-          if (s < in_stage) tc::tmem_st32_nowait(a_base + ar.s * 64, o);
-          stored = ar.s;
-          ar.next();
+          if (s < in_stage) tc::tmem_st32(a_base + ring.s * 64, o);
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc2::arrive_cluster(lead_full + ring.s * 8);
+          ring.next();
         }
         if (!ok) break;
         __syncwarp();  // the stage's codes are in registers
         if (lane == 0) mbar_arrive(bar(LY::B_CEMPTY + cr.s));
         cr.next();
-        pv = pnext;
       }
-      if (ok) publish();
-      stored = -1;
     };
     // ---- output of the k-th tile: group g takes every other 16 tokens.  The accumulators come in mma
     // fragments (thread (g8, t4): rows g8 + 8 i, tokens 2 t4, + 1 of eight), leave transposed through
@@ -331,35 +320,46 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
     bool left = false;  // a failure was seen by all warps: none meets the others again
     auto output = [&](int k, int lo, int hi, int n0, int64_t wbase) {
       const int b = k & 1;
-      ok = ok && __all_sync(0xffffffffu, wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1));
-      // the warps go on together or not at all: there are barriers among them below
-      ok = !tc2::any_of_group(5, !ok, DW * 32);
-      left = !ok;
-      if (!ok) return;
-      tc::fence_after();
       const int g8 = lane >> 2, t4 = lane & 3;
       const int row0 = n0 + (GATED ? (quarter & 1) * 32 : quarter * 32);  // of the warp's 32
       float rs[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         rs[i] = __ldg(p.row_scale[which] + wbase + min(row0 + g8 + 8 * i, p.n_out - 1));
+      ok = ok && __all_sync(0xffffffffu, wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1));
+      // the warps go on together or not at all: there are barriers among them below
+      ok = !tc2::any_of_group(15, !ok, DW * 32);
+      left = !ok;
+      if (!ok) return;
+      tc::fence_after();
       const int pair = group * 2 + (quarter & 1);
       float4* swap = reinterpret_cast<float4*>(smem + LY::OFF_SWAP) + pair * 256;
-      uint8_t* so = smem + LY::OFF_OUT + warp * (16 * kOutPitch);
+      uint8_t* so = smem + LY::OFF_OUT + warp * LY::OUT;
       // rows of the transposed 8 x 8 matrices: tokens lane % 8 (+ 8), weight rows 8 (lane / 8)
       const uint32_t st_addr = smem_u32(so) + (lane & 7) * kOutPitch + (lane >> 3) * 16;
       const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
       const int left_rows = p.n_out - (row0 + (lane & 3) * 8);  // from this lane's 8 output rows on
       int flip = 0;
+      float next[2][8];  // the next 16 tokens, loaded behind this one's work: [16 rows][token block, row
+                         // g8 or g8 + 8, token]
+      auto load = [&](int cb) {
+        tc::tmem_ld_16x16_nowait(tmem + cb + lane_base, next[0]);
+        tc::tmem_ld_16x16_nowait(tmem + cb + lane_base + (16u << 16), next[1]);
+      };
+      if (lo + group * 16 < hi) load(group * 16);
 #pragma unroll 1
       for (int cb = group * 16; lo + cb < hi; cb += 32, flip ^= 128) {
-        float v[2][8];  // [16 rows][token block, row g8 or g8 + 8, token]
-        tc::tmem_ld_16x16_nowait(tmem + cb + lane_base, v[0]);
-        tc::tmem_ld_16x16_nowait(tmem + cb + lane_base + (16u << 16), v[1]);
+        float v[2][8];
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[0][i] = next[0][i];
+          v[1][i] = next[1][i];
+        }
+        if (lo + cb + 32 < hi) load(cb + 32);
         float2 ts[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) ts[j] = *reinterpret_cast<const float2*>(tok_scale + b * 256 + cb + 8 * j + 2 * t4);
-        tc::tmem_wait_ld();
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -431,9 +431,9 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
         mbar_arrive(bar(LY::B_SEMPTY + b));
       }
     };
-    // The first AB steps of a tile are dequantized before the output of the one before it: they fill
+    // The first ST steps of a tile are dequantized before the output of the one before it: they fill
     // the operand buffers while its last MMAs run, and the next MMAs start with the output done.
-    constexpr int AHEAD = AB * SP / 4;  // stages
+    constexpr int AHEAD = LY::ST / 2;  // stages
     int k = 0, lo = 0, hi = 0, n0 = 0;
     int64_t wbase = 0;
     for (int tile = first; tile < tiles && ok; tile += step, ++k) {
@@ -464,8 +464,8 @@ __global__ void __launch_bounds__(PairLayout::THREADS, 1) linear_pair_kernel(con
       for (int j = max(0, issued_c - CS); j < issued_c; ++j)
         mbar_wait_bounded(bar(LY::B_CFULL + j % CS), (j / CS) & 1, kDrainNs);
     if (warp == X_WARP && lane == 0 && rank == 0)  // (both CTAs' loads complete on the leader's barriers)
-      for (int j = max(0, issued_x - XS); j < issued_x; ++j)
-        mbar_wait_bounded(bar(LY::B_XFULL + j % XS), (j / XS) & 1, kDrainNs);
+      for (int j = max(0, issued_x - ST); j < issued_x; ++j)
+        mbar_wait_bounded(bar(LY::B_FULL + j % ST), (j / ST) & 1, kDrainNs);
     if (warp == MMA_WARP && lane == 0 && mma_issued) {
       tc2::commit(bar(LY::B_DRAIN));
       mbar_wait_bounded(bar(LY::B_DRAIN), 0, kDrainNs);
@@ -488,14 +488,14 @@ static cudaError_t launch_pair_t(const PairParams& f, int clusters, int dev, cud
   static unsigned long long done = 0;
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
   if (!bit || !(__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) {
-    const cudaError_t err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, PairLayout::SMEM);
+    const cudaError_t err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, PairLayout<GATED>::SMEM);
     if (err != cudaSuccess) return err;
     if (bit) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * clusters);
-  cfg.blockDim = dim3(PairLayout::THREADS);
-  cfg.dynamicSmemBytes = PairLayout::SMEM;
+  cfg.blockDim = dim3(PairLayout<GATED>::THREADS);
+  cfg.dynamicSmemBytes = PairLayout<GATED>::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -522,13 +522,14 @@ cudaError_t launch_linear_pair(const LinearParams& p, cudaStream_t stream) {
   f.tile_tokens = 256;
   int64_t items = p.offsets != nullptr ? (int64_t)std::min(p.experts, p.rows) + p.rows / 256 : 0;
   if (p.offsets == nullptr) {
-    // One matrix: the cut of the tokens whose last round of tiles is fullest (a tile costs its tokens
-    // and about 24 more for its output and restart).
+    // One matrix: the cut of the tokens that ends first.  A step of 128 inputs measured 4.6 cycles a token
+    // (1178 for 256), 950 at least (the MMA thread), a tile's start and output 8000.
+    const double steps = (p.groups + 1) / 2;
     double best = 0.0;
-    for (int n = (p.rows + 255) / 256, tries = 0; tries < 4; ++n, ++tries) {
+    for (int n = (p.rows + 255) / 256, tries = 0; tries < 12; ++n, ++tries) {
       const int tokens = ((p.rows + n - 1) / n + 31) & ~31;
       const int64_t tiles = (int64_t)f.row_tiles * ((p.rows + tokens - 1) / tokens);
-      const double cost = (double)((tiles + pairs - 1) / pairs) * (tokens + 24);
+      const double cost = (double)((tiles + pairs - 1) / pairs) * (steps * std::max(4.6 * tokens, 950.0) + 8000.0);
       if (tries == 0 || cost < best) {
         best = cost;
         f.tile_tokens = tokens;
