@@ -175,4 +175,49 @@ __device__ __forceinline__ int find_item(const LinearParams& p, int item, int to
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
+// Two outputs as a pair of the call's type.
+__device__ __forceinline__ uint32_t pack_out(const LinearParams& p, float x, float y) {
+  if (p.bf16) {
+    const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&z);
+  }
+  return pack_half2(x, y);
+}
+
+// Bytes between tokens of a warp's 32 output rows in shared memory: 64, and 16 against bank conflicts.
+constexpr int kOutPitch = 80;
+
+// A warp writes output rows row0 .. row0 + 31 (weight rows) of 8 * BLOCKS tokens from `tok` on: q[j][i]
+// holds in mma fragments (thread (g, t): weight row 8 i + g, tokens 8 j + 2 t, + 1) pairs of
+// tokens.  They are transposed through 8 * BLOCKS * kOutPitch bytes of shared memory at `so`; a
+// token's 32 rows leave as 64 bytes.
+template <int BLOCKS>
+__device__ __forceinline__ void store_tokens(const LinearParams& p, uint8_t* so, const uint32_t (&q)[BLOCKS][4], int tok,
+                                             int hi, int row0) {
+  const int lane = threadIdx.x & 31;
+  const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  const int left = p.n_out - (row0 + (lane & 3) * 8);  // from this lane's 8 output rows on
+  const uint32_t st = smem_u32(so) + (lane & 7) * kOutPitch + (lane >> 3) * 16;
+#pragma unroll
+  for (int j = 0; j < BLOCKS; ++j) stsm_x4_trans(st + j * 8 * kOutPitch, q[j][0], q[j][1], q[j][2], q[j][3]);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < BLOCKS; ++j) {
+    const int at = tok + j * 8 + (lane >> 2);
+    const uint4 d = *reinterpret_cast<const uint4*>(so + (j * 8 + (lane >> 2)) * kOutPitch + (lane & 3) * 16);
+    if (at < hi && left > 0) {
+      uint16_t* dst = p.out + (int64_t)at * p.out_stride + row0 + (lane & 3) * 8;
+      if (wide && left >= 8) {
+        *reinterpret_cast<uint4*>(dst) = d;
+      } else {
+        const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < left) dst[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+  }
+  __syncwarp();
+}
+
 }  // namespace am

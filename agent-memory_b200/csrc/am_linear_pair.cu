@@ -71,8 +71,6 @@ __device__ __forceinline__ bool any_of_group(int id, bool v, int count) {
 
 }  // namespace tc2
 
-constexpr int kOutPitch = 80;  // bytes between tokens of a warp's 32 output rows: 64, and 16 against bank conflicts
-
 template <bool GATED>
 struct PairLayout {
   static constexpr int CS = 4;               // code stages (128 rows x 256 inputs)
@@ -138,7 +136,9 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
   float* tok_scale = reinterpret_cast<float*>(smem + LY::OFF_SCALE);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   auto wait = [&](int i, uint32_t parity) { return wait_quick(bar(i), parity, p.wait_ns, abort_flag); };
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (the warp index by a shuffle: uniform to the compiler, which then keeps the MMA operands in
+  // uniform registers)
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   griddep_launch_dependents();
   if (s_base & 1023u) {  // swizzled tiles need a 1024-byte aligned window (the whole grid returns)
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
   __syncthreads();
   cluster_sync_all();  // both CTAs' barriers exist before either arrives on the other's
   tc::fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   int issued_c = 0, issued_x = 0;  // loads issued (their own threads' counts)
   bool mma_issued = false;
@@ -221,42 +221,45 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
       }
     }
   } else if (warp == MMA_WARP) {
+    const bool lead = elect_one();
     PairRing<ST> ring;
     uint32_t dph = 1;
     for (int tile = first; tile < tiles && ok && rank == 0; tile += step, dph ^= 1u) {
       int lo, hi;
       find_item(p, tile / f.row_tiles, f.tile_tokens, lo, hi);
       const uint32_t id = tc::idesc(256, (hi - lo + 31) & ~31, false);
-      if (lane == 0) {
-        // One wait and one commit a step (8 MMAs of 128 cycles); the wait for step i + 1 stands before
-        // the last MMAs of step i.  With separate barriers for operand and activations the issuing
-        // thread itself took 1450 cycles a step.
-        ok = wait(LY::B_DEMPTY, dph) && wait(LY::B_FULL + ring.s, ring.ph);
-        for (int i = 0; i < steps && ok; ++i) {
-          tc::fence_after();
-          const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + ring.s * 2 * LY::XSLAB, 16, 1024);
-          const uint32_t a = tmem + LY::A_COL + ring.s * 64, done = bar(LY::B_EMPTY + ring.s);
-          const bool both = 2 * i + 1 < slabs;
-          ring.next();
+      // One wait and one commit a step (8 MMAs of 128 cycles); the wait for step i + 1 stands before the
+      // last MMAs of step i.  (With separate barriers for operand and activations the issuing thread
+      // itself took 1450 cycles a step.)  The warp stays converged and one lane issues, as in
+      // linear_tiles_kernel.
+      ok = __all_sync(0xffffffffu, wait(LY::B_DEMPTY, dph) && wait(LY::B_FULL + ring.s, ring.ph));
+      for (int i = 0; i < steps && ok; ++i) {
+        tc::fence_after();
+        const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + ring.s * 2 * LY::XSLAB, 16, 1024);
+        const uint32_t a = tmem + LY::A_COL + ring.s * 64, done = bar(LY::B_EMPTY + ring.s);
+        const bool both = 2 * i + 1 < slabs;
+        ring.next();
+        if (lead) {
           // (descriptor addresses count 16-byte units: 32 bytes of a swizzled row are 16 inputs)
           tc2::mma_ts(tmem, a, xd, id, i > 0 ? 1u : 0u);
 #pragma unroll
           for (int ks = 1; ks < 4; ++ks) tc2::mma_ts(tmem, a + ks * 8, xd + ks * 2, id, 1u);
-          mma_issued = true;
           if (both) {
             tc2::mma_ts(tmem, a + 32, xd + LY::XSLAB / 16, id, 1u);
             tc2::mma_ts(tmem, a + 40, xd + LY::XSLAB / 16 + 2, id, 1u);
           }
-          if (i + 1 < steps) ok = wait(LY::B_FULL + ring.s, ring.ph);
+        }
+        mma_issued = lead;
+        if (i + 1 < steps) ok = __all_sync(0xffffffffu, wait(LY::B_FULL + ring.s, ring.ph));
+        if (lead) {
           if (both) {
             tc2::mma_ts(tmem, a + 48, xd + LY::XSLAB / 16 + 4, id, 1u);
             tc2::mma_ts(tmem, a + 56, xd + LY::XSLAB / 16 + 6, id, 1u);
           }
           tc2::commit(done);
         }
-        if (ok) tc2::commit(bar(LY::B_DFULL));
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (ok && lead) tc2::commit(bar(LY::B_DFULL));
     }
   } else {
     // ---- dequantization (as in linear_tiles_kernel): a weight row a thread, slab `group` of every step
@@ -335,10 +338,6 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
       const int pair = group * 2 + (quarter & 1);
       float4* swap = reinterpret_cast<float4*>(smem + LY::OFF_SWAP) + pair * 256;
       uint8_t* so = smem + LY::OFF_OUT + warp * LY::OUT;
-      // rows of the transposed 8 x 8 matrices: tokens lane % 8 (+ 8), weight rows 8 (lane / 8)
-      const uint32_t st_addr = smem_u32(so) + (lane & 7) * kOutPitch + (lane >> 3) * 16;
-      const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-      const int left_rows = p.n_out - (row0 + (lane & 3) * 8);  // from this lane's 8 output rows on
       int flip = 0;
       float next[2][8];  // the next 16 tokens, loaded behind this one's work: [16 rows][token block, row
                          // g8 or g8 + 8, token]
@@ -364,14 +363,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[h][i] *= rs[2 * h + ((i >> 1) & 1)] * ((i & 1) ? ts[i >> 2].y : ts[i >> 2].x);
-        uint32_t q[2][4];  // [token block][8 rows]: pairs of tokens
-        auto pack = [&](float x, float y) -> uint32_t {
-          if (p.bf16) {
-            const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
-            return *reinterpret_cast<const uint32_t*>(&z);
-          }
-          return pack_half2(x, y);
-        };
+        uint32_t q[GATED ? 1 : 2][4];  // [token block][8 rows]: pairs of tokens
         if constexpr (GATED) {
           const int give = which == 0 ? 1 : 0;  // the token block the other warp finishes
           float keep[2][4];
@@ -390,38 +382,19 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
             float y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = which == 0 ? silu_mul(keep[h][i], o[i]) : silu_mul(o[i], keep[h][i]);
-            q[0][2 * h] = pack(y[0], y[1]);
-            q[0][2 * h + 1] = pack(y[2], y[3]);
+            q[0][2 * h] = pack_out(p, y[0], y[1]);
+            q[0][2 * h + 1] = pack_out(p, y[2], y[3]);
           }
         } else {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              q[j][2 * h] = pack(v[h][4 * j], v[h][4 * j + 1]);
-              q[j][2 * h + 1] = pack(v[h][4 * j + 2], v[h][4 * j + 3]);
+              q[j][2 * h] = pack_out(p, v[h][4 * j], v[h][4 * j + 1]);
+              q[j][2 * h + 1] = pack_out(p, v[h][4 * j + 2], v[h][4 * j + 3]);
             }
         }
-        stsm_x4_trans(st_addr, q[0][0], q[0][1], q[0][2], q[0][3]);
-        if constexpr (!GATED) stsm_x4_trans(st_addr + 8 * kOutPitch, q[1][0], q[1][1], q[1][2], q[1][3]);
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < (GATED ? 1 : 2); ++j) {
-          const int tok = lo + cb + (GATED ? which * 8 : j * 8) + (lane >> 2);
-          const uint4 d = *reinterpret_cast<const uint4*>(so + (j * 8 + (lane >> 2)) * kOutPitch + (lane & 3) * 16);
-          if (tok < hi && left_rows > 0) {
-            uint16_t* dst = p.out + (int64_t)tok * p.out_stride + row0 + (lane & 3) * 8;
-            if (wide && left_rows >= 8) {
-              *reinterpret_cast<uint4*>(dst) = d;
-            } else {
-              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (i < left_rows) dst[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
-            }
-          }
-        }
-        __syncwarp();
+        store_tokens(p, so, q, lo + cb + (GATED ? which * 8 : 0), hi, row0);
       }
       // the accumulator and the tokens' scales are read
       tc::fence_before();
@@ -466,7 +439,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
     if (warp == X_WARP && lane == 0 && rank == 0)  // (both CTAs' loads complete on the leader's barriers)
       for (int j = max(0, issued_x - ST); j < issued_x; ++j)
         mbar_wait_bounded(bar(LY::B_FULL + j % ST), (j / ST) & 1, kDrainNs);
-    if (warp == MMA_WARP && lane == 0 && mma_issued) {
+    if (warp == MMA_WARP && mma_issued) {
       tc2::commit(bar(LY::B_DRAIN));
       mbar_wait_bounded(bar(LY::B_DRAIN), 0, kDrainNs);
     }

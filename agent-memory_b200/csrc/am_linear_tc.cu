@@ -24,9 +24,9 @@
 // Every wait is bounded (LinearParams::wait_ns); on timeout the kernel flags AM_STATUS_TIMEOUT,
 // lets its copies and MMAs in flight finish, frees its TMEM and returns.
 //
-// The codes and parameters are read before griddepcontrol.wait: linear_rows_kernel starts only
-// when everything before it in the stream is complete (it is launched without programmatic
-// serialization), and it writes nothing but the activations.
+// The codes and parameters are read before griddepcontrol.wait: linear_rows_kernel lets this grid start
+// only after its own wait, when everything before it in the stream is complete, and it writes
+// nothing but the activations.
 #include <algorithm>
 #include <climits>
 
@@ -39,7 +39,8 @@ namespace am {
 // ---------------------------------------------------------------- activations
 __global__ void __launch_bounds__(128) linear_rows_kernel(const __grid_constant__ LinearParams p) {
   __shared__ uint32_t wmax[4];
-  griddep_launch_dependents();
+  griddep_wait();
+  griddep_launch_dependents();  // (not earlier: the next grid reads the weights before its own wait)
   const int row = blockIdx.x, tid = threadIdx.x;
   const int from = source_row(p, row);
   const uint4* src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(from, 0) * p.x_stride);
@@ -78,7 +79,7 @@ struct TilesLayout {
   static constexpr uint32_t TMEM_COLS = 512 / CTAS;
   static constexpr int SP = NT == 128 ? 2 : 1;             // slabs (64 inputs) of a pipeline step
   static constexpr int CS = NT == 128 ? 3 : 2;             // code stages (256 rows x 256 inputs)
-  static constexpr int XS = NT == 128 ? 3 : (NT == 64 ? 5 : 8);  // activation steps (NT x 64 SP inputs)
+  static constexpr int XS = NT == 128 ? 3 : (NT == 64 ? 4 : 8);  // activation steps (NT x 64 SP inputs)
   static constexpr int AB = (TMEM_COLS - 2 * NT) / (64 * SP);    // TMEM operand buffers (2 tiles x 32 SP columns)
   static constexpr int DW = 8 * SP;                        // dequantization warps: 8 a slab of the step
   static constexpr int THREADS = 32 * (DW + 4);            // + codes, activations, two MMA warps
@@ -88,8 +89,8 @@ struct TilesLayout {
   static constexpr int OFF_X = OFF_C + CS * CSTAGE;
   static constexpr int OFF_END = OFF_X + XS * SP * XSLAB;
   static constexpr int RED = 2 * NT * 128 * 4;             // fp32 sums of a split (over the rings)
-  static constexpr int OFF_OUT = OFF_END > RED ? OFF_END : RED;  // 1 KB a dequantization warp
-  static constexpr int OFF_SCALE = OFF_OUT + DW * 1024;    // two tiles' token scales
+  static constexpr int OFF_OUT = OFF_END > RED ? OFF_END : RED;  // kOutPitch bytes a token of a warp
+  static constexpr int OFF_SCALE = OFF_OUT + DW * 16 * kOutPitch;  // two tiles' token scales
   static constexpr int OFF_BAR = OFF_SCALE + 2 * NT * 4;
   static constexpr int B_CFULL = 0, B_CEMPTY = CS, B_XFULL = 2 * CS, B_XEMPTY = B_XFULL + XS;
   static constexpr int B_AFULL = B_XEMPTY + XS, B_AEMPTY = B_AFULL + AB, B_DFULL = B_AEMPTY + AB;
@@ -146,8 +147,12 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + LY::OFF_BAR + LY::B_COUNT * 8 + 4);
   float* tok_scale = reinterpret_cast<float*>(smem + LY::OFF_SCALE);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  auto wait = [&](int i, uint32_t parity) { return wait_or_abort(bar(i), parity, p.wait_ns, abort_flag); };
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (loads wait long, the others mostly not at all)
+  auto wait_long = [&](int i, uint32_t parity) { return wait_or_abort(bar(i), parity, p.wait_ns, abort_flag); };
+  auto wait = [&](int i, uint32_t parity) { return wait_quick(bar(i), parity, p.wait_ns, abort_flag); };
+  // (the warp index by a shuffle: uniform to the compiler, which then keeps the MMA operands in
+  // uniform registers)
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   griddep_launch_dependents();
   if (s_base & 1023u) {  // swizzled tiles need a 1024-byte aligned window (the whole grid returns)
@@ -177,7 +182,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   int issued_c = 0, issued_x = 0;  // loads issued (their own threads' counts)
   bool mma_issued = false;
@@ -190,7 +195,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
       const int y = e * p.n_out + tile % f.row_tiles * CTA_ROWS;
       if (lane == 0) {
         for (int c = q0; c < q1; ++c) {
-          ok = wait(LY::B_CEMPTY + ring.s, ring.ph ^ 1u);
+          ok = wait_long(LY::B_CEMPTY + ring.s, ring.ph ^ 1u);
           if (!ok) break;
           const uint32_t full = bar(LY::B_CFULL + ring.s), dst = s_base + LY::OFF_C + ring.s * LY::CSTAGE;
           mbar_arrive_expect_tx(full, LY::CSTAGE);
@@ -211,7 +216,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
       int lo, hi;
       find_item(p, tile / f.row_tiles, NT, lo, hi);
       for (int i = 0; i < steps; ++i) {
-        ok = __all_sync(0xffffffffu, wait(LY::B_XEMPTY + ring.s, ring.ph ^ 1u));
+        ok = __all_sync(0xffffffffu, wait_long(LY::B_XEMPTY + ring.s, ring.ph ^ 1u));
         if (!ok) break;
         const uint32_t full = bar(LY::B_XFULL + ring.s), dst = s_base + LY::OFF_X + ring.s * SP * LY::XSLAB;
         const int n = min(SP, slabs - i * SP);
@@ -233,23 +238,26 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
       }
     }
   } else if (warp >= MMA_WARP) {
-    // Two issuing threads, one a weight tile: the waits and commits of one hide behind the MMAs
-    // of the other (one thread for both left the tensor pipe idle half of the time).
-    if (lane == 0) {
-      constexpr uint32_t ID = tc::idesc(128, NT, false);
-      const int t = warp - MMA_WARP;
-      const uint32_t d = tmem + t * NT;
-      Ring<XS> xr;
-      Ring<AB> ar;
-      uint32_t dph = 1;
-      for (int tile = first; tile < tiles && ok; tile += step, dph ^= 1u) {
-        ok = wait(LY::B_DEMPTY, dph);
-        for (int i = 0; i < steps && ok; ++i) {
-          ok = wait(LY::B_XFULL + xr.s, xr.ph) && wait(LY::B_AFULL + ar.s, ar.ph);
-          if (!ok) break;
-          tc::fence_after();
-          const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + xr.s * SP * LY::XSLAB, 16, 1024);
-          const uint32_t a = tmem + LY::A_COL + ar.s * 64 * SP + t * 32;
+    // Two issuing warps, one a weight tile: the waits and commits of one hide behind the MMAs of the other
+    // (one for both left the tensor pipe idle half of the time).  The whole warp runs the loop,
+    // converged, and one lane issues: with a divergent loop every operand of every MMA moves to a
+    // uniform register first.
+    constexpr uint32_t ID = tc::idesc(128, NT, false);
+    const bool lead = elect_one();
+    const int t = warp - MMA_WARP;
+    const uint32_t d = tmem + t * NT;
+    Ring<XS> xr;
+    Ring<AB> ar;
+    uint32_t dph = 1;
+    for (int tile = first; tile < tiles && ok; tile += step, dph ^= 1u) {
+      ok = __all_sync(0xffffffffu, wait(LY::B_DEMPTY, dph));
+      for (int i = 0; i < steps && ok; ++i) {
+        ok = __all_sync(0xffffffffu, wait(LY::B_XFULL + xr.s, xr.ph) && wait(LY::B_AFULL + ar.s, ar.ph));
+        if (!ok) break;
+        tc::fence_after();
+        const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + xr.s * SP * LY::XSLAB, 16, 1024);
+        const uint32_t a = tmem + LY::A_COL + ar.s * 64 * SP + t * 32;
+        if (lead) {
           // (descriptor addresses count 16-byte units: 32 bytes of a swizzled row are 16 inputs)
           tc::mma_ts(d, a, xd, ID, i > 0 ? 1u : 0u);
 #pragma unroll
@@ -258,34 +266,23 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) tc::mma_ts(d, a + 64 + ks * 8, xd + LY::XSLAB / 16 + ks * 2, ID, 1u);
           }
-          mma_issued = true;
           tc::commit(bar(LY::B_XEMPTY + xr.s));
           tc::commit(bar(LY::B_AEMPTY + ar.s));
-          xr.next();
-          ar.next();
         }
-        if (ok) tc::commit(bar(LY::B_DFULL));
+        mma_issued = lead;
+        xr.next();
+        ar.next();
       }
+      if (ok && lead) tc::commit(bar(LY::B_DFULL));
     }
   } else {
-    // ---- dequantization: one weight row of tile t a thread, slab `group` of every step.  A slab's
-    // store into TMEM completes while the next one is dequantized, and only then is it handed
-    // to the MMA threads.
+    // ---- dequantization: one weight row of tile t a thread, slab `group` of every step
     const int group = warp >> 3, t = (warp >> 2) & 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t a_base = tmem + LY::A_COL + group * 64 + t * 32 + lane_base;
     Ring<CS> cr;
     Ring<AB> ar;
-    int stored = -1;  // buffer of the store in flight
-    auto publish = [&]() {
-      if (stored >= 0) {
-        tc::tmem_wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(LY::B_AFULL + stored));
-      }
-    };
     int k = 0;
     for (int tile = first; tile < tiles && ok; tile += step, ++k) {
       int lo, hi;
@@ -321,12 +318,13 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
               for (int q = 0; q < 4; ++q) o[4 * j + q] = d[q];
             }
           }
-          publish();
           ok = __all_sync(0xffffffffu, wait(LY::B_AEMPTY + ar.s, ar.ph ^ 1u));
           if (!ok) break;
           tc::fence_after();
-          if (s < in_stage) tc::tmem_st32_nowait(a_base + ar.s * 64 * SP, o);
-          stored = ar.s;
+          if (s < in_stage) tc::tmem_st32(a_base + ar.s * 64 * SP, o);  // (17 cycles with its wait)
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(LY::B_AFULL + ar.s));
           ar.next();
         }
         if (!ok) break;
@@ -336,8 +334,6 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
         pv = pnext;
       }
       if (!ok) break;
-      publish();
-      stored = -1;
       const int b = k & 1;
       ok = __all_sync(0xffffffffu, wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1));
       if (!ok) break;
@@ -355,61 +351,52 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
         }
         break;
       }
-      // ---- output: lane = weight row, columns = tokens; 16 tokens at a time through the warp's
-      // own shared memory, so that a token's 32 rows leave as 64 bytes
+      // ---- output: 16 tokens at a time, from mma fragments (thread (g8, t4): rows g8 + 8 i, tokens 2 t4, + 1
+      // of eight)
       constexpr int PARTS = GATED ? DW / 4 : DW / 8;  // warps that share a lane quarter (and tile)
       constexpr int COLS = NT / PARTS;
       const int part = GATED ? warp >> 2 : group;
+      const int g8 = lane >> 2, t4 = lane & 3;
       const int row0 = n0 + (GATED ? 0 : t * 128) + quarter * 32;
-      const int64_t wr = (int64_t)e * p.n_out + min(row0 + lane, p.n_out - 1);
-      const float rs0 = p.row_scale[0][wr], rs1 = GATED ? p.row_scale[1][wr] : 0.0f;
-      uint16_t* so = reinterpret_cast<uint16_t*>(smem + LY::OFF_OUT + warp * 1024);
-      const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+      float rs[GATED ? 2 : 1][4];
+#pragma unroll
+      for (int m = 0; m < (GATED ? 2 : 1); ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          rs[m][i] = __ldg(p.row_scale[m] + (int64_t)e * p.n_out + min(row0 + g8 + 8 * i, p.n_out - 1));
+      uint8_t* so = smem + LY::OFF_OUT + warp * 16 * kOutPitch;
 #pragma unroll 1
       for (int cb = part * COLS; cb < (part + 1) * COLS; cb += 16) {
         if (lo + cb >= hi) break;
-        float g[16], u[16];
-        tc::tmem_ld16(tmem + (GATED ? 0 : t * NT) + cb + lane_base, g);
-        if constexpr (GATED) tc::tmem_ld16(tmem + NT + cb + lane_base, u);
-        const float4* ts4 = reinterpret_cast<const float4*>(tok_scale + b * NT + cb);
+        float v[GATED ? 2 : 1][2][8];  // [matrix][16 rows][token block, row g8 or g8 + 8, token]
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float4 tv = ts4[j >> 2];
-          const float ts = (j & 3) == 0 ? tv.x : (j & 3) == 1 ? tv.y : (j & 3) == 2 ? tv.z : tv.w;
-          g[j] *= rs0 * ts;
-          if constexpr (GATED) g[j] = silu_mul(g[j], u[j] * (rs1 * ts));
-        }
+        for (int m = 0; m < (GATED ? 2 : 1); ++m)
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          uint32_t h;
-          if (p.bf16) {
-            const __nv_bfloat162 v = __floats2bfloat162_rn(g[j], g[j + 1]);
-            h = *reinterpret_cast<const uint32_t*>(&v);
-          } else {
-            h = pack_half2(g[j], g[j + 1]);
+          for (int h = 0; h < 2; ++h)
+            tc::tmem_ld_16x16_nowait(tmem + (GATED ? m * NT : t * NT) + cb + lane_base + (static_cast<uint32_t>(16 * h) << 16),
+                                     v[m][h]);
+        float2 ts[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) ts[j] = *reinterpret_cast<const float2*>(tok_scale + b * NT + cb + 8 * j + 2 * t4);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float f = (i & 1) ? ts[i >> 2].y : ts[i >> 2].x;
+            const int r4 = 2 * h + ((i >> 1) & 1);
+            v[0][h][i] *= rs[0][r4] * f;
+            if constexpr (GATED) v[0][h][i] = silu_mul(v[0][h][i], v[1][h][i] * (rs[1][r4] * f));
           }
-          so[j * 32 + lane] = static_cast<uint16_t>(h);
-          so[(j + 1) * 32 + lane] = static_cast<uint16_t>(h >> 16);
-        }
-        __syncwarp();
+        uint32_t q[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int tok = h * 8 + (lane >> 2), col = (lane & 3) * 8;
-          const int left = p.n_out - (row0 + col);
-          const uint4 d = *reinterpret_cast<const uint4*>(so + tok * 32 + col);
-          if (lo + cb + tok < hi && left > 0) {
-            uint16_t* dst = p.out + (int64_t)(lo + cb + tok) * p.out_stride + row0 + col;
-            if (wide && left >= 8) {
-              *reinterpret_cast<uint4*>(dst) = d;
-            } else {
-              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (j < left) dst[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
-            }
+          for (int h = 0; h < 2; ++h) {
+            q[j][2 * h] = pack_out(p, v[0][h][4 * j], v[0][h][4 * j + 1]);
+            q[j][2 * h + 1] = pack_out(p, v[0][h][4 * j + 2], v[0][h][4 * j + 3]);
           }
-        }
-        __syncwarp();
+        store_tokens(p, so, q, lo + cb, hi, row0);
       }
       // the accumulators and the tokens' scales are read
       tc::fence_before();
@@ -423,53 +410,55 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
   if (!ok) *abort_flag = 1;
   __syncwarp();
   if (f.ck > 1) {
-    // the ranks' sums of a token and row, added in rank order; a rank finishes its share of the
-    // tokens, two rows a thread
+    // the ranks' sums of a token and row, added in rank order; a rank finishes its share of the tokens,
+    // a thread four rows of every TL-th of them
     griddep_wait();
+    int lo, hi;
+    const int e = find_item(p, first / f.row_tiles, NT, lo, hi);
+    const int n0 = first % f.row_tiles * CTA_ROWS;
+    constexpr int QUADS = CTA_ROWS / 4, TL = LY::THREADS / QUADS;
+    const int rr = tid % QUADS * 4, tl = tid / QUADS, row = n0 + rr;
+    float rs[GATED ? 2 : 1][4];
+#pragma unroll
+    for (int m = 0; m < (GATED ? 2 : 1); ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rs[m][i] = __ldg(p.row_scale[m] + (int64_t)e * p.n_out + min(row + i, p.n_out - 1));
     cluster_sync_all();
-    if (!*abort_flag) {
-      int lo, hi;
-      const int e = find_item(p, first / f.row_tiles, NT, lo, hi);
-      const int n0 = first % f.row_tiles * CTA_ROWS;
+    if (!*abort_flag && tl < TL && row < p.n_out) {
       const int m = hi - lo;
       const int t0 = m * rank / f.ck, t1 = m * (rank + 1) / f.ck;
-      constexpr int PAIRS = CTA_ROWS / 2;
-      const bool wide = (p.out_stride & 1) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0;
-      for (int o = tid; o < PAIRS * (t1 - t0); o += LY::THREADS) {
-        const int tok = t0 + o / PAIRS, rr = (o % PAIRS) * 2;
-        const int row = n0 + rr;
-        if (row >= p.n_out) continue;
-        const uint32_t at = s_base + (((GATED ? 0 : rr >> 7) * NT + tok) * 128 + (rr & 127)) * 4;
-        float2 a[8], b[8];
+      const bool wide = (p.out_stride & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && row + 4 <= p.n_out;
+      const uint32_t at0 = s_base + ((GATED ? 0 : rr >> 7) * NT * 128 + (rr & 127)) * 4;
+      for (int tok = t0 + tl; tok < t1; tok += TL) {
+        float4 s[GATED ? 2 : 1] = {};
+#pragma unroll 8
+        for (int c = 0; c < f.ck; ++c) {
+          const uint32_t at = dsmem_addr(at0, c) + tok * 512;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          a[c] = c < f.ck ? ld_dsmem_f32x2(dsmem_addr(at, c)) : make_float2(0.0f, 0.0f);
-          if constexpr (GATED) b[c] = c < f.ck ? ld_dsmem_f32x2(dsmem_addr(at + NT * 128 * 4, c)) : make_float2(0.0f, 0.0f);
-        }
-#pragma unroll
-        for (int c = 1; c < 8; ++c) {
-          a[0].x += a[c].x;
-          a[0].y += a[c].y;
-          if constexpr (GATED) {
-            b[0].x += b[c].x;
-            b[0].y += b[c].y;
+          for (int k = 0; k < (GATED ? 2 : 1); ++k) {
+            const float4 v = ld_dsmem_f32x4(at + k * NT * 512);
+            s[k].x += v.x;
+            s[k].y += v.y;
+            s[k].z += v.z;
+            s[k].w += v.w;
           }
         }
         const float ts = tok_scale[tok];
-        const int64_t wr = (int64_t)e * p.n_out + row;
-        const bool two = row + 1 < p.n_out;
-        float y0 = a[0].x * (p.row_scale[0][wr] * ts), y1 = two ? a[0].y * (p.row_scale[0][wr + 1] * ts) : 0.0f;
+        float y[4] = {s[0].x, s[0].y, s[0].z, s[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] *= rs[0][i] * ts;
         if constexpr (GATED) {
-          y0 = silu_mul(y0, b[0].x * (p.row_scale[1][wr] * ts));
-          if (two) y1 = silu_mul(y1, b[0].y * (p.row_scale[1][wr + 1] * ts));
+          const float w[4] = {s[1].x, s[1].y, s[1].z, s[1].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = silu_mul(y[i], w[i] * (rs[1][i] * ts));
         }
-        const uint32_t h0 = p.bf16 ? f2h<true>(y0) : f2h<false>(y0), h1 = p.bf16 ? f2h<true>(y1) : f2h<false>(y1);
         uint16_t* dst = p.out + (int64_t)(lo + tok) * p.out_stride + row;
-        if (wide && two) {
-          *reinterpret_cast<uint32_t*>(dst) = h0 | (h1 << 16);
+        if (wide) {
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_out(p, y[0], y[1]), pack_out(p, y[2], y[3]));
         } else {
-          dst[0] = static_cast<uint16_t>(h0);
-          if (two) dst[1] = static_cast<uint16_t>(h1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (row + i < p.n_out) dst[i] = p.bf16 ? f2h<true>(y[i]) : f2h<false>(y[i]);
         }
       }
     }
@@ -486,7 +475,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     if (warp == X_WARP && lane == 0)
       for (int j = max(0, issued_x - XS); j < issued_x; ++j)
         mbar_wait_bounded(bar(LY::B_XFULL + j % XS), (j / XS) & 1, kDrainNs);
-    if (warp >= MMA_WARP && lane == 0 && mma_issued) {
+    if (warp >= MMA_WARP && mma_issued) {
       tc::commit(bar(LY::B_DRAIN + warp - MMA_WARP));
       mbar_wait_bounded(bar(LY::B_DRAIN + warp - MMA_WARP), 0, kDrainNs);
     }
@@ -564,8 +553,16 @@ static cudaError_t launch_tiles(const LinearParams& p, cudaStream_t stream) {
 }
 
 cudaError_t launch_linear_tiles(const LinearParams& p, bool pairs, cudaStream_t stream) {
-  linear_rows_kernel<<<p.rows, 128, 0, stream>>>(p);
-  cudaError_t err = cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.rows);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, linear_rows_kernel, p);
   if (err != cudaSuccess) return err;
   if (pairs) return launch_linear_pair(p, stream);
   switch (linear_token_tile(p.rows, p.experts, p.offsets != nullptr)) {

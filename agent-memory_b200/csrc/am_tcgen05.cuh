@@ -238,4 +238,13 @@ __device__ __forceinline__ bool wait_quick(uint32_t bar, uint32_t parity, uint64
   return done || wait_or_abort_slow(bar, parity, limit_ns, abort_flag);
 }
 
+// True on one lane of the (converged) warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(p));
+  return p != 0;
+}
+
 }  // namespace am
