@@ -37,38 +37,63 @@
 namespace am {
 
 // ---------------------------------------------------------------- activations
-__global__ void __launch_bounds__(128) linear_rows_kernel(const __grid_constant__ LinearParams p) {
-  __shared__ uint32_t wmax[4];
+// A team of TEAM threads a row (a warp up to 2048 inputs, else the CTA): all of its 16-byte vectors are
+// loaded before the first is used and stay in registers between the maximum and the conversion
+// (up to kRowVectors a thread; longer rows are read twice).
+constexpr int kRowThreads = 256, kRowVectors = 8;
+
+template <int TEAM>
+__global__ void __launch_bounds__(kRowThreads) linear_rows_kernel(const __grid_constant__ LinearParams p) {
+  __shared__ uint32_t wmax[kRowThreads / 32];
   griddep_wait();
   griddep_launch_dependents();  // (not earlier: the next grid reads the weights before its own wait)
-  const int row = blockIdx.x, tid = threadIdx.x;
+  const int row = blockIdx.x * (kRowThreads / TEAM) + threadIdx.x / TEAM, tid = threadIdx.x % TEAM;
+  if (row >= p.rows) return;  // (whole teams)
   const int from = source_row(p, row);
   const uint4* src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(from, 0) * p.x_stride);
   uint4* dst = reinterpret_cast<uint4*>(p.xh + (int64_t)row * p.n_in);
-  const int vecs = p.n_in / 8;
-  if (from < 0) {
-    for (int i = tid; i < vecs; i += 128) dst[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) p.xscale[row] = 1.0f;
-    return;
-  }
-  if (!p.bf16) {
-    for (int i = tid; i < vecs; i += 128) {
-      const uint4 u = src[i];
-      dst[i] = permute_f16(u);
-    }
-    if (tid == 0) p.xscale[row] = 1.0f;
-    return;
-  }
+  const int vecs = from < 0 ? 0 : p.n_in / 8;
+  const bool held = vecs <= TEAM * kRowVectors;
+  uint4 u[kRowVectors];
   uint32_t mx = 0;
-  for (int i = tid; i < vecs; i += 128) mx = max(mx, max_abs_bits(src[i]));
+  for (int i0 = 0; i0 < vecs; i0 += TEAM * kRowVectors) {
+#pragma unroll
+    for (int j = 0; j < kRowVectors; ++j) {
+      const int i = i0 + j * TEAM + tid;
+      u[j] = i < vecs ? src[i] : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < kRowVectors; ++j) mx = max(mx, max_abs_bits(u[j]));
+    if (!p.bf16) {  // fp16 values stay as they are
+#pragma unroll
+      for (int j = 0; j < kRowVectors; ++j) {
+        const int i = i0 + j * TEAM + tid;
+        if (i < vecs) dst[i] = permute_f16(u[j]);
+      }
+    }
+  }
+  if (!p.bf16 || from < 0) {
+    if (tid == 0) p.xscale[row] = 1.0f;
+    if (from < 0)
+      for (int i = tid; i < p.n_in / 8; i += TEAM) dst[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
   mx = __reduce_max_sync(0xffffffffu, mx);
-  if ((tid & 31) == 0) wmax[tid >> 5] = mx;
-  __syncthreads();
-  mx = max(max(wmax[0], wmax[1]), max(wmax[2], wmax[3]));
+  if constexpr (TEAM > 32) {
+    if ((tid & 31) == 0) wmax[tid >> 5] = mx;
+    __syncthreads();
+    mx = __reduce_max_sync(0xffffffffu, wmax[tid & (TEAM / 32 - 1)]);
+  }
   const int ex = row_exponent(mx);
-  const float inv = exp2f(static_cast<float>(-ex));
-  for (int i = tid; i < vecs; i += 128) dst[i] = permute_bf16(src[i], inv);
-  if (tid == 0) p.xscale[row] = exp2f(static_cast<float>(ex));
+  const float inv = exp2_int(-ex);
+  for (int i0 = 0; i0 < vecs; i0 += TEAM * kRowVectors) {
+#pragma unroll
+    for (int j = 0; j < kRowVectors; ++j) {
+      const int i = i0 + j * TEAM + tid;
+      if (i < vecs) dst[i] = permute_bf16(held ? u[j] : src[i], inv);
+    }
+  }
+  if (tid == 0) p.xscale[row] = exp2_int(ex);
 }
 
 // ---------------------------------------------------------------- tiles
@@ -554,15 +579,16 @@ static cudaError_t launch_tiles(const LinearParams& p, cudaStream_t stream) {
 
 cudaError_t launch_linear_tiles(const LinearParams& p, bool pairs, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.rows);
-  cfg.blockDim = dim3(128);
+  const int team = p.n_in <= 32 * 8 * kRowVectors ? 32 : kRowThreads;
+  cfg.gridDim = dim3((p.rows + kRowThreads / team - 1) / (kRowThreads / team));
+  cfg.blockDim = dim3(kRowThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, linear_rows_kernel, p);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, team == 32 ? linear_rows_kernel<32> : linear_rows_kernel<kRowThreads>, p);
   if (err != cudaSuccess) return err;
   if (pairs) return launch_linear_pair(p, stream);
   switch (linear_token_tile(p.rows, p.experts, p.offsets != nullptr)) {
