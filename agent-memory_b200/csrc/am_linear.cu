@@ -212,10 +212,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   }
 
   // ---- load side: walks the positions [p0, p1) D - 1 stages ahead of the sums.  A lane fetches 16
-  // bytes of rows lane / 8 + 4 j of the tile and a parameter of rows lane / 4 + 8 j.  (cp.async:
+  // bytes of rows lane / 8 + 4 j of the tile, lanes 0 to 15 the parameters of a row.  (cp.async:
   // tensor-map boxes of 16 rows reached 3.5 TB/s here, these copies 6.1.)
   const int row_bytes = p.n_in / 2;
-  const int64_t codes4 = (int64_t)4 * row_bytes, par8 = (int64_t)8 * p.pstride * 4;  // bytes to the next j
+  const int64_t codes4 = (int64_t)4 * row_bytes;  // bytes to the next j
   const int64_t tile_bytes = (int64_t)wr_n * TROWS * row_bytes - stages * 128;  // from a tile's end to the next
   const int64_t tile_par = (int64_t)wr_n * TROWS * p.pstride * 4 - stages * 16;
   const uint8_t *l_codes = nullptr, *l_par = nullptr;  // this lane's bytes of the next stage, matrix 0
@@ -223,9 +223,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
                                    : (int64_t)16 * row_bytes;
   const int64_t par_diff = GATED ? reinterpret_cast<const uint8_t*>(p.params[1]) - reinterpret_cast<const uint8_t*>(p.params[0])
                                  : (int64_t)16 * p.pstride * 4;
-  const uint32_t l_dst0 = smem_u32(ring) + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);  // row + 4: chunk ^ 4
-  const uint32_t l_flip = ((l_dst0 ^ 64) - l_dst0);
-  const uint32_t l_pdst0 = smem_u32(ring) + 2048 + (lane >> 2) * 16 + (lane & 3) * 4;
+  // chunk c of row r at c ^ 2 (r % 4): the eight bytes a lane reads of four rows lie in distinct banks
+  const uint32_t l_dst0 = smem_u32(ring) + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) << 1)) << 4);
+  const uint32_t l_pdst0 = smem_u32(ring) + 2048 + (lane & 15) * 16;
   const int item0 = p0 / f.tiles;
   int l_left = n_pos, l_item = item0, l_pos = p0 - item0 * f.tiles;  // (position in the item)
   int l_stage = 0;
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
     const int64_t row = (int64_t)max(e, 0) * p.n_out + first;
     l_rows = p.n_out - first;
     l_codes = reinterpret_cast<const uint8_t*>(p.codes[0]) + (row + (lane >> 3)) * row_bytes + qa * 128 + (lane & 7) * 16;
-    l_par = reinterpret_cast<const uint8_t*>(p.params[0]) + ((row + (lane >> 2)) * p.pstride + qa * 4 + (lane & 3)) * 4;
+    l_par = reinterpret_cast<const uint8_t*>(p.params[0]) + ((row + (lane & 15)) * p.pstride + qa * 4) * 4;
   };
   if (l_left > 0) l_open();
   auto fetch = [&]() {
@@ -251,11 +251,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
         for (int i = 0; i < MT; ++i) {
           const uint8_t* src = l_codes + i * codes_diff;
           cp_async16_s(dst + i * (kFewCodes + kFewPar), src);
-          cp_async16_s(dst + l_flip + i * (kFewCodes + kFewPar) + 512, src + codes4);
+          cp_async16_s(dst + i * (kFewCodes + kFewPar) + 512, src + codes4);
           cp_async16_s(dst + i * (kFewCodes + kFewPar) + 1024, src + 2 * codes4);
-          cp_async16_s(dst + l_flip + i * (kFewCodes + kFewPar) + 1536, src + 3 * codes4);
-          cp_async4_s(pdst + i * (kFewCodes + kFewPar), l_par + i * par_diff);
-          cp_async4_s(pdst + i * (kFewCodes + kFewPar) + 128, l_par + i * par_diff + par8);
+          cp_async16_s(dst + i * (kFewCodes + kFewPar) + 1536, src + 3 * codes4);
+          if (lane < 16) cp_async16_ca_s(pdst + i * (kFewCodes + kFewPar), l_par + i * par_diff);
         }
       } else {
 #pragma unroll 1
@@ -263,10 +262,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
           const int rows = l_rows - (GATED ? 0 : 16 * i);
           for (int j = 0; j < 4; ++j)
             if ((lane >> 3) + 4 * j < rows && (lane & 7) < chunks)
-              cp_async16_s(dst + (j & 1) * l_flip + i * (kFewCodes + kFewPar) + j * 512, l_codes + i * codes_diff + j * codes4);
-          for (int j = 0; j < 2; ++j)
-            if ((lane >> 2) + 8 * j < rows)
-              cp_async4_s(pdst + i * (kFewCodes + kFewPar) + j * 128, l_par + i * par_diff + j * par8);
+              cp_async16_s(dst + i * (kFewCodes + kFewPar) + j * 512, l_codes + i * codes_diff + j * codes4);
+          if (lane < min(rows, 16)) cp_async16_ca_s(pdst + i * (kFewCodes + kFewPar), l_par + i * par_diff);
         }
       }
       l_codes += 128;
@@ -336,7 +333,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   // activations and its two columns' sums in a group
   uint32_t woff[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) woff[q] = g8 * 128 + (((2 * q + (t4 >> 1)) ^ g8) << 4) + (t4 & 1) * 8;
+  for (int q = 0; q < 4; ++q) woff[q] = g8 * 128 + (((2 * q + (t4 >> 1)) ^ ((g8 & 3) << 1)) << 4) + (t4 & 1) * 8;
   const uint8_t* xlane = sx + (ga - ca) * XG + (g8 & (TK - 1)) * 64 + t4 * 16;
   const float* slane = sxsum + (ga - ca) * TK + ((2 * t4) & (TK - 1));
   int left = n_pos, it = item0, tile0 = p0 - item0 * f.tiles;
@@ -384,8 +381,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
             for (int h = 0; h < 2; ++h)
               pq[i][h] = *reinterpret_cast<const uint4*>(src + i * (kFewCodes + kFewPar) + 2048 + (g8 + 8 * h) * 16);
           auto group = [&](int q) {
-            const uint4 b0 = *reinterpret_cast<const uint4*>(xs + q * XG);
-            const uint4 b1 = *reinterpret_cast<const uint4*>(xs + q * XG + TK * 64);
+            // column g8 of B: the columns past TK are never read, and a 16-byte load costs a
+            // pass of shared memory for every eight lanes that take part
+            uint4 b0 = make_uint4(0, 0, 0, 0), b1 = b0;
+            if (TK == 8 || g8 < TK) {
+              b0 = *reinterpret_cast<const uint4*>(xs + q * XG);
+              b1 = *reinterpret_cast<const uint4*>(xs + q * XG + TK * 64);
+            }
             float2 sm;
             if constexpr (TK == 1)
               sm = make_float2(ss[q], 0.0f);
