@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
 
   griddep_launch_dependents();
   // positions [p0, p0 + n_pos) of the sequence of all items' positions
-  int items = (p.rows + kFewTokens - 1) / kFewTokens, p0, n_pos;
+  int items = (p.rows + TK - 1) / TK, p0, n_pos;
   auto share = [&]() {
     const int total = items * f.tiles, each = total / clusters, more = total - each * clusters;
     p0 = each * cluster + min(cluster, more);
@@ -205,12 +205,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
       }
     }
   }
-  griddep_wait();
-  if (p.offsets != nullptr) {
-    items = count_items(p, kFewTokens);
-    share();
-  }
-
   // ---- load side: walks the positions [p0, p1) D - 1 stages ahead of the sums.  A lane fetches 16
   // bytes of rows lane / 8 + 4 j of the tile, lanes 0 to 15 the parameters of a row.  (cp.async:
   // tensor-map boxes of 16 rows reached 3.5 TB/s here, these copies 6.1.)
@@ -226,21 +220,27 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   // chunk c of row r at c ^ 2 (r % 4): the eight bytes a lane reads of four rows lie in distinct banks
   const uint32_t l_dst0 = smem_u32(ring) + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) << 1)) << 4);
   const uint32_t l_pdst0 = smem_u32(ring) + 2048 + (lane & 15) * 16;
-  const int item0 = p0 / f.tiles;
-  int l_left = n_pos, l_item = item0, l_pos = p0 - item0 * f.tiles;  // (position in the item)
+  int item0, l_left, l_item, l_pos;  // (l_pos: position in the item)
   int l_stage = 0;
   uint32_t l_off = 0;  // of the next stage's buffer
   int l_rows = 0;      // weight rows from the tile's first one to the matrix's end
   auto l_open = [&]() {  // position l_pos of item l_item
     int lo, hi;
-    const int e = find_item(p, l_item, kFewTokens, lo, hi);
+    const int e = find_item(p, l_item, TK, lo, hi);
     const int first = (l_pos * wr_n + wr) * TROWS;
     const int64_t row = (int64_t)max(e, 0) * p.n_out + first;
     l_rows = p.n_out - first;
     l_codes = reinterpret_cast<const uint8_t*>(p.codes[0]) + (row + (lane >> 3)) * row_bytes + qa * 128 + (lane & 7) * 16;
     l_par = reinterpret_cast<const uint8_t*>(p.params[0]) + ((row + (lane & 15)) * p.pstride + qa * 4) * 4;
   };
-  if (l_left > 0) l_open();
+  auto l_begin = [&]() {
+    item0 = p0 / f.tiles;
+    l_left = n_pos;
+    l_item = item0;
+    l_pos = p0 - item0 * f.tiles;
+    if (l_left > 0) l_open();
+  };
+  if (p.offsets == nullptr) l_begin();
   auto fetch = [&]() {
     if (l_left > 0) {
       const uint32_t dst = l_dst0 + l_off, pdst = l_pdst0 + l_off;
@@ -284,36 +284,59 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
     }
     cp_async_commit();
   };
-#pragma unroll 1
-  for (int i = 0; i < D - 1; ++i) fetch();
 
   // ---- compute side
   int item = -1, e = 0, lo = 0, hi = 0, m = 0, buf = 0;
   // The item's activations of this CTA's inputs, the largest |x| of a token to [2^14, 2^15): 16 / TK
-  // warps a token, a lane's vectors read for the maximum and again (from L1) for the conversion.
-  constexpr int WPT = kFewWarps / TK;
+  // warps a token.  A lane holds its first XH vectors of 8 from the maximum to the conversion (4096
+  // inputs at 8 tokens), the others are read twice.  They are asked for before the item's codes:
+  // their way from L2 and the issue of the first copies take a microsecond each (1 token
+  // 4096x4096 5.9 -> 5.5 us, 8 tokens 8.8 -> 7.5).  The gated kernel has no registers for eight.
+  constexpr int WPT = kFewWarps / TK, XH = TK == 8 && !GATED ? 8 : 4;
+  const int vecs = (cb - ca) * 8;  // 16-byte vectors of a token
+  const int x_tok = warp / WPT, v0 = warp % WPT * 32 + lane;
+  uint4 held[XH];
+  auto open_item = [&](int i) {
+    e = find_item(p, i, TK, lo, hi);
+    item = i;
+    m = hi - lo;
+    const int x_row = x_tok < m ? source_row(p, lo + x_tok) : -1;
+    const uint4* x_src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(x_row, 0) * p.x_stride + (int64_t)ca * 64);
+#pragma unroll
+    for (int j = 0; j < XH; ++j) {
+      held[j] = make_uint4(0, 0, 0, 0);
+      if (x_row >= 0 && v0 + j * 32 * WPT < vecs) held[j] = x_src[v0 + j * 32 * WPT];
+    }
+  };
+  griddep_wait();
+  if (p.offsets != nullptr) {
+    items = count_items(p, TK);
+    share();
+    l_begin();
+  }
+  if (n_pos > 0) open_item(item0);
+#pragma unroll 1
+  for (int i = 0; i < D - 1; ++i) fetch();
+
   auto stage_x = [&]() {
-    const int tok = warp / WPT, part = warp % WPT;
-    const int vecs = (cb - ca) * 8;  // 16-byte vectors of the token
-    const int row = tok < m ? source_row(p, lo + tok) : -1;
-    const uint4* src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(row, 0) * p.x_stride + (int64_t)ca * 64);
-    const int v0 = part * 32 + lane;
+    const int x_tok = warp / WPT, v0 = warp % WPT * 32 + lane, vecs = (cb - ca) * 8;
+    const int x_row = x_tok < m ? source_row(p, lo + x_tok) : -1;
+    const uint4* x_src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(x_row, 0) * p.x_stride + (int64_t)ca * 64);
     uint32_t mx = 0;
-    if (row >= 0) {
-#pragma unroll 8
-      for (int v = v0; v < vecs; v += 32 * WPT) mx = max(mx, max_abs_bits(src[v]));
+#pragma unroll
+    for (int j = 0; j < XH; ++j) mx = max(mx, max_abs_bits(held[j]));
+    if (x_row >= 0) {
+#pragma unroll 4
+      for (int v = v0 + XH * 32 * WPT; v < vecs; v += 32 * WPT) mx = max(mx, max_abs_bits(x_src[v]));
     }
     mx = __reduce_max_sync(0xffffffffu, mx);
     if (lane == 0) sxmax[warp] = __uint_as_float(mx);
     __syncthreads();
-    if (tok < m) {
-      const uint32_t all = lane < WPT ? __float_as_uint(sxmax[tok * WPT + lane]) : 0u;
+    if (x_tok < m) {
+      const uint32_t all = lane < WPT ? __float_as_uint(sxmax[x_tok * WPT + lane]) : 0u;
       mx = __reduce_max_sync(0xffffffffu, all);
       const float inv = exp2_int(-(p.bf16 ? row_exponent(mx) : row_exponent_f16(mx)));
-#pragma unroll 2
-      for (int v = v0; v - lane < vecs; v += 32 * WPT) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (row >= 0 && v < vecs) u = src[v];
+      auto convert = [&](int v, uint4 u) {  // (u is zero where v is past the end)
         float sum;
         const uint4 o = p.bf16 ? stage_inputs<true>(u, inv, sum) : stage_inputs<false>(u, inv, sum);
 #pragma unroll
@@ -321,10 +344,16 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
         // word c of the group: lane c / 2 of the quad, half c & 1
         const int grp = v >> 3, c = v & 7;
         if (v < vecs) {
-          *reinterpret_cast<uint4*>(sx + grp * XG + ((c & 1) * TK + tok) * 64 + (c >> 1) * 16) = o;
-          if (c == 0) sxsum[grp * TK + tok] = sum;
+          *reinterpret_cast<uint4*>(sx + grp * XG + ((c & 1) * TK + x_tok) * 64 + (c >> 1) * 16) = o;
+          if (c == 0) sxsum[grp * TK + x_tok] = sum;
         }
-      }
+      };
+#pragma unroll
+      for (int j = 0; j < XH; ++j)
+        if (v0 - lane + j * 32 * WPT < vecs) convert(v0 + j * 32 * WPT, held[j]);
+#pragma unroll 2
+      for (int v = v0 + XH * 32 * WPT; v - lane < vecs; v += 32 * WPT)
+        convert(v, x_row >= 0 && v < vecs ? x_src[v] : make_uint4(0, 0, 0, 0));
     }
     __syncthreads();
   };
@@ -336,14 +365,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   for (int q = 0; q < 4; ++q) woff[q] = g8 * 128 + (((2 * q + (t4 >> 1)) ^ ((g8 & 3) << 1)) << 4) + (t4 & 1) * 8;
   const uint8_t* xlane = sx + (ga - ca) * XG + (g8 & (TK - 1)) * 64 + t4 * 16;
   const float* slane = sxsum + (ga - ca) * TK + ((2 * t4) & (TK - 1));
-  int left = n_pos, it = item0, tile0 = p0 - item0 * f.tiles;
+  int left = n_pos, it = item0, staged = -1, tile0 = p0 - item0 * f.tiles;
   float tscale[2] = {};  // powers of two of this lane's columns
   while (left > 0) {
     // a batch: positions of one item
-    if (it != item) {
-      e = find_item(p, it, kFewTokens, lo, hi);
-      item = it;
-      m = hi - lo;
+    if (it != staged) {
+      if (it != item) open_item(it);
+      staged = it;
       stage_x();  // (the last batch ended with a barrier after its last read of the activations)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -502,8 +530,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
 constexpr int kFewSmem = 227 * 1024;
 
 template <bool GATED, int MT, int TK>
-static cudaError_t launch_few_t(FewParams& f, int64_t items, cudaStream_t stream) {
+static cudaError_t launch_few_t(FewParams& f, cudaStream_t stream) {
   const LinearParams& p = f.p;
+  // items a grouped call is likely to have, and has at most
+  const int64_t likely = p.offsets != nullptr ? std::min(p.experts, p.rows) : (p.rows + TK - 1) / TK;
+  const int64_t items = p.offsets != nullptr ? likely + p.rows / TK : likely;
   int dev = 0;
   const int sms = sm_count(&dev);
   if (sms == 0) return cudaErrorInvalidDevice;
@@ -538,7 +569,7 @@ static cudaError_t launch_few_t(FewParams& f, int64_t items, cudaStream_t stream
   for (int k = 1; k <= kFewWarps; k *= 2) {
     if (k > 1 && quads < k * ck) break;
     const int wr = kFewWarps / k;
-    const int64_t positions = (int64_t)((row_tiles + wr - 1) / wr) * items;
+    const int64_t positions = (int64_t)((row_tiles + wr - 1) / wr) * likely;
     const double rounds = static_cast<double>((positions + ctas - 1) / ctas);
     const double cost = rounds * ((quads + k * ck - 1) / (k * ck) * 4 + 1.5);
     if (k == 1 || cost < best) {
@@ -570,11 +601,11 @@ static cudaError_t launch_few_t(FewParams& f, int64_t items, cudaStream_t stream
 }
 
 template <bool GATED, int MT, int MT8>
-static cudaError_t launch_few(FewParams& f, int tok, int64_t items, cudaStream_t stream) {
-  if (tok <= 1) return launch_few_t<GATED, MT, 1>(f, items, stream);
-  if (tok <= 2) return launch_few_t<GATED, MT, 2>(f, items, stream);
-  if (tok <= 4) return launch_few_t<GATED, MT, 4>(f, items, stream);
-  return launch_few_t<GATED, MT8, 8>(f, items, stream);
+static cudaError_t launch_few(FewParams& f, int64_t tok, cudaStream_t stream) {
+  if (tok <= 1) return launch_few_t<GATED, MT, 1>(f, stream);
+  if (tok <= 2) return launch_few_t<GATED, MT, 2>(f, stream);
+  if (tok <= 4) return launch_few_t<GATED, MT, 4>(f, stream);
+  return launch_few_t<GATED, MT8, 8>(f, stream);
 }
 
 // Which kernel: the mean number of rows of a matrix decides (a grouped call's counts are on the
@@ -586,13 +617,14 @@ bool linear_uses_tensor_tiles(int rows, int experts, bool grouped) {
 
 cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream) {
   if (p.rows == 0) return cudaSuccess;
-  const int64_t items = p.offsets != nullptr ? (int64_t)std::min(p.experts, p.rows) + p.rows / kFewTokens
-                                             : (p.rows + kFewTokens - 1) / kFewTokens;
   FewParams f{};
   f.p = p;
-  const int tok = std::min(p.rows, kFewTokens);
-  return p.codes[1] != nullptr ? launch_few<true, 2, 2>(f, tok, items, stream)
-                               : launch_few<false, 1, 1>(f, tok, items, stream);
+  // Tokens of an item: all rows of a plain call; for experts twice their mean number (one with
+  // more reads its weights again).  One token of 64 experts: 10.1 us with items of one token, 10.3
+  // with items of eight; 16 tokens, items of four and eight: 42.9 and 45.1.
+  int64_t tok = p.rows;
+  if (p.offsets != nullptr) tok = (2 * (int64_t)p.rows + p.experts - 1) / p.experts;
+  return p.codes[1] != nullptr ? launch_few<true, 2, 2>(f, tok, stream) : launch_few<false, 1, 1>(f, tok, stream);
 }
 
 }  // namespace am
