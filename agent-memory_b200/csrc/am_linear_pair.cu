@@ -121,7 +121,7 @@ struct PairRing {
   }
 };
 
-template <bool GATED>
+template <bool GATED, int PARTS>
 __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams f) {
   using LY = PairLayout<GATED>;
   constexpr int CS = LY::CS, ST = LY::ST, DW = LY::DW;
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
   const int tiles = count_items(p, f.tile_tokens) * f.row_tiles;
   if (first >= tiles) return;  // both CTAs of the pair
   const int stages = p.pstride >> 2;  // quads of groups
-  const int slabs = p.groups, steps = (slabs + 1) / 2;
+  const int slabs = p.groups, steps = (slabs + 1) / 2 * PARTS;  // (a step's parts follow one another)
 
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(tmem_slot)));
@@ -202,11 +202,11 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
         ok = __all_sync(0xffffffffu, wait(LY::B_EMPTY + ring.s, ring.ph ^ 1u));
         if (!ok) break;
         const uint32_t dst = s_base + LY::OFF_X + ring.s * 2 * LY::XSLAB;
-        const int n = min(2, slabs - 2 * i);
+        const int n = min(2, slabs - i / PARTS * 2);
         if (lane == 0) {
           const uint32_t full = bar(LY::B_FULL + ring.s);
           if (rank == 0) mbar_arrive_expect_tx(full, 2 * n * LY::XSLAB);  // both CTAs' bytes
-          for (int s = 0; s < n; ++s) tc2::tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, (2 * i + s) * 128, y, full);
+          for (int s = 0; s < n; ++s) tc2::tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, (i / PARTS * 2 + s) * 128, y, full);
         }
         ++issued_x;
         ring.next();
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
         tc::fence_after();
         const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + ring.s * 2 * LY::XSLAB, 16, 1024);
         const uint32_t a = tmem + LY::A_COL + ring.s * 64, done = bar(LY::B_EMPTY + ring.s);
-        const bool both = 2 * i + 1 < slabs;
+        const bool both = 2 * (i / PARTS) + 1 < slabs;
         ring.next();
         if (lead) {
           // (descriptor addresses count 16-byte units: 32 bytes of a swizzled row are 16 inputs)
@@ -286,29 +286,25 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
         for (int st = 0; st < 2; ++st) {
           if (st * 2 >= in_stage) break;
           const int s = st * 2 + group;
-          uint32_t o[32];
+          uint4 w0, w1;
           if (s < in_stage) {
-            const uint4 w0 = *reinterpret_cast<const uint4*>(crow + (((2 * s) ^ (r & 7)) << 4));
-            const uint4 w1 = *reinterpret_cast<const uint4*>(crow + (((2 * s + 1) ^ (r & 7)) << 4));
-            const uint32_t s24 = __byte_perm(ps[st], ps[st], 0x1010), bb = __byte_perm(ps[st], ps[st], 0x3232);
-            const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);
-            const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint32_t d[4];
-              dequant_word(words[j], s24, s20, bb, d);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) o[4 * j + q] = d[q];
-            }
+            w0 = *reinterpret_cast<const uint4*>(crow + (((2 * s) ^ (r & 7)) << 4));
+            w1 = *reinterpret_cast<const uint4*>(crow + (((2 * s + 1) ^ (r & 7)) << 4));
           }
-          ok = __all_sync(0xffffffffu, wait(LY::B_EMPTY + ring.s, ring.ph ^ 1u));
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) {
+            uint32_t o[32];
+            if (s < in_stage) dequant_group<PARTS>(w0, w1, ps[st], part, o);
+            ok = __all_sync(0xffffffffu, wait(LY::B_EMPTY + ring.s, ring.ph ^ 1u));
+            if (!ok) break;
+            tc::fence_after();
+            if (s < in_stage) tc::tmem_st32(a_base + ring.s * 64, o);
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc2::arrive_cluster(lead_full + ring.s * 8);
+            ring.next();
+          }
           if (!ok) break;
-          tc::fence_after();
-          if (s < in_stage) tc::tmem_st32(a_base + ring.s * 64, o);
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) tc2::arrive_cluster(lead_full + ring.s * 8);
-          ring.next();
         }
         if (!ok) break;
         __syncwarp();  // the stage's codes are in registers
@@ -406,7 +402,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
     };
     // The first ST steps of a tile are dequantized before the output of the one before it: they fill
     // the operand buffers while its last MMAs run, and the next MMAs start with the output done.
-    constexpr int AHEAD = LY::ST / 2;  // stages
+    constexpr int AHEAD = LY::ST / (2 * PARTS);  // stages
     int k = 0, lo = 0, hi = 0, n0 = 0;
     int64_t wbase = 0;
     for (int tile = first; tile < tiles && ok; tile += step, ++k) {
@@ -455,9 +451,9 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
 }
 
 // ---------------------------------------------------------------- host
-template <bool GATED>
+template <bool GATED, int PARTS>
 static cudaError_t launch_pair_t(const PairParams& f, int clusters, int dev, cudaStream_t stream) {
-  auto kfn = linear_pair_kernel<GATED>;
+  auto kfn = linear_pair_kernel<GATED, PARTS>;
   static unsigned long long done = 0;
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
   if (!bit || !(__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) {
@@ -487,7 +483,7 @@ cudaError_t launch_linear_pair(const LinearParams& p, cudaStream_t stream) {
   const int sms = sm_count(&dev);
   if (sms == 0) return cudaErrorInvalidDevice;
   const bool gated = p.codes[1] != nullptr;
-  const int rows = gated ? 128 : 256;
+  const int rows = gated ? 128 : 256, parts = weight_parts(gated, p.bf16);
   PairParams f{};
   f.p = p;
   f.row_tiles = (p.n_out + rows - 1) / rows;
@@ -497,7 +493,7 @@ cudaError_t launch_linear_pair(const LinearParams& p, cudaStream_t stream) {
   if (p.offsets == nullptr) {
     // One matrix: the cut of the tokens that ends first.  A step of 128 inputs measured 4.6 cycles a token
     // (1178 for 256), 950 at least (the MMA thread), a tile's start and output 8000.
-    const double steps = (p.groups + 1) / 2;
+    const double steps = (p.groups + 1) / 2 * parts;
     double best = 0.0;
     for (int n = (p.rows + 255) / 256, tries = 0; tries < 12; ++n, ++tries) {
       const int tokens = ((p.rows + n - 1) / n + 31) & ~31;
@@ -512,7 +508,8 @@ cudaError_t launch_linear_pair(const LinearParams& p, cudaStream_t stream) {
   }
   if (f.row_tiles * items > INT_MAX) return cudaErrorNotSupported;
   const int clusters = static_cast<int>(std::min<int64_t>(f.row_tiles * items, pairs));
-  return gated ? launch_pair_t<true>(f, clusters, dev, stream) : launch_pair_t<false>(f, clusters, dev, stream);
+  if (parts == 2) return launch_pair_t<true, 2>(f, clusters, dev, stream);
+  return gated ? launch_pair_t<true, 1>(f, clusters, dev, stream) : launch_pair_t<false, 1>(f, clusters, dev, stream);
 }
 
 }  // namespace am

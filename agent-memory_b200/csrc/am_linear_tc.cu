@@ -157,7 +157,7 @@ struct TilesParams {
   int32_t row_tiles;  // tiles of CTA_ROWS weight rows
 };
 
-template <int NT, bool GATED>
+template <int NT, bool GATED, int PARTS>
 __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTAS)
     linear_tiles_kernel(const __grid_constant__ TilesParams f) {
   using LY = TilesLayout<NT>;
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
   const int quads = p.pstride >> 2;
   const int q0 = quads * rank / f.ck, q1 = quads * (rank + 1) / f.ck;
   const int slabs = min(q1 * 4, p.groups) - q0 * 4;
-  const int steps = (slabs + SP - 1) / SP;
+  const int steps = (slabs + SP - 1) / SP * PARTS;  // (a step's parts follow one another)
 
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)),
@@ -244,11 +244,11 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
         ok = __all_sync(0xffffffffu, wait_long(LY::B_XEMPTY + ring.s, ring.ph ^ 1u));
         if (!ok) break;
         const uint32_t full = bar(LY::B_XFULL + ring.s), dst = s_base + LY::OFF_X + ring.s * SP * LY::XSLAB;
-        const int n = min(SP, slabs - i * SP);
+        const int n = min(SP, slabs - i / PARTS * SP);
         if (lane == 0) {
           mbar_arrive_expect_tx(full, n * LY::XSLAB);
           for (int s = 0; s < n; ++s)
-            tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, (q0 * 4 + i * SP + s) * 128, lo, full);
+            tma_load_2d(dst + s * LY::XSLAB, &p.tmap_x, (q0 * 4 + i / PARTS * SP + s) * 128, lo, full);
         }
         ++issued_x;
         ring.next();
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
           tc::mma_ts(d, a, xd, ID, i > 0 ? 1u : 0u);
 #pragma unroll
           for (int ks = 1; ks < 4; ++ks) tc::mma_ts(d, a + ks * 8, xd + ks * 2, ID, 1u);
-          if (SP == 2 && 2 * i + 1 < slabs) {
+          if (SP == 2 && 2 * (i / PARTS) + 1 < slabs) {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) tc::mma_ts(d, a + 64 + ks * 8, xd + LY::XSLAB / 16 + ks * 2, ID, 1u);
           }
@@ -327,30 +327,26 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
         for (int st = 0; st < STEPS; ++st) {
           if (st * SP >= in_stage) break;
           const int s = st * SP + group;
-          uint32_t o[32];
+          uint4 w0, w1;
           if (s < in_stage) {
-            const uint4 w0 = *reinterpret_cast<const uint4*>(crow + (((2 * s) ^ (r & 7)) << 4));
-            const uint4 w1 = *reinterpret_cast<const uint4*>(crow + (((2 * s + 1) ^ (r & 7)) << 4));
-            const uint32_t ps = SP == 1 || group == 0 ? pw[st * SP] : pw[(st * SP + 1) & 3];
-            const uint32_t s24 = __byte_perm(ps, ps, 0x1010), bb = __byte_perm(ps, ps, 0x3232);
-            const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);
-            const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint32_t d[4];
-              dequant_word(words[j], s24, s20, bb, d);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) o[4 * j + q] = d[q];
-            }
+            w0 = *reinterpret_cast<const uint4*>(crow + (((2 * s) ^ (r & 7)) << 4));
+            w1 = *reinterpret_cast<const uint4*>(crow + (((2 * s + 1) ^ (r & 7)) << 4));
           }
-          ok = __all_sync(0xffffffffu, wait(LY::B_AEMPTY + ar.s, ar.ph ^ 1u));
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) {
+            uint32_t o[32];
+            if (s < in_stage)
+              dequant_group<PARTS>(w0, w1, SP == 1 || group == 0 ? pw[st * SP] : pw[(st * SP + 1) & 3], part, o);
+            ok = __all_sync(0xffffffffu, wait(LY::B_AEMPTY + ar.s, ar.ph ^ 1u));
+            if (!ok) break;
+            tc::fence_after();
+            if (s < in_stage) tc::tmem_st32(a_base + ar.s * 64 * SP, o);  // (17 cycles with its wait)
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(LY::B_AFULL + ar.s));
+            ar.next();
+          }
           if (!ok) break;
-          tc::fence_after();
-          if (s < in_stage) tc::tmem_st32(a_base + ar.s * 64 * SP, o);  // (17 cycles with its wait)
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(LY::B_AFULL + ar.s));
-          ar.next();
         }
         if (!ok) break;
         __syncwarp();  // the stage's codes are in registers
@@ -378,8 +374,8 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
       }
       // ---- output: 16 tokens at a time, from mma fragments (thread (g8, t4): rows g8 + 8 i, tokens 2 t4, + 1
       // of eight)
-      constexpr int PARTS = GATED ? DW / 4 : DW / 8;  // warps that share a lane quarter (and tile)
-      constexpr int COLS = NT / PARTS;
+      constexpr int SHARES = GATED ? DW / 4 : DW / 8;  // warps that share a lane quarter (and tile)
+      constexpr int COLS = NT / SHARES;
       const int part = GATED ? warp >> 2 : group;
       const int g8 = lane >> 2, t4 = lane & 3;
       const int row0 = n0 + (GATED ? 0 : t * 128) + quarter * 32;
@@ -529,14 +525,14 @@ int linear_token_tile(int rows, int experts, bool grouped) {
   return mean <= 32 ? 32 : (mean <= 64 ? 64 : 128);
 }
 
-template <int NT, bool GATED>
+template <int NT, bool GATED, int PARTS>
 static cudaError_t launch_tiles_t(const LinearParams& p, int64_t items, cudaStream_t stream) {
   using LY = TilesLayout<NT>;
   int dev = 0;
   const int sms = sm_count(&dev);
   if (sms == 0) return cudaErrorInvalidDevice;
   cudaError_t err = cudaSuccess;
-  auto kfn = linear_tiles_kernel<NT, GATED>;
+  auto kfn = linear_tiles_kernel<NT, GATED, PARTS>;
   static unsigned long long done = 0;
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
   if (!bit || !(__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) {
@@ -574,7 +570,9 @@ template <int NT>
 static cudaError_t launch_tiles(const LinearParams& p, cudaStream_t stream) {
   const int64_t items = p.offsets != nullptr ? (int64_t)min(p.experts, p.rows) + p.rows / NT
                                              : ((int64_t)p.rows + NT - 1) / NT;
-  return p.codes[1] != nullptr ? launch_tiles_t<NT, true>(p, items, stream) : launch_tiles_t<NT, false>(p, items, stream);
+  const bool gated = p.codes[1] != nullptr;
+  if (weight_parts(gated, p.bf16) == 2) return launch_tiles_t<NT, true, 2>(p, items, stream);
+  return gated ? launch_tiles_t<NT, true, 1>(p, items, stream) : launch_tiles_t<NT, false, 1>(p, items, stream);
 }
 
 cudaError_t launch_linear_tiles(const LinearParams& p, bool pairs, cudaStream_t stream) {
