@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + LY::OFF_BAR + LY::B_COUNT * 8 + 4);
   float* tok_scale = reinterpret_cast<float*>(smem + LY::OFF_SCALE);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  auto wait = [&](int i, uint32_t parity) { return wait_quick(bar(i), parity, p.wait_ns, abort_flag); };
+  auto wait = [&](int i, uint32_t parity) { return wait_warp(bar(i), parity, p.wait_ns, abort_flag); };
   // (the warp index by a shuffle: uniform to the compiler, which then keeps the MMA operands in
   // uniform registers)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
       const int y = e * p.n_out + tile % f.row_tiles * 2 * CTA_ROWS + rank * CTA_ROWS;
       if (lane == 0) {
         for (int c = 0; c < stages; ++c) {
-          ok = wait(LY::B_CEMPTY + ring.s, ring.ph ^ 1u);
+          ok = wait_quick(bar(LY::B_CEMPTY + ring.s), ring.ph ^ 1u, p.wait_ns, abort_flag);
           if (!ok) break;
           const uint32_t full = bar(LY::B_CFULL + ring.s), dst = s_base + LY::OFF_C + ring.s * LY::CSTAGE;
           mbar_arrive_expect_tx(full, LY::CSTAGE);
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
       const int half = ((hi - lo + 31) & ~31) >> 1;  // tokens of a CTA
       const int y = lo + rank * half;
       for (int i = 0; i < steps; ++i) {
-        ok = __all_sync(0xffffffffu, wait(LY::B_EMPTY + ring.s, ring.ph ^ 1u));
+        ok = wait(LY::B_EMPTY + ring.s, ring.ph ^ 1u);
         if (!ok) break;
         const uint32_t dst = s_base + LY::OFF_X + ring.s * 2 * LY::XSLAB;
         const int n = min(2, slabs - i / PARTS * 2);
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
         ring.next();
         if (i == min(ST, steps) - 1) {  // behind the first loads: the tokens' powers of two
           const int b = k & 1;
-          ok = __all_sync(0xffffffffu, wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1));
+          ok = wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1);
           if (!ok) break;
           for (int j = lane; j < 256; j += 32) tok_scale[b * 256 + j] = lo + j < hi ? p.xscale[lo + j] : 0.0f;
           __syncwarp();
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
       // last MMAs of step i.  (With separate barriers for operand and activations the issuing thread
       // itself took 1450 cycles a step.)  The warp stays converged and one lane issues, as in
       // linear_tiles_kernel.
-      ok = __all_sync(0xffffffffu, wait(LY::B_DEMPTY, dph) && wait(LY::B_FULL + ring.s, ring.ph));
+      ok = wait(LY::B_DEMPTY, dph) && wait(LY::B_FULL + ring.s, ring.ph);
       for (int i = 0; i < steps && ok; ++i) {
         tc::fence_after();
         const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + ring.s * 2 * LY::XSLAB, 16, 1024);
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
           }
         }
         mma_issued = lead;
-        if (i + 1 < steps) ok = __all_sync(0xffffffffu, wait(LY::B_FULL + ring.s, ring.ph));
+        if (i + 1 < steps) ok = wait(LY::B_FULL + ring.s, ring.ph);
         if (lead) {
           if (both) {
             tc2::mma_ts(tmem, a + 48, xd + LY::XSLAB / 16 + 4, id, 1u);
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
       for (int c = c0; c < c1 && ok; ++c) {
         const uint32_t ps[2] = {group == 0 ? pv.x : pv.y, group == 0 ? pv.z : pv.w};
         pv = __ldg(prow + min(c + 1, stages - 1));
-        ok = __all_sync(0xffffffffu, wait(LY::B_CFULL + cr.s, cr.ph));
+        ok = wait(LY::B_CFULL + cr.s, cr.ph);
         if (!ok) break;
         const uint8_t* crow = smem + LY::OFF_C + cr.s * LY::CSTAGE + r * 128;
         const int in_stage = min(4, slabs - 4 * c);
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
           for (int part = 0; part < PARTS; ++part) {
             uint32_t o[32];
             if (s < in_stage) dequant_group<PARTS>(w0, w1, ps[st], part, o);
-            ok = __all_sync(0xffffffffu, wait(LY::B_EMPTY + ring.s, ring.ph ^ 1u));
+            ok = wait(LY::B_EMPTY + ring.s, ring.ph ^ 1u);
             if (!ok) break;
             tc::fence_after();
             if (s < in_stage) tc::tmem_st32(a_base + ring.s * 64, o);
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         rs[i] = __ldg(p.row_scale[which] + wbase + min(row0 + g8 + 8 * i, p.n_out - 1));
-      ok = ok && __all_sync(0xffffffffu, wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1));
+      ok = ok && wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1);
       // the warps go on together or not at all: there are barriers among them below
       ok = !tc2::any_of_group(15, !ok, DW * 32);
       left = !ok;

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   // (loads wait long, the others mostly not at all)
   auto wait_long = [&](int i, uint32_t parity) { return wait_or_abort(bar(i), parity, p.wait_ns, abort_flag); };
-  auto wait = [&](int i, uint32_t parity) { return wait_quick(bar(i), parity, p.wait_ns, abort_flag); };
+  auto wait = [&](int i, uint32_t parity) { return wait_warp(bar(i), parity, p.wait_ns, abort_flag); };
   // (the warp index by a shuffle: uniform to the compiler, which then keeps the MMA operands in
   // uniform registers)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
         ring.next();
         if (i == min(XS, steps) - 1) {  // behind the first loads: the tokens' powers of two
           const int b = k & 1;
-          ok = __all_sync(0xffffffffu, wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1));
+          ok = wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1);
           if (!ok) break;
           for (int j = lane; j < NT; j += 32) tok_scale[b * NT + j] = lo + j < hi ? p.xscale[lo + j] : 0.0f;
           __syncwarp();
@@ -275,9 +275,9 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     Ring<AB> ar;
     uint32_t dph = 1;
     for (int tile = first; tile < tiles && ok; tile += step, dph ^= 1u) {
-      ok = __all_sync(0xffffffffu, wait(LY::B_DEMPTY, dph));
+      ok = wait(LY::B_DEMPTY, dph);
       for (int i = 0; i < steps && ok; ++i) {
-        ok = __all_sync(0xffffffffu, wait(LY::B_XFULL + xr.s, xr.ph) && wait(LY::B_AFULL + ar.s, ar.ph));
+        ok = wait(LY::B_XFULL + xr.s, xr.ph) && wait(LY::B_AFULL + ar.s, ar.ph);
         if (!ok) break;
         tc::fence_after();
         const uint64_t xd = tc::sdesc(s_base + LY::OFF_X + xr.s * SP * LY::XSLAB, 16, 1024);
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     }
   } else {
     // ---- dequantization: one weight row of tile t a thread, slab `group` of every step
-    const int group = warp >> 3, t = (warp >> 2) & 1, quarter = warp & 3;
+    const int group = SP == 1 ? 0 : warp >> 3, t = (warp >> 2) & 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t a_base = tmem + LY::A_COL + group * 64 + t * 32 + lane_base;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
       uint4 pv = __ldg(prow + q0);
       for (int c = q0; c < q1; ++c) {
         const uint4 pnext = __ldg(prow + min(c + 1, q1 - 1));
-        ok = __all_sync(0xffffffffu, wait(LY::B_CFULL + cr.s, cr.ph));
+        ok = wait(LY::B_CFULL + cr.s, cr.ph);
         if (!ok) break;
         const uint8_t* crow = smem + LY::OFF_C + cr.s * LY::CSTAGE + t * (LY::CSTAGE / 2) + r * 128;
         const uint32_t pw[4] = {pv.x, pv.y, pv.z, pv.w};
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
             uint32_t o[32];
             if (s < in_stage)
               dequant_group<PARTS>(w0, w1, SP == 1 || group == 0 ? pw[st * SP] : pw[(st * SP + 1) & 3], part, o);
-            ok = __all_sync(0xffffffffu, wait(LY::B_AEMPTY + ar.s, ar.ph ^ 1u));
+            ok = wait(LY::B_AEMPTY + ar.s, ar.ph ^ 1u);
             if (!ok) break;
             tc::fence_after();
             if (s < in_stage) tc::tmem_st32(a_base + ar.s * 64 * SP, o);  // (17 cycles with its wait)
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
       }
       if (!ok) break;
       const int b = k & 1;
-      ok = __all_sync(0xffffffffu, wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1));
+      ok = wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1);
       if (!ok) break;
       tc::fence_after();
       if (f.ck > 1) {

@@ -238,6 +238,22 @@ __device__ __forceinline__ bool wait_quick(uint32_t bar, uint32_t parity, uint64
   return done || wait_or_abort_slow(bar, parity, limit_ns, abort_flag);
 }
 
+// The same for a whole converged warp, one answer for all its lanes: with the vote beside the try there is no
+// divergent branch, 10 instructions fewer a wait.  (A limit of 0 fails at the first barrier that is not
+// complete.)
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, uint64_t limit_ns,
+                                          const volatile int* abort_flag) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p, q;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "vote.sync.all.pred q, p, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (done) return true;
+  return __all_sync(0xffffffffu, wait_or_abort_slow(bar, parity, limit_ns, abort_flag));
+}
+
 // True on one lane of the (converged) warp, always the same one.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
