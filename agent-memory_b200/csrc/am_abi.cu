@@ -772,19 +772,19 @@ static int linear_params(LinearParams& p, const am_q4_weight* w, const am_q4_wei
 }
 
 // Workspace of the tensor-tile kernel: the activations as fp16 rows and one float a row.
-static size_t linear_workspace(const am_q4_weight* w, int32_t rows, bool grouped) {
+static size_t linear_workspace(const am_q4_weight* w, const am_q4_weight* up, int32_t rows, bool grouped) {
   if (w == nullptr || w->n_in <= 0 || w->experts <= 0 || rows <= 0 ||
-      !linear_uses_tensor_tiles(rows, w->experts, grouped))
+      !linear_uses_tensor_tiles(rows, w->experts, grouped, up != nullptr, w->n_out, w->n_in))
     return 0;
   return (size_t)rows * ((size_t)w->n_in * 2 + 4);
 }
 
-size_t am_q4_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight*, int32_t rows) {
-  return linear_workspace(w, rows, false);
+size_t am_q4_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up, int32_t rows) {
+  return linear_workspace(w, up, rows, false);
 }
 
-size_t am_q4_expert_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight*, int32_t rows) {
-  return linear_workspace(w, rows, true);
+size_t am_q4_expert_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up, int32_t rows) {
+  return linear_workspace(w, up, rows, true);
 }
 
 // A 2-D map over rows of `row_bytes` bytes, read in boxes of 128 bytes x box_rows with the
@@ -804,7 +804,7 @@ static bool encode_rows_map(CUtensorMap* m, const void* base, int64_t rows, int6
 static int run_linear(LinearParams& p, void* workspace, size_t workspace_bytes, void* stream, const char* fn) {
   if (p.rows == 0) return AM_OK;
   const bool grouped = p.offsets != nullptr;
-  if (!linear_uses_tensor_tiles(p.rows, p.experts, grouped))
+  if (!linear_uses_tensor_tiles(p.rows, p.experts, grouped, p.codes[1] != nullptr, p.n_out, p.n_in))
     return cuda_status(launch_linear_few(p, static_cast<cudaStream_t>(stream)), fn);
   const size_t need = (size_t)p.rows * ((size_t)p.n_in * 2 + 4);
   if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)) {

@@ -65,7 +65,7 @@ cudaError_t launch_weight_pack(const void* scales, const void* biases, bool bf16
                                int groups, uint32_t* params, float* row_scale, cudaStream_t stream);
 // Linear layers: the tensor-tile kernel (tcgen05, am_linear_tc.cu; it needs the workspace and the
 // tensor maps of LinearParams) or the few-token kernel (am_linear.cu).
-bool linear_uses_tensor_tiles(int rows, int experts, bool grouped);
+bool linear_uses_tensor_tiles(int rows, int experts, bool grouped, bool gated, int n_out, int n_in);
 // Rows of a token tile of the tensor-tile kernel for a call (the x map's box rows).
 int linear_token_tile(int rows, int experts, bool grouped);
 cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream);

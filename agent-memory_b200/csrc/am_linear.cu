@@ -608,11 +608,15 @@ static cudaError_t launch_few(FewParams& f, int64_t tok, cudaStream_t stream) {
   return launch_few_t<GATED, MT8, 8>(f, stream);
 }
 
-// Which kernel: the mean number of rows of a matrix decides (a grouped call's counts are on the
-// device).
-bool linear_uses_tensor_tiles(int rows, int experts, bool grouped) {
-  const int mean = grouped ? (rows + experts - 1) / experts : rows;
-  return mean > kFewTokens;
+// Which kernel.  One matrix: this one up to 8 tokens (4096x4096 at 8: 7.6 us, the tiles 12.8; 28672x8192
+// 42 and 39); a gated pair, whose sums at 8 tokens cost more than the tiles' longer start once the
+// pair is large, up to 4 of those (8 tokens, 33 million weights: 13.1 and 14.5 us; 117 million: 29.2 and
+// 24.4).  Experts: up to a mean of two rows (a grouped call's counts are on the device; 64 experts
+// of 2048x1408: mean 2 31.8 and 30.0 us, mean 1 24.1 and 25.4; 8 of 4096x14336 gated: mean 2 103
+// and 109, mean 3 143 and 111).
+bool linear_uses_tensor_tiles(int rows, int experts, bool grouped, bool gated, int n_out, int n_in) {
+  if (grouped) return (rows - 1) / experts >= 2;
+  return rows > kFewTokens || (gated && rows > 4 && 2LL * n_out * n_in > 56000000);
 }
 
 cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream) {
