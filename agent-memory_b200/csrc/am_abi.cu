@@ -879,6 +879,11 @@ int am_route_experts(const void* logits, int32_t dtype, int64_t stride, int32_t 
     set_error("am_route_experts: a buffer is NULL");
     return AM_ERR_INVALID;
   }
+  if (!aligned(logits, dtype == AM_DTYPE_F32 ? 4 : 2) || !aligned(experts, 4) || !aligned(weights, 4) ||
+      !aligned(offsets, 4) || !aligned(order, 4) || !aligned(positions, 4)) {
+    set_error("am_route_experts: buffers must be aligned to their elements");
+    return AM_ERR_INVALID;
+  }
   RouteParams p{};
   p.logits = logits;
   p.dtype = dtype;
@@ -905,9 +910,11 @@ int am_combine_experts(const void* y, int32_t dtype, int64_t y_stride, int32_t y
     return AM_ERR_INVALID;
   }
   if (tokens == 0 || width == 0) return AM_OK;
-  if (!y || !weights || !positions || !out || y_stride < width || out_stride < width ||
-      (residual && residual_stride < width)) {
-    set_error("am_combine_experts: y, weights, positions and out, with row strides of at least width, required");
+  if ((!y && y_rows > 0) || !weights || !positions || !out || y_stride < width || out_stride < width ||
+      (residual && residual_stride < width) || !aligned(y, 2) || !aligned(residual, 2) || !aligned(out, 2) ||
+      !aligned(weights, 4) || !aligned(positions, 4)) {
+    set_error("am_combine_experts: y, weights, positions and out, aligned to their elements and with row strides "
+              "of at least width, required");
     return AM_ERR_INVALID;
   }
   CombineParams p{};
