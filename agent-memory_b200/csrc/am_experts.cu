@@ -36,9 +36,10 @@ static cudaError_t launch_chained(K kfn, const P& p, dim3 grid, int threads, int
 //    warp walks its contiguous part 32 pairs at a time (match_any ranks equal experts among the
 //    lanes) with counters per (warp, expert); the counters' prefix over warps, CTAs (distributed
 //    shared memory) and experts gives the places.
-// Up to 64 tokens one CTA does both.  More go through a top-k launch over all SMs first (4096
-// tokens of 32 experts: 22 us with the top-k inside the sorting cluster).  Both are bound by the
-// launch and the barriers: the data of 4096 tokens are 0.8 MB.
+// Up to 16 tokens one CTA of 8 warps does both; more go through a top-k launch over all SMs first (16
+// tokens of 64 experts: 5.9 us and 6.6, 32: 8.5 and 6.7; 4096 of 32 experts: 22 and 10.2).  Both are
+// bound by the launches and the barriers: 1 token of 64 experts takes 4.2 us, and the data of 4096
+// are 0.8 MB.
 __device__ __forceinline__ float load_logit(const RouteParams& p, int64_t i) {
   const float v = p.dtype == AM_DTYPE_F32 ? static_cast<const float*>(p.logits)[i]
                                           : h2f_rt(static_cast<const uint16_t*>(p.logits)[i],
@@ -240,8 +241,7 @@ static cudaError_t launch_sort(const RouteParams& p, int ctas, int threads, cuda
 
 template <int PER>
 static cudaError_t launch_route_t(const RouteParams& p, cudaStream_t stream) {
-  // few tokens in a small CTA, whose barriers are cheaper
-  if (p.tokens <= 64) return launch_sort<PER>(p, 1, p.tokens <= 8 ? 256 : 1024, stream);
+  if (p.tokens <= 16) return launch_sort<PER>(p, 1, 256, stream);
   const cudaError_t err =
       launch_chained(route_topk_kernel<PER>, p, dim3((p.tokens + 7) / 8), 256, 0, 1, stream);
   if (err != cudaSuccess) return err;
@@ -259,7 +259,10 @@ cudaError_t launch_route(const RouteParams& p, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------- combine
-// HBM-bound: a thread sums VEC columns of a token, its rows' loads issued four at a time.
+// HBM-bound.  A CTA takes a part of a token's row, a thread VEC columns of it, with the loads of four rows at
+// once; the experts' rows are read here for the last time and leave the caches first.  4096 tokens of
+// 4 rows of 2880: 21 us, 6.7 TB/s (without the hint 24; with columns dealt out over whole CTAs, a
+// division a thread, 29).
 template <int VEC>
 struct Columns;
 template <>
@@ -287,10 +290,9 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Co
   using T = typename Columns<VEC>::T;
   griddep_launch_dependents();
   griddep_wait();
-  const int cols = p.width / VEC;
-  const int64_t all = (int64_t)p.tokens * cols;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int t = static_cast<int>(i / cols), c = static_cast<int>(i - (int64_t)t * cols) * VEC;
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  if (c >= p.width) return;
+  for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     const float* w = p.weights + (int64_t)t * p.top_k;
     const int32_t* at = p.positions + (int64_t)t * p.top_k;
     T res{};
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Co
           const int row = at[j0 + j];
           if (row >= 0 && row < p.y_rows) {
             wj[j] = w[j0 + j];
-            y[j] = *reinterpret_cast<const T*>(p.y + (int64_t)row * p.y_stride + c);
+            y[j] = __ldlu(reinterpret_cast<const T*>(p.y + (int64_t)row * p.y_stride + c));
           } else {
             flag_status(p.status, AM_STATUS_BAD_POSITION);
           }
@@ -338,10 +340,13 @@ cudaError_t launch_combine(const CombineParams& p, cudaStream_t stream) {
   // 16-byte columns where every row allows them (8x fewer, 8x larger accesses than one by one)
   const bool vec = p.width % 8 == 0 && wide(p.y, p.y_stride) && wide(p.out, p.out_stride) &&
                    (p.residual == nullptr || wide(p.residual, p.residual_stride));
-  const int64_t all = (int64_t)p.tokens * (vec ? p.width / 8 : p.width);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((all + 255) / 256, 1 << 20));
-  return vec ? launch_chained(combine_kernel<8>, p, dim3(grid), 256, 0, 1, stream)
-             : launch_chained(combine_kernel<1>, p, dim3(grid), 256, 0, 1, stream);
+  // CTAs of equal parts of a token's row, 256 columns or vectors at most
+  const int cols = vec ? p.width / 8 : p.width, parts = (cols - 1) / 256 + 1;
+  if (parts > 65535) return cudaErrorNotSupported;
+  const int threads = ((cols + parts - 1) / parts + 31) & ~31;
+  const dim3 grid(std::min(p.tokens, 1 << 20), parts);
+  return vec ? launch_chained(combine_kernel<8>, p, grid, threads, 0, 1, stream)
+             : launch_chained(combine_kernel<1>, p, grid, threads, 0, 1, stream);
 }
 
 }  // namespace am

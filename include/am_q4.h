@@ -310,8 +310,12 @@ int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int
  * y = x W^T (replaces mx.quantized_matmul(x, w, scales, biases, transpose=True)), or with a
  * second matrix `up` of the same shape y = silu(x W^T) * (x up^T).  x: device [rows, n_in],
  * out: device [rows, n_out], both of w->dtype, row strides in elements (x_stride % 8 == 0, x
- * 16-byte aligned).  Sums are fp32; y is rounded once.  Weights enter the products rounded
- * to fp16 (11 bits), activations exactly.
+ * 16-byte aligned).  Sums are fp32; y is rounded once.  A few tokens (up to 8, gated pairs 4
+ * to 8) multiply exact weights.  For more a weight enters as scale * code + bias rounded once
+ * to fp16, for a gated fp16 call as the sum of two such parts.  Activations are exact but for
+ * values below 2^-28 of their token's largest; infinite or NaN ones make their token's outputs
+ * infinite or NaN.  workspace: device memory, 256-byte aligned, of the size the query gives
+ * (0 for a few tokens); scratch of the call, free again when it has run.
  */
 size_t am_q4_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up, int32_t rows);
 int am_q4_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, int64_t x_stride,
@@ -324,7 +328,7 @@ int am_q4_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, i
  * x (order given), or from row r of x (order NULL).  offsets: device int32 [experts + 1],
  * non-decreasing, used clamped to [0, rows]; rows no expert holds are not written.  An order
  * entry that points outside [0, x_rows) reads as a row of zeros and sets
- * AM_STATUS_BAD_POSITION.
+ * AM_STATUS_BAD_POSITION.  Workspace as above (none up to a mean of two rows an expert).
  */
 size_t am_q4_expert_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up,
                                            int32_t rows);
