@@ -254,4 +254,31 @@ __device__ __forceinline__ void store_tokens(const LinearParams& p, uint8_t* so,
   __syncwarp();
 }
 
+// The same for 16 output rows of 16 tokens: q[j][h] are rows 8 h .. 8 h + 7 of tokens 8 j .. 8 j + 7, through
+// 16 * kOutPitch16 bytes at `so`; a token's 16 rows leave as 32 bytes.
+constexpr int kOutPitch16 = 48;
+__device__ __forceinline__ void store_tokens_16(const LinearParams& p, uint8_t* so, const uint32_t (&q)[2][2], int tok,
+                                                int hi, int row0) {
+  const int lane = threadIdx.x & 31;
+  const bool wide = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  const int left = p.n_out - (row0 + (lane & 1) * 8);
+  stsm_x4_trans(smem_u32(so) + ((lane >> 4) * 8 + (lane & 7)) * kOutPitch16 + ((lane >> 3) & 1) * 16, q[0][0], q[0][1],
+                q[1][0], q[1][1]);
+  __syncwarp();
+  const int at = tok + (lane >> 1);
+  const uint4 d = *reinterpret_cast<const uint4*>(so + (lane >> 1) * kOutPitch16 + (lane & 1) * 16);
+  if (at < hi && left > 0) {
+    uint16_t* dst = p.out + (int64_t)at * p.out_stride + row0 + (lane & 1) * 8;
+    if (wide && left >= 8) {
+      *reinterpret_cast<uint4*>(dst) = d;
+    } else {
+      const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) dst[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+  __syncwarp();
+}
+
 }  // namespace am

@@ -7,8 +7,8 @@
 // shared memory and read from it for 256 weight rows by each SM: at the power cap that these sizes
 // run at, the work saved beside the MMAs is clock rate gained for them.
 //
-// Per CTA: one thread streams the codes (plain: 128 rows of the matrix; gated: 64 rows of each, so
-// that a row's gate and its partner lie 64 TMEM lanes apart in the same CTA), one the
+// Per CTA: one thread streams the codes (plain: 128 rows of the matrix; gated: 64 rows of each, 16 and
+// 16 alternating in TMEM, so that one thread reads a row's gate and its partner), one the
 // activations; their full barrier, shared with the dequantized operand's, is the leader's.  8
 // warps dequantize (two groups of 4, a 64-input slab of a step each) and write the output: TMEM holds
 // the 256-column accumulator and eight operand slabs.  The MMA shape follows the item: N is its tokens
@@ -57,18 +57,6 @@ __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
 }
 
-// Whether any of the `count` threads that meet at named barrier `id` passes true.
-__device__ __forceinline__ bool any_of_group(int id, bool v, int count) {
-  uint32_t r;
-  asm volatile(
-      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, %2, %3, p;\n"
-      "selp.u32 %0, 1, 0, q;\n}\n"
-      : "=r"(r)
-      : "r"(static_cast<uint32_t>(v)), "r"(id), "r"(count)
-      : "memory");
-  return r != 0;
-}
-
 }  // namespace tc2
 
 template <bool GATED>
@@ -82,9 +70,8 @@ struct PairLayout {
   static constexpr int OFF_C = 0;
   static constexpr int OFF_X = OFF_C + CS * CSTAGE;
   static constexpr int OFF_OUT = OFF_X + ST * 2 * XSLAB;           // kOutPitch bytes a token of a warp
-  static constexpr int OUT = (GATED ? 8 : 16) * kOutPitch;
-  static constexpr int OFF_SWAP = OFF_OUT + DW * OUT;              // two buffers of 2 KB a pair of warps
-  static constexpr int OFF_SCALE = OFF_SWAP + (GATED ? DW / 2 * 4096 : 0);  // two tiles' token scales
+  static constexpr int OUT = 16 * (GATED ? kOutPitch16 : kOutPitch);
+  static constexpr int OFF_SCALE = OFF_OUT + DW * OUT;             // two tiles' token scales
   static constexpr int OFF_BAR = OFF_SCALE + 2 * 256 * 4;
   // FULL: a step's operand is in the TMEM of both CTAs and its activations in their shared memory (the
   // leader's copy); EMPTY: the step's MMAs are done (both copies).
@@ -264,9 +251,9 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
   } else {
     // ---- dequantization (as in linear_tiles_kernel): a weight row a thread, slab `group` of every step
     const int group = warp >> 2, quarter = warp & 3;
-    const int r = quarter * 32 + lane;
-    const int which = GATED ? quarter >> 1 : 0;      // the matrix of this lane's rows
-    const int rr = GATED ? r & 63 : r;               // output row within the CTA
+    const int which = GATED ? lane >> 4 : 0;                          // the matrix of this lane's row
+    const int rr = GATED ? quarter * 16 + (lane & 15) : quarter * 32 + lane;  // output row within the CTA
+    const int r = which * 64 + rr;                                    // row of the code stage
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t a_base = tmem + LY::A_COL + group * 32 + lane_base;
     const uint32_t lead_full = dsmem_addr(bar(LY::B_FULL), 0), lead_dempty = dsmem_addr(bar(LY::B_DEMPTY), 0);
@@ -313,28 +300,21 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
       }
     };
     // ---- output of the k-th tile: group g takes every other 16 tokens.  The accumulators come in mma
-    // fragments (thread (g8, t4): rows g8 + 8 i, tokens 2 t4, + 1 of eight), leave transposed through
-    // the warp's own shared memory, a token's 32 rows as 64 bytes.  Gated: the warps that hold a
-    // row's gate and its partner swap eight of the 16 tokens and finish the other eight each.
-    bool left = false;  // a failure was seen by all warps: none meets the others again
+    // fragments (thread (g8, t4): rows g8 + 8 i, tokens 2 t4, + 1 of eight; gated: of the gate for i < 2 and
+    // of its partner above), leave transposed through the warp's own shared memory, a token's 32
+    // rows as 64 bytes (gated 16, 32).
     auto output = [&](int k, int lo, int hi, int n0, int64_t wbase) {
       const int b = k & 1;
       const int g8 = lane >> 2, t4 = lane & 3;
-      const int row0 = n0 + (GATED ? (quarter & 1) * 32 : quarter * 32);  // of the warp's 32
+      const int row0 = n0 + quarter * (GATED ? 16 : 32);  // of the warp's
       float rs[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        rs[i] = __ldg(p.row_scale[which] + wbase + min(row0 + g8 + 8 * i, p.n_out - 1));
+        rs[i] = __ldg(p.row_scale[GATED ? i >> 1 : 0] + wbase + min(row0 + g8 + 8 * (GATED ? i & 1 : i), p.n_out - 1));
       ok = ok && wait(LY::B_DFULL, k & 1) && wait(LY::B_SFULL + b, (k >> 1) & 1);
-      // the warps go on together or not at all: there are barriers among them below
-      ok = !tc2::any_of_group(15, !ok, DW * 32);
-      left = !ok;
       if (!ok) return;
       tc::fence_after();
-      const int pair = group * 2 + (quarter & 1);
-      float4* swap = reinterpret_cast<float4*>(smem + LY::OFF_SWAP) + pair * 256;
       uint8_t* so = smem + LY::OFF_OUT + warp * LY::OUT;
-      int flip = 0;
       float next[2][8];  // the next 16 tokens, loaded behind this one's work: [16 rows][token block, row
                          // g8 or g8 + 8, token]
       auto load = [&](int cb) {
@@ -343,7 +323,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
       };
       if (lo + group * 16 < hi) load(group * 16);
 #pragma unroll 1
-      for (int cb = group * 16; lo + cb < hi; cb += 32, flip ^= 128) {
+      for (int cb = group * 16; lo + cb < hi; cb += 32) {
         float v[2][8];
         tc::tmem_wait_ld();
 #pragma unroll
@@ -359,29 +339,14 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[h][i] *= rs[2 * h + ((i >> 1) & 1)] * ((i & 1) ? ts[i >> 2].y : ts[i >> 2].x);
-        uint32_t q[GATED ? 1 : 2][4];  // [token block][8 rows]: pairs of tokens
         if constexpr (GATED) {
-          const int give = which == 0 ? 1 : 0;  // the token block the other warp finishes
-          float keep[2][4];
+          uint32_t q[2][2];  // [token block][8 rows]: pairs of tokens
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            swap[flip + (which * 2 + h) * 32 + lane] = give ? make_float4(v[h][4], v[h][5], v[h][6], v[h][7])
-                                                            : make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) keep[h][i] = give ? v[h][i] : v[h][4 + i];
-          }
-          asm volatile("bar.sync %0, 64;\n" ::"r"(1 + pair) : "memory");
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 o4 = swap[flip + ((which ^ 1) * 2 + h) * 32 + lane];
-            const float o[4] = {o4.x, o4.y, o4.z, o4.w};
-            float y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = which == 0 ? silu_mul(keep[h][i], o[i]) : silu_mul(o[i], keep[h][i]);
-            q[0][2 * h] = pack_out(p, y[0], y[1]);
-            q[0][2 * h + 1] = pack_out(p, y[2], y[3]);
-          }
+          for (int i = 0; i < 8; i += 2)
+            q[i >> 2][(i >> 1) & 1] = pack_out(p, silu_mul(v[0][i], v[1][i]), silu_mul(v[0][i + 1], v[1][i + 1]));
+          store_tokens_16(p, so, q, lo + cb, hi, row0);
         } else {
+          uint32_t q[2][4];
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -389,8 +354,8 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
               q[j][2 * h] = pack_out(p, v[h][4 * j], v[h][4 * j + 1]);
               q[j][2 * h + 1] = pack_out(p, v[h][4 * j + 2], v[h][4 * j + 3]);
             }
+          store_tokens(p, so, q, lo + cb, hi, row0);
         }
-        store_tokens(p, so, q, lo + cb + (GATED ? which * 8 : 0), hi, row0);
       }
       // the accumulator and the tokens' scales are read
       tc::fence_before();
@@ -413,14 +378,14 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
       prow = reinterpret_cast<const uint4*>(p.params[which] + (wbase_n + min(n0_n + rr, p.n_out - 1)) * p.pstride);
       pv = __ldg(prow);
       dequant(0, min(AHEAD, stages));
-      if (k > 0) output(k - 1, lo, hi, n0, wbase);
+      if (ok && k > 0) output(k - 1, lo, hi, n0, wbase);
       if (ok) dequant(min(AHEAD, stages), stages);
       lo = lo_n;
       hi = hi_n;
       n0 = n0_n;
       wbase = wbase_n;
     }
-    if (k > 0 && !left) output(k - 1, lo, hi, n0, wbase);
+    if (ok && k > 0) output(k - 1, lo, hi, n0, wbase);
   }
   if (!ok) *abort_flag = 1;
   __syncthreads();
