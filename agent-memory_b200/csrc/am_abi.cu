@@ -816,7 +816,7 @@ static int run_linear(LinearParams& p, void* workspace, size_t workspace_bytes, 
   p.wait_ns = wait_limit_ns();
   const bool gated = p.codes[1] != nullptr;
   const bool pairs = linear_uses_pairs(p.rows, p.experts, p.n_out, grouped, gated);
-  const int tile = pairs ? 128 : linear_token_tile(p.rows, p.experts, grouped);
+  const int tile = pairs ? 128 : linear_token_tile(p.rows, p.experts, p.n_out, grouped, gated);
   bool ok = encode_rows_map(&p.tmap_x, p.xh, p.rows, (int64_t)p.n_in * 2, tile);
   for (int i = 0; i < 2 && ok; ++i)
     if (p.codes[i] != nullptr)

@@ -67,7 +67,7 @@ cudaError_t launch_weight_pack(const void* scales, const void* biases, bool bf16
 // tensor maps of LinearParams) or the few-token kernel (am_linear.cu).
 bool linear_uses_tensor_tiles(int rows, int experts, bool grouped, bool gated, int n_out, int n_in);
 // Rows of a token tile of the tensor-tile kernel for a call (the x map's box rows).
-int linear_token_tile(int rows, int experts, bool grouped);
+int linear_token_tile(int rows, int experts, int n_out, bool grouped, bool gated);
 cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream);
 bool linear_uses_pairs(int rows, int experts, int n_out, bool grouped, bool gated);
 cudaError_t launch_linear_tiles(const LinearParams& p, bool pairs, cudaStream_t stream);

@@ -563,7 +563,34 @@ static cudaError_t launch_few_t(FewParams& f, cudaStream_t stream) {
   // about one and a half groups' time for the sums; a warp gets at least a whole stage.
   constexpr int TROWS = GATED ? 16 : 16 * MT;
   const int row_tiles = (p.n_out + TROWS - 1) / TROWS;
-  const int ctas = sms / ck;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(sms / ck * ck));
+  cfg.blockDim = dim3(kFewWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ck;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ck > 1 ? 2 : 1;
+  // CTAs, or clusters, that run at once: clusters lie within a GPC, so fewer of 4 or 8 fit than the SMs hold
+  // (8 tokens 8192x28672 in clusters of 8: 55.8 us with 18 of them, 52.6 with the 15 that fit)
+  int ctas = sms;
+  if (ck > 1) {
+    static int fit[64][4];  // by log2 of the cluster, once known
+    const int i = ck == 2 ? 1 : ck == 4 ? 2 : 3;
+    ctas = dev < 64 ? __atomic_load_n(&fit[dev][i], __ATOMIC_RELAXED) : 0;
+    if (ctas == 0) {
+      err = cudaOccupancyMaxActiveClusters(&ctas, kfn, &cfg);
+      if (err != cudaSuccess) return err;
+      if (ctas == 0) return cudaErrorNotSupported;
+      if (dev < 64) __atomic_store_n(&fit[dev][i], ctas, __ATOMIC_RELAXED);
+    }
+  }
   double best = 0.0;
   int wk = 1;
   for (int k = 1; k <= kFewWarps; k *= 2) {
@@ -583,20 +610,7 @@ static cudaError_t launch_few_t(FewParams& f, cudaStream_t stream) {
   const int wr = kFewWarps / wk;
   f.tiles = (row_tiles + wr - 1) / wr;
   if (items * f.tiles > INT_MAX) return cudaErrorNotSupported;
-  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(items * f.tiles, ctas)) * ck));
-  cfg.blockDim = dim3(kFewWarps * 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ck;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = ck > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kfn, f);
 }
 

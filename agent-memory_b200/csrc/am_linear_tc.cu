@@ -511,18 +511,26 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
 }
 
 // ---------------------------------------------------------------- host
-// Pairs of SMs where a matrix's mean number of rows fills most of a pair's 256 tokens and the tiles
-// fill the pairs.
+// Pairs of SMs where a matrix's mean number of rows passes the single tile's 128 tokens and the tiles
+// fill the pairs (experts, 32 of 2880x2880 gated: mean 96 147 us and 125 single, mean 144 167 and 222;
+// one matrix, 512 tokens: 14336x4096 gated, 224 tiles, 96 and 102; 4096x14336, 32 tiles, 59 and 50).
 bool linear_uses_pairs(int rows, int experts, int n_out, bool grouped, bool gated) {
   const int mean = grouped ? (rows + experts - 1) / experts : rows;
   const int64_t tiles = (int64_t)((n_out + (gated ? 127 : 255)) / (gated ? 128 : 256)) *
                         (grouped ? rows / 256 : (rows + 255) / 256);
-  return mean > 192 && tiles >= 64;
+  return mean > 128 && tiles >= 64;
 }
 
-int linear_token_tile(int rows, int experts, bool grouped) {
+// Tokens of a tile: what holds the rows of a matrix, for experts twice their mean up to 64 (32 of 2880x2880
+// gated, mean 8: 73 us with 32 tokens and 77 with 64, mean 32: 102 and 82, mean 96: 149 with 64 and
+// 125 with 128).  One matrix of few tiles is cut into 64 up to 128 tokens, for more SMs to work (128
+// tokens: 4096x4096, 32 tiles, 14.3 us and 16.9 uncut; 14336x4096, 112, 25.4 and 23.1).
+int linear_token_tile(int rows, int experts, int n_out, bool grouped, bool gated) {
   const int mean = grouped ? (rows + experts - 1) / experts : rows;
-  return mean <= 32 ? 32 : (mean <= 64 ? 64 : 128);
+  if (mean <= (grouped ? 16 : 32)) return 32;
+  if (mean <= 64) return 64;
+  const int tile_rows = gated ? 128 : 256;
+  return !grouped && mean <= 128 && (n_out + tile_rows - 1) / tile_rows <= 32 ? 64 : 128;
 }
 
 template <int NT, bool GATED, int PARTS>
@@ -546,11 +554,7 @@ static cudaError_t launch_tiles_t(const LinearParams& p, int64_t items, cudaStre
   const int quads = p.pstride / 4;
   TilesParams f{};
   f.p = p;
-  f.ck = 1;
-  while (f.ck < 8 && (int64_t)row_tiles * items * f.ck * 2 <= (int64_t)sms * LY::CTAS && f.ck * 4 <= quads) f.ck *= 2;
   cudaLaunchConfig_t cfg = {};
-  f.row_tiles = row_tiles;
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(row_tiles * items * f.ck, (int64_t)sms * LY::CTAS)));
   cfg.blockDim = dim3(LY::THREADS);
   cfg.dynamicSmemBytes = LY::SMEM;
   cfg.stream = stream;
@@ -558,10 +562,32 @@ static cudaError_t launch_tiles_t(const LinearParams& p, int64_t items, cudaStre
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = f.ck;
+  attr[1].val.clusterDim.x = 1;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
+  // The inputs are split while all tiles still run at once: clusters lie within a GPC, so fewer of 8 fit than
+  // the SMs would hold (128 tokens 4096x4096, 16 tiles: 29 us in clusters of 8 that came in two
+  // waves, 16.9 in clusters of 4).
+  static int fit[64][4];  // clusters of 2^i that fit on a device, once known
+  const int64_t tiles = row_tiles * items;
+  f.ck = 1;
+  f.row_tiles = row_tiles;
+  for (int i = 1; i < 4 && (4 << (i - 1)) <= quads && (tiles << i) <= (int64_t)sms * LY::CTAS; ++i) {
+    int n = dev < 64 ? __atomic_load_n(&fit[dev][i], __ATOMIC_RELAXED) : 0;
+    if (n == 0) {
+      cfg.gridDim = dim3(static_cast<unsigned>(sms * LY::CTAS) >> i << i);
+      attr[1].val.clusterDim.x = 1 << i;
+      cfg.numAttrs = 2;
+      err = cudaOccupancyMaxActiveClusters(&n, kfn, &cfg);
+      if (err != cudaSuccess) return err;
+      if (dev < 64) __atomic_store_n(&fit[dev][i], n, __ATOMIC_RELAXED);
+    }
+    if (tiles > n) break;
+    f.ck = 1 << i;
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles * f.ck, (int64_t)sms * LY::CTAS)));
+  attr[1].val.clusterDim.x = f.ck;
   cfg.numAttrs = f.ck > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kfn, f);
 }
@@ -589,7 +615,7 @@ cudaError_t launch_linear_tiles(const LinearParams& p, bool pairs, cudaStream_t 
   const cudaError_t err = cudaLaunchKernelEx(&cfg, team == 32 ? linear_rows_kernel<32> : linear_rows_kernel<kRowThreads>, p);
   if (err != cudaSuccess) return err;
   if (pairs) return launch_linear_pair(p, stream);
-  switch (linear_token_tile(p.rows, p.experts, p.offsets != nullptr)) {
+  switch (linear_token_tile(p.rows, p.experts, p.n_out, p.offsets != nullptr, p.codes[1] != nullptr)) {
     case 32: return launch_tiles<32>(p, stream);
     case 64: return launch_tiles<64>(p, stream);
     default: return launch_tiles<128>(p, stream);
