@@ -281,4 +281,17 @@ __device__ __forceinline__ void store_tokens_16(const LinearParams& p, uint8_t* 
   __syncwarp();
 }
 
+// Position in a ring of N buffers and the parity of its current round.
+template <int N>
+struct Ring {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      ph ^= 1u;
+    }
+  }
+};
+
 }  // namespace am
