@@ -47,7 +47,15 @@
 //
 // The attention grid is launched with programmatic stream serialization: its prologue (TMEM
 // allocation, barriers, the query tile) overlaps the end of the stage kernel, and the TMA
-// thread waits in griddepcontrol.wait before it reads the workspace.
+// thread waits in griddepcontrol.wait before it reads the workspace.  The queries and lengths
+// may be read before that wait because the stage kernel itself is launched plainly: it started
+// when everything before it was complete.  A call without a stage launch (am_q4_prefill_attend)
+// has no such grid before it, and may follow one that lets its dependents start early (a
+// linear layer that writes the queries): there every thread waits before its first read
+// (wait_first), and only asks L2 for the query rows before that.  What stands behind the wait
+// then, the lengths and the query tile, costs a call of the two-tile kernel 2.5 us (512 tokens
+// over a 4096-token prefix, stage and attention 109 -> 112 us a layer; waiting in front of the
+// whole prologue instead: 115); the K/V loads start beside it.
 //
 // Reference semantics: the compiled quantized SDPA (mlx_fused_attention.py:69-139) as used
 // by chunked prefill (batch_engine.py:339-456): the chunk's own K/V are already in the Q4
@@ -144,6 +152,16 @@ __device__ __forceinline__ void q_chunks_load(const uint16_t* src, bool ok, uint
   } else {
 #pragma unroll
     for (int c = 0; c < CH; ++c) raw[c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Asks L2 for the chunks of a row that may not be read yet (a prefetch reads nothing).
+template <int CH>
+__device__ __forceinline__ void q_chunks_prefetch(const uint16_t* src) {
+  if (src != nullptr) {
+#pragma unroll
+    for (int c = 0; c < CH; c += 8) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c * 8));
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(src + CH * 8 - 1));
   }
 }
 
@@ -498,6 +516,10 @@ struct PrefillLayout {
   static_assert((DV / CG) % 16 == 0, "O columns per softmax warp");
 };
 
+__device__ __forceinline__ void named_bar_sync(int id, int count) {
+  asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(count) : "memory");
+}
+
 // Named barrier over `count` threads that also ORs a flag across them: every thread gets the
 // same answer, so the warps of a lane quarter leave their loop together even if the shared
 // abort flag changes while their threads read it.
@@ -568,18 +590,7 @@ __global__ void __launch_bounds__(PrefillRoles<BN, QV4>::THREADS, 1)
   const int l0 = (gridDim.x - 1 - blockIdx.x) * tok_per_cta;
   const int l_last = min(l0 + tok_per_cta, p.q_len) - 1;
 
-  const int n = p.kv_len[b];
-  const int st = p.kv_start != nullptr ? p.kv_start[b] : 0;
-  int blo, bhi;  // the workspace plane holds keys [blo, blo + nw)
-  prefill_block_range(p, b, blo, bhi);
-  bhi = min(bhi, blo + p.nw);
-  const int pos_min = n - p.q_len + l0, pos_max = n - p.q_len + l_last;
-  int lo = blo, hi = bhi;  // keys this CTA's rows can see
-  if (!DENSE && p.window > 0) lo = max(lo, pos_min - p.window + 1);
-  if (p.causal) hi = min(hi, pos_max + 1);
-  const int n_tiles = hi > lo ? (hi - lo + BN - 1) / BN : 0;
-
-  // ---- setup
+  // ---- setup: barriers and TMEM, before the wait
   if (tid == 0) {
     for (int i = 0; i < LY::B_COUNT; ++i) {
       const bool pfull = i == LY::B_PFULL || i == LY::B_PFULL + 1;
@@ -595,29 +606,47 @@ __global__ void __launch_bounds__(PrefillRoles<BN, QV4>::THREADS, 1)
                  "r"(LY::TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
   }
-  if (tid < 256) {
-    // query row r -> fp16 with a power-of-two prescale (exact for fp16 / bf16 inputs); two
-    // threads per row (adjacent lanes), each staging half of it
-    const int r = tid >> 1, half = tid & 1;
-    constexpr int CH = DK / 16;
-    const int rl = r / n_rep;
-    const bool row_ok = r < tok_per_cta * n_rep && l0 + rl < p.q_len;
-    const int l = l0 + (row_ok ? rl : 0);
-    const int hq = h * n_rep + r % n_rep;
-    const uint16_t* qrow = p.q + (int64_t)b * p.qsb + (int64_t)hq * p.qsh + (int64_t)l * p.qsl;
-    uint4 raw[CH];
-    q_chunks_load<CH>(qrow + half * (DK / 2), row_ok, raw);
-    float amax = q_chunks_amax<CH>(raw, p.q_bf16 != 0);
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    const float pw = q_row_prescale(amax, p.scale_log2);
-    if (half == 0) sqf[r] = p.scale_log2 / pw;
-    q_chunks_store<CH>(smem + LY::OFF_Q, LY::QSLAB, raw, pw, p.q_bf16 != 0, r, half * CH);
-  }
-  fence_proxy_async_smem();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
+  // this thread's part of a query row; null past the tile's rows
+  constexpr int QCH = DK / 16;
+  const uint16_t* qrow = nullptr;
+  if (tid < 256) {
+    const int r = tid >> 1, l = l0 + r / n_rep, hq = h * n_rep + r % n_rep;
+    if (r < tok_per_cta * n_rep && l < p.q_len)
+      qrow = p.q + (int64_t)b * p.qsb + (int64_t)hq * p.qsh + (int64_t)l * p.qsl + (tid & 1) * (DK / 2);
+  }
+  if (p.wait_first) {
+    q_chunks_prefetch<QCH>(qrow);
+    griddep_wait();
+  }
+  uint4 raw[QCH];
+  q_chunks_load<QCH>(qrow, qrow != nullptr, raw);
+  const int n = p.kv_len[b];
+  const int st = p.kv_start != nullptr ? p.kv_start[b] : 0;
+  int blo, bhi;  // the workspace plane holds keys [blo, blo + nw)
+  prefill_block_range(p, b, blo, bhi);
+  bhi = min(bhi, blo + p.nw);
+  const int pos_min = n - p.q_len + l0, pos_max = n - p.q_len + l_last;
+  int lo = blo, hi = bhi;  // keys this CTA's rows can see
+  if (!DENSE && p.window > 0) lo = max(lo, pos_min - p.window + 1);
+  if (p.causal) hi = min(hi, pos_max + 1);
+  const int n_tiles = hi > lo ? (hi - lo + BN - 1) / BN : 0;
+
+  if (tid < 256) {
+    // query row r -> fp16 with a power-of-two prescale (exact for fp16 / bf16 inputs); two
+    // threads per row (adjacent lanes), each staging half of it
+    const int r = tid >> 1, half = tid & 1;
+    float amax = q_chunks_amax<QCH>(raw, p.q_bf16 != 0);
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    const float pw = q_row_prescale(amax, p.scale_log2);
+    if (half == 0) sqf[r] = p.scale_log2 / pw;
+    q_chunks_store<QCH>(smem + LY::OFF_Q, LY::QSLAB, raw, pw, p.q_bf16 != 0, r, half * QCH);
+  }
+  fence_proxy_async_smem();
+  if (warp != RL::TMA_WARP) named_bar_sync(5, RL::THREADS - 32);  // (the K/V loads need no query)
   constexpr uint32_t ID_S = tc::idesc(128, BN, false);
   constexpr uint32_t ID_O = tc::idesc(128, DV, true);
 
@@ -1131,18 +1160,7 @@ __global__ void __launch_bounds__(kTile2Threads, 1) prefill2_kernel(const __grid
   const int l0 = (gridDim.x - 1 - blockIdx.x) * 2 * tpq;
   const int l_last = min(l0 + 2 * tpq, p.q_len) - 1;
 
-  const int n = p.kv_len[b];
-  const int st = p.kv_start != nullptr ? p.kv_start[b] : 0;
-  int blo, bhi;  // the workspace plane holds keys [blo, blo + nw)
-  prefill_block_range(p, b, blo, bhi);
-  bhi = min(bhi, blo + p.nw);
-  const int pos_min = n - p.q_len + l0, pos_max = n - p.q_len + l_last;
-  int lo = blo, hi = bhi;  // keys the CTA's rows can see
-  if (!DENSE && p.window > 0) lo = max(lo, pos_min - p.window + 1);
-  if (p.causal) hi = min(hi, pos_max + 1);
-  const int n_tiles = hi > lo ? (hi - lo + BN - 1) / BN : 0;
-
-  // ---- setup
+  // ---- setup: barriers and TMEM, before the wait
   if (tid == 0) {
     for (int i = 0; i < LY::B_COUNT; ++i)
       mbar_init(bar(i), (i == LY::B_PFULL || i == LY::B_PFULL + 1) ? 128 : 1);
@@ -1155,27 +1173,45 @@ __global__ void __launch_bounds__(kTile2Threads, 1) prefill2_kernel(const __grid
                  "r"(LY::TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
   }
-  if (tid < 256) {
-    // query row R = tid of the CTA (tile R / 128, row R % 128) -> fp16 with a power-of-two
-    // prescale (exact for fp16 / bf16 inputs)
-    const int qt = tid >> 7, r = tid & 127;
-    constexpr int CH = DK / 8;
-    const int rl = r / n_rep;
-    const bool row_ok = r < tpq * n_rep && l0 + qt * tpq + rl < p.q_len;
-    const int l = l0 + qt * tpq + (row_ok ? rl : 0);
-    const int hq = h * n_rep + r % n_rep;
-    const uint16_t* qrow = p.q + (int64_t)b * p.qsb + (int64_t)hq * p.qsh + (int64_t)l * p.qsl;
-    uint4 raw[CH];
-    q_chunks_load<CH>(qrow, row_ok, raw);
-    const float pw = q_row_prescale(q_chunks_amax<CH>(raw, p.q_bf16 != 0), p.scale_log2);
-    sqf[tid] = p.scale_log2 / pw;
-    q_chunks_store<CH>(smem + LY::OFF_Q + qt * LY::QTILE, LY::QSLAB, raw, pw, p.q_bf16 != 0, r, 0);
-  }
-  fence_proxy_async_smem();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
+  // this thread's query row; null past the tile's rows
+  constexpr int QCH = DK / 8;
+  const uint16_t* qrow = nullptr;
+  if (tid < 256) {
+    const int r = tid & 127, l = l0 + (tid >> 7) * tpq + r / n_rep, hq = h * n_rep + r % n_rep;
+    if (r < tpq * n_rep && l < p.q_len)
+      qrow = p.q + (int64_t)b * p.qsb + (int64_t)hq * p.qsh + (int64_t)l * p.qsl;
+  }
+  if (p.wait_first) {
+    q_chunks_prefetch<QCH>(qrow);
+    griddep_wait();
+  }
+  const int n = p.kv_len[b];
+  const int st = p.kv_start != nullptr ? p.kv_start[b] : 0;
+  int blo, bhi;  // the workspace plane holds keys [blo, blo + nw)
+  prefill_block_range(p, b, blo, bhi);
+  bhi = min(bhi, blo + p.nw);
+  const int pos_min = n - p.q_len + l0, pos_max = n - p.q_len + l_last;
+  int lo = blo, hi = bhi;  // keys the CTA's rows can see
+  if (!DENSE && p.window > 0) lo = max(lo, pos_min - p.window + 1);
+  if (p.causal) hi = min(hi, pos_max + 1);
+  const int n_tiles = hi > lo ? (hi - lo + BN - 1) / BN : 0;
+
+  if (tid < 256) {
+    // query row R = tid of the CTA (tile R / 128, row R % 128) -> fp16 with a power-of-two
+    // prescale (exact for fp16 / bf16 inputs)
+    const int qt = tid >> 7, r = tid & 127;
+    uint4 raw[QCH];
+    q_chunks_load<QCH>(qrow, qrow != nullptr, raw);
+    const float pw = q_row_prescale(q_chunks_amax<QCH>(raw, p.q_bf16 != 0), p.scale_log2);
+    sqf[tid] = p.scale_log2 / pw;
+    q_chunks_store<QCH>(smem + LY::OFF_Q + qt * LY::QTILE, LY::QSLAB, raw, pw, p.q_bf16 != 0, r, 0);
+  }
+  fence_proxy_async_smem();
+  if (warp != TMA_WARP) named_bar_sync(1, kTile2Threads - 32);  // (the K/V loads need no query)
   constexpr uint32_t ID_S = tc::idesc(128, BN, false);
   constexpr uint32_t ID_O = tc::idesc(128, DV, true);
 
@@ -1621,6 +1657,7 @@ static cudaError_t launch_prefill_dims(const DecodeParams& p0, int batch, bool p
   DecodeParams p = p0;  // (the attention kernel's V dequantization reads the cache directly)
   p.paged = paged ? 1 : 0;
   p.scale_bf16 = sbf16 ? 1 : 0;
+  p.wait_first = parts & kPrefillStage ? 0 : 1;
   if (parts & kPrefillStage) {
     cudaError_t e = paged ? (sbf16 ? launch_stage_t<DK, DV, true, true>(p, batch, stream)
                                    : launch_stage_t<DK, DV, false, true>(p, batch, stream))

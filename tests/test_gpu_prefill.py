@@ -324,3 +324,34 @@ def test_paged_prefill_stage_before_append_then_attend(cuda, geom):
                                  causal=True, window=window, out_dtype=torch.float32)
     torch.cuda.synchronize(cuda)
     assert torch.equal(got, want), (got - want).abs().max()
+
+
+@pytest.mark.parametrize("geom", [(32, 8, 128, 128, 512), (16, 16, 192, 128, 300), (16, 8, 256, 256, 200)],
+                         ids=["llama_d128", "mla_k192_v128", "gemma_d256"])
+def test_attend_waits_for_the_projection_of_its_queries(cuda, geom):
+    """Stage, project, attend on one stream: the projection (a 4-bit linear layer) lets the next
+    grid start early, so the attention kernel of a call without a stage launch may not read the
+    queries before it is complete.  Repeated over a query buffer that holds NaN before each
+    projection; the result equals am_q4_prefill's over the finished queries, bit for bit."""
+    Hq, Hkv, Dk, Dv, L = geom
+    N, width = L + 300, 4096
+    _, kq, vq = make_case(1, Hq, Hkv, N, Dk, Dv, L=1, dtype=torch.bfloat16, cuda=cuda, seed=23)
+    view, _ = pkg.kernels.contiguous_view(kq, vq)
+    kv_len = torch.full((1,), N, dtype=torch.int32, device=cuda)
+    g = torch.Generator().manual_seed(6)
+    w = pkg.Q4Weight(*pkg.quantize((torch.randn(Hq * Dk, width, generator=g) * width ** -0.5).bfloat16().to(cuda)))
+    x = torch.randn(L, width, generator=g).bfloat16().to(cuda)
+    buf = torch.empty(L, Hq * Dk, dtype=torch.bfloat16, device=cuda)
+    q = buf.view(1, L, Hq, Dk).transpose(1, 2)
+    kw = dict(causal=True, out_dtype=torch.float32)
+    pkg.quantized_matmul(x, w, out=buf)
+    torch.cuda.synchronize(cuda)
+    want = pkg.kernels.attention(view, q, Dk ** -0.5, kv_len, N, mode="prefill", **kw)
+    nbytes = pkg.kernels.prefill_workspace_bytes(view, 1, Hq, L, N)
+    ws = torch.full((nbytes,), 255, dtype=torch.uint8, device=cuda)
+    for _ in range(50):
+        buf.fill_(float("nan"))
+        pkg.kernels.attention(view, q, Dk ** -0.5, kv_len, N, mode="prefill_stage", workspace=ws, **kw)
+        pkg.quantized_matmul(x, w, out=buf)
+        got = pkg.kernels.attention(view, q, Dk ** -0.5, kv_len, N, mode="prefill_attend", workspace=ws, **kw)
+        assert torch.equal(got, want), (got - want).abs().max()
