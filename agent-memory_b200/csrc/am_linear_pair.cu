@@ -120,12 +120,16 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
   griddep_launch_dependents();
   if (s_base & 1023u) {  // swizzled tiles need a 1024-byte aligned window (the whole grid returns)
     if (tid == 0) flag_status(p.status, AM_STATUS_BAD_POSITION);
+    griddep_wait();
     return;
   }
   const int rank = static_cast<int>(blockIdx.x) & 1;
   const int first = static_cast<int>(blockIdx.x) >> 1, step = static_cast<int>(gridDim.x) >> 1;
   const int tiles = count_items(p, f.tile_tokens) * f.row_tiles;
-  if (first >= tiles) return;  // both CTAs of the pair
+  if (first >= tiles) {  // both CTAs of the pair
+    griddep_wait();  // (a grid may not be complete before the one it depends on: the next one waits for this one only)
+    return;
+  }
   const int stages = p.pstride >> 2;  // quads of groups
   const int slabs = p.groups, steps = (slabs + 1) / 2 * PARTS;  // (a step's parts follow one another)
 

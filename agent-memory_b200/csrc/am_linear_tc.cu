@@ -173,12 +173,16 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
   griddep_launch_dependents();
   if (s_base & 1023u) {  // swizzled tiles need a 1024-byte aligned window (the whole grid returns)
     if (tid == 0) flag_status(p.status, AM_STATUS_BAD_POSITION);
+    griddep_wait();
     return;
   }
   const int rank = f.ck > 1 ? static_cast<int>(blockIdx.x) % f.ck : 0;
   const int first = static_cast<int>(blockIdx.x) / f.ck, step = static_cast<int>(gridDim.x) / f.ck;
   const int tiles = count_items(p, NT) * f.row_tiles;
-  if (first >= tiles) return;  // the whole cluster
+  if (first >= tiles) {  // the whole cluster
+    griddep_wait();  // (a grid may not be complete before the one it depends on: the next one waits for this one only)
+    return;
+  }
   constexpr int CTA_ROWS = GATED ? 128 : 256;
   // this CTA's inputs: quads of groups [q0, q1), slabs of 64 inputs, steps of SP slabs
   const int quads = p.pstride >> 2;

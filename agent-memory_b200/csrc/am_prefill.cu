@@ -655,8 +655,9 @@ __global__ void __launch_bounds__(PrefillRoles<BN, QV4>::THREADS, 1)
 
   if (warp == RL::TMA_WARP) {
     // ================================================================ TMA producer
-    if (lane == 0 && n_tiles > 0) {
-      griddep_wait();  // the stage kernel's workspace rows are complete and visible
+    if (lane == 0) {
+      griddep_wait();  // the stage kernel's workspace rows are complete and visible (without keys to
+                       // load too: this grid may not end before that one)
       const int y0 = (b * p.hkv + h) * p.nw + (lo - blo);
       bool ok = true;
       for (int j = 0; j < n_tiles; ++j) {
@@ -1220,8 +1221,9 @@ __global__ void __launch_bounds__(kTile2Threads, 1) prefill2_kernel(const __grid
 
   if (warp == TMA_WARP) {
     // ================================================================ TMA producer
-    if (lane == 0 && n_tiles > 0) {
-      griddep_wait();  // the stage kernel's workspace rows are complete and visible
+    if (lane == 0) {
+      griddep_wait();  // the stage kernel's workspace rows are complete and visible (without keys to
+                       // load too: this grid may not end before that one)
       const int y0 = (b * p.hkv + h) * p.nw + (lo - blo);
       bool ok = true;
       for (int j = 0; j < n_tiles; ++j) {
