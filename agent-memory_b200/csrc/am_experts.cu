@@ -233,8 +233,19 @@ static cudaError_t launch_sort(const RouteParams& p, int ctas, int threads, cuda
   const int smem = (threads / 32 * p.n_experts + 2 * p.n_experts + 32 + 2 * held) * 4;
   auto kfn = route_sort_kernel<PER>;
   if (smem > 48 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // once per device, to what the largest call needs: host threads share the attribute, and one that
+    // set it to its own call's size could lower it between another's setting and launch
+    constexpr int kLargest = (34 * 1024 + 32 + 2 * kRouteHeld) * 4;  // 1024 experts, 32 warps
+    static unsigned long long done = 0;
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (!bit || !(__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) {
+      err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargest);
+      if (err != cudaSuccess) return err;
+      if (bit) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
+    }
   }
   return launch_chained(kfn, p, dim3(ctas), threads, smem, ctas, stream);
 }
