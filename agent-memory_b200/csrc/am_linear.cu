@@ -531,6 +531,39 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
 }
 
 constexpr int kFewSmem = 227 * 1024;
+constexpr int kFewCluster = 8;  // CTAs, at most, that split the inputs
+
+// Tokens of an item: all rows of a plain call; for experts twice their mean number (one with
+// more reads its weights again).  One token of 64 experts: 10.1 us with items of one token, 10.3
+// with items of eight; 16 tokens, items of four and eight: 42.9 and 45.1.
+static int few_tokens(int rows, int experts, bool grouped) {
+  const int64_t tok = grouped ? (2 * (int64_t)rows + experts - 1) / experts : rows;
+  return tok <= 1 ? 1 : tok <= 2 ? 2 : tok <= 4 ? 4 : kFewTokens;
+}
+
+// Positions between two sums: 16 KB of sums.
+constexpr int few_batch(int mt, int tk) { return 16 / (mt * tk) > 1 ? 16 / (mt * tk) : 1; }
+
+// Shared memory of a CTA where `ck` of them split the inputs (quads of groups): the warps' rings, the
+// activations with their group sums, the partial sums.
+template <int MT, int TK>
+static int64_t few_smem(int quads, int ck) {
+  constexpr int64_t ring = kFewWarps * kFewDepth<MT, TK> * MT * (kFewCodes + kFewPar);
+  constexpr int64_t red = few_batch(MT, TK) * MT * kFewWarps * TK * 64;
+  return ring + (int64_t)((quads + ck - 1) / ck) * 4 * (128 + 4) * TK + kFewWarps * 4 + red;
+}
+
+// Whether the largest cluster holds the activations of a call: up to 49152 inputs at 8 tokens (a gated
+// pair 32768), 65536 at 4, 131072 at 2 and 264192 at 1.
+static bool few_fits(int tok, bool gated, int n_in) {
+  const int quads = ((n_in / 64) + 3) / 4;
+  int64_t smem = 0;
+  if (tok == 1) smem = gated ? few_smem<2, 1>(quads, kFewCluster) : few_smem<1, 1>(quads, kFewCluster);
+  if (tok == 2) smem = gated ? few_smem<2, 2>(quads, kFewCluster) : few_smem<1, 2>(quads, kFewCluster);
+  if (tok == 4) smem = gated ? few_smem<2, 4>(quads, kFewCluster) : few_smem<1, 4>(quads, kFewCluster);
+  if (tok == 8) smem = gated ? few_smem<2, 8>(quads, kFewCluster) : few_smem<1, 8>(quads, kFewCluster);
+  return smem <= kFewSmem;
+}
 
 template <bool GATED, int MT, int TK>
 static cudaError_t launch_few_t(FewParams& f, cudaStream_t stream) {
@@ -550,18 +583,12 @@ static cudaError_t launch_few_t(FewParams& f, cudaStream_t stream) {
     if (err != cudaSuccess) return err;
     if (bit) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
   }
-  constexpr int ring = kFewWarps * kFewDepth<MT, TK> * MT * (kFewCodes + kFewPar);
-  f.batch = std::max(1, 16 / (MT * TK));  // 16 KB of sums
-  const int red = f.batch * MT * kFewWarps * TK * 64;
+  f.batch = few_batch(MT, TK);
   const int quads = p.pstride / 4;
-  auto smem_for = [&](int ck) {
-    const int groups = (quads + ck - 1) / ck * 4;
-    return ring + groups * (128 + 4) * TK + kFewWarps * 4 + red;
-  };
   int ck = 1;
-  while (ck < 8 && smem_for(ck) > kFewSmem) ck *= 2;
-  const int smem = smem_for(ck);
-  if (smem > kFewSmem) return cudaErrorNotSupported;
+  while (ck < kFewCluster && few_smem<MT, TK>(quads, ck) > kFewSmem) ck *= 2;
+  if (few_smem<MT, TK>(quads, ck) > kFewSmem) return cudaErrorNotSupported;  // (few_fits said it would)
+  const int smem = static_cast<int>(few_smem<MT, TK>(quads, ck));
   // Warps along the inputs: the split whose CTAs finish first, a position costing its groups and
   // about one and a half groups' time for the sums; a warp gets at least a whole stage.
   constexpr int TROWS = GATED ? 16 : 16 * MT;
@@ -618,11 +645,13 @@ static cudaError_t launch_few_t(FewParams& f, cudaStream_t stream) {
 }
 
 template <bool GATED, int MT, int MT8>
-static cudaError_t launch_few(FewParams& f, int64_t tok, cudaStream_t stream) {
-  if (tok <= 1) return launch_few_t<GATED, MT, 1>(f, stream);
-  if (tok <= 2) return launch_few_t<GATED, MT, 2>(f, stream);
-  if (tok <= 4) return launch_few_t<GATED, MT, 4>(f, stream);
-  return launch_few_t<GATED, MT8, 8>(f, stream);
+static cudaError_t launch_few(FewParams& f, int tok, cudaStream_t stream) {
+  switch (tok) {
+    case 1: return launch_few_t<GATED, MT, 1>(f, stream);
+    case 2: return launch_few_t<GATED, MT, 2>(f, stream);
+    case 4: return launch_few_t<GATED, MT, 4>(f, stream);
+    default: return launch_few_t<GATED, MT8, 8>(f, stream);
+  }
 }
 
 // Which kernel.  One matrix: this one up to 8 tokens (4096x4096 at 8: 7.6 us, the tiles 12.8; 28672x8192
@@ -630,21 +659,19 @@ static cudaError_t launch_few(FewParams& f, int64_t tok, cudaStream_t stream) {
 // pair is large, up to 4 of those (8 tokens, 33 million weights: 13.1 and 14.5 us; 117 million: 29.2 and
 // 24.4).  Experts: up to a mean of two rows (a grouped call's counts are on the device; 64 experts
 // of 2048x1408: mean 2 31.8 and 30.0 us, mean 1 24.1 and 25.4; 8 of 4096x14336 gated: mean 2 103
-// and 109, mean 3 143 and 111).
+// and 109, mean 3 143 and 111).  In each case only where the activations fit.
 bool linear_uses_tensor_tiles(int rows, int experts, bool grouped, bool gated, int n_out, int n_in) {
-  if (grouped) return (rows - 1) / experts >= 2;
-  return rows > kFewTokens || (gated && rows > 4 && 2LL * n_out * n_in > 56000000);
+  if (grouped ? (rows - 1) / experts >= 2
+              : rows > kFewTokens || (gated && rows > 4 && 2LL * n_out * n_in > 56000000))
+    return true;
+  return !few_fits(few_tokens(rows, experts, grouped), gated, n_in);
 }
 
 cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream) {
   if (p.rows == 0) return cudaSuccess;
   FewParams f{};
   f.p = p;
-  // Tokens of an item: all rows of a plain call; for experts twice their mean number (one with
-  // more reads its weights again).  One token of 64 experts: 10.1 us with items of one token, 10.3
-  // with items of eight; 16 tokens, items of four and eight: 42.9 and 45.1.
-  int64_t tok = p.rows;
-  if (p.offsets != nullptr) tok = (2 * (int64_t)p.rows + p.experts - 1) / p.experts;
+  const int tok = few_tokens(p.rows, p.experts, p.offsets != nullptr);
   return p.codes[1] != nullptr ? launch_few<true, 2, 2>(f, tok, stream) : launch_few<false, 1, 1>(f, tok, stream);
 }
 

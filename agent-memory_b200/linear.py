@@ -27,8 +27,8 @@ from .kernels import GROUP_SIZE, _check_params, _half_code, as_codes, _require_c
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
-# With at most so many tokens one matrix, or a gated pair, needs no workspace.
-FEW_TOKENS, FEW_GATED_TOKENS = 8, 4
+# With at most so many tokens and inputs one matrix, or a gated pair, needs no workspace.
+FEW_TOKENS, FEW_GATED_TOKENS, FEW_INPUTS = 8, 4, 49152
 
 
 class Q4Weight:
@@ -144,7 +144,8 @@ def _linear_call(x, rows2, w, up, out):
     lib = _lib.load()
     up_ref = up.ref if up is not None else None
     need, ws = 0, None
-    if rows > (FEW_TOKENS if up is None else FEW_GATED_TOKENS):  # (scratch of the call from the caching allocator, on the call's stream)
+    # (scratch of the call from the caching allocator, on the call's stream)
+    if rows > (FEW_TOKENS if up is None else FEW_GATED_TOKENS) or w.n_in > FEW_INPUTS:
         need = int(lib.am_q4_linear_workspace_bytes(w.ref, up_ref, rows))
         ws = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
     rc = lib.am_q4_linear(w.ref, up_ref, rows2.data_ptr(), _row_stride(rows2), rows, out.data_ptr(),

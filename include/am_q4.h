@@ -311,7 +311,7 @@ int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int
  * second matrix `up` of the same shape y = silu(x W^T) * (x up^T).  x: device [rows, n_in],
  * out: device [rows, n_out], both of w->dtype, row strides in elements (x_stride % 8 == 0, x
  * 16-byte aligned).  Sums are fp32; y is rounded once.  A few tokens (up to 8, gated pairs 4
- * to 8) multiply exact weights.  For more a weight enters as scale * code + bias rounded once
+ * to 8, while their activations fit: 32768 inputs and more) multiply exact weights.  For more a weight enters as scale * code + bias rounded once
  * to fp16, for a gated fp16 call as the sum of two such parts.  Activations are exact but for
  * values below 2^-28 of their token's largest; infinite or NaN ones make their token's outputs
  * infinite or NaN.  workspace: device memory, 256-byte aligned, of the size the query gives

@@ -1,0 +1,36 @@
+"""4-bit linear and expert calls at the edges of what they take: many inputs, unusual rows, infinities."""
+
+import pytest
+import torch
+
+from conftest import pkg
+from test_gpu_linear import assert_within, expected, expected_experts, make_weight, make_x, routing_of, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("tokens,k", [(1, 49216), (4, 53248), (5, 14336), (8, 14336), (5, 49152), (5, 49216),
+                                      (8, 49152), (8, 53248), (9, 53248), (3, 69632), (2, 139264), (1, 278528)])
+def test_many_inputs(cuda, tokens, k):
+    """Few tokens of more inputs than a CTA, a cluster of 4 or 8, or the few-token kernel holds."""
+    w = make_weight((48, k), torch.bfloat16, cuda)
+    x = make_x(tokens, k, torch.bfloat16, cuda)
+    assert_within(run(x, [w]), *expected(x, [w]))
+
+
+@pytest.mark.parametrize("tokens,k", [(2, 139264), (4, 69632), (8, 14336), (5, 32768), (5, 32832), (8, 53248)])
+def test_many_inputs_gated(cuda, tokens, k):
+    ws = [make_weight((40, k), torch.float16, cuda, seed=i, scale=0.002) for i in range(2)]
+    x = make_x(tokens, k, torch.float16, cuda)
+    assert_within(run(x, ws), *expected(x, ws))
+
+
+def test_many_inputs_of_experts(cuda):
+    n_experts, k = 3, 139264
+    ws = [make_weight((n_experts, 24, k), torch.float16, cuda, seed=i, scale=0.002) for i in range(2)]
+    q = [pkg.Q4Weight(*w) for w in ws]
+    for tokens in (1, 3, 6):
+        r = routing_of((torch.arange(tokens, device=cuda) % n_experts)[:, None], n_experts)
+        x = make_x(tokens, k, torch.float16, cuda)
+        assert_within(pkg.expert_swiglu(x, *q, r), *expected_experts(x, ws, r, True))
+        assert_within(pkg.expert_matmul(x, q[0], r, gather=True), *expected_experts(x, ws[:1], r, True))

@@ -54,6 +54,22 @@ def test_workspace_sizes():
     assert int(lib.am_q4_linear_workspace_bytes(None, None, 100)) == 0
 
 
+def test_workspace_beyond_the_few_token_kernels_inputs():
+    """A few tokens of more inputs than one cluster's shared memory holds go the way of many, and need its
+    workspace; up to `linear.FEW_INPUTS` the Python calls need not ask."""
+    lib = pkg._lib.load()
+    size = lambda n_in, rows, gated=False: int(lib.am_q4_linear_workspace_bytes(  # noqa: E731
+        ctypes.byref(weight(n_in=n_in)), ctypes.byref(weight(n_in=n_in)) if gated else None, rows))
+    few = pkg.linear.FEW_INPUTS
+    assert [size(few, m) for m in range(1, pkg.linear.FEW_TOKENS + 1)] == [0] * pkg.linear.FEW_TOKENS
+    assert [size(few, m, True) for m in range(1, pkg.linear.FEW_GATED_TOKENS + 1)] == [0] * pkg.linear.FEW_GATED_TOKENS
+    for n_in, rows, gated in ((49408, 5, False), (53248, 8, False), (131072, 4, False), (278528, 1, False),
+                              (33024, 5, True), (131072, 3, True)):
+        assert size(n_in, rows, gated) == rows * (n_in * 2 + 4), (n_in, rows, gated)
+    e = weight(n_in=139264, experts=4)
+    assert int(lib.am_q4_expert_linear_workspace_bytes(ctypes.byref(e), None, 8)) == 8 * (139264 * 2 + 4)
+
+
 @pytest.mark.parametrize("field,value", [("codes", None), ("params", None), ("row_scale", None), ("codes", PTR + 4),
                                          ("n_in", 96), ("n_in", 0), ("n_out", 0), ("n_out", -3), ("experts", 0),
                                          ("dtype", 2), ("dtype", 9)])
