@@ -100,7 +100,7 @@ def _rows_of(x: torch.Tensor, w: Q4Weight) -> torch.Tensor:
     if len(shape) != 2:
         x = x.reshape(-1, w.n_in)
     stride = x.stride()
-    if stride[1] != 1 or x.data_ptr() % 16 or (stride[0] % 8 and x.shape[0] > 1):
+    if stride[1] != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (stride[0] % 8 or stride[0] < w.n_in)):
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()

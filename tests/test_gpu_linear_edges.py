@@ -34,3 +34,18 @@ def test_many_inputs_of_experts(cuda):
         x = make_x(tokens, k, torch.float16, cuda)
         assert_within(pkg.expert_swiglu(x, *q, r), *expected_experts(x, ws, r, True))
         assert_within(pkg.expert_matmul(x, q[0], r, gather=True), *expected_experts(x, ws[:1], r, True))
+
+
+@pytest.mark.parametrize("tokens", [2, 8, 40, 300])
+def test_rows_that_share_memory(cuda, tokens):
+    """A broadcast token (row stride 0) and overlapping windows of one sequence (row stride 64)."""
+    w, up = (make_weight((48, 256), torch.bfloat16, cuda, seed=i) for i in range(2))
+    experts = make_weight((3, 48, 256), torch.bfloat16, cuda)
+    r = routing_of((torch.arange(tokens, device=cuda) % 3)[:, None], 3)
+    flat = make_x(1, 256 + 64 * tokens, torch.bfloat16, cuda).flatten()
+    for x in (flat[:256].expand(tokens, -1), flat.as_strided((tokens, 256), (64, 1)), flat[64:320].expand(2, tokens, -1)):
+        assert_within(run(x, [w]), *expected(x, [w]), str(x.stride()))
+        assert_within(run(x, [w, up]), *expected(x, [w, up]), str(x.stride()))
+        if x.dim() == 2:
+            got = pkg.expert_matmul(x, pkg.Q4Weight(*experts), r, gather=True)
+            assert_within(got, *expected_experts(x, [experts], r, True), str(x.stride()))
