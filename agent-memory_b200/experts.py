@@ -21,7 +21,7 @@ from . import _lib
 from ._lib import check
 from .kernels import _half_code, dtype_code
 from .linear import (Q4Weight, _check_out, _check_pair, _current_device, _raw_stream, _row_stride,
-                     _rows_of)
+                     _rows_of, _status_ptr)
 
 MAX_EXPERTS, MAX_TOP_K = 1024, 32
 
@@ -46,14 +46,6 @@ def _int32(t: torch.Tensor, shape, device, what: str) -> torch.Tensor:
         raise ValueError(f"{what} must be int32 {tuple(shape)} on {device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return t if t.is_contiguous() else t.contiguous()
-
-
-def _status_ptr(status, device):
-    if status is None:
-        return None
-    if status.dtype is not torch.int32 or status.device != device or status.numel() < 1:
-        raise ValueError(f"status must be an int32 tensor on {device}")
-    return status.data_ptr()
 
 
 def route_experts(logits: torch.Tensor, top_k: int, *, normalize: bool = True) -> ExpertRouting:
@@ -146,7 +138,8 @@ def expert_matmul(x: torch.Tensor, weight: Q4Weight, routing: ExpertRouting, *, 
     """Row r of x [tokens * top_k, n_in], sorted by expert, times its expert's matrix (with
     ``gather`` x is [tokens, n_in] and each pair's row is fetched through ``routing.order``)
     -> [tokens * top_k, n_out] sorted by expert.  ``status``: optional int32 device word that
-    gets AM_STATUS_* bits for order entries outside x."""
+    gets AM_STATUS_* bits: for order entries outside x, and where a bounded wait of the tensor
+    tiles ran out (rows of the output are then unwritten)."""
     return _expert_linear(x, weight, None, routing, gather, out, status)
 
 

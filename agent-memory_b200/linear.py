@@ -123,17 +123,25 @@ def _check_out(out: torch.Tensor, w: Q4Weight, shape) -> None:
         raise ValueError(f"out must be a contiguous {w.dtype} tensor {tuple(shape)} on {w.device}")
 
 
-def _linear(x: torch.Tensor, w: Q4Weight, up: Q4Weight | None, out):
+def _status_ptr(status, device):
+    if status is None:
+        return None
+    if status.dtype is not torch.int32 or status.device != device or status.numel() < 1:
+        raise ValueError(f"status must be an int32 tensor on {device}")
+    return status.data_ptr()
+
+
+def _linear(x: torch.Tensor, w: Q4Weight, up: Q4Weight | None, out, status):
     if w.grouped:
         raise ValueError(f"{w} holds one matrix per expert: use expert_matmul / expert_swiglu")
     rows2 = _rows_of(x, w)
     if w.index != _current_device():
         with torch.cuda.device(w.device):
-            return _linear_call(x, rows2, w, up, out)
-    return _linear_call(x, rows2, w, up, out)
+            return _linear_call(x, rows2, w, up, out, status)
+    return _linear_call(x, rows2, w, up, out, status)
 
 
-def _linear_call(x, rows2, w, up, out):
+def _linear_call(x, rows2, w, up, out, status):
     rows = rows2.shape[0]
     if out is not None:
         _check_out(out, w, (*x.shape[:-1], w.n_out))
@@ -149,21 +157,25 @@ def _linear_call(x, rows2, w, up, out):
         need = int(lib.am_q4_linear_workspace_bytes(w.ref, up_ref, rows))
         ws = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
     rc = lib.am_q4_linear(w.ref, up_ref, rows2.data_ptr(), _row_stride(rows2), rows, out.data_ptr(),
-                          w.n_out, ws.data_ptr() if need else None, need, None, _raw_stream(w.index))
+                          w.n_out, ws.data_ptr() if need else None, need,
+                          _status_ptr(status, w.device), _raw_stream(w.index))
     if rc:
         check("am_q4_linear", rc)
     return out
 
 
-def quantized_matmul(x: torch.Tensor, weight: Q4Weight, *, out: torch.Tensor | None = None):
+def quantized_matmul(x: torch.Tensor, weight: Q4Weight, *, out: torch.Tensor | None = None,
+                     status: torch.Tensor | None = None):
     """x [..., n_in] times the weight's transpose -> [..., n_out] in x's type (see module
-    docstring).  One token is a matrix-vector product; any number of tokens is accepted."""
-    return _linear(x, weight, None, out)
+    docstring).  One token is a matrix-vector product; any number of tokens is accepted.
+    ``status``: optional int32 device word that gets AM_STATUS_TIMEOUT where a bounded wait of the
+    tensor tiles ran out (rows of the output are then unwritten)."""
+    return _linear(x, weight, None, out, status)
 
 
 def quantized_swiglu(x: torch.Tensor, gate: Q4Weight, up: Q4Weight, *,
-                     out: torch.Tensor | None = None):
+                     out: torch.Tensor | None = None, status: torch.Tensor | None = None):
     """silu(x gate^T) * (x up^T) -> [..., n_out] in x's type, both products in one kernel and the
-    gate's result never rounded in between."""
+    gate's result never rounded in between.  ``status`` as in quantized_matmul."""
     _check_pair(gate, up)
-    return _linear(x, gate, up, out)
+    return _linear(x, gate, up, out, status)

@@ -315,7 +315,8 @@ int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int
  * to fp16, for a gated fp16 call as the sum of two such parts.  Activations are exact but for
  * values below 2^-28 of their token's largest; infinite or NaN ones make their token's outputs
  * infinite or NaN.  workspace: device memory, 256-byte aligned, of the size the query gives
- * (0 for a few tokens); scratch of the call, free again when it has run.
+ * (0 for a few tokens); scratch of the call, free again when it has run.  status (device word
+ * or NULL) gets AM_STATUS_TIMEOUT where a bounded wait ran out: rows of out are then unwritten.
  */
 size_t am_q4_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up, int32_t rows);
 int am_q4_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, int64_t x_stride,

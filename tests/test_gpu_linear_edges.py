@@ -49,3 +49,26 @@ def test_rows_that_share_memory(cuda, tokens):
         if x.dim() == 2:
             got = pkg.expert_matmul(x, pkg.Q4Weight(*experts), r, gather=True)
             assert_within(got, *expected_experts(x, [experts], r, True), str(x.stride()))
+
+
+@pytest.mark.parametrize("tokens,n,gated", [(40, 512, False), (40, 40960, False), (100, 600, True), (600, 8448, True),
+                                            (1500, 4352, False)])
+def test_a_linear_call_reports_waits_that_ran_out(cuda, monkeypatch, tokens, n, gated):
+    """Tiles of one SM (split over a cluster and not) and of pairs of SMs whose waits give up at once say so
+    in the caller's status word; the next call is right and leaves it alone."""
+    ws = [make_weight((n, 640), torch.float16, cuda, seed=i) for i in range(1 + gated)]
+    q = [pkg.Q4Weight(*w) for w in ws]
+    x = make_x(tokens, 640, torch.float16, cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    f = lambda: (pkg.quantized_swiglu if gated else pkg.quantized_matmul)(x, *q, status=status)  # noqa: E731
+    monkeypatch.setenv("AM_Q4_TEST_WAIT_LIMIT_NS", "0")
+    f()
+    torch.cuda.synchronize(cuda)
+    assert int(status.item()) == pkg._lib.STATUS_TIMEOUT
+    monkeypatch.delenv("AM_Q4_TEST_WAIT_LIMIT_NS")
+    status.zero_()
+    assert_within(f(), *expected(x, ws))
+    assert int(status.item()) == 0
+    for bad in (status.long(), status.cpu(), status[:0]):
+        with pytest.raises(ValueError):
+            pkg.quantized_matmul(x, q[0], status=bad)
