@@ -440,7 +440,11 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
 #pragma unroll
       for (int i = 0; i < 4; ++i) rs[m][i] = __ldg(p.row_scale[m] + (int64_t)e * p.n_out + min(row + i, p.n_out - 1));
     cluster_sync_all();
-    if (!*abort_flag && tl < TL && row < p.n_out) {
+    if (!*abort_flag && tl < TL) {
+      // a rank that gave up has no sums: then nothing is stored (a lane asks one rank, ahead of the first
+      // sums, and the warp votes behind them; a lane asking all ranks cost 0.35 us)
+      int gave_up = 0;
+      if (lane < f.ck) gave_up = __float_as_int(ld_dsmem_f32(dsmem_addr(smem_u32(const_cast<const int*>(abort_flag)), lane)));
       const int m = hi - lo;
       const int t0 = m * rank / f.ck, t1 = m * (rank + 1) / f.ck;
       const bool wide = (p.out_stride & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && row + 4 <= p.n_out;
@@ -459,6 +463,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
             s[k].w += v.w;
           }
         }
+        if (__any_sync(0xffffffffu, gave_up)) break;
         const float ts = tok_scale[tok];
         float y[4] = {s[0].x, s[0].y, s[0].z, s[0].w};
 #pragma unroll

@@ -72,3 +72,23 @@ def test_a_linear_call_reports_waits_that_ran_out(cuda, monkeypatch, tokens, n, 
     for bad in (status.long(), status.cpu(), status[:0]):
         with pytest.raises(ValueError):
             pkg.quantized_matmul(x, q[0], status=bad)
+
+
+@pytest.mark.parametrize("tokens", [20, 40, 100])
+@pytest.mark.parametrize("gated", [False, True])
+def test_a_split_tile_that_gave_up_stores_nothing(cuda, monkeypatch, tokens, gated):
+    """Clusters of 8, 4 and 2 that split the inputs: no unfinished sum reaches the output."""
+    for n in (256, 2048, 8192):
+        ws = [make_weight((n, 2048), torch.bfloat16, cuda, seed=i) for i in range(1 + gated)]
+        q = [pkg.Q4Weight(*w) for w in ws]
+        x = make_x(tokens, 2048, torch.bfloat16, cuda)
+        out = torch.empty(tokens, n, dtype=torch.bfloat16, device=cuda)
+        f = lambda: (pkg.quantized_swiglu if gated else pkg.quantized_matmul)(x, *q, out=out)  # noqa: E731
+        assert_within(f(), *expected(x, ws))
+        out.fill_(7.0)
+        monkeypatch.setenv("AM_Q4_TEST_WAIT_LIMIT_NS", "0")
+        f()
+        torch.cuda.synchronize(cuda)
+        monkeypatch.delenv("AM_Q4_TEST_WAIT_LIMIT_NS")
+        assert bool((out == 7.0).all())
+        assert_within(f(), *expected(x, ws))
