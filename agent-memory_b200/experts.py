@@ -20,7 +20,7 @@ import torch
 from . import _lib
 from ._lib import check
 from .kernels import _half_code, dtype_code
-from .linear import (Q4Weight, _check_out, _check_pair, _current_device, _raw_stream, _row_stride,
+from .linear import (Q4Weight, _check_apart, _check_out, _check_pair, _current_device, _raw_stream, _row_stride,
                      _rows_of, _status_ptr)
 
 MAX_EXPERTS, MAX_TOP_K = 1024, 32
@@ -118,6 +118,7 @@ def _expert_linear(x, w: Q4Weight, up, routing: ExpertRouting, gather: bool, out
 def _expert_call(x, w, up, offsets, order, top_k, rows, out, status):
     if out is not None:
         _check_out(out, w, (rows, w.n_out))
+        _check_apart(out, x, "x")
     else:
         out = torch.empty(rows, w.n_out, dtype=w.dtype, device=w.device)
     lib = _lib.load()
@@ -156,7 +157,8 @@ def combine_experts(y: torch.Tensor, weights: torch.Tensor, positions: torch.Ten
                     residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
                     status: torch.Tensor | None = None):
     """out[t] = residual[t] + sum_j weights[t, j] * y[positions[t, j]]: y [rows, width] float16
-    or bfloat16, weights float32 and positions int32 [tokens, top_k].  fp32 sums, rounded once."""
+    or bfloat16, weights float32 and positions int32 [tokens, top_k].  fp32 sums, rounded once.
+    ``out`` may be the residual itself; it may not share memory with y."""
     if not y.is_cuda:
         raise ValueError("Q4 kernels run on CUDA tensors only (no CPU path)")
     if y.dim() != 2 or positions.dim() != 2:
@@ -185,6 +187,10 @@ def combine_experts(y: torch.Tensor, weights: torch.Tensor, positions: torch.Ten
     elif (out.shape != (tokens, width) or out.dtype is not y.dtype or out.device != dev
           or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous {y.dtype} tensor {(tokens, width)} on {dev}")
+    else:
+        _check_apart(out, y, "y")
+        if residual is not None and not (out.data_ptr() == res and res_stride == width):
+            _check_apart(out, residual, "residual other than row by row")
     args = (y.data_ptr(), code, _row_stride(y), y.shape[0], weights.data_ptr(), positions.data_ptr(),
             res, res_stride, out.data_ptr(), width, tokens, top_k, width, _status_ptr(status, dev),
             _raw_stream(dev.index))

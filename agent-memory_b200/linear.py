@@ -123,6 +123,19 @@ def _check_out(out: torch.Tensor, w: Q4Weight, shape) -> None:
         raise ValueError(f"out must be a contiguous {w.dtype} tensor {tuple(shape)} on {w.device}")
 
 
+def _check_apart(out: torch.Tensor, rows: torch.Tensor, what: str) -> None:
+    """Refuses a contiguous `out` that shares memory with the rows a call reads: CTAs store outputs
+    while others still read."""
+    if out.numel() == 0 or rows.numel() == 0:
+        return
+    start, width = rows.data_ptr(), rows.shape[1] * rows.element_size()
+    step = max(rows.stride(0) * rows.element_size(), width)
+    lo = out.data_ptr()
+    first = max((lo - width - start) // step + 1, 0)  # the first row that ends behind out's start
+    if first < rows.shape[0] and start + first * step < lo + out.numel() * out.element_size():
+        raise ValueError(f"out shares memory with {what}")
+
+
 def _status_ptr(status, device):
     if status is None:
         return None
@@ -145,6 +158,7 @@ def _linear_call(x, rows2, w, up, out, status):
     rows = rows2.shape[0]
     if out is not None:
         _check_out(out, w, (*x.shape[:-1], w.n_out))
+        _check_apart(out, rows2, "x")
     elif x.dim() == 2:
         out = torch.empty(rows, w.n_out, dtype=w.dtype, device=w.device)
     else:
@@ -167,7 +181,8 @@ def _linear_call(x, rows2, w, up, out, status):
 def quantized_matmul(x: torch.Tensor, weight: Q4Weight, *, out: torch.Tensor | None = None,
                      status: torch.Tensor | None = None):
     """x [..., n_in] times the weight's transpose -> [..., n_out] in x's type (see module
-    docstring).  One token is a matrix-vector product; any number of tokens is accepted.
+    docstring).  One token is a matrix-vector product; any number of tokens is accepted.  ``out``
+    may not share memory with x.
     ``status``: optional int32 device word that gets AM_STATUS_TIMEOUT where a bounded wait of the
     tensor tiles ran out (rows of the output are then unwritten)."""
     return _linear(x, weight, None, out, status)

@@ -310,7 +310,7 @@ int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int
  * y = x W^T (replaces mx.quantized_matmul(x, w, scales, biases, transpose=True)), or with a
  * second matrix `up` of the same shape y = silu(x W^T) * (x up^T).  x: device [rows, n_in],
  * out: device [rows, n_out], both of w->dtype, row strides in elements (x_stride % 8 == 0, x
- * 16-byte aligned).  Sums are fp32; y is rounded once.  A few tokens (up to 8, gated pairs 4
+ * 16-byte aligned); out may not share memory with x.  Sums are fp32; y is rounded once.  A few tokens (up to 8, gated pairs 4
  * to 8, while their activations fit: 32768 inputs and more) multiply exact weights.  For more a weight enters as scale * code + bias rounded once
  * to fp16, for a gated fp16 call as the sum of two such parts.  Activations are exact but for
  * values below 2^-28 of their token's largest; infinite or NaN ones make their token's outputs
@@ -359,7 +359,7 @@ int am_route_experts(const void* logits, int32_t dtype, int64_t stride, int32_t 
  * order, rounded once).  y: device [y_rows, width], residual (or NULL) and out: device
  * [tokens, width], of dtype F16 or BF16, row strides in elements; weights / positions: device
  * [tokens, top_k].  A position outside [0, y_rows) adds nothing and sets
- * AM_STATUS_BAD_POSITION.
+ * AM_STATUS_BAD_POSITION.  out may be the residual itself; it may not share memory with y.
  */
 int am_combine_experts(const void* y, int32_t dtype, int64_t y_stride, int32_t y_rows,
                        const float* weights, const int32_t* positions, const void* residual,

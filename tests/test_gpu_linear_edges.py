@@ -92,3 +92,41 @@ def test_a_split_tile_that_gave_up_stores_nothing(cuda, monkeypatch, tokens, gat
         monkeypatch.delenv("AM_Q4_TEST_WAIT_LIMIT_NS")
         assert bool((out == 7.0).all())
         assert_within(f(), *expected(x, ws))
+
+
+@pytest.mark.parametrize("tokens", [1, 4, 8, 40])
+def test_an_output_on_the_memory_of_the_input_is_refused(cuda, tokens):
+    k = 256
+    w = make_weight((k, k), torch.bfloat16, cuda)
+    q = pkg.Q4Weight(*w)
+    qe = pkg.Q4Weight(*make_weight((1, k, k), torch.bfloat16, cuda))
+    r = routing_of(torch.zeros(tokens, 1, dtype=torch.int64, device=cuda), 1)
+    buf = make_x(2 * tokens + 1, k, torch.bfloat16, cuda)
+    x = buf[:tokens]
+    for out in (x, buf[tokens - 1:2 * tokens - 1], buf.flatten()[8:8 + x.numel()].view(tokens, k)):
+        for call in (lambda: pkg.quantized_matmul(x, q, out=out), lambda: pkg.quantized_swiglu(x, q, q, out=out),
+                     lambda: pkg.expert_matmul(x, qe, r, out=out)):
+            with pytest.raises(ValueError, match="shares memory"):
+                call()
+    want = expected(x, [w])
+    assert_within(pkg.quantized_matmul(x, q, out=buf[tokens:2 * tokens]), *want)  # right behind x
+    wide = make_x(2, 4 * k, torch.bfloat16, cuda)
+    gap = wide.flatten()[k:2 * k].view(1, k)  # between two rows of a strided x
+    assert_within(pkg.quantized_matmul(wide[:1, :k], q, out=gap), *expected(wide[:1, :k], [w]))
+    every_other = make_x(tokens, 2 * k, torch.bfloat16, cuda)[:, ::2]  # copied: an output on it is no matter
+    want = expected(every_other, [w])
+    out = every_other._base.flatten()[:tokens * k].view(tokens, k) if every_other._base is not None else None
+    assert_within(pkg.quantized_matmul(every_other, q, out=out), *want)
+
+
+def test_a_combination_onto_its_inputs(cuda):
+    y = make_x(12, 64, torch.float16, cuda)
+    w = torch.rand(6, 2, device=cuda)
+    pos = torch.arange(12, dtype=torch.int32, device=cuda).view(6, 2)
+    res = make_x(7, 64, torch.float16, cuda, seed=3)
+    want = pkg.combine_experts(y, w, pos, residual=res[:6])
+    with pytest.raises(ValueError, match="shares memory with y"):
+        pkg.combine_experts(y, w, pos, out=y[3:9])
+    with pytest.raises(ValueError, match="residual"):
+        pkg.combine_experts(y, w, pos, residual=res[:6], out=res[1:])
+    assert torch.equal(pkg.combine_experts(y, w, pos, residual=res[:6], out=res[:6]), want)
