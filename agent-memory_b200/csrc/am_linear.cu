@@ -22,8 +22,11 @@ int sm_count(int* device) {
 
 // ---------------------------------------------------------------- weight parameters
 // One warp per weight row: the row's exponent e is the smallest with every |scale| * 2^(24-e)
-// and |bias| * 2^-e at most 2^15 (fp16 holds up to 65504), then the groups' pairs are scaled by
-// powers of two and stored as fp16.
+// and |bias| * 2^(20-e) at most 2^15 (fp16 holds up to 65504), then the groups' pairs are scaled by
+// these powers of two and stored as fp16.  The two reach their limit together at |bias| =
+// 16 scale, just above what a quantizer of 16 levels gives (0 to -15 scale), so both have fp16's
+// whole range below the row's largest: with L the larger of max |scale| and max |bias| / 16, a
+// scale is exact from 2^-28 L and a bias from 2^-24 L on (those of bf16 8 times further down).
 __device__ __forceinline__ int exponent_above(float v) {  // least e with v < 2^e (v > 0, finite)
   int e;
   frexpf(v, &e);
@@ -52,14 +55,14 @@ __global__ void __launch_bounds__(128) weight_pack_kernel(const uint16_t* scales
   constexpr float kMax = 3.0e38f;  // an infinite scale or bias stays infinite in the params
   int e = -126;
   if (ms > 0.0f) e = max(e, exponent_above(fminf(ms, kMax)) + 24 - 15);
-  if (mb > 0.0f) e = max(e, exponent_above(fminf(mb, kMax)) - 15);
+  if (mb > 0.0f) e = max(e, exponent_above(fminf(mb, kMax)) + 20 - 15);
   if (ms == 0.0f && mb == 0.0f) e = 0;
   e = min(e, 127);
   if (lane == 0) row_scale[row] = ldexpf(1.0f, e);
   const int pstride = (groups + 3) & ~3;
   for (int g = lane; g < pstride; g += 32) {
     uint32_t v = 0;
-    if (g < groups) v = pack_half2(ldexpf(h2f<BF16>(s[g]), 24 - e), ldexpf(h2f<BF16>(b[g]), -e));
+    if (g < groups) v = pack_half2(ldexpf(h2f<BF16>(s[g]), 24 - e), ldexpf(h2f<BF16>(b[g]), 20 - e));
     params[row * pstride + g] = v;
   }
 }
@@ -86,7 +89,7 @@ cudaError_t launch_weight_pack(const void* scales, const void* biases, bool bf16
 //   the tensor cores (exact products, fp32 sums), the rest in fp32: no weight is rounded.  One
 //   AND turns two nibbles of a word into fp16 subnormals code * 2^-24, or 16 code * 2^-24 for
 //   the odd nibbles, whose activations are staged divided by 16: 5 integer operations for 8
-//   weights; the parameters hold scale * 2^24 (am_q4_weight_pack).
+//   weights; the parameters hold scale * 2^24 and bias * 2^20 (am_q4_weight_pack).
 // * The inputs of a group are permuted over the MMA's k slots so that lane t of a quad owns words
 //   2t and 2t + 1 of its row.  The activations are staged in the same order, as fp16 under a
 //   power of two per token and slice (exact), in fragment order, with their group sums.
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   constexpr int STAGE = MT * (kFewCodes + kFewPar);
   uint8_t* ring = smem + warp * (D * STAGE);
   uint8_t* sx = smem + kFewWarps * D * STAGE;  // [group][half][TK][4] x 16 bytes
-  float* sxsum = reinterpret_cast<float*>(sx + cta_groups * XG);     // [group][TK]
+  float* sxsum = reinterpret_cast<float*>(sx + cta_groups * XG);     // [group][TK], times 2^-20
   float* sxmax = sxsum + cta_groups * TK;  // [warp]: largest |x| of its part of a token, as bits
   float* red = sxmax + kFewWarps;
   const int row_tiles = (p.n_out + TROWS - 1) / TROWS;
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
         const int grp = v >> 3, c = v & 7;
         if (v < vecs) {
           *reinterpret_cast<uint4*>(sx + grp * XG + ((c & 1) * TK + x_tok) * 64 + (c >> 1) * 16) = o;
-          if (c == 0) sxsum[grp * TK + x_tok] = sum;
+          if (c == 0) sxsum[grp * TK + x_tok] = sum * 0x1p-20f;  // (what the biases are multiplied by)
         }
       };
 #pragma unroll

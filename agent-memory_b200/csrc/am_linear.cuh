@@ -8,7 +8,7 @@ namespace am {
 // y = x W^T over 4-bit weights, plain or gated (up != null), for one matrix or per expert.
 struct LinearParams {
   const uint32_t* codes[2];   // [0] the matrix (gate), [1] its partner (up) or null
-  const uint32_t* params[2];  // [rows of weights][pstride]: half2 (scale * 2^(24-e), bias * 2^-e)
+  const uint32_t* params[2];  // [rows of weights][pstride]: half2 (scale * 2^(24-e), bias * 2^(20-e))
   const float* row_scale[2];  // [rows of weights]: 2^e
   int32_t n_out, n_in, groups, pstride;
   int32_t experts;
@@ -108,7 +108,7 @@ template <int PARTS>
 __device__ __forceinline__ void dequant_group(const uint4& w0, const uint4& w1, uint32_t params, int part,
                                               uint32_t (&o)[32]) {
   const uint32_t s24 = __byte_perm(params, params, 0x1010);
-  uint32_t b = __byte_perm(params, params, 0x3232);
+  uint32_t b = hfma2_bits(__byte_perm(params, params, 0x3232), 0x00100010u, 0x80008000u);  // * 2^-20
   const uint32_t s20 = hfma2_bits(s24, 0x2c002c00u, 0x80008000u);  // * 2^-4
   // 8 * scale = s24 * 2^-21
   if (PARTS == 2) b = part == 0 ? hfma2_bits(s24, 0x00080008u, b) : hfma2_bits(s24, 0x80088008u, 0x80008000u);

@@ -7,9 +7,11 @@ the codes as they are and lays the scales and biases out once.  ``quantized_matm
 gated half of an MLP, ``silu(x G^T) * (x U^T)``, in one pass over both matrices.
 
 Sums are fp32 and the result is rounded once to the activations' type.  A few tokens multiply
-exact weights.  For more tokens a weight is ``scale * code + bias`` rounded to fp16 (11 bits)
-under a power of two per weight row; in a gated float16 layer, where two such errors would be
-1.6 times the output's own rounding, it is the sum of two fp16 parts.  An activation is exact
+exact weights: scales and biases are held in fp16 under powers of two per weight row, which keeps
+a scale from 2**-28 and a bias from 2**-24 of the row's largest scale on (or of 1/16 of its largest
+bias, if that is larger).  For more tokens a weight is ``scale * code + bias`` rounded to fp16 (11
+bits, or 2**-14 of that largest scale if that is more); in a gated float16 layer, where two such
+errors would be 1.6 times the output's own rounding, it is the sum of two fp16 parts.  An activation is exact
 (bf16 values enter as fp16 under a power of two per token; only values below 2**-28 of their
 token's largest lose bits).  An infinite or NaN activation
 makes its token's outputs infinite or NaN.  The weights are frozen: there is no backward pass.

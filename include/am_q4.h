@@ -299,9 +299,10 @@ typedef struct am_q4_weight {
 /*
  * Lays out the scales and biases (device [rows, n_in/64] of dtype F16 or BF16) of `rows`
  * weight rows for the kernels: row_scale[r] = 2^e with e chosen so that every
- * scale * 2^(24-e) and bias * 2^-e of row r fits fp16, and params[r, g] = the two as fp16
- * (low half: the scale).  Both keep their value unless a group's is below about 2^-28 of
- * its row's largest; entries past n_in/64 of a params row are zero.
+ * scale * 2^(24-e) and bias * 2^(20-e) of row r fits fp16, and params[r, g] = the two as fp16
+ * (low half: the scale).  With L the larger of max |scale| and max |bias| / 16 of a row, a scale
+ * keeps its value from 2^-28 L on and a bias from 2^-24 L on, for L below 2^118.  Entries past
+ * n_in/64 of a params row are zero.
  */
 int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int64_t rows,
                       int32_t n_in, uint32_t* params, float* row_scale, void* stream);
@@ -310,10 +311,12 @@ int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int
  * y = x W^T (replaces mx.quantized_matmul(x, w, scales, biases, transpose=True)), or with a
  * second matrix `up` of the same shape y = silu(x W^T) * (x up^T).  x: device [rows, n_in],
  * out: device [rows, n_out], both of w->dtype, row strides in elements (x_stride % 8 == 0, x
- * 16-byte aligned); out may not share memory with x.  Sums are fp32; y is rounded once.  A few tokens (up to 8, gated pairs 4
- * to 8, while their activations fit: 32768 inputs and more) multiply exact weights.  For more a weight enters as scale * code + bias rounded once
- * to fp16, for a gated fp16 call as the sum of two such parts.  Activations are exact but for
- * values below 2^-28 of their token's largest; infinite or NaN ones make their token's outputs
+ * 16-byte aligned); out may not share memory with x.  Sums are fp32; y is rounded once.  A few
+ * tokens (up to 8, gated pairs 4 to 8, while their activations fit: 32768 inputs and more)
+ * multiply the weights as am_q4_weight_pack keeps them.  For more a weight enters as scale *
+ * code + bias rounded once to fp16, to 11 bits or 2^-14 L (above) if that is more, for a gated
+ * fp16 call as the sum of two such parts (2^-12 L).  Activations are exact but for values
+ * below 2^-28 of their token's largest; infinite or NaN ones make their token's outputs
  * infinite or NaN.  workspace: device memory, 256-byte aligned, of the size the query gives
  * (0 for a few tokens); scratch of the call, free again when it has run.  status (device word
  * or NULL) gets AM_STATUS_TIMEOUT where a bounded wait ran out: rows of out are then unwritten.

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from conftest import pkg
-from test_gpu_linear import assert_within, expected, expected_experts, make_weight, make_x, routing_of, run
+from test_gpu_linear import (GROUP, assert_within, expected, expected_experts, make_weight, make_x, product,
+                             routing_of, run)
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +131,55 @@ def test_a_combination_onto_its_inputs(cuda):
     with pytest.raises(ValueError, match="residual"):
         pkg.combine_experts(y, w, pos, residual=res[:6], out=res[1:])
     assert torch.equal(pkg.combine_experts(y, w, pos, residual=res[:6], out=res[:6]), want)
+
+
+def spread_weight(n, k, dtype, dev, r, seed=0):
+    """A weight whose first group's scales and biases are 2^r times the others'."""
+    codes, s, b = make_weight((n, k), torch.float32, dev, seed=seed, scale=0.25)
+    f = torch.full((k // GROUP,), 2.0 ** -r, device=dev)
+    f[0] = 1.0
+    return codes, (s * f).to(dtype), (b * f).to(dtype)
+
+
+SPREADS = [(torch.float16, 6), (torch.float16, 10), (torch.float16, 14), (torch.float16, 18),
+           (torch.bfloat16, 8), (torch.bfloat16, 14), (torch.bfloat16, 20), (torch.bfloat16, 24)]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype,r", SPREADS)
+def test_groups_far_below_their_rows_largest(cuda, dtype, r, gated):
+    """Activations of zero at a row's largest group leave the small groups alone to count.  Few tokens
+    multiply them exactly; the tiles round a weight to 11 bits or to 2^-14 of the row's largest scale
+    (two parts: 2^-12), which is more than their few bits below 2^-10 of it."""
+    n, k = 72, 320
+    ws = [spread_weight(n, k, dtype, cuda, r, seed=i) for i in range(1 + gated)]
+    q = [pkg.Q4Weight(*w) for w in ws]
+    for tokens in (1, 2, 4, 7, 8, 9, 40, 150, 600):
+        x = (make_x(tokens, k, torch.float32, cuda, seed=tokens) * 2.0 ** min(r, 12)).to(dtype)  # (fp16: finite)
+        x[:, :GROUP] = 0
+        tiles = tokens > 8
+        largest = torch.stack([w[1].double().abs().amax(-1).maximum(w[2].double().abs().amax(-1) / 16) for w in ws])
+        floor = largest * (0.0 if not tiles else 2.0 ** -12 if gated and dtype == torch.float16 else 2.0 ** -14)
+        size = x.double().abs().sum(-1, keepdim=True)
+        y, e = product(x, ws[0])
+        e = e + floor[0] * size
+        if gated:
+            u, eu = product(x, ws[1])
+            eu = eu + floor[1] * size
+            s = y * torch.sigmoid(y)
+            y, e = s * u, 1.1 * e * (u.abs() + eu) + s.abs() * eu + 2.0 ** -20 * (s * u).abs()
+        got = pkg.quantized_swiglu(x, *q) if gated else pkg.quantized_matmul(x, *q)
+        assert_within(got, y, e, f"{tokens} tokens, 2^-{r}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ratio", [0.0, 1.0, 16.0, 64.0, 1024.0])
+def test_biases_of_every_size_beside_their_scales(cuda, dtype, ratio):
+    """Rows that are all scale, and rows that are nearly all bias (weights far from zero)."""
+    codes, s, _ = make_weight((72, 320), torch.float32, cuda, scale=2.0 ** -10)
+    g = torch.Generator(device="cpu").manual_seed(9)
+    b = s * ratio * (0.5 + torch.rand(s.shape, generator=g).to(cuda))
+    w = codes, s.to(dtype), b.to(dtype)
+    for tokens in (1, 5, 12, 200):
+        x = make_x(tokens, 320, dtype, cuda)
+        assert_within(run(x, [w]), *expected(x, [w]), f"{tokens} tokens, bias / scale {ratio}")
