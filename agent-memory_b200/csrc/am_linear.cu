@@ -117,8 +117,8 @@ struct FewParams {
 };
 
 // Ring depth of a warp: what leaves room for the activations of a few thousand inputs.
-template <int MT, int TK>
-constexpr int kFewDepth = MT == 2 ? 2 : (TK == 8 ? 3 : 4);
+template <bool GATED, int TK>
+constexpr int kFewDepth = GATED ? 2 : (TK == 8 ? 3 : 4);
 
 // D = A x B with a zero accumulator.
 __device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -159,12 +159,12 @@ __device__ __forceinline__ uint4 stage_inputs(uint4 u, float f, float& sum) {
 }
 
 // TK: tokens of an item, padded to 1, 2, 4 or 8.
-template <bool GATED, int MT, int TK>
+template <bool GATED, int TK>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __grid_constant__ FewParams f) {
-  constexpr int TROWS = GATED ? 16 : 16 * MT;  // output rows of a tile
-  constexpr int D = kFewDepth<MT, TK>;
+  constexpr int TROWS = 16;          // output rows of a tile
+  constexpr int MT = GATED ? 2 : 1;  // matrices
+  constexpr int D = kFewDepth<GATED, TK>;
   constexpr int XG = 128 * TK;  // staged bytes of a group
-  static_assert(!GATED || MT == 2, "a gated tile holds 16 rows of each matrix");
   const LinearParams& p = f.p;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -202,9 +202,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
     if (p0 < f.tiles) {
 #pragma unroll 1
       for (int i = 0; i < MT; ++i) {
-        const int64_t n = (int64_t)((p0 << lwr) + wr) * TROWS + (lane >> 1) + (GATED ? 0 : 16 * i);
+        const int64_t n = (int64_t)((p0 << lwr) + wr) * TROWS + (lane >> 1);
         if (n < p.n_out) {
-          const char* c = reinterpret_cast<const char*>(p.codes[GATED ? i : 0] + n * (p.n_in / 8));
+          const char* c = reinterpret_cast<const char*>(p.codes[i] + n * (p.n_in / 8));
           for (int g = ga + (lane & 1) * 4; g < min(gb, ga + 16); g += 8)
             asm volatile("prefetch.global.L2 [%0];" ::"l"(c + g * 32));
         }
@@ -219,10 +219,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   const int64_t tile_bytes = (int64_t)wr_n * TROWS * row_bytes - stages * 128;  // from a tile's end to the next
   const int64_t tile_par = (int64_t)wr_n * TROWS * p.pstride * 4 - stages * 16;
   const uint8_t *l_codes = nullptr, *l_par = nullptr;  // this lane's bytes of the next stage, matrix 0
-  const int64_t codes_diff = GATED ? reinterpret_cast<const uint8_t*>(p.codes[1]) - reinterpret_cast<const uint8_t*>(p.codes[0])
-                                   : (int64_t)16 * row_bytes;
-  const int64_t par_diff = GATED ? reinterpret_cast<const uint8_t*>(p.params[1]) - reinterpret_cast<const uint8_t*>(p.params[0])
-                                 : (int64_t)16 * p.pstride * 4;
+  const int64_t codes_diff =  // from a matrix to its partner
+      GATED ? reinterpret_cast<const uint8_t*>(p.codes[1]) - reinterpret_cast<const uint8_t*>(p.codes[0]) : 0;
+  const int64_t par_diff =
+      GATED ? reinterpret_cast<const uint8_t*>(p.params[1]) - reinterpret_cast<const uint8_t*>(p.params[0]) : 0;
   // chunk c of row r at c ^ 2 (r % 4): the eight bytes a lane reads of four rows lie in distinct banks
   const uint32_t l_dst0 = smem_u32(ring) + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) << 1)) << 4);
   const uint32_t l_pdst0 = smem_u32(ring) + 2048 + (lane & 15) * 16;
@@ -265,11 +265,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
       } else {
 #pragma unroll 1
         for (int i = 0; i < MT; ++i) {
-          const int rows = l_rows - (GATED ? 0 : 16 * i);
           for (int j = 0; j < 4; ++j)
-            if ((lane >> 3) + 4 * j < rows && (lane & 7) < chunks)
+            if ((lane >> 3) + 4 * j < l_rows && (lane & 7) < chunks)
               cp_async16_s(dst + i * (kFewCodes + kFewPar) + j * 512, l_codes + i * codes_diff + j * codes4);
-          if (lane < min(rows, 16)) cp_async16_ca_s(pdst + i * (kFewCodes + kFewPar), l_par + i * par_diff);
+          if (lane < min(l_rows, 16)) cp_async16_ca_s(pdst + i * (kFewCodes + kFewPar), l_par + i * par_diff);
         }
       }
       l_codes += 128;
@@ -397,8 +396,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int n = tile * TROWS + (GATED ? 0 : 16 * i) + g8 + 8 * h;
-          rs[i][h] = n < p.n_out ? __ldg(p.row_scale[GATED ? i : 0] + (int64_t)e * p.n_out + n) : 0.0f;
+          const int n = tile * TROWS + g8 + 8 * h;
+          rs[i][h] = n < p.n_out ? __ldg(p.row_scale[i] + (int64_t)e * p.n_out + n) : 0.0f;
         }
       const uint8_t* xs = xlane;
       const float* ss = slane;
@@ -475,7 +474,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
         __syncwarp();  // the stage is read before it is loaded again
         if ((buf += STAGE) == D * STAGE) buf = 0;
       }
-      // partial sums [batch][matrix or half][wr][slice][token][16 rows]
+      // partial sums [batch][matrix][wr][slice][token][16 rows]
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int tok = 2 * t4 + (c & 1);
@@ -492,7 +491,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
       cluster_sync_all();
     else
       __syncthreads();
-    constexpr int LROWS = TROWS == 16 ? 4 : 5, LTK = TK == 1 ? 0 : TK == 2 ? 1 : TK == 4 ? 2 : 3;
+    constexpr int LROWS = 4, LTK = TK == 1 ? 0 : TK == 2 ? 1 : TK == 4 ? 2 : 3;
     const int outs = nb << (lwr + LROWS + LTK);
     const uint32_t red_addr = smem_u32(red);
     for (int o = tid + rank * kFewWarps * 32; o < outs; o += kFewWarps * 32 << f.lck) {
@@ -500,11 +499,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
       const int tok = rest & (TK - 1), b = rest >> LTK;
       const int n = (((tile0 + b) << lwr) + w) * TROWS + r;
       if (n >= p.n_out || tok >= m) continue;
-      float sum[2];
+      float sum[MT];
 #pragma unroll
-      for (int i = 0; i < (GATED ? 2 : 1); ++i) {
-        const int half = GATED ? i : r >> 4;
-        const int at = ((((((b * MT + half) << lwr) + w) << f.lwk) * TK + tok) << 4) + (r & 15);
+      for (int i = 0; i < MT; ++i) {
+        const int at = ((((((b * MT + i) << lwr) + w) << f.lwk) * TK + tok) << 4) + r;
         float s = 0.0f;
         if (f.lck > 0) {
           for (int c = 0; c < 1 << f.lck; ++c) {
@@ -518,7 +516,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
         }
         sum[i] = s;
       }
-      const float y = GATED ? silu_mul(sum[0], sum[1]) : sum[0];
+      const float y = GATED ? silu_mul(sum[0], sum[MT - 1]) : sum[0];
       p.out[(int64_t)(lo + tok) * p.out_stride + n] = p.bf16 ? f2h<true>(y) : f2h<false>(y);
     }
     if (f.lck > 0)
@@ -545,14 +543,15 @@ static int few_tokens(int rows, int experts, bool grouped) {
 }
 
 // Positions between two sums: 16 KB of sums.
-constexpr int few_batch(int mt, int tk) { return 16 / (mt * tk) > 1 ? 16 / (mt * tk) : 1; }
+constexpr int few_batch(bool gated, int tk) { return 16 / ((gated ? 2 : 1) * tk); }
 
 // Shared memory of a CTA where `ck` of them split the inputs (quads of groups): the warps' rings, the
 // activations with their group sums, the partial sums.
-template <int MT, int TK>
+template <bool GATED, int TK>
 static int64_t few_smem(int quads, int ck) {
-  constexpr int64_t ring = kFewWarps * kFewDepth<MT, TK> * MT * (kFewCodes + kFewPar);
-  constexpr int64_t red = few_batch(MT, TK) * MT * kFewWarps * TK * 64;
+  constexpr int MT = GATED ? 2 : 1;
+  constexpr int64_t ring = kFewWarps * kFewDepth<GATED, TK> * MT * (kFewCodes + kFewPar);
+  constexpr int64_t red = few_batch(GATED, TK) * MT * kFewWarps * TK * 64;
   return ring + (int64_t)((quads + ck - 1) / ck) * 4 * (128 + 4) * TK + kFewWarps * 4 + red;
 }
 
@@ -561,14 +560,14 @@ static int64_t few_smem(int quads, int ck) {
 static bool few_fits(int tok, bool gated, int n_in) {
   const int quads = ((n_in / 64) + 3) / 4;
   int64_t smem = 0;
-  if (tok == 1) smem = gated ? few_smem<2, 1>(quads, kFewCluster) : few_smem<1, 1>(quads, kFewCluster);
-  if (tok == 2) smem = gated ? few_smem<2, 2>(quads, kFewCluster) : few_smem<1, 2>(quads, kFewCluster);
-  if (tok == 4) smem = gated ? few_smem<2, 4>(quads, kFewCluster) : few_smem<1, 4>(quads, kFewCluster);
-  if (tok == 8) smem = gated ? few_smem<2, 8>(quads, kFewCluster) : few_smem<1, 8>(quads, kFewCluster);
+  if (tok == 1) smem = gated ? few_smem<true, 1>(quads, kFewCluster) : few_smem<false, 1>(quads, kFewCluster);
+  if (tok == 2) smem = gated ? few_smem<true, 2>(quads, kFewCluster) : few_smem<false, 2>(quads, kFewCluster);
+  if (tok == 4) smem = gated ? few_smem<true, 4>(quads, kFewCluster) : few_smem<false, 4>(quads, kFewCluster);
+  if (tok == 8) smem = gated ? few_smem<true, 8>(quads, kFewCluster) : few_smem<false, 8>(quads, kFewCluster);
   return smem <= kFewSmem;
 }
 
-template <bool GATED, int MT, int TK>
+template <bool GATED, int TK>
 static cudaError_t launch_few_t(FewParams& f, cudaStream_t stream) {
   const LinearParams& p = f.p;
   // items a grouped call is likely to have, and has at most
@@ -579,23 +578,22 @@ static cudaError_t launch_few_t(FewParams& f, cudaStream_t stream) {
   if (sms == 0) return cudaErrorInvalidDevice;
   cudaError_t err = cudaSuccess;
   static unsigned long long done = 0;
-  auto kfn = linear_few_kernel<GATED, MT, TK>;
+  auto kfn = linear_few_kernel<GATED, TK>;
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
   if (!bit || !(__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) {
     err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
     if (err != cudaSuccess) return err;
     if (bit) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
   }
-  f.batch = few_batch(MT, TK);
+  f.batch = few_batch(GATED, TK);
   const int quads = p.pstride / 4;
   int ck = 1;
-  while (ck < kFewCluster && few_smem<MT, TK>(quads, ck) > kFewSmem) ck *= 2;
-  if (few_smem<MT, TK>(quads, ck) > kFewSmem) return cudaErrorNotSupported;  // (few_fits said it would)
-  const int smem = static_cast<int>(few_smem<MT, TK>(quads, ck));
+  while (ck < kFewCluster && few_smem<GATED, TK>(quads, ck) > kFewSmem) ck *= 2;
+  if (few_smem<GATED, TK>(quads, ck) > kFewSmem) return cudaErrorNotSupported;  // (few_fits said it would)
+  const int smem = static_cast<int>(few_smem<GATED, TK>(quads, ck));
   // Warps along the inputs: the split whose CTAs finish first, a position costing its groups and
   // about one and a half groups' time for the sums; a warp gets at least a whole stage.
-  constexpr int TROWS = GATED ? 16 : 16 * MT;
-  const int row_tiles = (p.n_out + TROWS - 1) / TROWS;
+  const int row_tiles = (p.n_out + 15) / 16;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(sms / ck * ck));
   cfg.blockDim = dim3(kFewWarps * 32);
@@ -647,13 +645,13 @@ static cudaError_t launch_few_t(FewParams& f, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kfn, f);
 }
 
-template <bool GATED, int MT, int MT8>
+template <bool GATED>
 static cudaError_t launch_few(FewParams& f, int tok, cudaStream_t stream) {
   switch (tok) {
-    case 1: return launch_few_t<GATED, MT, 1>(f, stream);
-    case 2: return launch_few_t<GATED, MT, 2>(f, stream);
-    case 4: return launch_few_t<GATED, MT, 4>(f, stream);
-    default: return launch_few_t<GATED, MT8, 8>(f, stream);
+    case 1: return launch_few_t<GATED, 1>(f, stream);
+    case 2: return launch_few_t<GATED, 2>(f, stream);
+    case 4: return launch_few_t<GATED, 4>(f, stream);
+    default: return launch_few_t<GATED, 8>(f, stream);
   }
 }
 
@@ -675,7 +673,7 @@ cudaError_t launch_linear_few(const LinearParams& p, cudaStream_t stream) {
   FewParams f{};
   f.p = p;
   const int tok = few_tokens(p.rows, p.experts, p.offsets != nullptr);
-  return p.codes[1] != nullptr ? launch_few<true, 2, 2>(f, tok, stream) : launch_few<false, 1, 1>(f, tok, stream);
+  return p.codes[1] != nullptr ? launch_few<true>(f, tok, stream) : launch_few<false>(f, tok, stream);
 }
 
 }  // namespace am
