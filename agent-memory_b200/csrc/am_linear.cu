@@ -158,6 +158,29 @@ __device__ __forceinline__ uint4 stage_inputs(uint4 u, float f, float& sum) {
                     pack_half2(v[3] * k, v[7] * k));
 }
 
+// The share [p0, p0 + n) of `total` positions of one of the clusters.
+__device__ __forceinline__ void few_share(int total, int cluster, int clusters, int& p0, int& n) {
+  const int each = total / clusters, more = total - each * clusters;
+  p0 = each * cluster + min(cluster, more);
+  n = each + (cluster < more);
+}
+
+// The positions of this CTA's cluster again, as far as their tokens are not finite (store_nonfinite; by the
+// CTAs whose inputs those are).
+static __device__ __noinline__ void few_store_nonfinite(const FewParams& f, int tk) {
+  const LinearParams& p = f.p;
+  const int clusters = static_cast<int>(gridDim.x) >> f.lck, cluster = static_cast<int>(blockIdx.x) >> f.lck;
+  const int items = p.offsets == nullptr ? (p.rows + tk - 1) / tk : count_items(p, tk);
+  const int rows = 16 << (kFewLogWarps - f.lwk);
+  int p0, n_pos;
+  few_share(items * f.tiles, cluster, clusters, p0, n_pos);
+  for (int q = p0; q < p0 + n_pos; ++q) {
+    int lo, hi;
+    const int e = find_item(p, q / f.tiles, tk, lo, hi);
+    store_nonfinite(p, nullptr, e, lo, hi, q % f.tiles * rows, (q % f.tiles + 1) * rows);
+  }
+}
+
 // TK: tokens of an item, padded to 1, 2, 4 or 8.
 template <bool GATED, int TK>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __grid_constant__ FewParams f) {
@@ -185,17 +208,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
   uint8_t* sx = smem + kFewWarps * D * STAGE;  // [group][half][TK][4] x 16 bytes
   float* sxsum = reinterpret_cast<float*>(sx + cta_groups * XG);     // [group][TK], times 2^-20
   float* sxmax = sxsum + cta_groups * TK;  // [warp]: largest |x| of its part of a token, as bits
-  float* red = sxmax + kFewWarps;
+  volatile int* marked = reinterpret_cast<volatile int*>(sxmax + kFewWarps);  // a token is not finite
+  float* red = sxmax + kFewWarps + 4;
+  *marked = 0;  // (by every thread; stage_x has a barrier before it is set)
   const int row_tiles = (p.n_out + TROWS - 1) / TROWS;
 
   griddep_launch_dependents();
   // positions [p0, p0 + n_pos) of the sequence of all items' positions
   int items = (p.rows + TK - 1) / TK, p0, n_pos;
-  auto share = [&]() {
-    const int total = items * f.tiles, each = total / clusters, more = total - each * clusters;
-    p0 = each * cluster + min(cluster, more);
-    n_pos = each + (cluster < more);
-  };
+  auto share = [&]() { few_share(items * f.tiles, cluster, clusters, p0, n_pos); };
   if (p.offsets == nullptr) {
     share();
     // L2 prefetch of the first tiles' codes: a lane pair a row
@@ -340,6 +361,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
     if (x_tok < m) {
       const uint32_t all = lane < WPT ? __float_as_uint(sxmax[x_tok * WPT + lane]) : 0u;
       mx = __reduce_max_sync(0xffffffffu, all);
+      if (mx >= nonfinite_bits(p)) *marked = 1;
       const float inv = exp2_int(-(p.bf16 ? row_exponent(mx) : row_exponent_f16(mx)));
       auto convert = [&](int v, uint4 u) {  // (u is zero where v is past the end)
         float sum;
@@ -529,6 +551,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
       ++it;
     }
   }
+  if (*marked) few_store_nonfinite(f, TK);  // (every thread cleared it, and the last batch ended with a barrier)
 }
 
 constexpr int kFewSmem = 227 * 1024;
@@ -552,7 +575,7 @@ static int64_t few_smem(int quads, int ck) {
   constexpr int MT = GATED ? 2 : 1;
   constexpr int64_t ring = kFewWarps * kFewDepth<GATED, TK> * MT * (kFewCodes + kFewPar);
   constexpr int64_t red = few_batch(GATED, TK) * MT * kFewWarps * TK * 64;
-  return ring + (int64_t)((quads + ck - 1) / ck) * 4 * (128 + 4) * TK + kFewWarps * 4 + red;
+  return ring + (int64_t)((quads + ck - 1) / ck) * 4 * (128 + 4) * TK + (kFewWarps + 4) * 4 + red;
 }
 
 // Whether the largest cluster holds the activations of a call: up to 49152 inputs at 8 tokens (a gated

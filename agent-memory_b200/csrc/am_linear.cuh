@@ -218,6 +218,77 @@ __device__ __forceinline__ uint32_t pack_out(const LinearParams& p, float x, flo
   return pack_half2(x, y);
 }
 
+// ---- tokens with infinite or NaN activations
+// The kernels' sums are not what the formula gives there: a scale and a bias meet an infinity apart, a
+// weight that rounds to zero or is the sum of two parts makes it a NaN.  A kernel that has seen such
+// a token stores its outputs again behind the others.
+
+// The least fp16 or bf16 bits (without the sign) that are no finite number.
+__device__ __forceinline__ uint32_t nonfinite_bits(const LinearParams& p) { return p.bf16 ? 0x7f80u : 0x7c00u; }
+
+// The product of weight row `wrow` with x row `x_row` as far as infinite and NaN activations determine it
+// (under the weight row's power of two); false where there is none.
+__device__ __forceinline__ bool nonfinite_sum(const LinearParams& p, int matrix, int64_t wrow, int x_row, float& sum) {
+  const uint16_t* x = p.x + (int64_t)x_row * p.x_stride;
+  const uint32_t* codes = p.codes[matrix] + wrow * (p.n_in / 8);
+  const uint32_t* params = p.params[matrix] + wrow * p.pstride;
+  const uint32_t limit = nonfinite_bits(p);
+  bool any = false;
+  sum = 0.0f;
+#pragma unroll 1
+  for (int k = 0; k < p.n_in; k += 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(x + k);
+    if (max_abs_bits(u) < limit) continue;
+    any = true;
+    const uint32_t v = params[k >> 6];
+    const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t bits = (w[j >> 1] >> (16 * (j & 1))) & 0xffffu;
+      if ((bits & 0x7fffu) < limit) continue;
+      const float code = static_cast<float>((codes[k >> 3] >> (4 * j)) & 15u);
+      sum += h2f_rt(static_cast<uint16_t>(bits), p.bf16) * fmaf(code * 0x1p-24f, sb.x, sb.y * 0x1p-20f);
+    }
+    if (isnan(sum)) break;  // (and stays so)
+  }
+  return any;
+}
+
+// Stores again such tokens among output rows [lo, hi), weight rows [n0, n1) of expert e, by the whole
+// CTA.  scale (or null): the tokens' powers of two from row lo on; linear_rows_kernel gives such a
+// token a NaN.
+__device__ __forceinline__ void store_nonfinite(const LinearParams& p, const float* scale, int e, int lo, int hi, int n0,
+                                                int n1) {
+  for (int r = lo + static_cast<int>(threadIdx.x >> 5); r < hi; r += blockDim.x >> 5) {
+    if (scale != nullptr && !isnan(scale[r - lo])) continue;
+    const int x_row = source_row(p, r);
+    if (x_row < 0) continue;
+    for (int n = n0 + static_cast<int>(threadIdx.x & 31); n < min(n1, p.n_out); n += 32) {
+      float y, u;
+      if (!nonfinite_sum(p, 0, (int64_t)e * p.n_out + n, x_row, y)) break;
+      if (p.codes[1] != nullptr) {
+        nonfinite_sum(p, 1, (int64_t)e * p.n_out + n, x_row, u);
+        y = silu_mul(y, u);
+      }
+      p.out[(int64_t)r * p.out_stride + n] = p.bf16 ? f2h<true>(y) : f2h<false>(y);
+    }
+  }
+}
+
+// The same for the tiles of CTA `cta` of `ctas`: items of `tok` rows x row_tiles tiles, of which this CTA
+// makes weight rows [row0, row0 + rows) of every tile_rows, and tokens rank / ck to (rank + 1) / ck.
+__device__ __forceinline__ void store_nonfinite_tiles(const LinearParams& p, int tok, int row_tiles, int tile_rows,
+                                                          int row0, int rows, int cta, int ctas, int rank, int ck) {
+  griddep_wait();
+  const int tiles = count_items(p, tok) * row_tiles;
+  for (int tile = cta; tile < tiles; tile += ctas) {
+    int lo, hi;
+    const int e = find_item(p, tile / row_tiles, tok, lo, hi);
+    const int n0 = tile % row_tiles * tile_rows + row0, t0 = lo + (hi - lo) * rank / ck;
+    store_nonfinite(p, p.xscale + t0, e, t0, lo + (hi - lo) * (rank + 1) / ck, n0, n0 + rows);
+  }
+}
+
 // Bytes between tokens of a warp's 32 output rows in shared memory: 64, and 16 against bank conflicts.
 constexpr int kOutPitch = 80;
 

@@ -98,6 +98,14 @@ struct PairParams {
   int32_t tile_tokens;  // tokens of an item, at most: a multiple of 32 up to 256
 };
 
+// (out of line and with nothing kept for it: the kernel's loops do not notice)
+template <int CTA_ROWS>
+__device__ __noinline__ void pair_store_nonfinite(const PairParams& f) {
+  const int b = static_cast<int>(blockIdx.x);
+  store_nonfinite_tiles(f.p, f.tile_tokens, f.row_tiles, 2 * CTA_ROWS, (b & 1) * CTA_ROWS, CTA_ROWS, b >> 1,
+                        static_cast<int>(gridDim.x) >> 1, 0, 1);
+}
+
 template <bool GATED, int PARTS>
 __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams f) {
   using LY = PairLayout<GATED>;
@@ -110,6 +118,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + LY::OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + LY::OFF_BAR + LY::B_COUNT * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + LY::OFF_BAR + LY::B_COUNT * 8 + 4);
+  volatile int* nonfinite = abort_flag + 1;  // one of this CTA's tokens is not finite
   float* tok_scale = reinterpret_cast<float*>(smem + LY::OFF_SCALE);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   auto wait = [&](int i, uint32_t parity) { return wait_warp(bar(i), parity, p.wait_ns, abort_flag); };
@@ -138,7 +147,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::);
   } else if (warp == CODES_WARP) {
     for (int i = lane; i < LY::B_COUNT; i += 32) mbar_init(bar(i), LY::arrivals(i));
-    if (lane == 0) *abort_flag = 0;
+    if (lane == 0) *abort_flag = *nonfinite = 0;
     fence_mbar_init();
   }
   tc::fence_before();
@@ -195,7 +204,13 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
           const int b = k & 1;
           ok = wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1);
           if (!ok) break;
-          for (int j = lane; j < 256; j += 32) tok_scale[b * 256 + j] = lo + j < hi ? p.xscale[lo + j] : 0.0f;
+          bool marked = false;
+          for (int j = lane; j < 256; j += 32) {
+            const float ts = lo + j < hi ? p.xscale[lo + j] : 0.0f;
+            tok_scale[b * 256 + j] = ts;
+            marked |= isnan(ts);
+          }
+          if (__any_sync(0xffffffffu, marked)) *nonfinite = 1;  // (the warp together: a divergent store made the loops spill)
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(LY::B_SFULL + b));
         }
@@ -407,6 +422,7 @@ __global__ void __launch_bounds__(PairLayout<GATED>::THREADS, 1) linear_pair_ker
     tc::fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
   }
+  if (*nonfinite) pair_store_nonfinite<CTA_ROWS>(f);
 }
 
 // ---------------------------------------------------------------- host

@@ -76,10 +76,9 @@ __global__ void __launch_bounds__(kRowThreads) linear_rows_kernel(const __grid_c
       }
     }
   }
-  if (!p.bf16 || from < 0) {
+  if (from < 0) {
     if (tid == 0) p.xscale[row] = 1.0f;
-    if (from < 0)
-      for (int i = tid; i < p.n_in / 8; i += TEAM) dst[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < p.n_in / 8; i += TEAM) dst[i] = make_uint4(0, 0, 0, 0);
     return;
   }
   mx = __reduce_max_sync(0xffffffffu, mx);
@@ -87,6 +86,11 @@ __global__ void __launch_bounds__(kRowThreads) linear_rows_kernel(const __grid_c
     if ((tid & 31) == 0) wmax[tid >> 5] = mx;
     __syncthreads();
     mx = __reduce_max_sync(0xffffffffu, wmax[tid & (TEAM / 32 - 1)]);
+  }
+  // (a row with an infinity or a NaN is marked by a NaN as its power of two)
+  if (!p.bf16) {
+    if (tid == 0) p.xscale[row] = mx < 0x7c00u ? 1.0f : __int_as_float(0x7fffffff);
+    return;
   }
   const int ex = row_exponent(mx);
   const float inv = exp2_int(-ex);
@@ -97,7 +101,7 @@ __global__ void __launch_bounds__(kRowThreads) linear_rows_kernel(const __grid_c
       if (i < vecs) dst[i] = permute_bf16(held ? u[j] : src[i], inv);
     }
   }
-  if (tid == 0) p.xscale[row] = exp2_int(ex);
+  if (tid == 0) p.xscale[row] = mx < 0x7f80u ? exp2_int(ex) : __int_as_float(0x7fffffff);
 }
 
 // ---------------------------------------------------------------- tiles
@@ -148,6 +152,14 @@ struct TilesParams {
   int32_t row_tiles;  // tiles of CTA_ROWS weight rows
 };
 
+// (out of line and with nothing kept for it: the kernel's loops do not notice)
+template <int NT, int CTA_ROWS>
+__device__ __noinline__ void tiles_store_nonfinite(const TilesParams& f) {
+  const int b = static_cast<int>(blockIdx.x);
+  store_nonfinite_tiles(f.p, NT, f.row_tiles, CTA_ROWS, 0, CTA_ROWS, b / f.ck, static_cast<int>(gridDim.x) / f.ck, b % f.ck,
+                        f.ck);
+}
+
 template <int NT, bool GATED, int PARTS>
 __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTAS)
     linear_tiles_kernel(const __grid_constant__ TilesParams f) {
@@ -161,6 +173,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + LY::OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + LY::OFF_BAR + LY::B_COUNT * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + LY::OFF_BAR + LY::B_COUNT * 8 + 4);
+  volatile int* nonfinite = abort_flag + 1;  // one of this CTA's tokens is not finite
   float* tok_scale = reinterpret_cast<float*>(smem + LY::OFF_SCALE);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   // (loads wait long, the others mostly not at all)
@@ -196,7 +209,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
   } else if (warp == CODES_WARP) {
     for (int i = lane; i < LY::B_COUNT; i += 32) mbar_init(bar(i), LY::arrivals(i));
-    if (lane == 0) *abort_flag = 0;
+    if (lane == 0) *abort_flag = *nonfinite = 0;
     fence_mbar_init();
   }
   tc::fence_before();
@@ -251,7 +264,13 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
           const int b = k & 1;
           ok = wait(LY::B_SEMPTY + b, ((k >> 1) & 1) ^ 1);
           if (!ok) break;
-          for (int j = lane; j < NT; j += 32) tok_scale[b * NT + j] = lo + j < hi ? p.xscale[lo + j] : 0.0f;
+          bool marked = false;
+          for (int j = lane; j < NT; j += 32) {
+            const float ts = lo + j < hi ? p.xscale[lo + j] : 0.0f;
+            tok_scale[b * NT + j] = ts;
+            marked |= isnan(ts);
+          }
+          if (__any_sync(0xffffffffu, marked)) *nonfinite = 1;  // (the warp together: a divergent store made the loops spill)
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(LY::B_SFULL + b));
         }
@@ -508,6 +527,7 @@ __global__ void __launch_bounds__(TilesLayout<NT>::THREADS, TilesLayout<NT>::CTA
     tc::fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(LY::TMEM_COLS));
   }
+  if (*nonfinite) tiles_store_nonfinite<NT, CTA_ROWS>(f);
 }
 
 // ---------------------------------------------------------------- host

@@ -13,8 +13,8 @@ bias, if that is larger).  For more tokens a weight is ``scale * code + bias`` r
 bits, or 2**-14 of that largest scale if that is more); in a gated float16 layer, where two such
 errors would be 1.6 times the output's own rounding, it is the sum of two fp16 parts.  An activation is exact
 (bf16 values enter as fp16 under a power of two per token; only values below 2**-28 of their
-token's largest lose bits).  An infinite or NaN activation
-makes its token's outputs infinite or NaN.  The weights are frozen: there is no backward pass.
+token's largest lose bits).  A token with infinite
+or NaN activations gets the infinities and NaN of the formula.  The weights are frozen: there is no backward pass.
 """
 
 from __future__ import annotations

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from conftest import pkg
-from test_gpu_linear import (GROUP, assert_within, expected, expected_experts, make_weight, make_x, product,
+from test_gpu_linear import (GROUP, assert_within, dense, expected, expected_experts, make_weight, make_x, product,
                              routing_of, run)
 
 pytestmark = pytest.mark.gpu
@@ -183,3 +183,81 @@ def test_biases_of_every_size_beside_their_scales(cuda, dtype, ratio):
     for tokens in (1, 5, 12, 200):
         x = make_x(tokens, 320, dtype, cuda)
         assert_within(run(x, [w]), *expected(x, [w]), f"{tokens} tokens, bias / scale {ratio}")
+
+
+def formula(x, ws):
+    """The layer as it is defined, infinities and NaN with it: sums in 64 bits over the tokens' own values."""
+    y = x.double() @ dense(ws[0]).mT
+    return y / (1 + torch.exp(-y)) * (x.double() @ dense(ws[1]).mT) if len(ws) == 2 else y
+
+
+def put_nonfinite(x):
+    """Tokens with one infinity, two of both signs, a NaN, and one of each at the ends."""
+    inf, k = float("inf"), x.shape[1]
+    at = [(0, [(7, inf)]), (1, [(k - 1, -inf)]), (2, [(64, inf), (65, -inf)]), (4, [(3, float("nan"))]),
+          (5, [(0, -inf), (k - 2, -inf)]), (x.shape[0] - 1, [(100, inf)])]
+    for row, values in at:
+        for col, v in values if row < x.shape[0] else ():
+            x[row, col] = v
+    return ~torch.isfinite(x).all(-1)
+
+
+def assert_same_kind(got, want):
+    same = (got.double() == want) | (torch.isnan(got) & torch.isnan(want))
+    assert bool(same.all()), f"{int((~same).sum())} of {same.numel()} differ: {got[~same][:4]} for {want[~same][:4]}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("tokens,n,k", [(1, 130, 320), (2, 130, 14336), (4, 130, 320), (8, 300, 14336), (20, 130, 704),
+                                        (40, 4100, 320), (60, 40000, 320), (150, 1030, 1344), (700, 8450, 320)])
+def test_infinities_and_nan_as_the_formula_has_them(cuda, tokens, n, k, gated, dtype):
+    """A token with infinite or NaN activations gives the infinities and NaN of the formula in every
+    kernel (few tokens, tiles split and whole, pairs); the other tokens do not notice.  Some
+    weights are zero."""
+    ws = [make_weight((n, k), dtype, cuda, seed=i) for i in range(1 + gated)]
+    for _, s, b in ws:
+        s[3], b[3] = 0, 0
+        s[5, 1], b[5, 1] = 0, 0
+        b[7] = -3 * s[7]
+    x = make_x(tokens, k, dtype, cuda)
+    clean = x.clone()
+    bad = put_nonfinite(x)
+    got = run(x, ws)
+    assert_same_kind(got[bad], formula(x[bad], ws))
+    want, bound = expected(clean[~bad], ws)
+    assert_within(got[~bad], want, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [6, 60, 2400])
+def test_infinities_and_nan_through_experts(cuda, tokens, dtype):
+    n_experts, n, k = 6, 700, 320
+    ws = [make_weight((n_experts, n, k), dtype, cuda, seed=i) for i in range(2)]
+    q = [pkg.Q4Weight(*w) for w in ws]
+    r = routing_of((torch.arange(tokens, device=cuda) % n_experts)[:, None], n_experts)
+    x = make_x(tokens, k, dtype, cuda)
+    bad = put_nonfinite(x)
+    for many in (1, 2):
+        got = pkg.expert_swiglu(x, *q, r) if many == 2 else pkg.expert_matmul(x, q[0], r, gather=True)
+        for t in torch.nonzero(bad)[:, 0].tolist():
+            e = int(r.experts[t, 0])
+            want = formula(x[t:t + 1], [[p[e] for p in w] for w in ws[:many]])
+            assert_same_kind(got[r.positions[t].long()], want)
+        keep = ~bad[r.order.long()]
+        want, bound = expected_experts(x.masked_fill(bad[:, None], 0), ws[:many], r, True)
+        assert_within(got[keep], want[keep], bound[keep])
+
+
+@pytest.mark.parametrize("tokens", [8, 100, 1024])
+def test_tokens_of_nothing_but_nan_or_infinity(cuda, tokens):
+    """Every token: all NaN, all infinite, or finite (the calls end in ordinary time)."""
+    ws = [make_weight((2304, 1024), torch.float16, cuda, seed=i) for i in range(2)]
+    x = make_x(tokens, 1024, torch.float16, cuda)
+    x[0::3] = float("nan")
+    x[1::3] = float("inf")
+    got = run(x, ws)
+    bad = ~torch.isfinite(x).all(-1)
+    assert_same_kind(got[bad], formula(x[bad], ws))
+    want, bound = expected(x[~bad], ws)
+    assert_within(got[~bad], want, bound)
