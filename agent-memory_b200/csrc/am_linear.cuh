@@ -66,16 +66,19 @@ __device__ __forceinline__ void expert_range(const LinearParams& p, int e, int& 
   }
 }
 
-// The x row that output row r is made from; -1 (and the status bit) for a bad order entry.
-__device__ __forceinline__ int source_row(const LinearParams& p, int r) {
-  if (p.order == nullptr) return r;
-  const int pair = p.order[r];
+// The x row that output row r (of pair order[r]) is made from; -1 (and the status bit) for a bad order
+// entry.
+__device__ __forceinline__ int source_row_of(const LinearParams& p, int pair) {
+  if (p.order == nullptr) return pair;
   const int t = pair / p.top_k;
   if (pair < 0 || t >= p.x_rows) {
     flag_status(p.status, AM_STATUS_BAD_POSITION);
     return -1;
   }
   return t;
+}
+__device__ __forceinline__ int source_row(const LinearParams& p, int r) {
+  return source_row_of(p, p.order != nullptr ? p.order[r] : r);
 }
 
 __device__ __forceinline__ uint32_t hfma2_bits(uint32_t a, uint32_t b, uint32_t c) {

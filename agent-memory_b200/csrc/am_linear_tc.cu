@@ -53,7 +53,12 @@ __global__ void __launch_bounds__(kRowThreads) linear_rows_kernel(const __grid_c
   griddep_launch_dependents();  // (not earlier: the next grid reads the weights before its own wait)
   const int row = blockIdx.x * (kRowThreads / TEAM) + threadIdx.x / TEAM, tid = threadIdx.x % TEAM;
   if (row >= p.rows) return;  // (whole teams)
-  const int from = source_row(p, row);
+  // rows that no expert holds are left alone: their order entries mean nothing (all three loads at once)
+  const int pair = p.order != nullptr ? p.order[row] : row;
+  const int held_lo = p.offsets != nullptr ? p.offsets[0] : 0;
+  const int held_hi = p.offsets != nullptr ? p.offsets[p.experts] : p.rows;
+  if (row < held_lo || row >= held_hi) return;
+  const int from = source_row_of(p, pair);
   const uint4* src = reinterpret_cast<const uint4*>(p.x + (int64_t)max(from, 0) * p.x_stride);
   uint4* dst = reinterpret_cast<uint4*>(p.xh + (int64_t)row * p.n_in);
   const int vecs = from < 0 ? 0 : p.n_in / 8;

@@ -330,9 +330,9 @@ int am_q4_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, i
  * The same with one matrix per expert (replaces mx.gather_qmm over sorted rows): output row
  * r in [offsets[e], offsets[e+1]) is made with expert e's matrix from row order[r] / top_k of
  * x (order given), or from row r of x (order NULL).  offsets: device int32 [experts + 1],
- * non-decreasing, used clamped to [0, rows]; rows no expert holds are not written.  An order
- * entry that points outside [0, x_rows) reads as a row of zeros and sets
- * AM_STATUS_BAD_POSITION.  Workspace as above (none up to a mean of two rows an expert).
+ * non-decreasing, used clamped to [0, rows]; rows no expert holds are not written and their
+ * order entries mean nothing.  An order entry that points outside [0, x_rows) reads as a row of
+ * zeros and sets AM_STATUS_BAD_POSITION.  Workspace as above (none up to a mean of two rows an expert).
  */
 size_t am_q4_expert_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up,
                                            int32_t rows);

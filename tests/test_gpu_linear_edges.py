@@ -261,3 +261,31 @@ def test_tokens_of_nothing_but_nan_or_infinity(cuda, tokens):
     assert_same_kind(got[bad], formula(x[bad], ws))
     want, bound = expected(x[~bad], ws)
     assert_within(got[~bad], want, bound)
+
+
+@pytest.mark.parametrize("tokens", [6, 90, 700])
+def test_order_entries_of_rows_that_no_expert_holds(cuda, tokens):
+    """Offsets that leave rows out at both ends, whose order entries point nowhere: no status bit, the
+    rows stay as they were, the others are right."""
+    n_experts, top_k = 4, 2
+    ws = [make_weight((n_experts, 72, 256), torch.bfloat16, cuda, seed=i) for i in range(2)]
+    q = [pkg.Q4Weight(*w) for w in ws]
+    r = routing_of(torch.stack([torch.arange(tokens, device=cuda) % n_experts,
+                                (torch.arange(tokens, device=cuda) + 1) % n_experts], 1), n_experts)
+    x = make_x(tokens, 256, torch.bfloat16, cuda)
+    off, order = r.offsets.clone(), r.order.clone()
+    lo, hi = int(off[1]), int(off[-2])
+    off[0], off[-1] = lo, hi
+    order[:lo], order[hi:] = -1, 10 ** 9
+    r2 = r._replace(offsets=off, order=order)
+    for many in (1, 2):
+        status = torch.zeros(1, dtype=torch.int32, device=cuda)
+        out = torch.full((2 * tokens, 72), 5.0, dtype=torch.bfloat16, device=cuda)
+        if many == 2:
+            pkg.expert_swiglu(x, *q, r2, out=out, status=status)
+        else:
+            pkg.expert_matmul(x, q[0], r2, gather=True, out=out, status=status)
+        want, bound = expected_experts(x, ws[:many], r, True)
+        assert_within(out[lo:hi], want[lo:hi], bound[lo:hi])
+        assert bool((out[:lo] == 5.0).all()) and bool((out[hi:] == 5.0).all())
+        assert int(status) == 0
