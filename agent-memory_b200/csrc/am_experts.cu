@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(1024) route_sort_kernel(const __grid_constant_
 
 template <int PER>
 static cudaError_t launch_sort(const RouteParams& p, int ctas, int threads, cudaStream_t stream) {
-  const int held = std::min((p.tokens + ctas - 1) / ctas * p.top_k, kRouteHeld);
+  const int held = static_cast<int>(std::min<int64_t>(((int64_t)p.tokens + ctas - 1) / ctas * p.top_k, kRouteHeld));
   const int smem = (threads / 32 * p.n_experts + 2 * p.n_experts + 32 + 2 * held) * 4;
   auto kfn = route_sort_kernel<PER>;
   if (smem > 48 * 1024) {
@@ -254,7 +254,7 @@ template <int PER>
 static cudaError_t launch_route_t(const RouteParams& p, cudaStream_t stream) {
   if (p.tokens <= 16) return launch_sort<PER>(p, 1, 256, stream);
   const cudaError_t err =
-      launch_chained(route_topk_kernel<PER>, p, dim3((p.tokens + 7) / 8), 256, 0, 1, stream);
+      launch_chained(route_topk_kernel<PER>, p, dim3((p.tokens - 1) / 8 + 1), 256, 0, 1, stream);
   if (err != cudaSuccess) return err;
   int ctas = 1;  // a CTA for every 1024 pairs: one pair a thread
   while (ctas < 8 && (int64_t)p.tokens * p.top_k > ctas * 1024) ctas *= 2;
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Co
   griddep_wait();
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
   if (c >= p.width) return;
-  for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+  for (uint32_t t = blockIdx.x; t < static_cast<uint32_t>(p.tokens); t += gridDim.x) {  // (up to 2^31 - 1)
     const float* w = p.weights + (int64_t)t * p.top_k;
     const int32_t* at = p.positions + (int64_t)t * p.top_k;
     T res{};

@@ -289,3 +289,20 @@ def test_order_entries_of_rows_that_no_expert_holds(cuda, tokens):
         assert_within(out[lo:hi], want[lo:hi], bound[lo:hi])
         assert bool((out[:lo] == 5.0).all()) and bool((out[hi:] == 5.0).all())
         assert int(status) == 0
+
+
+def test_a_combination_of_two_billion_tokens(cuda):
+    """As many tokens as the interface can count (the walk over them passes 31 bits)."""
+    tokens = 2 ** 31 - 1
+    if torch.cuda.mem_get_info(cuda)[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    y = torch.full((3, 1), 1.5, dtype=torch.float16, device=cuda)
+    w = torch.full((1, 1), 2.0, device=cuda).expand(tokens, 1).contiguous()
+    pos = torch.ones(tokens, 1, dtype=torch.int32, device=cuda)
+    pos[-1] = 7  # out of range: adds nothing
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = pkg.combine_experts(y, w, pos, status=status)
+    assert bool((out[:-1] == 3.0).all()) and float(out[-1]) == 0.0
+    assert int(status) == pkg._lib.STATUS_BAD_POSITION
+    del y, w, pos, out
+    torch.cuda.empty_cache()
