@@ -704,15 +704,18 @@ int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int
                      "am_q4_weight_pack");
 }
 
+// Weight rows of a call, all experts': the kernels count them in 32 bits, in tiles of up to 512 past the last.
+constexpr int64_t kMaxWeightRows = INT_MAX - 1024;
+
 static int check_weight(const am_q4_weight* w, const char* fn) {
   if (w == nullptr || !w->codes || !w->params || !w->row_scale) {
     set_error("%s: a packed weight (codes, params, row_scale) is required", fn);
     return AM_ERR_INVALID;
   }
   if (!valid_half_dtype(w->dtype) || w->n_out <= 0 || w->n_in <= 0 || w->n_in % 64 || w->experts <= 0 ||
-      (int64_t)w->experts * w->n_out > (int64_t)INT_MAX) {
-    set_error("%s: weight needs F16 or BF16, n_out > 0, n_in %% 64 == 0, experts > 0 (got %d, %d, %d, %d)", fn,
-              w->dtype, w->n_out, w->n_in, w->experts);
+      (int64_t)w->experts * w->n_out > kMaxWeightRows) {
+    set_error("%s: weight needs F16 or BF16, n_out > 0, n_in %% 64 == 0, experts > 0 and experts * n_out < "
+              "2^31 - 1024 (got %d, %d, %d, %d)", fn, w->dtype, w->n_out, w->n_in, w->experts);
     return AM_ERR_INVALID;
   }
   if (!aligned(w->codes, 16) || !aligned(w->params, 16) || !aligned(w->row_scale, 4)) {

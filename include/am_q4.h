@@ -292,7 +292,7 @@ typedef struct am_q4_weight {
   const float* row_scale;     /* device [experts, n_out] */
   int32_t n_out;
   int32_t n_in;               /* multiple of 64 */
-  int32_t experts;            /* 1 for a plain matrix */
+  int32_t experts;            /* 1 for a plain matrix; experts * n_out < 2^31 - 1024 */
   int32_t dtype;              /* AM_DTYPE_F16 or AM_DTYPE_BF16: activations and outputs */
 } am_q4_weight;
 

@@ -83,6 +83,16 @@ def test_a_bad_weight_is_refused(field, value):
     assert lib.am_last_error()
 
 
+def test_weights_whose_rows_pass_the_kernels_counts_are_refused():
+    """Tiles reach up to 512 rows past the last one: row numbers have to stay below 2^31 there too."""
+    lib = pkg._lib.load()
+    for n_out, experts, want in ((2 ** 31 - 1, 1, INVALID), (2 ** 31 - 1024, 1, INVALID), (2 ** 20, 2048, INVALID),
+                                 (2 ** 31 - 1025, 1, WORKSPACE), (2 ** 20, 2047, WORKSPACE)):
+        w = weight(n_out=n_out, experts=experts)
+        assert lib.am_q4_expert_linear(ctypes.byref(w), None, PTR, 128, 2 ** 13, PTR, None, 1, 2 ** 13, PTR, n_out,
+                                       None, 0, None, None) == want, (n_out, experts)
+
+
 def test_linear_arguments_are_refused():
     lib = pkg._lib.load()
     w, other, grouped = weight(), weight(n_out=32), weight(experts=4)
