@@ -119,9 +119,9 @@ __global__ void __launch_bounds__(256) route_topk_kernel(const __grid_constant__
 constexpr int kRouteHeld = 4096;  // pairs of a CTA whose expert and rank stay in shared memory
 
 // Shared memory: counters [warps][n_experts], totals and first places [n_experts], a word a warp,
-// then the held pairs' expert and rank.  PER > 0: the top-k too.
+// then the held pairs' expert and rank.  PER > 0: the top-k too, by a CTA of 256 threads.
 template <int PER>
-__global__ void __launch_bounds__(1024) route_sort_kernel(const __grid_constant__ RouteParams p) {
+__global__ void __launch_bounds__(PER > 0 ? 256 : 1024) route_sort_kernel(const __grid_constant__ RouteParams p) {
   extern __shared__ int32_t counts[];
   const int E = p.n_experts, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int threads = blockDim.x, warps = threads >> 5;
