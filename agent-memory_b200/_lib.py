@@ -15,7 +15,7 @@ PKG_DIR = Path(__file__).resolve().parent
 LIB_NAME = "libamq4.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 # Status codes / enums (mirrors include/am_q4.h)
 AM_OK = 0
@@ -111,7 +111,7 @@ class AttnArgs(ctypes.Structure):
         ("mask_kind", c_int32),
         ("mask", c_void_p),
         ("mask_dtype", c_int32),
-        ("reserved0", c_int32),
+        ("queries_ready", c_int32),
         ("mask_stride_b", c_int64),
         ("mask_stride_h", c_int64),
         ("mask_stride_l", c_int64),

@@ -530,6 +530,7 @@ static int prefill_call(const am_q4_cache* cache, const am_attn_args* a, void* w
   const int bn = prefill_key_tile(cache->k_dim, cache->v_dim);
   const int64_t hi_eff = std::min<int64_t>(key_hi, static_cast<int64_t>(a->max_kv_len) + bn);
   const int64_t range_rows = std::max<int64_t>(hi_eff - key_lo, 0);
+  p.wait_first = (parts & kPrefillStage) || a->queries_ready ? 0 : 1;
   p.stage_lo = key_lo;
   p.stage_hi = static_cast<int32_t>(hi_eff);
   p.stage_blocks = range_rows + kStageRowsHost < pl.nw

@@ -412,8 +412,8 @@ struct DecodeParams {
   // layout (table, block_tokens) or contiguous rows, and the scale / bias type.
   int32_t paged;
   int32_t scale_bf16;
-  // The prefill attention kernel waits for the grid before it as its first step: its call has no
-  // stage launch of its own, and that grid may be the one that writes the queries.
+  // The prefill attention kernel waits for the grid before it ahead of its first read: its call has
+  // no stage launch of its own, and that grid may be the one that writes the queries.
   int32_t wait_first;
   alignas(64) CUtensorMap tmap_kd;
   alignas(64) CUtensorMap tmap_vd;

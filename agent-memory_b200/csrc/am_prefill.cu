@@ -52,10 +52,11 @@
 // when everything before it was complete.  A call without a stage launch (am_q4_prefill_attend)
 // has no such grid before it, and may follow one that lets its dependents start early (a
 // linear layer that writes the queries): there every thread waits before its first read
-// (wait_first), and only asks L2 for the query rows before that.  What stands behind the wait
-// then, the lengths and the query tile, costs a call of the two-tile kernel 2.5 us (512 tokens
-// over a 4096-token prefix, stage and attention 109 -> 112 us a layer; waiting in front of the
-// whole prologue instead: 115); the K/V loads start beside it.
+// (wait_first), and only asks L2 for the query rows before that.  What stands behind the wait then,
+// the lengths and the query tile, costs a call of the two-tile kernel 2.5 us (512 tokens over a
+// 4096-token prefix, append, stage and attention 109 -> 112 us a layer; waiting in front of the
+// whole prologue instead: 115); the K/V loads start beside it.  A caller who promises that a stage
+// call directly precedes and the queries were complete before it (queries_ready) keeps the 109.
 //
 // Reference semantics: the compiled quantized SDPA (mlx_fused_attention.py:69-139) as used
 // by chunked prefill (batch_engine.py:339-456): the chunk's own K/V are already in the Q4
@@ -1659,7 +1660,6 @@ static cudaError_t launch_prefill_dims(const DecodeParams& p0, int batch, bool p
   DecodeParams p = p0;  // (the attention kernel's V dequantization reads the cache directly)
   p.paged = paged ? 1 : 0;
   p.scale_bf16 = sbf16 ? 1 : 0;
-  p.wait_first = parts & kPrefillStage ? 0 : 1;
   if (parts & kPrefillStage) {
     cudaError_t e = paged ? (sbf16 ? launch_stage_t<DK, DV, true, true>(p, batch, stream)
                                    : launch_stage_t<DK, DV, false, true>(p, batch, stream))

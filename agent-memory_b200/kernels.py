@@ -367,14 +367,17 @@ def attention(view: CacheView, queries: torch.Tensor, scale: float, kv_len: torc
               out: torch.Tensor | None = None, status: torch.Tensor | None = None,
               mode: str = "auto", sinks: torch.Tensor | None = None,
               workspace: torch.Tensor | None = None,
-              stage_keys: tuple[int, int] | None = None) -> torch.Tensor:
+              stage_keys: tuple[int, int] | None = None,
+              queries_ready: bool = False) -> torch.Tensor:
     """Attention of queries [B, Hq, L, Dk] over the cache -> [B, Hq, L, Dv].
 
     kv_len/kv_start: int32 device tensors [B].  mode: "auto" (library dispatch), "decode"
     (split-KV kernel) or "prefill" (tcgen05 kernel); "prefill_stage" dequantizes only the
     keys at positions stage_keys = (lo, hi) (default: all) into `workspace`, and
     "prefill_attend" runs only the attention kernel over a workspace that stage calls have
-    filled (am_q4_prefill_stage / am_q4_prefill_attend).  sinks: optional [Hq]
+    filled (am_q4_prefill_stage / am_q4_prefill_attend).  queries_ready ("prefill_attend" only):
+    the caller's promise that the queries, lengths, mask and sinks were complete before the
+    stage call that directly precedes this one on the stream.  sinks: optional [Hq]
     attention-sink logits (scaled-score units).  workspace: a contiguous uint8 device tensor
     of at least the call's workspace bytes (256-byte aligned); by default the workspace the
     chosen kernel needs (split-KV partials, or the prefill kernel's fp16 rows of the visible
@@ -383,6 +386,10 @@ def attention(view: CacheView, queries: torch.Tensor, scale: float, kv_len: torc
     a, keep, out = attention_args(view, queries, scale, kv_len, max_kv_len, kv_start=kv_start,
                                   causal=causal, window=window, mask=mask, out_dtype=out_dtype,
                                   out=out, status=status, sinks=sinks)
+    if queries_ready:
+        if mode != "prefill_attend":
+            raise ValueError('queries_ready is a promise to mode "prefill_attend" only')
+        a.queries_ready = 1
     dev = out.device
     L_ = _lib.load()
     fn = {"decode": "am_q4_decode", "prefill": "am_q4_prefill",

@@ -642,6 +642,8 @@ def measure_prefill(am, dev, steps, warmup, gen, workload="prefill"):
         win = [0 if is_global[l] else window for l in range(layers)]
         args = [am.kernels.attention_args(views[l], q[l], dk ** -0.5, kv_len, N, causal=True,
                                           window=win[l], out=out[l]) for l in range(layers)]
+        for call in args:  # (complete long before each layer's stage call, which attend follows directly)
+            call[0].queries_ready = 1
         nbytes = max(am.kernels.prefill_workspace_bytes(views[l], B, hq, L, N, window=win[l])
                      for l in range(layers))
         ws = [torch.empty(nbytes, dtype=torch.uint8, device=dev) for _ in range(2)]

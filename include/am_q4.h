@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define AM_ABI_VERSION 4
+#define AM_ABI_VERSION 5
 
 enum {
   AM_OK = 0,
@@ -110,7 +110,10 @@ typedef struct am_attn_args {
   int32_t mask_kind;          /* AM_MASK_* */
   const void* mask;           /* device, element strides below (0 = broadcast) */
   int32_t mask_dtype;         /* additive: AM_DTYPE_F16/BF16/F32; bool: AM_DTYPE_U8 */
-  int32_t reserved0;
+  /* am_q4_prefill_attend only: nonzero promises that q, kv_len, kv_start, mask and sinks were
+   * complete before the am_q4_prefill_stage call that directly precedes this one on the
+   * stream, whose end then hides the reading of the queries (0: no such promise). */
+  int32_t queries_ready;
   int64_t mask_stride_b, mask_stride_h, mask_stride_l, mask_stride_n;
   int32_t* status;            /* device word or NULL: kernels OR AM_STATUS_* bits into it */
   /* Attention sinks (replaces the fp16 detour of mlx_sink_compat.py:46-69): device fp32

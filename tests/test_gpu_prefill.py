@@ -355,3 +355,35 @@ def test_attend_waits_for_the_projection_of_its_queries(cuda, geom):
         pkg.quantized_matmul(x, w, out=buf)
         got = pkg.kernels.attention(view, q, Dk ** -0.5, kv_len, N, mode="prefill_attend", workspace=ws, **kw)
         assert torch.equal(got, want), (got - want).abs().max()
+
+
+@pytest.mark.parametrize("geom", [(32, 8, 128, 128, 512), (16, 16, 192, 128, 300), (16, 8, 256, 256, 200)],
+                         ids=["llama_d128", "mla_k192_v128", "gemma_d256"])
+def test_attend_with_queries_promised_before_the_stage_call(cuda, geom):
+    """Project, stage, attend with `queries_ready`: am_q4_prefill's bits, 50 times over; the promise is
+    taken by the attend call alone."""
+    Hq, Hkv, Dk, Dv, L = geom
+    N, width = L + 300, 4096
+    _, kq, vq = make_case(1, Hq, Hkv, N, Dk, Dv, L=1, dtype=torch.bfloat16, cuda=cuda, seed=29)
+    view, _ = pkg.kernels.contiguous_view(kq, vq)
+    kv_len = torch.full((1,), N, dtype=torch.int32, device=cuda)
+    g = torch.Generator().manual_seed(7)
+    w = pkg.Q4Weight(*pkg.quantize((torch.randn(Hq * Dk, width, generator=g) * width ** -0.5).bfloat16().to(cuda)))
+    x = torch.randn(L, width, generator=g).bfloat16().to(cuda)
+    buf = pkg.quantized_matmul(x, w)
+    q = buf.view(1, L, Hq, Dk).transpose(1, 2)
+    kw = dict(causal=True, out_dtype=torch.float32)
+    want = pkg.kernels.attention(view, q, Dk ** -0.5, kv_len, N, mode="prefill", **kw)
+    nbytes = pkg.kernels.prefill_workspace_bytes(view, 1, Hq, L, N)
+    ws = torch.full((nbytes,), 255, dtype=torch.uint8, device=cuda)
+    for _ in range(50):
+        buf.fill_(float("nan"))
+        ws.fill_(255)
+        pkg.quantized_matmul(x, w, out=buf)
+        pkg.kernels.attention(view, q, Dk ** -0.5, kv_len, N, mode="prefill_stage", workspace=ws, **kw)
+        got = pkg.kernels.attention(view, q, Dk ** -0.5, kv_len, N, mode="prefill_attend", workspace=ws,
+                                    queries_ready=True, **kw)
+        assert torch.equal(got, want), (got - want).abs().max()
+    for mode in ("prefill", "prefill_stage", "decode"):
+        with pytest.raises(ValueError, match="queries_ready"):
+            pkg.kernels.attention(view, q, Dk ** -0.5, kv_len, N, mode=mode, workspace=ws, queries_ready=True, **kw)
