@@ -52,11 +52,12 @@
 // when everything before it was complete.  A call without a stage launch (am_q4_prefill_attend)
 // has no such grid before it, and may follow one that lets its dependents start early (a
 // linear layer that writes the queries): there every thread waits before its first read
-// (wait_first), and only asks L2 for the query rows before that.  What stands behind the wait then,
-// the lengths and the query tile, costs a call of the two-tile kernel 2.5 us (512 tokens over a
-// 4096-token prefix, append, stage and attention 109 -> 112 us a layer; waiting in front of the
-// whole prologue instead: 115); the K/V loads start beside it.  A caller who promises that a stage
-// call directly precedes and the queries were complete before it (queries_ready) keeps the 109.
+// (wait_first).  The two-tile kernel sets up its barriers and TMEM and asks L2 for the query rows
+// before that, and its K/V loads start beside the query tile: 512 tokens over a 4096-token prefix
+// take 109 us a layer (append, stage, attention), 112 with the wait and 115 with one in front of
+// the whole prologue, where the one-tile kernel has it (Gemma-3 shape 253 -> 259 us).  A caller who
+// promises that a stage call directly precedes and the queries were complete before it
+// (queries_ready) has no such wait.
 //
 // Reference semantics: the compiled quantized SDPA (mlx_fused_attention.py:69-139) as used
 // by chunked prefill (batch_engine.py:339-456): the chunk's own K/V are already in the Q4
@@ -591,7 +592,19 @@ __global__ void __launch_bounds__(PrefillRoles<BN, QV4>::THREADS, 1)
   const int l0 = (gridDim.x - 1 - blockIdx.x) * tok_per_cta;
   const int l_last = min(l0 + tok_per_cta, p.q_len) - 1;
 
-  // ---- setup: barriers and TMEM, before the wait
+  if (p.wait_first) griddep_wait();
+  const int n = p.kv_len[b];
+  const int st = p.kv_start != nullptr ? p.kv_start[b] : 0;
+  int blo, bhi;  // the workspace plane holds keys [blo, blo + nw)
+  prefill_block_range(p, b, blo, bhi);
+  bhi = min(bhi, blo + p.nw);
+  const int pos_min = n - p.q_len + l0, pos_max = n - p.q_len + l_last;
+  int lo = blo, hi = bhi;  // keys this CTA's rows can see
+  if (!DENSE && p.window > 0) lo = max(lo, pos_min - p.window + 1);
+  if (p.causal) hi = min(hi, pos_max + 1);
+  const int n_tiles = hi > lo ? (hi - lo + BN - 1) / BN : 0;
+
+  // ---- setup
   if (tid == 0) {
     for (int i = 0; i < LY::B_COUNT; ++i) {
       const bool pfull = i == LY::B_PFULL || i == LY::B_PFULL + 1;
@@ -607,47 +620,29 @@ __global__ void __launch_bounds__(PrefillRoles<BN, QV4>::THREADS, 1)
                  "r"(LY::TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
   }
-  tc::fence_before();
-  __syncthreads();
-  tc::fence_after();
-  const uint32_t tmem = *tmem_slot;
-  // this thread's part of a query row; null past the tile's rows
-  constexpr int QCH = DK / 16;
-  const uint16_t* qrow = nullptr;
-  if (tid < 256) {
-    const int r = tid >> 1, l = l0 + r / n_rep, hq = h * n_rep + r % n_rep;
-    if (r < tok_per_cta * n_rep && l < p.q_len)
-      qrow = p.q + (int64_t)b * p.qsb + (int64_t)hq * p.qsh + (int64_t)l * p.qsl + (tid & 1) * (DK / 2);
-  }
-  if (p.wait_first) {
-    q_chunks_prefetch<QCH>(qrow);
-    griddep_wait();
-  }
-  uint4 raw[QCH];
-  q_chunks_load<QCH>(qrow, qrow != nullptr, raw);
-  const int n = p.kv_len[b];
-  const int st = p.kv_start != nullptr ? p.kv_start[b] : 0;
-  int blo, bhi;  // the workspace plane holds keys [blo, blo + nw)
-  prefill_block_range(p, b, blo, bhi);
-  bhi = min(bhi, blo + p.nw);
-  const int pos_min = n - p.q_len + l0, pos_max = n - p.q_len + l_last;
-  int lo = blo, hi = bhi;  // keys this CTA's rows can see
-  if (!DENSE && p.window > 0) lo = max(lo, pos_min - p.window + 1);
-  if (p.causal) hi = min(hi, pos_max + 1);
-  const int n_tiles = hi > lo ? (hi - lo + BN - 1) / BN : 0;
-
   if (tid < 256) {
     // query row r -> fp16 with a power-of-two prescale (exact for fp16 / bf16 inputs); two
     // threads per row (adjacent lanes), each staging half of it
     const int r = tid >> 1, half = tid & 1;
-    float amax = q_chunks_amax<QCH>(raw, p.q_bf16 != 0);
+    constexpr int CH = DK / 16;
+    const int rl = r / n_rep;
+    const bool row_ok = r < tok_per_cta * n_rep && l0 + rl < p.q_len;
+    const int l = l0 + (row_ok ? rl : 0);
+    const int hq = h * n_rep + r % n_rep;
+    const uint16_t* qrow = p.q + (int64_t)b * p.qsb + (int64_t)hq * p.qsh + (int64_t)l * p.qsl;
+    uint4 raw[CH];
+    q_chunks_load<CH>(qrow + half * (DK / 2), row_ok, raw);
+    float amax = q_chunks_amax<CH>(raw, p.q_bf16 != 0);
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     const float pw = q_row_prescale(amax, p.scale_log2);
     if (half == 0) sqf[r] = p.scale_log2 / pw;
-    q_chunks_store<QCH>(smem + LY::OFF_Q, LY::QSLAB, raw, pw, p.q_bf16 != 0, r, half * QCH);
+    q_chunks_store<CH>(smem + LY::OFF_Q, LY::QSLAB, raw, pw, p.q_bf16 != 0, r, half * CH);
   }
   fence_proxy_async_smem();
-  if (warp != RL::TMA_WARP) named_bar_sync(5, RL::THREADS - 32);  // (the K/V loads need no query)
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
   constexpr uint32_t ID_S = tc::idesc(128, BN, false);
   constexpr uint32_t ID_O = tc::idesc(128, DV, true);
 
