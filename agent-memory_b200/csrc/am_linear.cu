@@ -99,9 +99,11 @@ cudaError_t launch_weight_pack(const void* scales, const void* biases, bool bf16
 //   cp.async ring: the warps of a SM keep 74 to 110 KB in flight, across tile and expert ends.
 // * Partial sums meet in shared memory every few tiles, in a fixed order.
 // * The work of all experts is one sequence of row tiles, cut evenly over the CTAs.
-// * Bound by instruction issue (70 a warp for 16 weight rows x 64 inputs, 50 in the loop) a little below
-//   HBM: 1 token 128256x4096 55.5 us, 5.3 TB/s (a plain read of the bytes 45.7), 8 tokens 67;
-//   small matrices by a start of 3 us: 1 token 4096x4096 5.5 to 5.8 us.
+// * What bounds it (ncu, 128256x4096): no unit alone.  1 token 56 us, 5.3 TB/s (a plain read of the
+//   bytes 45.7): issue slots 65 % busy (70 instructions a warp for 16 weight rows x 64 inputs), ALU
+//   60 %, shared memory 55 %.  8 tokens 70 us: shared memory 70 % (23 wavefronts for the same piece, 8
+//   of them the activations read again for every row tile), issue 60 % (83 instructions), DRAM 50 %.
+//   Small matrices by a start of 3 us: 1 token 4096x4096 5.6 us; 8 tokens 4096x14336 14.9.
 // * Before griddepcontrol.wait the CTA only asks L2 for its first codes (a prefetch reads
 //   nothing, so it may run before the previous kernel is done).
 constexpr int kFewWarps = 16, kFewLogWarps = 4;

@@ -210,6 +210,9 @@ __device__ __forceinline__ int find_item(const LinearParams& p, int item, int to
   return -1;
 }
 
+// silu(g) * u by the fast exponential (off by up to 2 + 1.2 |g| ulp) and division (2 ulp): 2^-18 of
+// silu at g = -20, beside the output's own rounding of 2^-12 (fp16) or 2^-9.  Below g = -87.3 it
+// is 0, where |silu| is less than 1.1e-36.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 // Two outputs as a pair of the call's type.

@@ -12,8 +12,8 @@
 // activations; their full barrier, shared with the dequantized operand's, is the leader's.  8
 // warps dequantize (two groups of 4, a 64-input slab of a step each) and write the output: TMEM holds
 // the 256-column accumulator and eight operand slabs.  The MMA shape follows the item: N is its tokens
-// rounded up to 32.  4096 tokens 14336x4096 gated: 672 us, 1.43 PFLOP/s, in a burst and 780 at the power
-// cap, which bounds it; a tile of few inputs is bound by its output (32 experts 2880x2880 gated, 512
+// rounded up to 32.  4096 tokens 14336x4096 gated: 668 us, 1.44 PFLOP/s, in a burst and 780 at the power
+// cap, which bounds it (ncu, 2048 tokens 16384x4096 gated: tensor pipe 81 % busy, issue slots 34 %); a tile of few inputs is bound by its output (32 experts 2880x2880 gated, 512
 // rows each: 510 to 540 us, 1.0 to 1.07 PFLOP/s).  Waits are bounded as in am_linear_tc.cu; the CTAs of a pair leave together.
 #include <algorithm>
 #include <climits>

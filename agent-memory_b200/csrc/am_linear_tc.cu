@@ -21,10 +21,12 @@
 //    gridDim.x; the loads of its next tile run during the output of the last one.
 //    With few tiles the inputs are split over the CTAs of a cluster, whose fp32 sums meet in
 //    distributed shared memory, in rank order.
-// Up to 64 tokens two CTAs share a SM and the kernel is bound by the instructions of the dequantization
-// (150 a warp for 32 rows x 64 inputs, waits among them) and the latency of a slab's chain: 37
-// tokens 15360x3840 gated 25 us, 2.7 TB/s; 128 tokens 14336x4096 gated 31 us.  With few tiles the
-// start, the activations' launch and the join take 10 us: 37 tokens 4096x4096 12 to 13 us.
+// Up to 64 tokens two CTAs share a SM.  No unit is saturated (ncu, 37 tokens 65536x4096 gated, 85 us:
+// issue slots 59 % busy, tensor pipe 48 %, shared memory 35 %, DRAM 45 %; most stalls wait for the
+// TMEM stores and barriers): what bounds it is the latency of a slab's chain, codes to
+// commit, which two CTAs hide only in part.  At 128 tokens the tensor pipe is 62 % busy.  37 tokens
+// 15360x3840 gated 26 us, 2.6 TB/s; 128 tokens 14336x4096 gated 33 us.  With few tiles the
+// start, the activations' launch and the join take 10 us: 37 tokens 4096x4096 13 us.
 // Every wait is bounded (LinearParams::wait_ns); on timeout the kernel flags AM_STATUS_TIMEOUT,
 // lets its copies and MMAs in flight finish, frees its TMEM and returns.
 //
