@@ -11,10 +11,10 @@ exact weights: scales and biases are held in fp16 under powers of two per weight
 a scale from 2**-28 and a bias from 2**-24 of the row's largest scale on (or of 1/16 of its largest
 bias, if that is larger).  For more tokens a weight is ``scale * code + bias`` rounded to fp16 (11
 bits, or 2**-14 of that largest scale if that is more); in a gated float16 layer, where two such
-errors would be 1.6 times the output's own rounding, it is the sum of two fp16 parts.  An activation is exact
-(bf16 values enter as fp16 under a power of two per token; only values below 2**-28 of their
-token's largest lose bits).  A token with infinite
-or NaN activations gets the infinities and NaN of the formula.  The weights are frozen: there is no backward pass.
+errors would be 1.6 times the output's own rounding, it is the sum of two fp16 parts.  An
+activation enters as fp16 under a power of two per token: only values below 2**-24 of their
+token's largest lose bits (and keep 2**-35 of that).  A token with infinite or NaN activations gets
+the infinities and NaN of the formula.  The weights are frozen: there is no backward pass.
 """
 
 from __future__ import annotations

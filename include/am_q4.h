@@ -319,10 +319,10 @@ int am_q4_weight_pack(const void* scales, const void* biases, int32_t dtype, int
  * multiply the weights as am_q4_weight_pack keeps them.  For more a weight enters as scale *
  * code + bias rounded once to fp16, to 11 bits or 2^-14 L (above) if that is more, for a gated
  * fp16 call as the sum of two such parts (2^-12 L).  Activations are exact but for values
- * below 2^-28 of their token's largest; a token with infinite or NaN ones gets the
- * infinities and NaN of the formula.  workspace: device memory, 256-byte aligned, of the size the query gives
- * (0 for a few tokens); scratch of the call, free again when it has run.  status (device word
- * or NULL) gets AM_STATUS_TIMEOUT where a bounded wait ran out: rows of out are then unwritten.
+ * below 2^-24 of their token's largest, which keep 2^-35 of that; a token with infinite or NaN
+ * ones gets the infinities and NaN of the formula.  workspace: device memory, 256-byte aligned,
+ * of the size the query gives (0 for a few tokens); scratch of the call, free again when it has
+ * run.  status (device word or NULL) gets AM_STATUS_TIMEOUT where a bounded wait ran out: rows of out are then unwritten.
  */
 size_t am_q4_linear_workspace_bytes(const am_q4_weight* w, const am_q4_weight* up, int32_t rows);
 int am_q4_linear(const am_q4_weight* w, const am_q4_weight* up, const void* x, int64_t x_stride,
